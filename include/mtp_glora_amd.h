@@ -425,6 +425,122 @@ int mga_soft_ce_bwd(const void *student, int64_t student_row_stride,
                     const float *grad_output, const float *stats,
                     void *grad, int64_t grad_row_stride, void *stream);
 
+/*
+ * The k largest logits of each row, in order (value descending, lower column
+ * first among equals; -0 equals +0, NaN stands below -inf): values [n_rows, k]
+ * in the logits' dtype, ids [n_rows, k] their columns; lse [n_rows] (may be
+ * null) the row's log sum_j exp(x_j / temperature) in fp32 (-inf for a row of
+ * -inf alone, NaN where the row holds a NaN). Rows of n_cols <= 1 048 576
+ * logits, row r at logits + r * row_stride elements, columns contiguous;
+ * 1 <= k <= min(n_cols, 1024); temperature positive and finite.
+ * No counterpart in the reference, which keeps a teacher's whole rows
+ * (mtp_glora/core/mtp.py:121-126): what is kept of them here feeds
+ * mga_top_logits_ce_*.
+ */
+int mga_top_logits(const void *logits, int64_t row_stride, int32_t n_rows, int32_t n_cols, int32_t dtype,
+                   int32_t k, float temperature, void *values, int32_t *ids, float *lse, void *stream);
+
+/*
+ * Cross-entropy of student logits x [n_rows, n_cols] against the k logits t that
+ * were kept of each teacher row (values [n_rows, k] in values_dtype, any of the
+ * three; ids [n_rows, k] their columns, int64 if ids_are_int64 else int32), with
+ * tau = temperature:
+ *   an entry whose id is outside [0, n_cols) does not count (padding);
+ *   q_k = exp(t_k / tau - teacher_lse[r]); with teacher_lse null the softmax of
+ *   t / tau over the row's entries; 0 for t_k = -inf and for teacher_lse = -inf;
+ *   Q = sum_k q_k,  p = softmax(x / tau),
+ *   row_loss[r] = tau^2 (Q log sum_j exp(x_j / tau) - sum_k q_k x_{id_k} / tau).
+ * loss_sum: the row losses added in a fixed order. q [n_rows, k] (null: not kept)
+ * and stats [3, n_rows] = (max x, sum exp((x - max) / tau), Q) are what the
+ * backward reads. A row without an entry of q > 0 has loss and gradient 0,
+ * whatever its logits are; a student logit of -inf at an entry of q > 0 gives an
+ * infinite loss; NaN and +inf among other rows' student logits give NaN. An id
+ * may stand in a row more than once: its q add up.
+ * 1 <= k <= 1024. workspace: mga_top_logits_ce_workspace_floats fp32 values.
+ * Stands beside mga_soft_ce_* (loss.py:259-330), which reads whole teacher rows.
+ */
+int64_t mga_top_logits_ce_workspace_floats(int32_t n_rows, int32_t n_cols);
+int mga_top_logits_ce_fwd(const void *student, int64_t student_row_stride, const void *values,
+                          int64_t values_row_stride, int32_t values_dtype, const void *ids, int64_t ids_row_stride,
+                          int32_t ids_are_int64, const float *teacher_lse, int32_t n_rows, int32_t n_cols, int32_t k,
+                          float temperature, int32_t dtype, float *q, float *stats, float *row_loss, float *loss_sum,
+                          float *workspace, void *stream);
+
+/*
+ * Its backward for the student (the teacher gets none):
+ *   grad[r, j] = grad_output * tau * (Q p_j - sum over k with id_k = j of q_k),
+ * in the student's dtype, one rounding; grad_output: one fp32 value in device
+ * memory.
+ */
+int mga_top_logits_ce_bwd(const void *student, int64_t student_row_stride, const void *ids, int64_t ids_row_stride,
+                          int32_t ids_are_int64, const float *q, const float *stats, int32_t n_rows, int32_t n_cols,
+                          int32_t k, float temperature, int32_t dtype, const float *grad_output, void *grad,
+                          int64_t grad_row_stride, void *stream);
+
+/*
+ * Loss and gradient in one call, with an upstream gradient that the host knows:
+ * loss_sum as mga_top_logits_ce_fwd, grad as mga_top_logits_ce_bwd with
+ * grad_output = scale. Rows of up to 163 840 16-bit or 81 920 fp32 logits are
+ * read once; longer ones as by the two calls. grad may not overlap student.
+ * workspace: mga_top_logits_ce_step_workspace_floats fp32 values.
+ */
+int64_t mga_top_logits_ce_step_workspace_floats(int32_t n_rows, int32_t n_cols, int32_t k);
+int mga_top_logits_ce_step(const void *student, int64_t student_row_stride, const void *values,
+                           int64_t values_row_stride, int32_t values_dtype, const void *ids, int64_t ids_row_stride,
+                           int32_t ids_are_int64, const float *teacher_lse, int32_t n_rows, int32_t n_cols, int32_t k,
+                           float temperature, float scale, int32_t dtype, float *row_loss, float *loss_sum, void *grad,
+                           int64_t grad_row_stride, float *workspace, void *stream);
+
+/*
+ * One token a row from its logits and one given uniform number u in [0, 1):
+ *   T = temperature <= 0 (or NaN): the first of the row's largest logits;
+ *   else, with the tokens in order (logit descending, lower column first) and
+ *   w = exp((x - max x) / T) (in a row with +inf: 1 for those, else 0), three
+ *   filters leave
+ *     the first top_k tokens (top_k <= 0 or >= n_cols: all),
+ *     of those the shortest leading run with at least top_p of their weight
+ *     (top_p >= 1: all; at least the first),
+ *     of those the tokens with w >= min_p (min_p <= 0: all; the largest stays),
+ *   and the token is the first, by ascending column, at which the running sum of
+ *   the weights that are left exceeds u times their total.
+ * Weights are computed in 64 bits and held in whole multiples of 2^-45 (2^-42 at
+ * the largest n_cols) of the largest, whose sums are exact. NaN and -inf logits are never drawn; a row with no
+ * other gives -1; u < 0 or NaN draws as 0, u >= 1 the last token that is left.
+ * temperature, top_k, top_p and min_p: one value a row in device memory, or
+ * null for the *_all value. n_cols <= 1 048 576. No counterpart in the reference
+ * (its sampler head is trained, never run; mtp_glora/core/mtp.py:28-144).
+ */
+int mga_sample(const void *logits, int64_t row_stride, int32_t n_rows, int32_t n_cols, int32_t dtype,
+               const float *uniform, const float *temperature, float temperature_all, const int32_t *top_k,
+               int32_t top_k_all, const float *top_p, float top_p_all, const float *min_p, float min_p_all,
+               int64_t *token, void *stream);
+
+/*
+ * Scaled embedding lookup: out[n, :] = T(scale * weight[ids[n], :]) for n_ids ids
+ * (int64 if ids_are_int64 else int32) of a [n_rows, width] table, T = rounding to
+ * the dtype; zeros for an id outside the table. The lookup at the start of
+ * Qwen3Model.forward (mtp_glora/models/modeling_qwen3.py:436); the table is the one
+ * that resize_token_embeddings grows (:616).
+ */
+int mga_embedding_fwd(const void *ids, int32_t ids_are_int64, int32_t n_ids, const void *weight,
+                      int64_t weight_row_stride, int32_t n_rows, int32_t width, float scale, int32_t dtype, void *out,
+                      int64_t out_row_stride, void *stream);
+
+/*
+ * Its gradient: grad_weight[v, :] = T(scale * sum over n with ids[n] = v of
+ * grad_out[n, :]), summed in fp32 in ascending order of n; ids equal to
+ * padding_idx (-1: none) or outside the table count nowhere. The whole of
+ * grad_weight [n_rows, width] is written, or, with accumulate, the sums are added
+ * to it (one rounding) and rows without a token are left as they are.
+ * grad_weight_dtype: dtype, or MGA_DTYPE_F32. workspace:
+ * mga_embedding_workspace_bytes bytes, 16-byte aligned.
+ */
+int64_t mga_embedding_workspace_bytes(int32_t n_ids, int32_t width);
+int mga_embedding_bwd(const void *grad_out, int64_t grad_out_row_stride, const void *ids, int32_t ids_are_int64,
+                      int32_t n_ids, float scale, int64_t padding_idx, int32_t n_rows, int32_t width, int32_t dtype,
+                      void *grad_weight, int64_t grad_weight_row_stride, int32_t grad_weight_dtype,
+                      int32_t accumulate, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

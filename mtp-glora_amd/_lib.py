@@ -81,10 +81,24 @@ SIGNATURES = {
     "mga_soft_ce_fwd": [_P, _I64, _P, _I64, _I32, _I32, _I32, _P, _P, _P, _P],
     "mga_soft_ce_loss": [_P, _I64, _P, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P],
     "mga_soft_ce_bwd": [_P, _I64, _P, _I64, _I32, _I32, _I32, _P, _P, _P, _I64, _P],
+    "mga_top_logits": [_P, _I64, _I32, _I32, _I32, _I32, _F32, _P, _P, _P, _P],
+    "mga_top_logits_ce_workspace_floats": [_I32, _I32],
+    "mga_top_logits_ce_fwd": [_P, _I64, _P, _I64, _I32, _P, _I64, _I32, _P, _I32, _I32, _I32, _F32, _I32,
+                              _P, _P, _P, _P, _P, _P],
+    "mga_top_logits_ce_bwd": [_P, _I64, _P, _I64, _I32, _P, _P, _I32, _I32, _I32, _F32, _I32, _P, _P, _I64, _P],
+    "mga_top_logits_ce_step_workspace_floats": [_I32, _I32, _I32],
+    "mga_top_logits_ce_step": [_P, _I64, _P, _I64, _I32, _P, _I64, _I32, _P, _I32, _I32, _I32, _F32, _F32, _I32,
+                               _P, _P, _P, _I64, _P, _P],
+    "mga_sample": [_P, _I64, _I32, _I32, _I32, _P, _P, _F32, _P, _I32, _P, _F32, _P, _F32, _P, _P],
+    "mga_embedding_fwd": [_P, _I32, _I32, _P, _I64, _I32, _I32, _F32, _I32, _P, _I64, _P],
+    "mga_embedding_workspace_bytes": [_I32, _I32],
+    "mga_embedding_bwd": [_P, _I64, _P, _I32, _I32, _F32, _I64, _I32, _I32, _I32, _P, _I64, _I32, _I32, _P, _I64, _P],
 }
 _RESTYPES = {"mga_last_error": ctypes.c_char_p, "mga_soft_ce_workspace_floats": ctypes.c_int64,
              "mga_gated_lora_workspace_bytes": ctypes.c_int64, "mga_attn_workspace_bytes": ctypes.c_int64,
-             "mga_header_hash": ctypes.c_uint64}
+             "mga_top_logits_ce_workspace_floats": ctypes.c_int64,
+             "mga_top_logits_ce_step_workspace_floats": ctypes.c_int64,
+             "mga_embedding_workspace_bytes": ctypes.c_int64, "mga_header_hash": ctypes.c_uint64}
 
 
 class MGAError(RuntimeError):

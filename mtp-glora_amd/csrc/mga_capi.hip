@@ -841,4 +841,208 @@ int mga_soft_ce_bwd(const void *student, int64_t student_row_stride, const void 
   return check_launch("mga_soft_ce_bwd");
 }
 
+
+// ---- vocabulary operators ------------------------------------------------------
+
+namespace {
+
+constexpr int32_t kMaxVocab = 1 << 20, kMaxTopLogits = 1024;
+
+// A [n_rows, n_cols] operand of 16-bit or fp32 elements.
+int check_matrix(const char *fn, const char *name, const void *p, int64_t rs, int32_t n_rows, int32_t n_cols,
+                 int32_t dtype) {
+  const int eb = elem_bytes(dtype);
+  if (!eb) return fail(MGA_ERR_INVALID, "%s: unknown dtype code %d", fn, dtype);
+  if (n_rows <= 0 || n_cols <= 0) return fail(MGA_ERR_INVALID, "%s: bad sizes (rows=%d cols=%d)", fn, n_rows, n_cols);
+  if (!p) return fail(MGA_ERR_INVALID, "%s: %s is null", fn, name);
+  if (rs < n_cols) return fail(MGA_ERR_INVALID, "%s: %s row stride %lld < %d columns", fn, name, (long long)rs, n_cols);
+  if (reinterpret_cast<uintptr_t>(p) % eb)
+    return fail(MGA_ERR_INVALID, "%s: %s is not aligned to its elements", fn, name);
+  return MGA_OK;
+}
+
+int check_positive(const char *fn, const char *name, float v) {
+  if (v > 0.f && v < __builtin_huge_valf()) return MGA_OK;
+  return fail(MGA_ERR_INVALID, "%s: %s must be positive and finite (got %g)", fn, name, (double)v);
+}
+
+int check_top_k(const char *fn, int32_t k) {
+  if (k >= 1 && k <= kMaxTopLogits) return MGA_OK;
+  return fail(MGA_ERR_INVALID, "%s: k must be 1 to %d (got %d)", fn, kMaxTopLogits, k);
+}
+
+int check_top_ce(const char *fn, const mga::TopLogitsCeArgs &a, int32_t dtype) {
+  int rc = check_matrix(fn, "student", a.x, a.xs, a.N, a.V, dtype);
+  if (rc == MGA_OK) rc = check_top_k(fn, a.K);
+  if (rc == MGA_OK) rc = check_positive(fn, "temperature", a.tau);
+  if (rc != MGA_OK) return rc;
+  if (!a.ids || a.ids_rs < a.K) return fail(MGA_ERR_INVALID, "%s: ids null or with a row stride below k", fn);
+  if (reinterpret_cast<uintptr_t>(a.ids) % (a.ids64 ? 8 : 4))
+    return fail(MGA_ERR_INVALID, "%s: ids are not aligned to their elements", fn);
+  return MGA_OK;
+}
+
+int check_teacher(const char *fn, const mga::TopLogitsCeArgs &a, const float *workspace) {
+  const int rc = check_matrix(fn, "values", a.values, a.values_rs, a.N, a.K, a.values_dtype);
+  if (rc != MGA_OK) return rc;
+  if (!a.loss || !a.sum || !workspace) return fail(MGA_ERR_INVALID, "%s: null output or workspace", fn);
+  return MGA_OK;
+}
+
+int check_embedding(const char *fn, const void *ids, int32_t ids64, int32_t n, int32_t n_rows, int32_t width,
+                    int32_t dtype) {
+  if (!elem_bytes(dtype)) return fail(MGA_ERR_INVALID, "%s: unknown dtype code %d", fn, dtype);
+  if (n < 0 || n_rows <= 0 || width <= 0)
+    return fail(MGA_ERR_INVALID, "%s: bad sizes (ids=%d rows=%d width=%d)", fn, n, n_rows, width);
+  if (n > 0 && (!ids || reinterpret_cast<uintptr_t>(ids) % (ids64 ? 8 : 4)))
+    return fail(MGA_ERR_INVALID, "%s: ids null or not aligned to their elements", fn);
+  return MGA_OK;
+}
+
+bool vec_rows(const void *p, int64_t rs, int eb) { return aligned16(p) && (rs * eb) % 16 == 0; }
+
+}  // namespace
+
+int mga_top_logits(const void *logits, int64_t row_stride, int32_t n_rows, int32_t n_cols, int32_t dtype, int32_t k,
+                   float temperature, void *values, int32_t *ids, float *lse, void *stream) {
+  const char *fn = "mga_top_logits";
+  int rc = check_matrix(fn, "logits", logits, row_stride, n_rows, n_cols, dtype);
+  if (rc == MGA_OK) rc = check_top_k(fn, k);
+  if (rc == MGA_OK) rc = check_positive(fn, "temperature", temperature);
+  if (rc != MGA_OK) return rc;
+  if (k > n_cols || n_cols > kMaxVocab)
+    return fail(MGA_ERR_INVALID, "%s: k=%d of %d columns (at most %d)", fn, k, n_cols, kMaxVocab);
+  if (!values || !ids) return fail(MGA_ERR_INVALID, "%s: null output", fn);
+  mga::launch_top_logits(logits, row_stride, n_rows, n_cols, dtype, k, temperature, values, ids, lse,
+                         (hipStream_t)stream);
+  return check_launch(fn);
+}
+
+int64_t mga_top_logits_ce_workspace_floats(int32_t n_rows, int32_t n_cols) {
+  return n_rows <= 0 || n_cols <= 0 ? 0 : mga::top_ce_workspace_floats(n_rows, n_cols);
+}
+
+int64_t mga_top_logits_ce_step_workspace_floats(int32_t n_rows, int32_t n_cols, int32_t k) {
+  if (n_rows <= 0 || n_cols <= 0 || k <= 0) return 0;
+  return mga::top_ce_workspace_floats(n_rows, n_cols) + (3 + (int64_t)k) * n_rows;
+}
+
+int mga_top_logits_ce_fwd(const void *student, int64_t student_row_stride, const void *values,
+                          int64_t values_row_stride, int32_t values_dtype, const void *ids, int64_t ids_row_stride,
+                          int32_t ids_are_int64, const float *teacher_lse, int32_t n_rows, int32_t n_cols, int32_t k,
+                          float temperature, int32_t dtype, float *q, float *stats, float *row_loss, float *loss_sum,
+                          float *workspace, void *stream) {
+  const char *fn = "mga_top_logits_ce_fwd";
+  const mga::TopLogitsCeArgs a{student, student_row_stride, values, values_row_stride, ids, ids_row_stride, teacher_lse,
+                               q, stats, row_loss, loss_sum, nullptr, nullptr, 0, temperature, 1.f, n_rows, n_cols, k,
+                               values_dtype, ids_are_int64 != 0};
+  int rc = check_top_ce(fn, a, dtype);
+  if (rc == MGA_OK) rc = check_teacher(fn, a, workspace);
+  if (rc != MGA_OK) return rc;
+  if (!stats) return fail(MGA_ERR_INVALID, "%s: null stats", fn);
+  mga::launch_top_ce_fwd(a, dtype, workspace, (hipStream_t)stream);
+  return check_launch(fn);
+}
+
+int mga_top_logits_ce_bwd(const void *student, int64_t student_row_stride, const void *ids, int64_t ids_row_stride,
+                          int32_t ids_are_int64, const float *q, const float *stats, int32_t n_rows, int32_t n_cols,
+                          int32_t k, float temperature, int32_t dtype, const float *grad_output, void *grad,
+                          int64_t grad_row_stride, void *stream) {
+  const char *fn = "mga_top_logits_ce_bwd";
+  const mga::TopLogitsCeArgs a{student, student_row_stride, nullptr, 0, ids, ids_row_stride, nullptr,
+                               const_cast<float *>(q), const_cast<float *>(stats), nullptr, nullptr, grad_output, grad,
+                               grad_row_stride, temperature, 1.f, n_rows, n_cols, k, 0, ids_are_int64 != 0};
+  int rc = check_top_ce(fn, a, dtype);
+  if (rc == MGA_OK) rc = check_matrix(fn, "grad", grad, grad_row_stride, n_rows, n_cols, dtype);
+  if (rc != MGA_OK) return rc;
+  if (!q || !stats || !grad_output) return fail(MGA_ERR_INVALID, "%s: null q, stats or grad_output", fn);
+  mga::launch_top_ce_bwd(a, dtype, (hipStream_t)stream);
+  return check_launch(fn);
+}
+
+int mga_top_logits_ce_step(const void *student, int64_t student_row_stride, const void *values,
+                           int64_t values_row_stride, int32_t values_dtype, const void *ids, int64_t ids_row_stride,
+                           int32_t ids_are_int64, const float *teacher_lse, int32_t n_rows, int32_t n_cols, int32_t k,
+                           float temperature, float scale, int32_t dtype, float *row_loss, float *loss_sum, void *grad,
+                           int64_t grad_row_stride, float *workspace, void *stream) {
+  const char *fn = "mga_top_logits_ce_step";
+  float *stats = workspace, *q = stats ? stats + 3 * (int64_t)n_rows : nullptr;
+  const mga::TopLogitsCeArgs a{student, student_row_stride, values, values_row_stride, ids, ids_row_stride, teacher_lse,
+                               q, stats, row_loss, loss_sum, nullptr, grad, grad_row_stride, temperature, scale, n_rows,
+                               n_cols, k, values_dtype, ids_are_int64 != 0};
+  int rc = check_top_ce(fn, a, dtype);
+  if (rc == MGA_OK) rc = check_teacher(fn, a, workspace);
+  if (rc == MGA_OK) rc = check_matrix(fn, "grad", grad, grad_row_stride, n_rows, n_cols, dtype);
+  if (rc != MGA_OK) return rc;
+  const uintptr_t eb = elem_bytes(dtype), x0 = reinterpret_cast<uintptr_t>(student), g0 = reinterpret_cast<uintptr_t>(grad);
+  const uintptr_t x1 = x0 + ((uintptr_t)(n_rows - 1) * student_row_stride + n_cols) * eb;
+  const uintptr_t g1 = g0 + ((uintptr_t)(n_rows - 1) * grad_row_stride + n_cols) * eb;
+  if (x0 < g1 && g0 < x1) return fail(MGA_ERR_INVALID, "%s: grad overlaps student", fn);
+  mga::launch_top_ce_step(a, dtype, q + (int64_t)n_rows * k, (hipStream_t)stream);
+  return check_launch(fn);
+}
+
+int mga_sample(const void *logits, int64_t row_stride, int32_t n_rows, int32_t n_cols, int32_t dtype,
+               const float *uniform, const float *temperature, float temperature_all, const int32_t *top_k,
+               int32_t top_k_all, const float *top_p, float top_p_all, const float *min_p, float min_p_all,
+               int64_t *token, void *stream) {
+  const char *fn = "mga_sample";
+  const int rc = check_matrix(fn, "logits", logits, row_stride, n_rows, n_cols, dtype);
+  if (rc != MGA_OK) return rc;
+  if (n_cols > kMaxVocab) return fail(MGA_ERR_INVALID, "%s: %d columns (at most %d)", fn, n_cols, kMaxVocab);
+  if (!uniform || !token) return fail(MGA_ERR_INVALID, "%s: null uniform or token", fn);
+  mga::launch_sample(logits, row_stride, n_rows, n_cols, dtype, uniform,
+                     {temperature, top_k, top_p, min_p, temperature_all, top_k_all, top_p_all, min_p_all}, token,
+                     (hipStream_t)stream);
+  return check_launch(fn);
+}
+
+int mga_embedding_fwd(const void *ids, int32_t ids_are_int64, int32_t n_ids, const void *weight,
+                      int64_t weight_row_stride, int32_t n_rows, int32_t width, float scale, int32_t dtype, void *out,
+                      int64_t out_row_stride, void *stream) {
+  const char *fn = "mga_embedding_fwd";
+  int rc = check_embedding(fn, ids, ids_are_int64, n_ids, n_rows, width, dtype);
+  if (rc == MGA_OK) rc = check_matrix(fn, "weight", weight, weight_row_stride, n_rows, width, dtype);
+  if (rc != MGA_OK || n_ids == 0) return rc;
+  rc = check_matrix(fn, "out", out, out_row_stride, n_ids, width, dtype);
+  if (rc != MGA_OK) return rc;
+  if ((int64_t)n_ids * (width / 1024 + 1) >= int64_t(1) << 32)
+    return fail(MGA_ERR_INVALID, "%s: %d ids of width %d are too many", fn, n_ids, width);
+  const int eb = elem_bytes(dtype);
+  const mga::EmbedArgs a{ids, weight, weight_row_stride, nullptr, 0, out, out_row_stride, scale, -1, 0, n_ids, n_rows,
+                         width, ids_are_int64 != 0};
+  mga::launch_embed_fwd(a, dtype, (int64_t)width * eb % 16 == 0 && vec_rows(weight, weight_row_stride, eb) &&
+                        vec_rows(out, out_row_stride, eb), (hipStream_t)stream);
+  return check_launch(fn);
+}
+
+int64_t mga_embedding_workspace_bytes(int32_t n_ids, int32_t width) {
+  return n_ids <= 0 || width <= 0 ? 0 : mga::embed_workspace_bytes(n_ids, width);
+}
+
+int mga_embedding_bwd(const void *grad_out, int64_t grad_out_row_stride, const void *ids, int32_t ids_are_int64,
+                      int32_t n_ids, float scale, int64_t padding_idx, int32_t n_rows, int32_t width, int32_t dtype,
+                      void *grad_weight, int64_t grad_weight_row_stride, int32_t grad_weight_dtype,
+                      int32_t accumulate, void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *fn = "mga_embedding_bwd";
+  int rc = check_embedding(fn, ids, ids_are_int64, n_ids, n_rows, width, dtype);
+  if (rc == MGA_OK && n_ids > 0)
+    rc = check_matrix(fn, "grad_out", grad_out, grad_out_row_stride, n_ids, width, dtype);
+  if (rc == MGA_OK)
+    rc = check_matrix(fn, "grad_weight", grad_weight, grad_weight_row_stride, n_rows, width, grad_weight_dtype);
+  if (rc != MGA_OK) return rc;
+  if (grad_weight_dtype != dtype && grad_weight_dtype != MGA_DTYPE_F32)
+    return fail(MGA_ERR_INVALID, "%s: grad_weight is neither of the gradients' dtype nor fp32", fn);
+  if (n_ids > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < mga::embed_workspace_bytes(n_ids, width)))
+    return fail(MGA_ERR_INVALID, "%s: workspace null, not 16-byte aligned or smaller than %lld bytes", fn,
+                (long long)mga::embed_workspace_bytes(n_ids, width));
+  const int eb = elem_bytes(dtype), ob = elem_bytes(grad_weight_dtype);
+  const mga::EmbedArgs a{ids, nullptr, 0, grad_out, grad_out_row_stride, grad_weight, grad_weight_row_stride, scale,
+                         padding_idx, 0, n_ids, n_rows, width, ids_are_int64 != 0};
+  const bool vec = (int64_t)width * eb % 16 == 0 && (n_ids == 0 || vec_rows(grad_out, grad_out_row_stride, eb)) &&
+                   vec_rows(grad_weight, grad_weight_row_stride, ob);
+  mga::launch_embed_bwd(a, dtype, grad_weight_dtype, vec, accumulate != 0, workspace, (hipStream_t)stream);
+  return check_launch(fn);
+}
+
 }  // extern "C"

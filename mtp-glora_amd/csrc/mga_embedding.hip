@@ -1,0 +1,388 @@
+// Scaled embedding lookup, out[n] = T(scale W[id_n]), and its gradient by sorted
+// tokens, dW[v] = T(scale sum_{n: id_n = v} dY[n]).
+//
+// In an MTP chunk D of every 1 + D tokens can be the one mask token: a scatter of
+// atomic additions queues hundreds to thousands of rows up at one row of dW. Here
+// the tokens are put in order of (id, position) and summed in that order, in fp32,
+// with one rounding: every run is bit-for-bit repeatable. Both directions are bound
+// by memory, the gradient by writing dW (1.2 GB at 151 936 x 4 096 bf16).
+//
+//   embed_sort_kernel    - a workgroup per kTile tokens sorts its (id, position)
+//       pairs in LDS; the other workgroups clear dW meanwhile;
+//   embed_merge_kernel   - more than one tile: every pair's place among all;
+//   embed_sum_kernel     - grid (chunk of sorted tokens, column slice): sums the
+//       runs of equal ids; a run that lies within its chunk is written, the parts
+//       of one that crosses chunks go to the workspace;
+//   embed_join_kernel    - adds the parts of each crossing run, in order.
+#include <algorithm>
+
+#include "mga_common.hpp"
+#include "mga_internal.hpp"
+
+namespace mga {
+
+namespace {
+
+constexpr int kTile = 8192;
+constexpr int kSortThreads = 1024;
+constexpr int kThreads = 256;
+constexpr uint32_t kNoId = 0xFFFFFFFFu;   // padding and ids outside the table: last in order, summed nowhere
+
+template <typename T> constexpr int kW = 16 / (int)sizeof(T);
+
+__device__ __forceinline__ int64_t token_id(const void *ids, bool ids64, int64_t n) {
+  return ids64 ? static_cast<const int64_t *>(ids)[n] : static_cast<const int32_t *>(ids)[n];
+}
+
+// kW<T> elements from p as fp32: one 16-byte load (VEC), or those of the n <= kW
+// that there are.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_elems(const T *p, int n, float *f) {
+  if constexpr (VEC) {
+    const i32x4 v = *reinterpret_cast<const i32x4 *>(p);
+    if constexpr (sizeof(T) == 4) {
+      const f32x4 x = __builtin_bit_cast(f32x4, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = x[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[2 * e] = pair_lo<T>((uint32_t)v[e]);
+        f[2 * e + 1] = pair_hi<T>((uint32_t)v[e]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kW<T>; ++e) f[e] = e < n ? (float)p[e] : 0.f;
+  }
+}
+// N elements f to p in TO's type; n of them where not VEC
+template <typename TO, bool VEC, int N>
+__device__ __forceinline__ void store_elems(TO *p, int n, const float *f) {
+  if constexpr (VEC) {
+#pragma unroll
+    for (int e = 0; e < N; e += 4) store4(p + e, f[e], f[e + 1], f[e + 2], f[e + 3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < n) p[e] = (TO)f[e];
+  }
+}
+
+}  // namespace
+
+// A wave per part of up to 256 vectors of a token's row, all loads in flight.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kThreads) void embed_fwd_kernel(EmbedArgs a, int32_t parts) {
+  constexpr int W = kW<T>, U = 4;
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  const int64_t n = unit / parts;
+  if (n >= a.N) return;
+  const int part = (int)(unit - n * parts);
+  const int64_t id = token_id(a.ids, a.ids64, n);
+  const bool ok = id >= 0 && id < a.V;
+  const T *w = static_cast<const T *>(a.w) + (ok ? id : 0) * a.w_rs;
+  T *o = static_cast<T *>(a.out) + n * a.out_rs;
+  float f[U][W];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int c = ((part * U + u) * 64 + lane) * W;
+    if (c < a.H && ok) load_elems<T, VEC>(w + c, a.H - c, f[u]);
+    else
+#pragma unroll
+      for (int e = 0; e < W; ++e) f[u][e] = 0.f;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int c = ((part * U + u) * 64 + lane) * W;
+    if (c >= a.H) continue;
+#pragma unroll
+    for (int e = 0; e < W; ++e) f[u][e] *= ok ? a.scale : 0.f;
+    store_elems<T, VEC, W>(o + c, a.H - c, f[u]);
+  }
+}
+
+// Clears [V, H] (row stride rs) a row a wave at a time.
+template <typename TO, bool VEC, bool NT>
+__device__ __forceinline__ void clear_rows(TO *out, int64_t rs, int32_t V, int32_t H, int64_t block, int64_t blocks) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t v = block * (kSortThreads / 64) + (threadIdx.x >> 6); v < V; v += blocks * (kSortThreads / 64)) {
+    TO *o = out + v * rs;
+    if constexpr (VEC) {
+      const i32x4 zero = {0, 0, 0, 0};
+#pragma unroll 4
+      for (int c = lane * kW<TO>; c < H; c += 64 * kW<TO>) {
+        if constexpr (NT) __builtin_nontemporal_store(zero, reinterpret_cast<i32x4 *>(o + c));
+        else *reinterpret_cast<i32x4 *>(o + c) = zero;
+      }
+    } else {
+      for (int c = lane; c < H; c += 64) o[c] = (TO)0.f;
+    }
+  }
+}
+
+template <typename TO, bool VEC, bool NT>
+__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a, int32_t tiles, bool clear,
+                                                                  uint64_t *__restrict__ sorted) {
+  __shared__ uint64_t key[kTile];
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x >= tiles) {
+    if (clear)
+      clear_rows<TO, VEC, NT>(static_cast<TO *>(a.out), a.out_rs, a.V, a.H, blockIdx.x - tiles, gridDim.x - tiles);
+    return;
+  }
+  const int64_t n0 = (int64_t)blockIdx.x * kTile;
+  const int n = (int)min((int64_t)kTile, a.N - n0);
+  int size = 64;
+  while (size < n) size <<= 1;
+  for (int i = tid; i < size; i += kSortThreads) {
+    uint64_t k = ~uint64_t(0);
+    if (i < n) {
+      const int64_t id = token_id(a.ids, a.ids64, n0 + i);
+      const bool ok = id >= 0 && id < a.V && id != a.padding_idx;
+      k = (uint64_t)(ok ? (uint32_t)id : kNoId) << 32 | (uint32_t)(n0 + i);
+    }
+    key[i] = k;
+  }
+  __syncthreads();
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int t = tid; t < size / 2; t += kSortThreads) {
+        const int p = 2 * t - (t & (j - 1)), q = p + j;
+        const uint64_t x = key[p], y = key[q];
+        if ((x > y) == ((p & k) == 0)) {
+          key[p] = y;
+          key[q] = x;
+        }
+      }
+      __syncthreads();
+    }
+  for (int i = tid; i < n; i += kSortThreads) sorted[n0 + i] = key[i];
+}
+
+// Each pair's place: those before it in its own tile and in the others.
+__global__ __launch_bounds__(kThreads) void embed_merge_kernel(const uint64_t *__restrict__ tiles_in, int32_t N,
+                                                               int32_t tiles, uint64_t *__restrict__ sorted) {
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= N) return;
+  const uint64_t k = tiles_in[i];
+  const int own = (int)(i / kTile);
+  int64_t place = i - (int64_t)own * kTile;
+  for (int t = 0; t < tiles; ++t) {
+    if (t == own) continue;
+    const uint64_t *p = tiles_in + (int64_t)t * kTile;
+    int lo = 0, hi = (int)min((int64_t)kTile, N - (int64_t)t * kTile);
+    while (lo < hi) {   // pairs are all different
+      const int mid = (lo + hi) >> 1;
+      if (p[mid] < k) lo = mid + 1;
+      else hi = mid;
+    }
+    place += lo;
+  }
+  sorted[place] = k;
+}
+
+namespace {
+
+__device__ __forceinline__ uint32_t id_at(const uint64_t *sorted, int64_t i) { return (uint32_t)(sorted[i] >> 32); }
+
+// scale f into out[id], added to what is there where ADD
+template <typename TO, bool VEC, bool ADD, int N>
+__device__ __forceinline__ void put_row(const EmbedArgs &a, uint32_t id, int col, float *f) {
+  TO *o = static_cast<TO *>(a.out) + (int64_t)id * a.out_rs + col;
+  const int n = a.H - col;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    f[e] *= a.scale;
+    if constexpr (ADD)
+      if (VEC || e < n) f[e] += (float)o[e];
+  }
+  store_elems<TO, VEC, N>(o, n, f);
+}
+
+}  // namespace
+
+constexpr int kMaxChunk = 64;
+
+template <typename T, typename TO, bool VEC, bool ADD>
+__global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedArgs a, const uint64_t *__restrict__ sorted,
+                                                             int32_t chunk, float *__restrict__ part) {
+  constexpr int W = kW<T>, U = 8;
+  __shared__ uint64_t key[kMaxChunk + 2];   // the chunk's, with its neighbours on both sides
+  const int tid = threadIdx.x;
+  const int64_t n0 = (int64_t)blockIdx.x * chunk;
+  const int n = (int)min((int64_t)chunk, a.N - n0);
+  if (tid < n + 2) {
+    const int64_t i = n0 - 1 + tid;
+    key[tid] = i >= 0 && i < a.N ? sorted[i] : (uint64_t)kNoId << 32;
+  }
+  __syncthreads();
+  const int col = (blockIdx.y * kThreads + tid) * W;
+  if (col >= a.H) return;
+  auto id = [&](int i) { return (uint32_t)(key[i + 1] >> 32); };
+  const T *dy = static_cast<const T *>(a.dy) + col;
+  float acc[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) acc[e] = 0.f;
+  bool whole = id(0) != id(-1);   // the run began in this chunk
+  for (int i0 = 0; i0 < n && id(i0) != kNoId; i0 += U) {
+    float f[U][W];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = (uint32_t)key[min(i0 + u, n - 1) + 1];   // past the end: the last one again
+      load_elems<T, VEC>(dy + at * a.dy_rs, a.H - col, f[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u;
+      if (i >= n || id(i) == kNoId) break;
+#pragma unroll
+      for (int e = 0; e < W; ++e) acc[e] += f[u][e];
+      const bool ends = id(i + 1) != id(i);
+      if (!ends && i + 1 < n) continue;
+      if (whole && ends) {
+        put_row<TO, VEC, ADD, W>(a, id(i), col, acc);
+      } else {   // slot 0: came from the chunk before, 1: began here
+        float *p = part + ((int64_t)blockIdx.x * 2 + (whole ? 1 : 0)) * a.part_rs + col;
+        store_elems<float, true, W>(p, W, acc);
+      }
+#pragma unroll
+      for (int e = 0; e < W; ++e) acc[e] = 0.f;
+      whole = true;
+    }
+  }
+}
+
+// grid (chunk, slice of 256 columns): where a run begins in the chunk and goes on
+// behind it, the sum of its parts. Four waves take a quarter of the parts each.
+template <typename TO, bool VEC, bool ADD>
+__global__ __launch_bounds__(kThreads) void embed_join_kernel(EmbedArgs a, const uint64_t *__restrict__ sorted,
+                                                              int32_t chunk, const float *__restrict__ part) {
+  const int64_t n0 = (int64_t)blockIdx.x * chunk, n1 = n0 + chunk;
+  if (n1 >= a.N) return;
+  const uint32_t id = id_at(sorted, n1);
+  if (id == kNoId || id_at(sorted, n1 - 1) != id) return;
+  if (n0 > 0 && id_at(sorted, n0) == id && id_at(sorted, n0 - 1) == id) return;   // began further back
+  int64_t lo = n1, hi = a.N;   // the run's end
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (id_at(sorted, mid) <= id) lo = mid + 1;
+    else hi = mid;
+  }
+  const int64_t c0 = blockIdx.x, count = (lo - 1) / chunk - c0 + 1;   // slot 1 of c0, slot 0 of the others
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = (blockIdx.y * 64 + lane) * 4;
+  __shared__ f32x4 sums[kThreads / 64][64];
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int64_t per = (count + 3) / 4, from = wave * per, to = min(count, from + per);
+  if (col < a.H) {
+    auto slot = [&](int64_t i) {
+      return *reinterpret_cast<const f32x4 *>(part + ((c0 + i) * 2 + (i == 0)) * a.part_rs + col);
+    };
+    int64_t i = from;
+    for (; i + 8 <= to; i += 8) {
+      f32x4 f[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) f[u] = slot(i + u);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += f[u][e];
+    }
+    for (; i < to; ++i) {
+      const f32x4 f = slot(i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += f[e];
+    }
+  }
+  sums[wave][lane] = acc;
+  __syncthreads();
+  if (wave || col >= a.H) return;
+  float f[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = (sums[0][lane][e] + sums[1][lane][e]) + (sums[2][lane][e] + sums[3][lane][e]);
+  put_row<TO, VEC, ADD, 4>(a, id, col, f);
+}
+
+namespace {
+
+// Sorted tokens a chunk: about a thousand workgroups over all slices.
+int chunk_of(int32_t N, int32_t H, int W) {
+  const int64_t slices = ((int64_t)H + kThreads * W - 1) / (kThreads * W);
+  return (int)std::min<int64_t>(kMaxChunk, std::max<int64_t>(8, (int64_t)N * slices / 1024));
+}
+
+constexpr int64_t kCachedBytes = 200 << 20;   // of dW that are written into the last-level cache
+
+template <typename T, bool VEC>
+void fwd_typed(const EmbedArgs &a, hipStream_t st) {
+  const int32_t parts = (a.H + 256 * kW<T> - 1) / (256 * kW<T>);
+  const int64_t units = (int64_t)a.N * parts;
+  hipLaunchKernelGGL((embed_fwd_kernel<T, VEC>), dim3((unsigned)((units + 3) / 4)), dim3(kThreads), 0, st, a, parts);
+}
+
+template <typename T, typename TO, bool VEC>
+void bwd_typed(EmbedArgs a, bool add, char *ws, hipStream_t st) {
+  const int tiles = (a.N + kTile - 1) / kTile;
+  uint64_t *sorted = reinterpret_cast<uint64_t *>(ws), *raw = sorted;
+  ws += ((int64_t)a.N * 8 + 15) / 16 * 16;
+  if (tiles > 1) {
+    raw = reinterpret_cast<uint64_t *>(ws);
+    ws += ((int64_t)a.N * 8 + 15) / 16 * 16;
+  }
+  float *part = reinterpret_cast<float *>(ws);
+  const int64_t rows = add ? 0 : ((int64_t)a.V + 15) / 16;
+  const unsigned clear = (unsigned)std::min<int64_t>(rows, 2048);
+  if (tiles + clear == 0) return;
+  if ((int64_t)a.V * a.H * (int64_t)sizeof(TO) > kCachedBytes)
+    hipLaunchKernelGGL((embed_sort_kernel<TO, VEC, true>), dim3(tiles + clear), dim3(kSortThreads), 0, st, a, tiles,
+                       !add, raw);
+  else
+    hipLaunchKernelGGL((embed_sort_kernel<TO, VEC, false>), dim3(tiles + clear), dim3(kSortThreads), 0, st, a, tiles,
+                       !add, raw);
+  if (a.N == 0) return;
+  if (tiles > 1)
+    hipLaunchKernelGGL(embed_merge_kernel, dim3((a.N + kThreads - 1) / kThreads), dim3(kThreads), 0, st, raw, a.N,
+                       tiles, sorted);
+  const int chunk = chunk_of(a.N, a.H, kW<T>);
+  const unsigned chunks = (a.N + chunk - 1) / chunk;
+  const dim3 grid(chunks, (a.H + kThreads * kW<T> - 1) / (kThreads * kW<T>)), join(chunks, (a.H + 255) / 256);
+  auto run = [&](auto sum, auto joined) {
+    hipLaunchKernelGGL(sum, grid, dim3(kThreads), 0, st, a, sorted, chunk, part);
+    if (chunks > 1) hipLaunchKernelGGL(joined, join, dim3(kThreads), 0, st, a, sorted, chunk, part);
+  };
+  if (add) run(embed_sum_kernel<T, TO, VEC, true>, embed_join_kernel<TO, VEC, true>);
+  else run(embed_sum_kernel<T, TO, VEC, false>, embed_join_kernel<TO, VEC, false>);
+}
+
+}  // namespace
+
+int64_t embed_part_stride(int32_t H) { return ((int64_t)H + 15) / 16 * 16; }
+
+int64_t embed_workspace_bytes(int32_t N, int32_t H) {
+  const int64_t keys = ((int64_t)N * 8 + 15) / 16 * 16;
+  const int chunk = std::min(chunk_of(N, H, 4), chunk_of(N, H, 8));
+  return keys * (N > kTile ? 2 : 1) + ((int64_t)N + chunk - 1) / chunk * 2 * embed_part_stride(H) * 4;
+}
+
+void launch_embed_fwd(const EmbedArgs &a, int dtype, bool vec, hipStream_t st) {
+  auto run = dtype == kDtF32   ? (vec ? fwd_typed<float, true> : fwd_typed<float, false>)
+             : dtype == kDtF16 ? (vec ? fwd_typed<f16_t, true> : fwd_typed<f16_t, false>)
+                               : (vec ? fwd_typed<bf16_t, true> : fwd_typed<bf16_t, false>);
+  run(a, st);
+}
+
+void launch_embed_bwd(const EmbedArgs &a, int dtype, int out_dtype, bool vec, bool add, void *ws, hipStream_t st) {
+  EmbedArgs b = a;
+  b.part_rs = embed_part_stride(a.H);
+  auto run = dtype == kDtF32 ? (vec ? bwd_typed<float, float, true> : bwd_typed<float, float, false>)
+             : dtype == kDtF16
+                 ? (out_dtype == kDtF32 ? (vec ? bwd_typed<f16_t, float, true> : bwd_typed<f16_t, float, false>)
+                                        : (vec ? bwd_typed<f16_t, f16_t, true> : bwd_typed<f16_t, f16_t, false>))
+                 : (out_dtype == kDtF32 ? (vec ? bwd_typed<bf16_t, float, true> : bwd_typed<bf16_t, float, false>)
+                                        : (vec ? bwd_typed<bf16_t, bf16_t, true> : bwd_typed<bf16_t, bf16_t, false>));
+  run(b, add, static_cast<char *>(ws), st);
+}
+
+}  // namespace mga

@@ -202,6 +202,62 @@ void launch_soft_ce_bwd(const void *x, int64_t xs, const void *t, int64_t ts, in
                         bool vec, const float *grad_out, const float *stats, void *g, int64_t gs,
                         hipStream_t stream);
 
+// Top logits (mga_top_logits.hip): the k largest of each row in order; lse may be null.
+void launch_top_logits(const void *x, int64_t xs, int32_t N, int32_t V, int dtype, int32_t k, float tau, void *values,
+                       int32_t *ids, float *lse, hipStream_t stream);
+
+// Cross-entropy against a teacher's top logits (mga_top_logits_ce.hip).
+struct TopLogitsCeArgs {
+  const void *x; int64_t xs;           // student [N, V], row stride
+  const void *values; int64_t values_rs;   // teacher's values [N, K], dtype values_dtype
+  const void *ids; int64_t ids_rs;     // their columns [N, K], int64 (ids64) or int32; outside [0, V): no entry
+  const float *lse;                    // teacher's log-sum-exp [N], or null: renormalised over the K
+  float *q;                            // [N, K] teacher weights (forward: out, or null; backward: in)
+  float *stats;                        // [3, N]: max, sum, Q
+  float *loss, *sum;                   // [N], and their sum
+  const float *go;                     // backward: upstream gradient, or null (= 1)
+  void *grad; int64_t gs;              // [N, V]
+  float tau, scale;                    // scale: of the gradient, beside go
+  int32_t N, V, K, values_dtype;
+  bool ids64;
+};
+int64_t top_ce_workspace_floats(int32_t N, int32_t V);
+void launch_top_ce_fwd(const TopLogitsCeArgs &a, int dtype, float *ws, hipStream_t stream);
+void launch_top_ce_bwd(const TopLogitsCeArgs &a, int dtype, hipStream_t stream);
+// loss and gradient; q and stats are written too where the rows do not fit registers
+void launch_top_ce_step(const TopLogitsCeArgs &a, int dtype, float *ws, hipStream_t stream);
+
+// Scaled embedding and its gradient (mga_embedding.hip).
+struct EmbedArgs {
+  const void *ids;                     // [N], int64 (ids64) or int32
+  const void *w; int64_t w_rs;         // forward: table [V, H]
+  const void *dy; int64_t dy_rs;       // backward: [N, H]
+  void *out; int64_t out_rs;           // forward: [N, H]; backward: dW [V, H]
+  float scale;
+  int64_t padding_idx;                 // backward: tokens of this id have no gradient; -1: none
+  int64_t part_rs;                     // set by the launcher
+  int32_t N, V, H;
+  bool ids64;
+};
+int64_t embed_workspace_bytes(int32_t N, int32_t H);
+// vec: 16-byte vectors (rows 16-byte aligned, H a multiple of 16 bytes)
+void launch_embed_fwd(const EmbedArgs &a, int dtype, bool vec, hipStream_t stream);
+// add: dW is added to and its other rows are left as they are
+void launch_embed_bwd(const EmbedArgs &a, int dtype, int out_dtype, bool vec, bool add, void *ws, hipStream_t stream);
+
+// Sampling (mga_sample.hip): one value a row where the pointer is set, else the
+// one for all rows.
+struct SampleParams {
+  const float *temperature;
+  const int32_t *top_k;
+  const float *top_p, *min_p;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all, min_p_all;
+};
+void launch_sample(const void *x, int64_t xs, int32_t N, int32_t V, int dtype, const float *uniform,
+                   const SampleParams &prm, int64_t *token, hipStream_t stream);
+
 // Compute units of the current device (queried once per device).
 int device_cu_count();
 

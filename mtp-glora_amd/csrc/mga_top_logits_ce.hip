@@ -1,0 +1,477 @@
+// Cross-entropy of student logits x against the top logits that were kept of a
+// teacher's row (K values t with their columns), forward and backward.
+//
+//   q_k = e^{t_k / tau - lse}, or the softmax of t / tau over the row's K;
+//   Q = sum_k q_k; p = softmax(x / tau);
+//   row loss = tau^2 (Q log sum_j e^{x_j / tau} - sum_k q_k x_{id_k} / tau)
+//            = tau^2 sum_k q_k ((m - x_{id_k}) / tau + log d),
+//              m = max x, d = sum_j e^{(x_j - m) / tau} (no difference of large
+//              numbers where student and teacher agree);
+//   grad_j = go tau (Q p_j - sum_{k: id_k = j} q_k).
+// The K columns are a few cache lines; all three kernels are bound by the rows of
+// x (read) and of the gradient (written).
+//
+// Forward: column ranges of the rows to (m, d), then a wave per row joins them,
+// forms q and the row's loss; the last workgroup adds the rows in a fixed order.
+// Backward: one more pass over x. Both in one (step): a workgroup holds the row in
+// registers between the sum and the gradient, so x is read once.
+#include "mga_internal.hpp"
+#include "mga_vocab_row.hpp"
+
+namespace mga {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ float ex2(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// (m, d) of a part of a row, d = sum e^{(x - m) c ln 2}.
+struct RowSum {
+  float m = kRowNegInf, d = 0.f;
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N], float c) {
+    float g = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) g = fmaxf(g, x[i]);
+    if (g > m) {
+      d *= ex2((m - g) * c);   // 0 while m = -inf
+      m = g;
+    }
+    const float base = m == kRowNegInf ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) d += ex2((x[i] - base) * c);
+  }
+  __device__ __forceinline__ void merge(float om, float od, float c) {
+    const float n = fmaxf(m, om);
+    if (n != kRowNegInf) {
+      d = d * ex2((m - n) * c) + od * ex2((om - n) * c);
+      m = n;
+    } else {
+      d += od;   // NaN stays
+    }
+  }
+  __device__ __forceinline__ void merge_lanes(float c) {
+#pragma unroll
+    for (int s = 32; s >= 1; s >>= 1) merge(__shfl_xor(m, s, 64), __shfl_xor(d, s, 64), c);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ i32x4 pack_vec(const float *v) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(i32x4, f32x4{v[0], v[1], v[2], v[3]});
+  else
+    return i32x4{(int)cvt2<T>(v[0], v[1]), (int)cvt2<T>(v[2], v[3]), (int)cvt2<T>(v[4], v[5]), (int)cvt2<T>(v[6], v[7])};
+}
+
+__device__ __forceinline__ float teacher_value(const TopLogitsCeArgs &a, int64_t row, int k) {
+  const int64_t at = row * a.values_rs + k;
+  return a.values_dtype == kDtF32 ? static_cast<const float *>(a.values)[at]
+         : a.values_dtype == kDtF16 ? (float)static_cast<const f16_t *>(a.values)[at]
+                                    : (float)static_cast<const bf16_t *>(a.values)[at];
+}
+// -1 outside the row
+__device__ __forceinline__ int teacher_id(const TopLogitsCeArgs &a, int64_t row, int k) {
+  const int64_t at = row * a.ids_rs + k;
+  const int64_t id = a.ids64 ? static_cast<const int64_t *>(a.ids)[at] : static_cast<const int32_t *>(a.ids)[at];
+  return id >= 0 && id < a.V ? (int)id : -1;
+}
+// q of a teacher value before the division by its sum (no lse) or as it is (lse)
+__device__ __forceinline__ float teacher_weight(float t, int id, float norm, float itau) {
+  const float s = t * itau;
+  if (id < 0 || s == kRowNegInf || norm == kRowNegInf) return 0.f;
+  return ex2((s - norm) * kLog2e);
+}
+
+__device__ __forceinline__ float loss_term(float q, float x, float m, float logd, float itau) {
+  if (q == 0.f) return 0.f;
+  if (x == kRowNegInf) return -kRowNegInf;   // all of the row among them (m = -inf)
+  return q * ((m - x) * itau + logd);
+}
+
+// What the gradient's elements of a row have in common.
+struct GradRow {
+  float base, c, a;   // a e^{(x - base) c ln 2}
+  bool dead;          // nothing of the teacher's row is left: zeros, whatever x holds
+  __device__ __forceinline__ GradRow(float m, float d, float Q, float c_, float coef)
+      : base(m == kRowNegInf ? 0.f : m), c(c_), a(d == 0.f ? 0.f : coef * Q / d), dead(Q == 0.f) {}
+  __device__ __forceinline__ float operator()(float x) const { return dead ? 0.f : a * ex2((x - base) * c); }
+};
+
+// Sum of sq[j] over the j with ids[j] == id, in order; 0 where an earlier j than k has it.
+__device__ __forceinline__ bool owned_sum(const int *ids, const float *q, int K, int k, float *sum) {
+  const int id = ids[k];
+  float s = 0.f;
+  for (int j = 0; j < K; ++j) {
+    if (ids[j] != id) continue;
+    if (j < k) return false;
+    s += q[j];
+  }
+  *sum = s;
+  return true;
+}
+
+}  // namespace
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void top_ce_partial_kernel(const T *__restrict__ x, int64_t xs, int32_t V,
+                                                                  float c, int32_t chunk, int32_t nsplit,
+                                                                  float *__restrict__ part, int *__restrict__ done) {
+  constexpr int W = RowElem<T>::W;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x / nsplit;
+  const int sp = blockIdx.x - row * nsplit, c0 = sp * chunk, c1 = min(V, c0 + chunk);
+  if (blockIdx.x == 0 && tid == 0) *done = 0;   // for the combine kernel
+  const T *xr = x + row * xs + c0;
+  const int n = c1 - c0;
+  const int off = (int)((reinterpret_cast<uintptr_t>(xr) & 15) / sizeof(T));
+  const int head = min(n, off ? W - off : 0), nvec = (n - head) / W;
+  RowSum st;
+  const i32x4 *vp = reinterpret_cast<const i32x4 *>(xr + head);
+  auto add = [&](const i32x4 &v) {
+    float f[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) f[e] = RowElem<T>::get(v, e);
+    st.add(f, c);
+  };
+  // four vectors a turn, the next turn's loads issued before this turn's arithmetic
+  const int nturn = nvec / (4 * kThreads);
+  if (nturn > 0) {
+    const i32x4 *q = vp + tid;
+    i32x4 a0 = q[0], a1 = q[kThreads], a2 = q[2 * kThreads], a3 = q[3 * kThreads];
+    for (int i = 1; i <= nturn; ++i) {
+      const i32x4 *r = vp + tid + min(i, nturn - 1) * 4 * kThreads;   // the last turn reads its own again
+      const i32x4 b0 = r[0], b1 = r[kThreads], b2 = r[2 * kThreads], b3 = r[3 * kThreads];
+      add(a0);
+      add(a1);
+      add(a2);
+      add(a3);
+      a0 = b0; a1 = b1; a2 = b2; a3 = b3;
+    }
+  }
+  for (int i = nturn * 4 * kThreads + tid; i < nvec; i += kThreads) add(vp[i]);
+  const int tail0 = head + nvec * W;
+  if (tid < head) {
+    const float f[1] = {(float)xr[tid]};
+    st.add(f, c);
+  }
+  if (tid < n - tail0) {
+    const float f[1] = {(float)xr[tail0 + tid]};
+    st.add(f, c);
+  }
+  st.merge_lanes(c);
+  __shared__ float wm[kThreads / 64], wd[kThreads / 64];
+  if ((tid & 63) == 0) {
+    wm[tid >> 6] = st.m;
+    wd[tid >> 6] = st.d;
+  }
+  __syncthreads();
+  if (tid == 0) {
+#pragma unroll
+    for (int w = 1; w < kThreads / 64; ++w) st.merge(wm[w], wd[w], c);
+    part[2 * blockIdx.x] = st.m;
+    part[2 * blockIdx.x + 1] = st.d;
+  }
+}
+
+// The losses added in a fixed order by one workgroup of kThreads; on thread 0.
+__device__ __forceinline__ float sum_rows(const float *loss, int N) {
+  float s = 0.f;
+  for (int64_t r0 = 0; r0 < N; r0 += 8 * kThreads) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t r = r0 + u * kThreads + threadIdx.x;
+      v[u] = r < N ? __hip_atomic_load(loss + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += v[u];
+  }
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
+  __shared__ float ws[kThreads / 64];
+  if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = s;
+  __syncthreads();
+  return threadIdx.x ? 0.f : (ws[0] + ws[1]) + (ws[2] + ws[3]);
+}
+
+// A wave per row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void top_ce_combine_kernel(TopLogitsCeArgs a, const float *__restrict__ part,
+                                                                  int32_t nsplit, int *__restrict__ done) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  const float itau = 1.f / a.tau, c = itau * kLog2e;
+  if (row < a.N) {
+    RowSum st;
+    for (int sp = lane; sp < nsplit; sp += 64) {
+      const float *p = part + 2 * (row * nsplit + sp);
+      st.merge(p[0], p[1], c);
+    }
+    st.merge_lanes(c);
+    float norm = kRowNegInf, inv = 1.f;
+    if (a.lse) norm = a.lse[row];
+    else {
+      for (int k = lane; k < a.K; k += 64)
+        if (teacher_id(a, row, k) >= 0) norm = fmaxf(norm, teacher_value(a, row, k) * itau);
+#pragma unroll
+      for (int m = 32; m >= 1; m >>= 1) norm = fmaxf(norm, __shfl_xor(norm, m, 64));
+      float s = 0.f;
+      for (int k = lane; k < a.K; k += 64)
+        s += teacher_weight(teacher_value(a, row, k), teacher_id(a, row, k), norm, itau);
+#pragma unroll
+      for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
+      inv = s == 0.f ? 0.f : 1.f / s;
+    }
+    const T *xr = static_cast<const T *>(a.x) + row * a.xs;
+    const float logd = logf(st.d);
+    float loss = 0.f, Q = 0.f;
+    for (int k = lane; k < a.K; k += 64) {
+      const int id = teacher_id(a, row, k);
+      const float q = teacher_weight(teacher_value(a, row, k), id, norm, itau) * inv;
+      if (a.q) a.q[row * a.K + k] = q;
+      Q += q;
+      if (id >= 0) loss += loss_term(q, (float)xr[id], st.m, logd, itau);
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+      loss += __shfl_xor(loss, m, 64);
+      Q += __shfl_xor(Q, m, 64);
+    }
+    if (lane == 0) {
+      __hip_atomic_store(a.loss + row, a.tau * a.tau * loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      a.stats[row] = st.m;
+      a.stats[a.N + row] = st.d;
+      a.stats[2 * (int64_t)a.N + row] = Q;
+    }
+  }
+  // the workgroup that finishes last adds the rows
+  __shared__ int last;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(done, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  const float s = sum_rows(a.loss, a.N);
+  if (threadIdx.x == 0) *a.sum = s;
+}
+
+__global__ __launch_bounds__(kThreads) void top_ce_sum_kernel(const float *__restrict__ loss, int32_t N,
+                                                              float *__restrict__ sum) {
+  const float s = sum_rows(loss, N);
+  if (threadIdx.x == 0) *sum = s;
+}
+
+// Walks the columns as the forward does, from the end: what the last-level cache
+// still holds of x are its last columns.
+template <typename T, bool NT>
+__global__ __launch_bounds__(kThreads) void top_ce_bwd_kernel(TopLogitsCeArgs a, int32_t chunk, int32_t nsplit) {
+  constexpr int W = RowElem<T>::W;
+  __shared__ int ids[kMaxTop];
+  __shared__ float qs[kMaxTop];
+  const int tid = threadIdx.x;
+  const unsigned b = gridDim.x - 1 - blockIdx.x;
+  const int64_t row = b / nsplit;
+  const int sp = b - row * nsplit, c0 = sp * chunk, c1 = min(a.V, c0 + chunk), n = c1 - c0;
+  for (int k = tid; k < a.K; k += kThreads) {
+    ids[k] = teacher_id(a, row, k);
+    qs[k] = a.q[row * a.K + k];
+  }
+  const float coef = a.scale * a.tau * (a.go ? *a.go : 1.f);
+  const GradRow gradient(a.stats[row], a.stats[a.N + row], a.stats[2 * (int64_t)a.N + row], kLog2e / a.tau, coef);
+  const T *xr = static_cast<const T *>(a.x) + row * a.xs + c0;
+  T *gr = static_cast<T *>(a.grad) + row * a.gs + c0;
+  const int off = (int)((reinterpret_cast<uintptr_t>(gr) & 15) / sizeof(T));
+  const bool same = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(gr)) & 15) == 0;
+  const int head = min(n, off ? W - off : 0), nvec = (n - head) / W, tail0 = head + nvec * W;
+  if (tid < head) gr[tid] = (T)gradient((float)xr[tid]);
+  if (tid < n - tail0) gr[tail0 + tid] = (T)gradient((float)xr[tail0 + tid]);
+  auto put = [&](int i, const i32x4 &v) {
+    float g[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) g[e] = gradient(RowElem<T>::get(v, e));
+    i32x4 *out = reinterpret_cast<i32x4 *>(gr + head) + i;
+    if constexpr (NT) __builtin_nontemporal_store(pack_vec<T>(g), out);
+    else *out = pack_vec<T>(g);
+  };
+  if (same) {
+    const i32x4 *vp = reinterpret_cast<const i32x4 *>(xr + head);
+    const int nturn = nvec / (4 * kThreads);
+    for (int i = nturn * 4 * kThreads + tid; i < nvec; i += kThreads) put(i, vp[i]);
+    if (nturn > 0) {
+      int at = (nturn - 1) * 4 * kThreads + tid;
+      i32x4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = vp[at + u * kThreads];
+      while (true) {
+        const int next = max(at - 4 * kThreads, tid);   // the last turn reads its own again
+        i32x4 w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = vp[next + u * kThreads];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) put(at + u * kThreads, v[u]);
+        if (at == tid) break;
+        at = next;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = w[u];
+      }
+    }
+  } else {
+    for (int i = tid; i < nvec; i += kThreads) {
+      const T *p = xr + head + i * W;
+      float g[W];
+#pragma unroll
+      for (int e = 0; e < W; ++e) g[e] = gradient((float)p[e]);
+      *(reinterpret_cast<i32x4 *>(gr + head) + i) = pack_vec<T>(g);
+    }
+  }
+  // the teacher's columns over what was just written
+  __syncthreads();
+  for (int k = tid; k < a.K; k += kThreads) {
+    const int id = ids[k];
+    float s;
+    if (id >= c0 && id < c1 && owned_sum(ids, qs, a.K, k, &s))
+      gr[id - c0] = (T)(gradient((float)xr[id - c0]) - coef * s);
+  }
+}
+
+// Loss and gradient of a row in one pass over x.
+template <typename T, int NB, bool NT>
+__global__ __launch_bounds__(kRowThreads) void top_ce_step_kernel(TopLogitsCeArgs a) {
+  constexpr int W = RowElem<T>::W;
+  __shared__ int ids[kMaxTop];
+  __shared__ float qs[kMaxTop];
+  __shared__ RowPart sh;
+  const int tid = threadIdx.x;
+  const int64_t n = blockIdx.x;
+  const float itau = 1.f / a.tau, c = itau * kLog2e;
+  Row<T, NB> row;
+  row.load(static_cast<const T *>(a.x) + n * a.xs, a.V);
+  // the teacher's side, a thread per entry, while the row is on its way
+  const int id = tid < a.K ? teacher_id(a, n, tid) : -1;
+  const float t = id >= 0 ? teacher_value(a, n, tid) : kRowNegInf;
+  const float xk = id >= 0 ? (float)row.p[id] : 0.f;
+  float norm, inv = 1.f;
+  if (a.lse) norm = a.lse[n];
+  else norm = block_max(t * itau, sh);
+  float q = teacher_weight(t, id, norm, itau);
+  if (!a.lse) {
+    const float s = block_sum(q, sh);
+    inv = s == 0.f ? 0.f : 1.f / s;
+  }
+  q *= inv;
+  const float Q = block_sum(q, sh);
+  if (tid < a.K) {
+    ids[tid] = id;
+    qs[tid] = q;
+  }
+  RowSum st;
+  row.each_vec([&](const i32x4 &v, int, int) {
+    float f[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) f[e] = RowElem<T>::get(v, e);
+    st.add(f, c);
+  });
+  if (row.ecol >= 0) {
+    const float f[1] = {row.edge};
+    st.add(f, c);
+  }
+  const float m = block_max(st.m, sh);
+  const float d = block_sum(st.d * (st.m == m ? 1.f : ex2((st.m - m) * c)), sh);
+  const float loss = block_sum(loss_term(q, xk, m, logf(d), itau), sh);
+  if (tid == 0) a.loss[n] = a.tau * a.tau * loss;
+  const float coef = a.scale * a.tau;
+  const GradRow gradient(m, d, Q, c, coef);
+  T *gr = static_cast<T *>(a.grad) + n * a.gs;
+  const bool whole = ((reinterpret_cast<uintptr_t>(gr + row.head)) & 15) == 0;
+  row.each_vec([&](const i32x4 &v, int col, int) {
+    if (col >= a.V) return;
+    float g[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) g[e] = gradient(RowElem<T>::get(v, e));
+    if (whole) {
+      i32x4 *out = reinterpret_cast<i32x4 *>(gr + col);
+      if constexpr (NT) __builtin_nontemporal_store(pack_vec<T>(g), out);
+      else *out = pack_vec<T>(g);
+    } else {
+#pragma unroll
+      for (int e = 0; e < W; ++e) gr[col + e] = (T)g[e];
+    }
+  });
+  if (row.ecol >= 0) gr[row.ecol] = (T)gradient(row.edge);
+  __syncthreads();
+  float s;
+  if (id >= 0 && owned_sum(ids, qs, a.K, tid, &s)) gr[id] = (T)(gradient(xk) - coef * s);
+}
+
+namespace {
+
+// Column split of the rows: enough workgroups to fill the chip (about 1024).
+void split_plan(int32_t N, int32_t V, int32_t *nsplit, int32_t *chunk) {
+  const int64_t want = (1024 + (int64_t)N - 1) / N, most = ((int64_t)V + 4095) / 4096;
+  const int64_t s = std::max<int64_t>(1, std::min(want, most));
+  const int64_t c = ((V + s - 1) / s + 2047) / 2048 * 2048;
+  *chunk = (int32_t)std::min<int64_t>(c, V);
+  *nsplit = (int32_t)((V + c - 1) / c);
+}
+
+// Bytes of x and its gradient up to which the last-level cache holds both; the
+// gradient is then written into it, where the next operation finds it.
+constexpr int64_t kCachedBytes = 200 << 20;
+template <typename T>
+bool past_cache(const TopLogitsCeArgs &a) { return 2 * (int64_t)a.N * a.V * (int64_t)sizeof(T) > kCachedBytes; }
+
+template <typename T>
+void fwd_typed(const TopLogitsCeArgs &a, float *ws, hipStream_t st) {
+  int32_t ns, ch;
+  split_plan(a.N, a.V, &ns, &ch);
+  int *done = reinterpret_cast<int *>(ws);
+  hipLaunchKernelGGL((top_ce_partial_kernel<T>), dim3((unsigned)((int64_t)a.N * ns)), dim3(kThreads), 0, st,
+                     static_cast<const T *>(a.x), a.xs, a.V, kLog2e / a.tau, ch, ns, ws + 4, done);
+  hipLaunchKernelGGL((top_ce_combine_kernel<T>), dim3((a.N + 3) / 4), dim3(kThreads), 0, st, a, ws + 4, ns, done);
+}
+
+template <typename T>
+void bwd_typed(const TopLogitsCeArgs &a, hipStream_t st) {
+  int32_t ns, ch;
+  split_plan(a.N, a.V, &ns, &ch);
+  const dim3 grid((unsigned)((int64_t)a.N * ns));
+  if (past_cache<T>(a)) hipLaunchKernelGGL((top_ce_bwd_kernel<T, true>), grid, dim3(kThreads), 0, st, a, ch, ns);
+  else hipLaunchKernelGGL((top_ce_bwd_kernel<T, false>), grid, dim3(kThreads), 0, st, a, ch, ns);
+}
+
+template <typename T>
+void step_typed(const TopLogitsCeArgs &a, float *ws, hipStream_t st) {
+  with_row_blocks<T>(a.V, [&](auto nb) {
+    constexpr int NB = decltype(nb)::value;
+    if constexpr (NB == 0) {   // rows that registers do not hold
+      fwd_typed<T>(a, ws, st);
+      bwd_typed<T>(a, st);
+    } else {
+      if (past_cache<T>(a)) hipLaunchKernelGGL((top_ce_step_kernel<T, NB, true>), dim3(a.N), dim3(kRowThreads), 0, st, a);
+      else hipLaunchKernelGGL((top_ce_step_kernel<T, NB, false>), dim3(a.N), dim3(kRowThreads), 0, st, a);
+      hipLaunchKernelGGL(top_ce_sum_kernel, dim3(1), dim3(kThreads), 0, st, a.loss, a.N, a.sum);
+    }
+  });
+}
+
+}  // namespace
+
+int64_t top_ce_workspace_floats(int32_t N, int32_t V) {
+  int32_t ns, ch;
+  split_plan(N, V, &ns, &ch);
+  return 4 + 2 * (int64_t)N * ns;
+}
+
+void launch_top_ce_fwd(const TopLogitsCeArgs &a, int dtype, float *ws, hipStream_t st) {
+  (dtype == kDtF32 ? fwd_typed<float> : dtype == kDtF16 ? fwd_typed<f16_t> : fwd_typed<bf16_t>)(a, ws, st);
+}
+void launch_top_ce_bwd(const TopLogitsCeArgs &a, int dtype, hipStream_t st) {
+  (dtype == kDtF32 ? bwd_typed<float> : dtype == kDtF16 ? bwd_typed<f16_t> : bwd_typed<bf16_t>)(a, st);
+}
+void launch_top_ce_step(const TopLogitsCeArgs &a, int dtype, float *ws, hipStream_t st) {
+  (dtype == kDtF32 ? step_typed<float> : dtype == kDtF16 ? step_typed<f16_t> : step_typed<bf16_t>)(a, ws, st);
+}
+
+}  // namespace mga

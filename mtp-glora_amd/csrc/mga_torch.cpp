@@ -37,7 +37,9 @@ using torch::autograd::variable_list;
   X(mga_header_hash) X(mga_kv_append) X(mga_attn_workspace_bytes) X(mga_attn_fwd_ws) X(mga_attn_bwd_ws) \
   X(mga_qk_norm_rope_stage_fwd) X(mga_qk_norm_rope_bwd) X(mga_gated_lora_workspace_bytes)             \
   X(mga_gated_lora_fwd) X(mga_gated_lora_bwd) X(mga_soft_ce_workspace_floats) X(mga_soft_ce_loss)     \
-  X(mga_soft_ce_bwd)
+  X(mga_soft_ce_bwd) X(mga_top_logits) X(mga_top_logits_ce_workspace_floats) X(mga_top_logits_ce_fwd)  \
+  X(mga_top_logits_ce_bwd) X(mga_top_logits_ce_step_workspace_floats) X(mga_top_logits_ce_step)          \
+  X(mga_sample) X(mga_embedding_fwd) X(mga_embedding_workspace_bytes) X(mga_embedding_bwd)
 struct Api {
 #define X(f) decltype(&::f) f = nullptr;
   MGA_API(X)
@@ -493,6 +495,229 @@ std::optional<Tensor> soft_ce(const Tensor &x, const Tensor &t) {
   return SoftCE::apply(x, t);
 }
 
+// ---- vocabulary rows -----------------------------------------------------------------
+
+// Rows of a [..., cols] tensor with unit stride on the last dimension.
+struct Rows {
+  int64_t n = 1, stride = 0;
+  int32_t cols = 0;
+  void *data = nullptr;
+};
+std::optional<Rows> rows_of(const Tensor &t) {
+  Rows r;
+  const int64_t d = t.dim();
+  if (d < 1 || t.numel() == 0 || t.stride(d - 1) != 1 || t.size(d - 1) > INT32_MAX) return std::nullopt;
+  r.cols = (int32_t)t.size(d - 1);
+  for (int64_t i = d - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (r.n == 1) r.stride = t.stride(i);
+    else if (t.stride(i) != r.stride * r.n) return std::nullopt;
+    r.n *= t.size(i);
+  }
+  if (r.n == 1) r.stride = r.cols;
+  if (r.stride < r.cols || r.n > INT32_MAX) return std::nullopt;
+  r.data = t.data_ptr();
+  return r;
+}
+
+constexpr int64_t kMaxTop = 1024, kMaxVocab = 1 << 20;
+
+std::optional<std::tuple<Tensor, Tensor, Tensor>> top_logits(const Tensor &x, int64_t k, double temperature) {
+  if (!eager() || !plain(x) || dtype_code(x.scalar_type()) < 0) return std::nullopt;
+  const auto r = rows_of(x);
+  if (!r || k < 1 || k > kMaxTop || k > r->cols || r->cols > kMaxVocab) return std::nullopt;
+  const at::DeviceGuard guard(x.device());
+  auto lead = x.sizes().vec();
+  lead.back() = k;
+  const auto opt = x.options().requires_grad(false);
+  Tensor values = at::empty(lead, opt), ids = at::empty(lead, opt.dtype(at::kInt));
+  lead.pop_back();
+  Tensor lse = at::empty(lead, opt.dtype(at::kFloat));
+  check_rc("mga_top_logits",
+           g.mga_top_logits(r->data, r->stride, (int32_t)r->n, r->cols, dtype_code(x.scalar_type()), (int32_t)k,
+                            (float)temperature, values.data_ptr(), ids.data_ptr<int32_t>(), lse.data_ptr<float>(),
+                            stream(x)));
+  return std::make_tuple(values, ids, lse);
+}
+
+// The operands of a call against a teacher's top logits, of their plain form.
+struct TopCe {
+  Rows x, values, ids;
+  int dtype, values_dtype;
+  bool ids64;
+  const float *lse = nullptr;
+};
+std::optional<TopCe> top_ce_operands(const Tensor &x, const Tensor &values, const Tensor &ids,
+                                     const std::optional<Tensor> &lse) {
+  if (!eager()) return std::nullopt;
+  for (const Tensor *t : {&x, &values, &ids})
+    if (!plain(*t) || t->device() != x.device() || t->dim() != x.dim()) return std::nullopt;
+  TopCe o;
+  o.dtype = dtype_code(x.scalar_type());
+  o.values_dtype = dtype_code(values.scalar_type());
+  o.ids64 = ids.scalar_type() == at::kLong;
+  if (o.dtype < 0 || o.values_dtype < 0 || (!o.ids64 && ids.scalar_type() != at::kInt) || values.sizes() != ids.sizes())
+    return std::nullopt;
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  if (values.sizes().slice(0, x.dim() - 1) != lead || values.size(-1) > kMaxTop) return std::nullopt;
+  const auto rx = rows_of(x), rv = rows_of(values), ri = rows_of(ids);
+  if (!rx || !rv || !ri) return std::nullopt;
+  if (lse) {
+    if (!plain(*lse) || lse->device() != x.device() || lse->scalar_type() != at::kFloat || lse->sizes() != lead ||
+        !lse->is_contiguous())
+      return std::nullopt;
+    o.lse = lse->data_ptr<float>();
+  }
+  o.x = *rx;
+  o.values = *rv;
+  o.ids = *ri;
+  return o;
+}
+
+struct TopLogitsCE : public Function<TopLogitsCE> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &values, const Tensor &ids,
+                        const std::optional<Tensor> &lse, double tau) {
+    const TopCe o = *top_ce_operands(x, values, ids, lse);
+    const int32_t N = (int32_t)o.x.n, V = o.x.cols, K = o.ids.cols;
+    const auto opt = x.options().requires_grad(false).dtype(at::kFloat);
+    // what the backward reads, and what only this call does
+    Tensor keep = at::empty({N * (3 + (int64_t)K)}, opt), total = at::empty({}, opt);
+    Tensor ws = at::empty({g.mga_top_logits_ce_workspace_floats(N, V) + N}, opt);
+    float *stats = keep.data_ptr<float>(), *w = ws.data_ptr<float>();
+    check_rc("mga_top_logits_ce_fwd",
+             g.mga_top_logits_ce_fwd(o.x.data, o.x.stride, o.values.data, o.values.stride, o.values_dtype, o.ids.data,
+                                     o.ids.stride, o.ids64, o.lse, N, V, K, (float)tau, o.dtype, stats + 3 * (int64_t)N,
+                                     stats, w + ws.numel() - N, total.data_ptr<float>(), w, stream(x)));
+    ctx->save_for_backward({x.detach(), ids.detach(), keep});
+    ctx->saved_data["tau"] = tau;
+    return total;
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &grad) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &ids = s[1];
+    const at::DeviceGuard guard(x.device());
+    const Rows rx = *rows_of(x), ri = *rows_of(ids);
+    const float *stats = s[2].data_ptr<float>();
+    const Tensor go = grad[0].detach().reshape({1}).to(x.device(), at::kFloat).contiguous();
+    Tensor gx = at::empty(x.sizes(), x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+    check_rc("mga_top_logits_ce_bwd",
+             g.mga_top_logits_ce_bwd(rx.data, rx.stride, ri.data, ri.stride, ids.scalar_type() == at::kLong,
+                                     stats + 3 * rx.n, stats, (int32_t)rx.n, rx.cols, ri.cols,
+                                     (float)ctx->saved_data["tau"].toDouble(), dtype_code(x.scalar_type()),
+                                     go.data_ptr<float>(), gx.data_ptr(), rx.cols, stream(x)));
+    return {gx, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::optional<Tensor> top_logits_ce(const Tensor &x, const Tensor &values, const Tensor &ids,
+                                    const std::optional<Tensor> &lse, double tau) {
+  if (!top_ce_operands(x, values, ids, lse)) return std::nullopt;
+  const at::DeviceGuard guard(x.device());
+  return TopLogitsCE::apply(x, values.detach(), ids, lse ? std::optional<Tensor>(lse->detach()) : lse, tau);
+}
+
+std::optional<std::tuple<Tensor, Tensor>> top_logits_step(const Tensor &x, const Tensor &values, const Tensor &ids,
+                                                          const std::optional<Tensor> &lse, double tau, double scale) {
+  const auto o = top_ce_operands(x, values, ids, lse);
+  if (!o) return std::nullopt;
+  const at::DeviceGuard guard(x.device());
+  const int32_t N = (int32_t)o->x.n, V = o->x.cols, K = o->ids.cols;
+  const auto opt = x.options().requires_grad(false);
+  Tensor total = at::empty({}, opt.dtype(at::kFloat));
+  Tensor gx = at::empty(x.sizes(), opt.memory_format(at::MemoryFormat::Contiguous));
+  Tensor ws = at::empty({g.mga_top_logits_ce_step_workspace_floats(N, V, K) + N}, opt.dtype(at::kFloat));
+  float *w = ws.data_ptr<float>();
+  check_rc("mga_top_logits_ce_step",
+           g.mga_top_logits_ce_step(o->x.data, o->x.stride, o->values.data, o->values.stride, o->values_dtype,
+                                    o->ids.data, o->ids.stride, o->ids64, o->lse, N, V, K, (float)tau, (float)scale,
+                                    o->dtype, w + ws.numel() - N, total.data_ptr<float>(), gx.data_ptr(), V, w,
+                                    stream(x)));
+  return std::make_tuple(total, gx);
+}
+
+// A sampling setting: a dense tensor with one value a row, or none (the number counts).
+bool setting(const std::optional<Tensor> &t, const Tensor &x, int64_t n, at::ScalarType type) {
+  return !t || (plain(*t) && t->device() == x.device() && t->scalar_type() == type && t->is_contiguous() &&
+                t->numel() == n);
+}
+
+std::optional<Tensor> sample(const Tensor &x, const Tensor &u, const std::optional<Tensor> &temperature,
+                             const std::optional<Tensor> &top_k, const std::optional<Tensor> &top_p,
+                             const std::optional<Tensor> &min_p, double temperature_all, int64_t top_k_all,
+                             double top_p_all, double min_p_all) {
+  if (!eager() || !plain(x) || !plain(u) || dtype_code(x.scalar_type()) < 0) return std::nullopt;
+  const auto r = rows_of(x);
+  if (!r || r->cols > kMaxVocab || u.device() != x.device() || u.scalar_type() != at::kFloat || !u.is_contiguous() ||
+      u.sizes() != x.sizes().slice(0, x.dim() - 1))
+    return std::nullopt;
+  if (!setting(temperature, x, r->n, at::kFloat) || !setting(top_k, x, r->n, at::kInt) ||
+      !setting(top_p, x, r->n, at::kFloat) || !setting(min_p, x, r->n, at::kFloat))
+    return std::nullopt;
+  const at::DeviceGuard guard(x.device());
+  Tensor token = at::empty(u.sizes(), x.options().requires_grad(false).dtype(at::kLong));
+  auto f32 = [](const std::optional<Tensor> &t) { return t ? t->data_ptr<float>() : nullptr; };
+  const int32_t k = (int32_t)std::max<int64_t>(-1, std::min(top_k_all, kMaxVocab));
+  check_rc("mga_sample",
+           g.mga_sample(r->data, r->stride, (int32_t)r->n, r->cols, dtype_code(x.scalar_type()), u.data_ptr<float>(),
+                        f32(temperature), (float)temperature_all, top_k ? top_k->data_ptr<int32_t>() : nullptr, k,
+                        f32(top_p), (float)top_p_all, f32(min_p), (float)min_p_all, token.data_ptr<int64_t>(),
+                        stream(x)));
+  return token;
+}
+
+// ---- embedding -----------------------------------------------------------------------
+
+struct Embedding : public Function<Embedding> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &ids, const Tensor &w, double scale, int64_t padding_idx) {
+    auto shape = ids.sizes().vec();
+    shape.push_back(w.size(1));
+    Tensor out = at::empty(shape, w.options().requires_grad(false));
+    check_rc("mga_embedding_fwd",
+             g.mga_embedding_fwd(ids.data_ptr(), ids.scalar_type() == at::kLong, (int32_t)ids.numel(), w.data_ptr(),
+                                 w.stride(0), (int32_t)w.size(0), (int32_t)w.size(1), (float)scale,
+                                 dtype_code(w.scalar_type()), out.data_ptr(), w.size(1), stream(w)));
+    ctx->save_for_backward({ids});
+    ctx->saved_data["rows"] = w.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["pad"] = padding_idx;
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &grad) {
+    if (!ctx->needs_input_grad(1)) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto s = ctx->get_saved_variables();
+    const Tensor &ids = s[0];
+    const at::DeviceGuard guard(ids.device());
+    Tensor dy = grad[0].detach();
+    auto r = rows_of(dy);
+    if (!r) {
+      dy = dy.contiguous();
+      r = rows_of(dy);
+    }
+    const int64_t V = ctx->saved_data["rows"].toInt();
+    const int32_t n = (int32_t)ids.numel(), H = r->cols;
+    Tensor dw = at::empty({V, H}, dy.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+    const int64_t wn = g.mga_embedding_workspace_bytes(n, H);
+    Tensor ws = bytes(wn, dy);
+    check_rc("mga_embedding_bwd",
+             g.mga_embedding_bwd(r->data, r->stride, ids.data_ptr(), ids.scalar_type() == at::kLong, n,
+                                 (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["pad"].toInt(), (int32_t)V,
+                                 H, dtype_code(dy.scalar_type()), dw.data_ptr(), H, dtype_code(dy.scalar_type()), 0,
+                                 ws.data_ptr(), wn, stream(dy)));
+    return {Tensor(), dw, Tensor(), Tensor()};
+  }
+};
+
+std::optional<Tensor> embedding(const Tensor &ids, const Tensor &w, double scale, int64_t padding_idx) {
+  if (!eager() || !plain(ids) || !plain(w) || dtype_code(w.scalar_type()) < 0 || ids.device() != w.device())
+    return std::nullopt;
+  if ((ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) || !ids.is_contiguous() || ids.numel() == 0 ||
+      ids.numel() > INT32_MAX || w.dim() != 2 || w.numel() == 0 || w.stride(1) != 1 || w.stride(0) < w.size(1) ||
+      w.size(0) > INT32_MAX || w.size(1) > INT32_MAX)
+    return std::nullopt;
+  const at::DeviceGuard guard(w.device());
+  return Embedding::apply(ids, w, scale, padding_idx);
+}
+
 }  // namespace
 
 #define MGA_DEF(f) m.def(#f, torch::wrap_pybind_function_no_gil(f))
@@ -504,4 +729,9 @@ PYBIND11_MODULE(_mga_torch, m) {
   MGA_DEF(norm_rope_stage);
   MGA_DEF(gated_lora);
   MGA_DEF(soft_ce);
+  MGA_DEF(top_logits);
+  MGA_DEF(top_logits_ce);
+  MGA_DEF(top_logits_step);
+  MGA_DEF(sample);
+  MGA_DEF(embedding);
 }

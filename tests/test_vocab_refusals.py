@@ -1,0 +1,129 @@
+"""Arguments that the vocabulary operators' C entry points refuse before any device
+work, each with a message (so these run without a GPU), and CPU tensors at the
+Python entry points."""
+import ctypes
+
+import pytest
+import torch
+
+P = ctypes.c_void_p(64)
+
+
+def refused(mga, rc, text=b""):
+    assert rc == mga._lib.MGA_ERR_INVALID
+    msg = mga.load_library().mga_last_error()
+    assert msg and text in msg
+
+
+def _top(lib, **kw):
+    a = dict(x=P, rs=100, n=2, v=100, dtype=0, k=4, t=1.0, values=P, ids=P, lse=None)
+    a.update(kw)
+    return lib.mga_top_logits(a["x"], a["rs"], a["n"], a["v"], a["dtype"], a["k"], a["t"], a["values"], a["ids"],
+                              a["lse"], None)
+
+
+@pytest.mark.parametrize("kw", [dict(x=None), dict(rs=99), dict(n=0), dict(v=0), dict(dtype=3), dict(k=0), dict(k=101),
+                                dict(v=2000, rs=2000, k=1025), dict(v=(1 << 20) + 1, rs=1 << 21), dict(t=0.0),
+                                dict(t=-1.0), dict(t=float("inf")), dict(t=float("nan")), dict(values=None),
+                                dict(ids=None), dict(x=ctypes.c_void_p(65)), dict(x=ctypes.c_void_p(66), dtype=1)])
+def test_top_logits(mga, kw):
+    refused(mga, _top(mga.load_library(), **kw))
+
+
+def _fwd(lib, step=False, **kw):
+    a = dict(x=P, rs=100, values=P, vrs=4, vd=0, ids=P, irs=4, i64=0, lse=None, n=2, v=100, k=4, t=1.0, scale=1.0,
+             dtype=0, q=P, stats=P, loss=P, sum=P, grad=ctypes.c_void_p(1 << 20), gs=100, ws=P)
+    a.update(kw)
+    head = (a["x"], a["rs"], a["values"], a["vrs"], a["vd"], a["ids"], a["irs"], a["i64"], a["lse"], a["n"], a["v"],
+            a["k"], a["t"])
+    if step:
+        return lib.mga_top_logits_ce_step(*head, a["scale"], a["dtype"], a["loss"], a["sum"], a["grad"], a["gs"],
+                                          a["ws"], None)
+    return lib.mga_top_logits_ce_fwd(*head, a["dtype"], a["q"], a["stats"], a["loss"], a["sum"], a["ws"], None)
+
+
+COMMON = [dict(x=None), dict(rs=99), dict(n=0), dict(dtype=5), dict(k=0), dict(k=1025, vrs=1025, irs=1025),
+          dict(t=0.0), dict(t=float("nan")), dict(ids=None), dict(irs=3), dict(ids=ctypes.c_void_p(68), i64=1),
+          dict(values=None), dict(vrs=3), dict(vd=7), dict(loss=None), dict(sum=None), dict(ws=None)]
+
+
+@pytest.mark.parametrize("step", [False, True])
+@pytest.mark.parametrize("kw", COMMON)
+def test_top_logits_ce(mga, kw, step):
+    refused(mga, _fwd(mga.load_library(), step, **kw))
+
+
+def test_top_logits_ce_outputs(mga):
+    lib = mga.load_library()
+    refused(mga, _fwd(lib, stats=None), b"stats")
+    refused(mga, _fwd(lib, True, grad=None), b"grad")
+    refused(mga, _fwd(lib, True, gs=99), b"grad")
+    refused(mga, _fwd(lib, True, grad=P), b"overlaps")
+    refused(mga, _fwd(lib, True, grad=ctypes.c_void_p(64 + 2 * 199)), b"overlaps")
+    bwd = lambda **kw: lib.mga_top_logits_ce_bwd(   # noqa: E731
+        P, 100, P, 4, 0, kw.get("q", P), kw.get("stats", P), 2, 100, 4, 1.0, 0, kw.get("go", P), kw.get("grad", P),
+        kw.get("gs", 100), None)
+    for kw in (dict(q=None), dict(stats=None), dict(go=None), dict(grad=None), dict(gs=50)):
+        refused(mga, bwd(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(x=None), dict(rs=9), dict(n=0), dict(v=(1 << 20) + 1, rs=1 << 21), dict(dtype=4),
+                                dict(u=None), dict(token=None)])
+def test_sample(mga, kw):
+    a = dict(x=P, rs=10, n=1, v=10, dtype=0, u=P, token=P)
+    a.update(kw)
+    refused(mga, mga.load_library().mga_sample(a["x"], a["rs"], a["n"], a["v"], a["dtype"], a["u"], None, 1.0, None, 0,
+                                               None, 1.0, None, 0.0, a["token"], None))
+
+
+@pytest.mark.parametrize("kw", [dict(ids=None), dict(n=-1), dict(w=None), dict(rs=7), dict(v=0), dict(h=0),
+                                dict(dtype=3), dict(out=None), dict(ors=7), dict(ids=ctypes.c_void_p(68), i64=1),
+                                dict(n=2 ** 31 - 1, h=4096, rs=4096, ors=4096)])
+def test_embedding_fwd(mga, kw):
+    a = dict(ids=P, i64=0, n=3, w=P, rs=8, v=10, h=8, dtype=0, out=P, ors=8)
+    a.update(kw)
+    refused(mga, mga.load_library().mga_embedding_fwd(a["ids"], a["i64"], a["n"], a["w"], a["rs"], a["v"], a["h"], 1.0,
+                                                      a["dtype"], a["out"], a["ors"], None))
+
+
+@pytest.mark.parametrize("kw", [dict(dy=None), dict(drs=7), dict(ids=None), dict(n=-1), dict(v=0), dict(h=0),
+                                dict(dtype=3), dict(dw=None), dict(wrs=7), dict(wd=2), dict(dtype=1, wd=0),
+                                dict(ws=None), dict(wn=0), dict(ws=ctypes.c_void_p(72))])
+def test_embedding_bwd(mga, kw):
+    lib = mga.load_library()
+    a = dict(dy=P, drs=8, ids=P, i64=0, n=3, v=10, h=8, dtype=0, dw=P, wrs=8, wd=0, ws=P,
+             wn=int(lib.mga_embedding_workspace_bytes(3, 8)))
+    a.update(kw)
+    refused(mga, lib.mga_embedding_bwd(a["dy"], a["drs"], a["ids"], a["i64"], a["n"], 1.0, -1, a["v"], a["h"],
+                                       a["dtype"], a["dw"], a["wrs"], a["wd"], 0, a["ws"], a["wn"], None))
+
+
+def test_workspace_sizes_of_no_work(mga):
+    lib = mga.load_library()
+    assert lib.mga_embedding_workspace_bytes(0, 8) == 0
+    assert lib.mga_top_logits_ce_workspace_floats(0, 8) == 0
+    assert lib.mga_top_logits_ce_step_workspace_floats(4, 8, 0) == 0
+
+
+def test_cpu_tensors(mga):
+    x, ids = torch.randn(2, 9), torch.zeros(2, 3, dtype=torch.int32)
+    for call in (lambda: mga.top_logits(x, 3), lambda: mga.top_logits_cross_entropy(x, torch.zeros(2, 3), ids),
+                 lambda: mga.top_logits_loss_and_grad(x, torch.zeros(2, 3), ids),
+                 lambda: mga.sample_tokens(x, torch.zeros(2)), lambda: mga.scaled_embedding(ids, x),
+                 lambda: mga.embedding_grad(torch.zeros(2, 3, 4), ids, 5)):
+        with pytest.raises(RuntimeError, match="GPU tensor"):
+            call()
+    for t in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="temperature"):
+            mga.top_logits_cross_entropy(x, torch.zeros(2, 3), ids, None, t)
+
+
+def test_layer_keeps_the_parameter(mga):
+    base = torch.nn.Embedding(6, 4, padding_idx=2)
+    layer = mga.ScaledEmbedding.wrap(base, 3.0)
+    assert layer.weight is base.weight and layer.padding_idx == 2 and layer.scale == 3.0
+    assert list(layer.state_dict()) == list(base.state_dict())
+    own = mga.ScaledEmbedding(6, 4, scale=2.0, dtype=torch.bfloat16)
+    assert own.weight.dtype == torch.bfloat16 and list(own.state_dict()) == ["weight"]
+    with pytest.raises(NotImplementedError):
+        mga.ScaledEmbedding.wrap(torch.nn.Embedding(6, 4, max_norm=1.0))
