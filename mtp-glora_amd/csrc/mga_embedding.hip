@@ -24,7 +24,7 @@ namespace mga {
 namespace {
 
 constexpr int kTile = 8192;
-constexpr int kSortThreads = 1024;
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kRounds = kTile / kSortThreads;
 constexpr int kThreads = 256;
 constexpr uint32_t kNoId = 0xFFFFFFFFu;   // padding and ids outside the table: last in order, summed nowhere
 
@@ -126,6 +126,7 @@ template <typename TO, bool VEC, bool NT>
 __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a, int32_t tiles, bool clear,
                                                                   uint64_t *__restrict__ sorted) {
   __shared__ uint64_t key[kTile];
+  __shared__ uint32_t count[kSortThreads], sums[kSortWaves];
   const int tid = threadIdx.x;
   if ((int)blockIdx.x >= tiles) {
     if (clear)
@@ -134,31 +135,72 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a, i
   }
   const int64_t n0 = (int64_t)blockIdx.x * kTile;
   const int n = (int)min((int64_t)kTile, a.N - n0);
-  int size = 64;
-  while (size < n) size <<= 1;
-  for (int i = tid; i < size; i += kSortThreads) {
-    uint64_t k = ~uint64_t(0);
-    if (i < n) {
+  // the tile in order of position: a wave's part is contiguous, 64 pairs a round
+  const int rounds = (n + kSortThreads - 1) / kSortThreads, lane = tid & 63, wave = tid >> 6;
+  const int at0 = wave * rounds * 64 + lane;
+  uint64_t k[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int i = at0 + r * 64;
+    k[r] = (uint64_t)kNoId << 32;
+    if (r < rounds && i < n) {
       const int64_t id = token_id(a.ids, a.ids64, n0 + i);
       const bool ok = id >= 0 && id < a.V && id != a.padding_idx;
-      k = (uint64_t)(ok ? (uint32_t)id : kNoId) << 32 | (uint32_t)(n0 + i);
+      k[r] = (uint64_t)(ok ? (uint32_t)id : kNoId) << 32 | (uint32_t)(n0 + i);
     }
-    key[i] = k;
   }
-  __syncthreads();
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int t = tid; t < size / 2; t += kSortThreads) {
-        const int p = 2 * t - (t & (j - 1)), q = p + j;
-        const uint64_t x = key[p], y = key[q];
-        if ((x > y) == ((p & k) == 0)) {
-          key[p] = y;
-          key[q] = x;
-        }
+  // By digits of six bits from the lowest, each pass stable: lane d of a wave counts
+  // digit d, and a pair's place is what has its digit in earlier waves, earlier
+  // rounds and lower lanes, behind all lower digits. The pairs that are none, and
+  // the places past n, have the digit 63 in every pass and stay last (the last
+  // pass has a spare bit for them).
+  const int bits = 33 - __builtin_clz(a.V);
+  for (int shift = 0; shift < bits; shift += 6) {
+    uint32_t place[kRounds], mine = 0;   // mine: of digit `lane`, in the rounds so far
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      if (r >= rounds) break;
+      const uint32_t d = (uint32_t)(k[r] >> (32 + shift)) & 63;
+      uint64_t same = ~uint64_t(0), own = ~uint64_t(0);   // lanes of my digit, of the digit I count
+#pragma unroll
+      for (int b = 0; b < 6; ++b) {
+        const uint64_t set = __ballot((d >> b) & 1);
+        same &= (d >> b) & 1 ? set : ~set;
+        own &= (lane >> b) & 1 ? set : ~set;
       }
-      __syncthreads();
+      place[r] = __shfl(mine, d, 64) + __popcll(same & lanes_below());
+      mine += __popcll(own);
     }
-  for (int i = tid; i < n; i += kSortThreads) sorted[n0 + i] = key[i];
+    count[lane * kSortWaves + wave] = mine;
+    __syncthreads();
+    // sums over (digit, wave) in that order, an entry a thread
+    const uint32_t c = count[tid];
+    uint32_t in = c;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const uint32_t o = __shfl_up(in, s, 64);
+      if (lane >= s) in += o;
+    }
+    if (lane == 63) sums[wave] = in;
+    __syncthreads();
+    uint32_t before = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) before += w < wave ? sums[w] : 0;
+    count[tid] = before + in - c;
+    __syncthreads();
+    const uint32_t base = count[lane * kSortWaves + wave];
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r)
+      if (r < rounds) key[__shfl(base, (int)(k[r] >> (32 + shift)) & 63, 64) + place[r]] = k[r];
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r)
+      if (r < rounds) k[r] = key[at0 + r * 64];
+    __syncthreads();
+  }
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r)
+    if (r < rounds && at0 + r * 64 < n) sorted[n0 + at0 + r * 64] = k[r];
 }
 
 // Each pair's place: those before it in its own tile and in the others.
