@@ -1,10 +1,12 @@
-// One row of vocabulary logits, held by one workgroup of kRowThreads threads:
+// One row of vocabulary logits, taken by one workgroup of kRowThreads threads:
 // what the kernels that put a row's tokens in order (top logits, sampling) share.
 //
-// A row of 151 936 16-bit logits (304 KB) fits the register file of a compute
-// unit (512 KB) and not its LDS (160 KB): it is loaded once, 16 bytes a thread
-// and load, and every later pass over it reads registers. Longer rows (and fp32
-// rows past 81 920 columns) are read again in each pass, from the caches.
+// A row of 151 936 16-bit logits (304 KB) does not fit LDS (160 KB). Holding it in
+// the register file (512 KB a compute unit) leaves room for one workgroup there,
+// whose read, arithmetic and latency then follow each other: 132 us for the top
+// logits of 1 024 such rows. So a row is read in one pass that keeps what later
+// steps need, the largest element of each run of vectors, and the few vectors that
+// matter are read again from the caches.
 //
 // Order of a row's elements: value descending, then column ascending; -0 equals
 // +0, NaN stands below -inf. As one number (rank_of): the value's bits made
@@ -12,7 +14,6 @@
 #pragma once
 
 #include <algorithm>
-#include <type_traits>
 
 #include "mga_common.hpp"
 
@@ -70,19 +71,15 @@ __device__ __forceinline__ float rank_value(uint64_t r) {   // NaN where the key
 
 // ---- the row ----------------------------------------------------------------
 
-// NB > 0: NB blocks of four vectors a thread stay in registers; NB = 0: the
-// blocks are loaded again by every pass. Loops over a block's vectors stay
-// rolled (the vector is picked by a uniform index), so that a pass is a few KB
-// of code: a single row's time would otherwise go into fetching instructions.
-// Elements before the first 16-byte boundary and after the last are single
-// ones of the threads 0 .. W-1 and W .. 2W-1.
-template <typename T, int NB>
+// Vectors of 16 bytes, a block of four of them a thread and turn; elements before
+// the first 16-byte boundary and after the last are single ones of the threads
+// 0 .. W-1 and W .. 2W-1.
+template <typename T>
 struct Row {
   static constexpr int W = RowElem<T>::W;
   const T *p;
   int V, head, nvec, ecol;   // ecol: column of this thread's single element, or -1
   float edge;
-  i32x16 r[NB > 0 ? NB : 1];
 
   __device__ __forceinline__ i32x16 load_block(int b) const {
     const i32x4 *vp = reinterpret_cast<const i32x4 *>(p + head) + threadIdx.x;
@@ -107,31 +104,29 @@ struct Row {
     const int tail0 = head + nvec * W;
     ecol = tid < W ? (tid < head ? tid : -1) : (tid < 2 * W && tail0 + tid - W < n ? tail0 + tid - W : -1);
     edge = ecol >= 0 ? (float)row[ecol] : kRowNegInf;
-    if constexpr (NB > 0) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b) r[b] = load_block(b);
-    }
   }
 
+  // blocks of four vectors a thread that hold the row's vectors
+  __device__ __forceinline__ int blocks() const { return (nvec + 4 * kRowThreads - 1) / (4 * kRowThreads); }
+
   // f(v, col, i): the i-th vector of every thread (all lanes take part; a thread
-  // without one has -inf and a column of at least V), in ascending order of i.
+  // without one has -inf and a column of at least V), in ascending order of i. The
+  // next block is on its way meanwhile.
   template <typename F>
   __device__ __forceinline__ void each_vec(F f) const {
-    const int n = (nvec + kRowThreads - 1) / kRowThreads;
-    auto block = [&](const i32x16 &q, int b) {
-      const int left = min(4, n - 4 * b);
+    const int n = blocks();
+    i32x16 q = load_block(0);
 #pragma unroll 1
-      for (int j = 0; j < left; ++j) {
+    for (int b = 0; b < n; ++b) {
+      i32x16 next = q;
+      if (b + 1 < n) next = load_block(b + 1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
         const int i = 4 * b + j, vi = i * kRowThreads + (int)threadIdx.x;
         const i32x4 v = {q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]};
         f(v, vi < nvec ? head + vi * W : V, i);
       }
-    };
-    if constexpr (NB > 0) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b) block(r[b], b);
-    } else {
-      for (int b = 0; 4 * b < n; ++b) block(load_block(b), b);
+      q = next;
     }
   }
 
@@ -146,48 +141,7 @@ struct Row {
     });
     if (ecol >= 0) f(edge, ecol);
   }
-
-  // f(x, col) of every element with x >= least (NaN: never).
-  template <typename F>
-  __device__ __forceinline__ void each_from(float least, F f) const {
-    each_vec([&](const i32x4 &v, int col, int) {
-      float m = RowElem<T>::get(v, 0);
-#pragma unroll
-      for (int e = 1; e < W; ++e) m = fmaxf(m, RowElem<T>::get(v, e));
-      if (m >= least && col < V) {
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const float x = RowElem<T>::get(v, e);
-          if (x >= least) f(x, col + e);
-        }
-      }
-    });
-    if (ecol >= 0 && edge >= least) f(edge, ecol);
-  }
 };
-
-// f(std::integral_constant NB) for the rows of V columns: the fewest blocks that
-// hold them, 0 where five (80 registers) do not.
-template <typename T, typename F>
-void with_row_blocks(int32_t V, F f) {
-  const int64_t block = 4 * (int64_t)kRowThreads * RowElem<T>::W;
-  if (V <= block) f(std::integral_constant<int, 1>());
-  else if (V <= 2 * block) f(std::integral_constant<int, 2>());
-  else if (V <= 4 * block) f(std::integral_constant<int, 4>());
-  else if (V <= 5 * block) f(std::integral_constant<int, 5>());
-  else f(std::integral_constant<int, 0>());
-}
-
-// Largest element of this thread (-inf without one; NaN left out).
-template <typename T, int NB>
-__device__ __forceinline__ float thread_max(const Row<T, NB> &row) {
-  float m = fmaxf(row.edge, kRowNegInf);
-  row.each_vec([&](const i32x4 &v, int, int) {
-#pragma unroll
-    for (int e = 0; e < RowElem<T>::W; ++e) m = fmaxf(m, RowElem<T>::get(v, e));
-  });
-  return m;
-}
 
 // ---- the workgroup -----------------------------------------------------------
 
@@ -252,8 +206,14 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, RowShared &sh, uint64
   return before + in - v;
 }
 
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
+  const uint32_t lo = __shfl_xor((uint32_t)v, m, 64), hi = __shfl_xor((uint32_t)(v >> 32), m, 64);
+  return (uint64_t)hi << 32 | lo;
+}
+
 // sh.list[0, n) in descending order. Up to 256 entries by counting those above
-// each (n / 2 broadcast reads a thread), else by a bitonic network.
+// each (n broadcast reads a thread); up to 1 024 by a bitonic network with an
+// entry a thread, whose steps within a wave need no barrier; more by one in LDS.
 __device__ __forceinline__ void sort_list(RowShared &sh, int n) {
   const int tid = threadIdx.x;
   __syncthreads();
@@ -269,6 +229,27 @@ __device__ __forceinline__ void sort_list(RowShared &sh, int n) {
   }
   int size = 512;
   while (size < n) size <<= 1;
+  if (size <= kRowThreads) {
+    uint64_t v = tid < n ? sh.list[tid] : 0;
+    for (int k = 2; k <= size; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        uint64_t o;
+        if (j >= 64) {
+          __syncthreads();
+          sh.list[tid] = v;
+          __syncthreads();
+          o = sh.list[tid ^ j];
+        } else {
+          o = shfl_xor64(v, j);
+        }
+        const bool larger = ((tid & j) == 0) == ((tid & k) == 0);
+        if ((v < o) == larger) v = o;
+      }
+    __syncthreads();
+    sh.list[tid] = v;
+    __syncthreads();
+    return;
+  }
   for (int i = n + tid; i < size; i += kRowThreads) sh.list[i] = 0;
   __syncthreads();
   for (int k = 2; k <= size; k <<= 1)
@@ -301,38 +282,61 @@ __device__ __forceinline__ void add_bin(uint64_t *bins, uint32_t bin, uint64_t w
   atomicAdd((unsigned long long *)&bins[bin], (unsigned long long)w);
 }
 
-// The bin in which the running sum of sh.bins[0, nbins) (from the top bin down,
+// The bin in which the running sum of bins[0, nbins) (from the top bin down,
 // or from bin 0 up) reaches need, and the sum before it (sh.found). *total: of
 // all bins. need(total) >= 1 gives what has to be reached, at most the total.
 template <typename F>
-__device__ __forceinline__ void find_bin(RowShared &sh, int nbins, bool down, F need, uint64_t *total) {
+__device__ __forceinline__ void find_bin(RowShared &sh, const uint64_t *bins, int nbins, bool down, F need,
+                                         uint64_t *total) {
   const int tid = threadIdx.x, per = nbins <= kRowThreads ? 1 : nbins / kRowThreads;
   uint64_t s = 0;
   const int b0 = tid * per;
   __syncthreads();
   if (b0 < nbins)
-    for (int i = 0; i < per; ++i) s += sh.bins[down ? nbins - 1 - b0 - i : b0 + i];
+    for (int i = 0; i < per; ++i) s += bins[down ? nbins - 1 - b0 - i : b0 + i];
   uint64_t before = block_scan(s, sh, total);
   const uint64_t want = need(*total);
   if (before < want && want <= before + s)
     for (int i = 0; i < per; ++i) {
       const int b = down ? nbins - 1 - b0 - i : b0 + i;
-      if (before + sh.bins[b] >= want) {
+      if (before + bins[b] >= want) {
         sh.found[0] = b;
         sh.found[1] = before;
         break;
       }
-      before += sh.bins[b];
+      before += bins[b];
     }
   __syncthreads();
+}
+
+// The rank of the element that is number `ties` by column among those of `key` (and
+// of at least `floor`): more than that have the key. Uses sh.list.
+template <typename T>
+__device__ uint64_t column_threshold(const Row<T> &row, RowShared &sh, uint64_t floor, uint32_t key, uint64_t ties) {
+  uint32_t prefix = 0;
+  uint64_t total;
+  for (int shift = 20; shift > 0; shift -= 10) {
+    for (int i = threadIdx.x; i < 1024; i += kRowThreads) sh.list[i] = 0;
+    __syncthreads();
+    row.each([&](float x, int col) {
+      const uint64_t r = rank_of(x, col);
+      if ((uint32_t)(r >> 32) != key || r < floor || (shift < 20 && (uint32_t)col >> shift != prefix)) return;
+      add_bin(sh.list, ((uint32_t)col >> (shift - 10)) & 1023u, 1, true);
+    });
+    find_bin(sh, sh.list, 1024, false, [&](uint64_t) { return ties; }, &total);
+    ties -= sh.found[1];
+    prefix = prefix << 10 | (uint32_t)sh.found[0];
+    __syncthreads();
+  }
+  return (uint64_t)key << 32 | (uint32_t)~prefix;
 }
 
 // The largest rank such that the elements of at least that rank (among those of
 // at least `floor`) weigh need(total) or more. weight(x) is 1 (ONES) or a whole
 // number that depends on the value alone. Digits of the key from the top, 12
 // bits at first, then of the columns of the elements that share the last key.
-template <bool ONES, typename T, int NB, typename WF, typename NF>
-__device__ uint64_t radix_threshold(const Row<T, NB> &row, RowShared &sh, uint64_t floor, WF weight, NF need) {
+template <bool ONES, typename T, typename WF, typename NF>
+__device__ uint64_t radix_threshold(const Row<T> &row, RowShared &sh, uint64_t floor, WF weight, NF need) {
   uint64_t want = 0, total = 0;
   uint32_t prefix = 0;
   int shift = 32;
@@ -350,7 +354,7 @@ __device__ uint64_t radix_threshold(const Row<T, NB> &row, RowShared &sh, uint64
       if (ONES || w) add_bin(sh.bins, (key >> next) & mask, w, ONES);
     });
     const bool first = shift == 32;
-    find_bin(sh, 1 << width, true, [&](uint64_t t) { return first ? need(t) : want; }, &total);
+    find_bin(sh, sh.bins, 1 << width, true, [&](uint64_t t) { return first ? need(t) : want; }, &total);
     if (first) want = need(total);
     want -= sh.found[1];
     in_bin = sh.bins[sh.found[0]];
@@ -365,34 +369,127 @@ __device__ uint64_t radix_threshold(const Row<T, NB> &row, RowShared &sh, uint64
   }
   // elements of this key that are needed, of those there are
   const uint64_t w = ONES ? 1 : weight(rank_value((uint64_t)key << 32));
-  uint64_t ties = (want + w - 1) / w;
-  if (ties >= in_bin / w) return (uint64_t)key << 32;
-  uint32_t cprefix = 0;
-  for (int cshift = 20; cshift > 0; cshift -= 10) {
-    for (int i = threadIdx.x; i < 1024; i += kRowThreads) sh.bins[i] = 0;
-    __syncthreads();
-    row.each([&](float x, int col) {
-      const uint64_t r = rank_of(x, col);
-      if ((uint32_t)(r >> 32) != key || r < floor || (cshift < 20 && (uint32_t)col >> cshift != cprefix)) return;
-      add_bin(sh.bins, ((uint32_t)col >> (cshift - 10)) & 1023u, 1, true);
-    });
-    find_bin(sh, 1024, false, [&](uint64_t) { return ties; }, &total);
-    ties -= sh.found[1];
-    cprefix = cprefix << 10 | (uint32_t)sh.found[0];
-    __syncthreads();
+  const uint64_t ties = (want + w - 1) / w;
+  return ties >= in_bin / w ? (uint64_t)key << 32 : column_threshold(row, sh, floor, key, ties);
+}
+
+// A running maximum and sum of exponentials, (m, d = sum e^{(x - m) c ln 2}).
+struct RowSum {
+  float m = kRowNegInf, d = 0.f;
+  // elements with the largest of them, g (NaN left out)
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N], float g, float c) {
+    if (g > m) {
+      d *= __builtin_amdgcn_exp2f((m - g) * c);   // 0 while m = -inf
+      m = g;
+    }
+    const float base = m == kRowNegInf ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) d += __builtin_amdgcn_exp2f((x[i] - base) * c);
   }
-  return (uint64_t)key << 32 | (uint32_t)~cprefix;
+  __device__ __forceinline__ void merge(float om, float od, float c) {
+    const float n = fmaxf(m, om);
+    if (n != kRowNegInf) {
+      d = d * __builtin_amdgcn_exp2f((m - n) * c) + od * __builtin_amdgcn_exp2f((om - n) * c);
+      m = n;
+    } else {
+      d += od;   // NaN stays
+    }
+  }
+};
+
+// ---- the first elements in order ------------------------------------------------
+
+// A pass over the row that leaves, for each thread, the largest element of every
+// `group` blocks of four vectors (sh.bins, as floats; the thread's own column)
+// and of all its elements (the result). With those, the few vectors that hold an
+// element above a bound are found, and read again, without another pass.
+// With SUM the elements' exponentials are added too.
+constexpr int kGroups = 8;
+template <bool SUM, typename T>
+__device__ __forceinline__ float scan_row(const Row<T> &row, RowShared &sh, int group, float c, RowSum &st) {
+  constexpr int W = RowElem<T>::W;
+  float *tops = reinterpret_cast<float *>(sh.bins) + threadIdx.x;
+  const int nblocks = row.blocks();
+  float tmax = fmaxf(row.edge, kRowNegInf), gmax = kRowNegInf;
+  if constexpr (SUM) {
+    if (row.ecol >= 0) {
+      const float f[1] = {row.edge};
+      st.add(f, tmax, c);
+    }
+  }
+  i32x16 q = row.load_block(0);
+  int g = 0, left = group;
+#pragma unroll 1
+  for (int b = 0; b < nblocks; ++b) {
+    i32x16 next = q;
+    if (b + 1 < nblocks) next = row.load_block(b + 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const i32x4 v = {q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]};
+      float f[W];
+      float m = f[0] = RowElem<T>::get(v, 0);
+#pragma unroll
+      for (int e = 1; e < W; ++e) m = fmaxf(m, f[e] = RowElem<T>::get(v, e));
+      m = fmaxf(m, kRowNegInf);
+      gmax = fmaxf(gmax, m);
+      if constexpr (SUM) st.add(f, m, c);
+    }
+    q = next;
+    if (--left == 0 || b == nblocks - 1) {
+      tops[g * kRowThreads] = gmax;
+      tmax = fmaxf(tmax, gmax);
+      gmax = kRowNegInf;
+      left = group;
+      ++g;
+    }
+  }
+  return tmax;
+}
+
+// Blocks a group, for kGroups groups to hold any row of V columns.
+template <typename T>
+int row_group(int32_t V) {
+  const int64_t block = 4 * (int64_t)kRowThreads * RowElem<T>::W;
+  return (int)((((int64_t)V + block - 1) / block + kGroups - 1) / kGroups);
+}
+
+// f(x, col) of the elements that are >= least, by what scan_row left.
+template <typename T, typename F>
+__device__ __forceinline__ void scan_hits(const Row<T> &row, const RowShared &sh, int group, float least, F f) {
+  constexpr int W = RowElem<T>::W;
+  const float *tops = reinterpret_cast<const float *>(sh.bins) + threadIdx.x;
+  const int nblocks = row.blocks(), ngroups = (nblocks + group - 1) / group;
+  if (row.ecol >= 0 && row.edge >= least) f(row.edge, row.ecol);
+  for (int g = 0;; ++g) {
+    while (g < ngroups && !(tops[g * kRowThreads] >= least)) ++g;   // each lane to its own next one
+    if (g >= ngroups) break;
+    for (int b = g * group; b < min(nblocks, (g + 1) * group); ++b) {
+      const i32x16 q = row.load_block(b);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int vi = (4 * b + j) * kRowThreads + (int)threadIdx.x;
+        if (vi >= row.nvec) continue;
+        const i32x4 v = {q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]};
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const float x = RowElem<T>::get(v, e);
+          if (x >= least) f(x, row.head + vi * W + e);
+        }
+      }
+    }
+  }
 }
 
 // The k <= kMaxTop first elements of the row in sh.list[0, k), in order (the
-// row has k). tmax: this thread's largest element.
+// row has k), after scan_row, which gave tmax.
 //
 // Each wave puts its threads' largest in order; with j = ceil(k / 16) the least of
 // the 16 waves' j-th ones has at least 16 j >= k elements at or above it, and for
 // ordinary rows few more: those are taken into LDS and put in order there. A row
 // with too many of them (equal values) has its threshold found digit by digit.
-template <typename T, int NB>
-__device__ void top_list(const Row<T, NB> &row, RowShared &sh, float tmax, int k) {
+template <typename T>
+__device__ void top_list(const Row<T> &row, RowShared &sh, int group, float tmax, int k) {
   const int tid = threadIdx.x, lane = tid & 63;
   float v = tmax;
 #pragma unroll
@@ -402,17 +499,16 @@ __device__ void top_list(const Row<T, NB> &row, RowShared &sh, float tmax, int k
       const float o = __shfl_xor(v, stride, 64);
       v = ((lane & stride) == 0) == ((lane & size) == 0) ? fmaxf(v, o) : fminf(v, o);
     }
-  const float least = -block_max(-__shfl(v, (k + kRowWaves - 1) / kRowWaves - 1, 64), sh);
   if (tid == 0) sh.count = 0;
-  __syncthreads();
-  row.each_from(least, [&](float x, int col) {
+  const float least = -block_max(-__shfl(v, (k + kRowWaves - 1) / kRowWaves - 1, 64), sh);
+  scan_hits(row, sh, group, least, [&](float x, int col) {
     const int at = atomicAdd(&sh.count, 1);
     if (at < kListCap) sh.list[at] = rank_of(x, col);
   });
   __syncthreads();
   int n = sh.count;
-  __syncthreads();
   if (n > kListCap || n < k) {   // n < k: NaN among the first
+    __syncthreads();
     const uint64_t thr = radix_threshold<true>(row, sh, 0, [](float) { return uint64_t(1); },
                                                [&](uint64_t) { return (uint64_t)k; });
     if (tid == 0) sh.count = 0;
