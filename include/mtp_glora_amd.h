@@ -456,7 +456,8 @@ int mga_top_logits(const void *logits, int64_t row_stride, int32_t n_rows, int32
  * whatever its logits are; a student logit of -inf at an entry of q > 0 gives an
  * infinite loss; NaN and +inf among other rows' student logits give NaN. An id
  * may stand in a row more than once: its q add up.
- * 1 <= k <= 1024. workspace: mga_top_logits_ce_workspace_floats fp32 values.
+ * 1 <= k <= 1024. workspace: mga_top_logits_ce_workspace_floats fp32 values,
+ * 16-byte aligned.
  * Stands beside mga_soft_ce_* (loss.py:259-330), which reads whole teacher rows.
  */
 int64_t mga_top_logits_ce_workspace_floats(int32_t n_rows, int32_t n_cols);
@@ -480,9 +481,10 @@ int mga_top_logits_ce_bwd(const void *student, int64_t student_row_stride, const
 /*
  * Loss and gradient in one call, with an upstream gradient that the host knows:
  * loss_sum as mga_top_logits_ce_fwd, grad as mga_top_logits_ce_bwd with
- * grad_output = scale. Rows of up to 163 840 16-bit or 81 920 fp32 logits are
- * read once; longer ones as by the two calls. grad may not overlap student.
- * workspace: mga_top_logits_ce_step_workspace_floats fp32 values.
+ * grad_output = scale. With 128 rows and more a row's second reading follows its
+ * first and comes from the caches; fewer are taken as by the two calls. grad may
+ * not overlap student.
+ * workspace: mga_top_logits_ce_step_workspace_floats fp32 values, 16-byte aligned.
  */
 int64_t mga_top_logits_ce_step_workspace_floats(int32_t n_rows, int32_t n_cols, int32_t k);
 int mga_top_logits_ce_step(const void *student, int64_t student_row_stride, const void *values,

@@ -886,7 +886,13 @@ int check_teacher(const char *fn, const mga::TopLogitsCeArgs &a, const float *wo
   const int rc = check_matrix(fn, "values", a.values, a.values_rs, a.N, a.K, a.values_dtype);
   if (rc != MGA_OK) return rc;
   if (!a.loss || !a.sum || !workspace) return fail(MGA_ERR_INVALID, "%s: null output or workspace", fn);
+  if (!aligned16(workspace)) return fail(MGA_ERR_INVALID, "%s: workspace not 16-byte aligned", fn);
   return MGA_OK;
+}
+
+// where the step's stats begin in its workspace, behind the forward's
+int64_t step_stats_at(int32_t n_rows, int32_t n_cols) {
+  return (mga::top_ce_workspace_floats(n_rows, n_cols) + 3) / 4 * 4;
 }
 
 int check_embedding(const char *fn, const void *ids, int32_t ids64, int32_t n, int32_t n_rows, int32_t width,
@@ -924,7 +930,7 @@ int64_t mga_top_logits_ce_workspace_floats(int32_t n_rows, int32_t n_cols) {
 
 int64_t mga_top_logits_ce_step_workspace_floats(int32_t n_rows, int32_t n_cols, int32_t k) {
   if (n_rows <= 0 || n_cols <= 0 || k <= 0) return 0;
-  return mga::top_ce_workspace_floats(n_rows, n_cols) + (3 + (int64_t)k) * n_rows;
+  return step_stats_at(n_rows, n_cols) + (3 + (int64_t)k) * n_rows;
 }
 
 int mga_top_logits_ce_fwd(const void *student, int64_t student_row_stride, const void *values,
@@ -966,7 +972,8 @@ int mga_top_logits_ce_step(const void *student, int64_t student_row_stride, cons
                            float temperature, float scale, int32_t dtype, float *row_loss, float *loss_sum, void *grad,
                            int64_t grad_row_stride, float *workspace, void *stream) {
   const char *fn = "mga_top_logits_ce_step";
-  float *stats = workspace, *q = stats ? stats + 3 * (int64_t)n_rows : nullptr;
+  float *stats = workspace && n_rows > 0 && n_cols > 0 ? workspace + step_stats_at(n_rows, n_cols) : nullptr;
+  float *q = stats ? stats + 3 * (int64_t)n_rows : nullptr;
   const mga::TopLogitsCeArgs a{student, student_row_stride, values, values_row_stride, ids, ids_row_stride, teacher_lse,
                                q, stats, row_loss, loss_sum, nullptr, grad, grad_row_stride, temperature, scale, n_rows,
                                n_cols, k, values_dtype, ids_are_int64 != 0};
@@ -978,7 +985,7 @@ int mga_top_logits_ce_step(const void *student, int64_t student_row_stride, cons
   const uintptr_t x1 = x0 + ((uintptr_t)(n_rows - 1) * student_row_stride + n_cols) * eb;
   const uintptr_t g1 = g0 + ((uintptr_t)(n_rows - 1) * grad_row_stride + n_cols) * eb;
   if (x0 < g1 && g0 < x1) return fail(MGA_ERR_INVALID, "%s: grad overlaps student", fn);
-  mga::launch_top_ce_step(a, dtype, q + (int64_t)n_rows * k, (hipStream_t)stream);
+  mga::launch_top_ce_step(a, dtype, workspace, (hipStream_t)stream);
   return check_launch(fn);
 }
 

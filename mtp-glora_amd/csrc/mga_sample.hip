@@ -70,107 +70,145 @@ __device__ __forceinline__ uint64_t mass_needed(float p, uint64_t total) {
 
 // ---- bf16: the weights of the values that occur ----------------------------------
 
-// Positions 0 .. kTable - 1 in descending order of the value: the positive values of
-// kOctaves octaves, then the negative ones. The top octave is that of the largest
-// magnitude with a weight; the values below the window (2^-27 of that) are few, and
-// stand between the halves.
-constexpr int kOctaves = 28, kHalf = kOctaves * 128, kTable = 2 * kHalf, kPerThread = kTable / kRowThreads;
-static_assert(kTable == kPerThread * kRowThreads && kHalf % kPerThread == 0, "a thread's positions are of one sign");
+// The table has the positive values of kOctaves octaves at [0, kHalf) by magnitude,
+// then the negative ones. The top octave is one above that of the largest magnitude
+// that has a weight; what is larger still (-inf, NaN) shares its last entries, which
+// have none. Values below the window (2^-31 of that magnitude) are few: they are
+// computed.
+constexpr int kOctaves = 32, kHalf = kOctaves * 128, kTable = 2 * kHalf, kPerThread = kTable / kRowThreads;
 
 struct TableShared {
-  uint64_t weight[kTable + 1];   // the last: no weight
-  uint32_t count[kTable];
+  uint64_t weight[kTable];
   uint64_t small_weight;
   uint32_t small_count;
 };
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
 struct Window {
-  uint32_t lo, gap;
-  // values as whole numbers in descending order: 0 .. 0x7FFF positive, 0x8000 .. negative
-  __device__ __forceinline__ static uint32_t descending(uint32_t bits) { return bits ^ (bits & 0x8000u ? 0u : 0x7FFFu); }
-  // kTable: none (below the window, past its ends, NaN)
-  __device__ __forceinline__ uint32_t position(uint32_t bits) const {
-    const uint32_t e = descending(bits) - lo, neg = e - gap;
-    return e < (uint32_t)kHalf ? e : neg - (uint32_t)kHalf < (uint32_t)kHalf ? neg : (uint32_t)kTable;
+  uint32_t mag0;   // the smallest magnitude, bits of a bf16
+  // Two values' entries in the halves of a word. Where one is below the window its
+  // bit 15 is set (13 bits are the entry).
+  __device__ __forceinline__ uint32_t entries(uint32_t two) const {
+    const u16x2 low = (u16x2)(uint16_t)mag0, high = (u16x2)(uint16_t)(mag0 + kHalf - 1);
+    const u16x2 m = __builtin_elementwise_min(__builtin_bit_cast(u16x2, two & 0x7FFF7FFFu), high) - low;
+    return __builtin_bit_cast(uint32_t, m) | (two >> 3 & 0x10001000u);
   }
-  __device__ __forceinline__ bool small(uint32_t bits) const { return descending(bits) - lo - (uint32_t)kHalf < gap; }
-  __device__ __forceinline__ float value(int pos) const {
-    return __builtin_bit_cast(float, descending(lo + pos + (pos >= kHalf ? gap : 0)) << 16);
+  __device__ __forceinline__ float value(int entry) const {
+    const uint32_t bits = mag0 + (entry & (kHalf - 1)) + (entry & kHalf ? 0x8000u : 0u);
+    return __builtin_bit_cast(float, bits << 16);
   }
 };
+static_assert(kHalf == 0x1000, "the sign's place in entries()");
+constexpr uint32_t kBelow = 0x80008000u;
 
-__device__ __forceinline__ uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x) >> 16; }
+// Entries in descending order of the value.
+__device__ __forceinline__ int entry_at(int place) { return place < kHalf ? kHalf - 1 - place : place; }
 
-// Weight of a bf16 value from the table.
+// Weight of a value that is at least `least`, computed.
+struct Computed {
+  Weight weight;
+  float least;
+  __device__ __forceinline__ uint64_t operator()(float x) const { return x >= least ? weight(x) : 0; }
+};
+
+// The same for bf16, from the table.
 struct Tabulated {
   Weight weight;
+  float least;
   Window win;
-  const TableShared *tab;
+  TableShared *tab;
   __device__ __forceinline__ uint64_t operator()(float x) const {
-    const uint32_t b = bits_of(x);
-    return win.small(b) ? weight(x) : tab->weight[win.position(b)];
+    const uint32_t e = win.entries(__builtin_bit_cast(uint32_t, x) >> 16);
+    return e & 0x8000u ? (x >= least ? weight(x) : 0) : tab->weight[e & (kTable - 1)];
+  }
+  // Values below v have no weight from here on.
+  __device__ __forceinline__ void raise(float v) {
+    least = v;
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) {
+      const int e = (int)threadIdx.x + j * kRowThreads;
+      if (win.value(e) < v) tab->weight[e] = 0;
+    }
+    __syncthreads();
   }
 };
 
-// Weights of the window's values; the counts cleared. top is finite.
-__device__ __forceinline__ Window make_table(TableShared &tab, const Weight &weight) {
+// The window for values up to weight.top; false where none will do.
+__device__ __forceinline__ bool find_window(const Weight &weight, Window *win) {
   const double least = weight.topd - (weight.s + 2) / weight.c;   // nothing below it has a weight
-  const float big = fminf(fmaxf(fabsf((float)least), fabsf(weight.top)), 3.3895314e38f);
-  const uint32_t octave = max(__builtin_bit_cast(uint32_t, big) >> 23, (uint32_t)kOctaves);
-  const uint32_t mag0 = (octave + 1 - kOctaves) << 7;   // the window's smallest magnitude
-  const Window win{0x7FFFu - (mag0 + kHalf - 1), 2 * mag0};
-#pragma unroll 1
+  const float big = fmaxf(fabsf((float)least), fabsf(weight.top));
+  const uint32_t octave = max((__builtin_bit_cast(uint32_t, big) >> 23) + 1, (uint32_t)kOctaves - 1);
+  win->mag0 = ((octave + 1) << 7) - kHalf;
+  return octave <= 254;   // no octave of infinities
+}
+
+__device__ __forceinline__ void make_table(TableShared &tab, const Weight &weight, const Window &win) {
+#pragma unroll
   for (int j = 0; j < kPerThread; ++j) {
-    const int pos = (int)threadIdx.x + j * kRowThreads;
-    const float v = win.value(pos);
-    tab.weight[pos] = v <= weight.top ? weight(v) : 0;
-    tab.count[pos] = 0;
+    const int e = (int)threadIdx.x + j * kRowThreads;
+    const float v = win.value(e);
+    const uint64_t w = weight(fminf(v, weight.top));
+    tab.weight[e] = v <= weight.top ? w : 0;
   }
   if (threadIdx.x == 0) {
-    tab.weight[kTable] = 0;
     tab.small_weight = 0;
     tab.small_count = 0;
   }
   __syncthreads();
-  return win;
 }
 
-// Threshold of top_k and top_p by the histogram of the row's values, and how many
-// elements it leaves; what scan_row left stays. False where a cut falls among the values below the window.
+// Threshold of top_k and top_p by the histogram of the row's values (counted in
+// sh.list), and how many elements it leaves; what scan_row left stays. False where
+// a cut falls among the values below the window.
 __device__ bool table_threshold(const Row<bf16_t> &row, RowShared &sh, TableShared &tab, const Tabulated &t, bool by_k,
                                 uint64_t top_k, bool by_p, float top_p, uint64_t *thr, uint64_t *kept) {
   const int tid = threadIdx.x;
-  auto tally = [&](uint32_t bits) {
-    const uint32_t pos = t.win.position(bits);
-    if (pos < (uint32_t)kTable) atomicAdd(&tab.count[pos], 1u);
-    else if (t.win.small(bits)) {
-      atomicAdd(&tab.small_count, 1u);
-      atomicAdd((unsigned long long *)&tab.small_weight,
-                (unsigned long long)t.weight(__builtin_bit_cast(float, bits << 16)));
-    }
+  static_assert(sizeof(sh.list) >= kTable * sizeof(uint32_t), "the counts");
+  uint32_t *count = reinterpret_cast<uint32_t *>(sh.list);
+  for (int i = tid; i < kTable; i += kRowThreads) count[i] = 0;
+  __syncthreads();
+  auto tally = [&](uint32_t e) {   // the last entries have no weight, and may be most of a masked row
+    if ((e & (kHalf - 1)) != kHalf - 1) atomicAdd(&count[e & (kTable - 1)], 1u);
+  };
+  auto one = [&](uint32_t bits) {
+    const uint32_t e = t.win.entries(bits);
+    if (!(e & 0x8000u)) return tally(e);
+    atomicAdd(&tab.small_count, 1u);
+    atomicAdd((unsigned long long *)&tab.small_weight,
+              (unsigned long long)t.weight(__builtin_bit_cast(float, bits << 16)));
   };
   row.each_vec([&](const i32x4 &v, int col, int) {
     if (col >= row.V) return;
-#pragma unroll 2
+    uint32_t e[4], below = 0;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) below |= e[d] = t.win.entries((uint32_t)v[d]);
+    if (below & kBelow) {
+#pragma unroll 1
+      for (int d = 0; d < 8; ++d) one((uint32_t)v[d >> 1] >> (d & 1) * 16 & 0xFFFFu);
+      return;
+    }
+#pragma unroll
     for (int d = 0; d < 4; ++d) {
-      tally((uint32_t)v[d] & 0xFFFFu);
-      tally((uint32_t)v[d] >> 16);
+      tally(e[d] & 0xFFFFu);
+      tally(e[d] >> 16);
     }
   });
-  if (row.ecol >= 0) tally(bits_of(row.edge));
+  if (row.ecol >= 0) one(__builtin_bit_cast(uint32_t, row.edge) >> 16);
   __syncthreads();
-  // a thread's positions; the values below the window stand before thread kHalf / kPerThread's
+  // a thread's entries, in descending order; the values below the window stand
+  // before those of the first thread of the negative half
   const int p0 = tid * kPerThread;
   const uint32_t between = p0 == kHalf ? tab.small_count : 0;
   uint32_t c[kPerThread];
   uint64_t cs = between, total;
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) cs += c[j] = tab.count[p0 + j];
+  for (int j = 0; j < kPerThread; ++j) cs += c[j] = count[entry_at(p0 + j)];
   const uint64_t before = block_scan(cs, sh, &total);
-  int cut = kTable;        // position of the last kept value, -1: below the window
+  int cut = kTable;        // place of the last kept value, -1: below the window
   uint64_t ties = 0;       // kept elements of it
-  auto share = [&](int pos, uint64_t n, uint64_t left) {   // by the one thread that has it
-    sh.count = pos;
+  auto share = [&](int place, uint64_t n, uint64_t left) {   // by the one thread that has it
+    sh.count = place;
     sh.found[0] = n;
     sh.found[1] = left;
   };
@@ -186,16 +224,16 @@ __device__ bool table_threshold(const Row<bf16_t> &row, RowShared &sh, TableShar
   if (by_k && total > top_k) {
     if (before < top_k && top_k <= before + cs) {
       uint64_t run = before + between;
-      int pos = run >= top_k ? -1 : -2;
+      int place = run >= top_k ? -1 : -2;
 #pragma unroll
       for (int j = 0; j < kPerThread; ++j) {
-        if (pos == -2 && run + c[j] >= top_k) {
-          pos = p0 + j;
-          share(pos, top_k - run, top_k);
+        if (place == -2 && run + c[j] >= top_k) {
+          place = p0 + j;
+          share(place, top_k - run, top_k);
         }
         run += c[j];
       }
-      if (pos == -1) share(-1, 0, 0);
+      if (place == -1) share(-1, 0, 0);
     }
     shared();
     if (cut < 0) return false;
@@ -206,31 +244,33 @@ __device__ bool table_threshold(const Row<bf16_t> &row, RowShared &sh, TableShar
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j) {
       if (p0 + j >= cut) c[j] = p0 + j == cut ? (uint32_t)ties : 0;
-      ms += c[j] * tab.weight[p0 + j];
+      ms += c[j] * tab.weight[entry_at(p0 + j)];
     }
     const uint64_t mb = block_scan(ms, sh, &z), want = mass_needed(top_p, z);
     if (mb < want && want <= mb + ms) {
       uint64_t run = mb + mid, left = before + between;
-      int pos = run >= want ? -1 : -2;
+      int place = run >= want ? -1 : -2;
 #pragma unroll
       for (int j = 0; j < kPerThread; ++j) {
-        const uint64_t w = tab.weight[p0 + j], m = c[j] * w;
-        if (pos == -2 && m && run + m >= want) {
+        const uint64_t w = tab.weight[entry_at(p0 + j)], m = c[j] * w;
+        if (place == -2 && m && run + m >= want) {
           const uint64_t n = (want - run + w - 1) / w;
-          pos = p0 + j;
-          share(pos, n, left + n);
+          place = p0 + j;
+          share(place, n, left + n);
         }
         run += m;
         left += c[j];
       }
-      if (pos == -1) share(-1, 0, 0);
+      if (place == -1) share(-1, 0, 0);
     }
     shared();
     if (cut < 0) return false;
   }
   if (cut == kTable) return true;
-  const uint32_t key = value_key(t.win.value(cut));
-  *thr = ties >= tab.count[cut] ? (uint64_t)key << 32 : column_threshold(row, sh, 0, key, ties);
+  const uint32_t key = value_key(t.win.value(entry_at(cut)));
+  const uint32_t there = count[entry_at(cut)];
+  __syncthreads();   // the counts are over
+  *thr = ties >= there ? (uint64_t)key << 32 : column_threshold(row, sh, 0, key, ties);
   return true;
 }
 
@@ -243,9 +283,33 @@ template <typename WF>
 __device__ int pick_in_list(RowShared &sh, int n, const WF &weight, float u) {
   constexpr int kEach = kListCap / kRowThreads;
   const int tid = threadIdx.x;
+  __syncthreads();
+  if (n <= 256) {   // each entry adds those of columns up to its own
+    const uint64_t r = tid < n ? sh.list[tid] : 0;
+    const int col = rank_col(r);
+    const uint64_t w = tid < n ? weight(rank_value(r)) : 0;
+    if (tid < 256) {
+      sh.bins[2 * tid] = w;
+      sh.bins[2 * tid + 1] = (uint64_t)col;
+    }
+    __syncthreads();
+    if (tid < n) {
+      uint64_t upto = 0, all = 0;
+      for (int i = 0; i < n; i += 8)   // those past n have no weight
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const uint64_t o = sh.bins[2 * (i + u)];
+          all += o;
+          upto += (int)sh.bins[2 * (i + u) + 1] <= col ? o : 0;
+        }
+      const uint64_t target = target_of(u, all);
+      if (w && upto >= target && upto - w < target) sh.count = col;
+    }
+    __syncthreads();
+    return sh.count;
+  }
   uint64_t w[kEach];
   int col[kEach];
-  __syncthreads();
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int at = tid + i * kRowThreads;
@@ -275,21 +339,48 @@ __device__ int pick_in_list(RowShared &sh, int n, const WF &weight, float u) {
   return token;
 }
 
-// The same among all elements of at least `thr`.
+// The weights of a vector's elements, added.
+template <typename T>
+__device__ __forceinline__ uint64_t vector_sum(const Computed &weight, const i32x4 &v) {
+  uint64_t s = 0;
+#pragma unroll
+  for (int e = 0; e < RowElem<T>::W; ++e) s += weight(RowElem<T>::get(v, e));
+  return s;
+}
+template <typename T>
+__device__ __forceinline__ uint64_t vector_sum(const Tabulated &t, const i32x4 &v) {
+  uint32_t e[4], below = 0;
+  uint64_t s = 0;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    below |= e[d] = t.win.entries((uint32_t)v[d]);
+    s += t.tab->weight[e[d] & (kTable - 1)] + t.tab->weight[e[d] >> 16 & (kTable - 1)];
+  }
+  if (below & kBelow) {
+    s = 0;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) s += t(RowElem<T>::get(v, i));
+  }
+  return s;
+}
+
+// The same among all elements of at least `thr`. `weight` is 0 for smaller values.
 template <typename T, typename WF>
 __device__ int pick_in_row(const Row<T> &row, RowShared &sh, uint64_t thr, const WF &weight, float u) {
   constexpr int W = RowElem<T>::W;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const float least = thr >> 32 > 1 ? rank_value(thr) : kRowNegInf;
-  const int last = (uint32_t)thr ? rank_col(thr) : row.V;   // of the elements equal to least, the last column that counts
-  auto kept = [&](float x, int col) {
-    return x > least || (x == least && col <= last) ? weight(x) : uint64_t(0);
-  };
+  // of the elements equal to least, the last column that counts
+  const int last = (uint32_t)thr ? rank_col(thr) : row.V;
+  auto kept = [&](float x, int col) { return x == weight.least && col > last ? uint64_t(0) : weight(x); };
   auto lane_sum = [&](const i32x4 &v, int col) {
     uint64_t s = 0;
-    if (col < row.V) {
-#pragma unroll
-      for (int e = 0; e < W; ++e) s += kept(RowElem<T>::get(v, e), col + e);
+    if (col + W - 1 > last) {
+      if (col < row.V) {
+#pragma unroll 1
+        for (int e = 0; e < W; ++e) s += kept(RowElem<T>::get(v, e), col + e);
+      }
+    } else {
+      s = vector_sum<T>(weight, v);
     }
     return s;
   };
@@ -376,7 +467,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict
   Row<T> row;
   row.load(x + n * xs, V);
   RowSum none;
-  const float tmax = scan_row<false>(row, sh, group, 0.f, none), top = block_max(tmax, sh);
+  const float tmax = scan_row<false, 2>(row, sh, group, 0.f, none), top = block_max(tmax, sh);
   if (top == kRowNegInf) {   // nothing to draw from
     if (tid == 0) token[n] = -1;
     return;
@@ -438,27 +529,33 @@ __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict
         thr = radix_threshold<false>(row, sh, thr, weight, [&](uint64_t total) { return mass_needed(top_p, total); });
       thr = max(thr, floor);
     };
-    if (listed <= kListCap) {
-      t = pick_in_list(sh, listed, weight, u);
-    } else if constexpr (sizeof(SampleShared<T>) > sizeof(RowShared)) {
+    bool done = listed <= kListCap;
+    if (done) t = pick_in_list(sh, listed, weight, u);
+    if constexpr (sizeof(SampleShared<T>) > sizeof(RowShared)) {
       // up to kTable columns, their own weights are no more work than the table's
-      if (top < -kRowNegInf && V > kTable) {
-        const Tabulated tw{weight, make_table(sh.tab, weight), &sh.tab};
+      Window win;
+      if (!done && top < -kRowNegInf && V > kTable && find_window(weight, &win)) {
+        make_table(sh.tab, weight, win);
+        Tabulated tw{weight, kRowNegInf, win, &sh.tab};
         bool found = true;
         if (by_k || by_p) {
           found = table_threshold(row, sh, sh.tab, tw, by_k, top_k, by_p, top_p, &thr, &kept);
           if (!found) threshold();
           thr = max(thr, floor);
+          if (found && kept <= kListCap && thr >> 32 > 1) listed = gather();
         }
-        if (found && kept <= kListCap && thr >> 32 > 1) listed = gather();
-        t = listed <= kListCap ? pick_in_list(sh, listed, tw, u) : pick_in_row(row, sh, thr, tw, u);
-      } else {
-        threshold();
-        t = pick_in_row(row, sh, thr, weight, u);
+        if (listed <= kListCap) {
+          t = pick_in_list(sh, listed, tw, u);
+        } else {
+          if (thr >> 32 > 1) tw.raise(rank_value(thr));
+          t = pick_in_row(row, sh, thr, tw, u);
+        }
+        done = true;
       }
-    } else {
+    }
+    if (!done) {
       threshold();
-      t = pick_in_row(row, sh, thr, weight, u);
+      t = pick_in_row(row, sh, thr, Computed{weight, thr >> 32 > 1 ? rank_value(thr) : kRowNegInf}, u);
     }
   }
   if (tid == 0) token[n] = t;

@@ -33,7 +33,7 @@ __device__ __forceinline__ void merge_lanes(RowSum &st, float c) {
 
 // Four vectors of x a turn of the workgroup of B threads, upwards; f(vector).
 template <int B, typename F>
-__device__ __forceinline__ void vectors_up(const i32x4 *vp, int nvec, F f) {
+__device__ __forceinline__ void vectors_up(const i32x4 *vp, int nvec, const i32x4 &none, F f) {
   const int tid = threadIdx.x, nturn = nvec / (4 * B);
   i32x4 a[4], b[4];
   if (nturn > 0) {
@@ -50,7 +50,8 @@ __device__ __forceinline__ void vectors_up(const i32x4 *vp, int nvec, F f) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) a[u] = b[u];
   }
-  for (int i = nturn * 4 * B + tid; i < nvec; i += B) f(vp[i]);
+  // every lane of a wave calls f, with -inf where it has none
+  for (int i = nturn * 4 * B + tid; i - (tid & 63) < nvec; i += B) f(i < nvec ? vp[i] : none);
 }
 // The same downwards; f(index, vector).
 template <int B, typename F>
@@ -81,18 +82,19 @@ __device__ __forceinline__ RowSum sum_elements(const T *p, int n, float c) {
   const int tid = threadIdx.x, off = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
   const int head = min(n, off ? W - off : 0), nvec = (n - head) / W, tail0 = head + nvec * W;
   RowSum st;
-  auto one = [&](float x) {
+  auto one = [&](float x) {   // every lane, -inf where there is none
     const float f[1] = {x};
     st.add(f, fmaxf(x, kRowNegInf), c);
   };
-  vectors_up<B>(reinterpret_cast<const i32x4 *>(p + head), nvec, [&](const i32x4 &v) {
+  constexpr int fill = RowElem<T>::kFill;
+  vectors_up<B>(reinterpret_cast<const i32x4 *>(p + head), nvec, i32x4{fill, fill, fill, fill}, [&](const i32x4 &v) {
     float f[W], g = kRowNegInf;
 #pragma unroll
     for (int e = 0; e < W; ++e) g = fmaxf(g, f[e] = RowElem<T>::get(v, e));
     st.add(f, g, c);
   });
-  if (tid < head) one((float)p[tid]);
-  if (tid < n - tail0) one((float)p[tail0 + tid]);
+  one(tid < head ? (float)p[tid] : kRowNegInf);
+  one(tid < n - tail0 ? (float)p[tail0 + tid] : kRowNegInf);
   return st;
 }
 
@@ -128,13 +130,17 @@ __device__ __forceinline__ float loss_term(float q, float x, float m, float logd
   return q * ((m - x) * itau + logd);
 }
 
-// What the gradient's elements of a row have in common.
+// What the gradient's elements of a row have in common: a 2^{x c - mc}; zeros,
+// whatever x holds, where nothing of the teacher's row is left (dead).
 struct GradRow {
-  float base, c, a;   // a e^{(x - base) c ln 2}
-  bool dead;          // nothing of the teacher's row is left: zeros, whatever x holds
+  float mc, c, a;
+  bool dead;
   __device__ __forceinline__ GradRow(float m, float d, float Q, float c_, float coef)
-      : base(m == kRowNegInf ? 0.f : m), c(c_), a(d == 0.f ? 0.f : coef * Q / d), dead(Q == 0.f) {}
-  __device__ __forceinline__ float operator()(float x) const { return dead ? 0.f : a * ex2((x - base) * c); }
+      : mc(scaled(m, c_)), c(c_), a(d == 0.f ? 0.f : sum_at_max(m, coef * Q / d, c_)), dead(Q == 0.f) {}
+  __device__ __forceinline__ float operator()(float x) const { return a * ex2(__builtin_fmaf(x, c, -mc)); }
+};
+struct ZeroRow {
+  __device__ __forceinline__ float operator()(float) const { return 0.f; }
 };
 
 // Sum of q[j] over the j with ids[j] == id, in order; 0 where an earlier j than k has it.
@@ -197,7 +203,8 @@ __device__ __forceinline__ float sum_rows(const float *loss, int N) {
   return threadIdx.x ? 0.f : (ws[0] + ws[1]) + (ws[2] + ws[3]);
 }
 
-// A wave per row.
+// A wave per row. Latency-bound (a few hundred bytes a row): everything that does
+// not depend on another load is asked for first, two entries a lane (K <= 128).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void top_ce_combine_kernel(TopLogitsCeArgs a, const float *__restrict__ part,
                                                                   int32_t nsplit, int *__restrict__ done) {
@@ -205,35 +212,66 @@ __global__ __launch_bounds__(kThreads) void top_ce_combine_kernel(TopLogitsCeArg
   const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   const float itau = 1.f / a.tau, c = itau * kLog2e;
   if (row < a.N) {
-    RowSum st;
-    for (int sp = lane; sp < nsplit; sp += 64) {
-      const float *p = part + 2 * (row * nsplit + sp);
-      st.merge(p[0], p[1], c);
+    const T *xr = static_cast<const T *>(a.x) + row * a.xs;
+    const float2 *pr = reinterpret_cast<const float2 *>(part) + row * nsplit;
+    float2 p = {kRowNegInf, 0.f};
+    if (lane < nsplit) p = pr[lane];
+    constexpr int kEach = 2;
+    int id[kEach];
+    float t[kEach], xk[kEach], q[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int k = lane + 64 * i;
+      id[i] = k < a.K ? teacher_id(a, row, k) : -1;
+      t[i] = k < a.K ? teacher_value(a, row, k) : kRowNegInf;
     }
-    merge_lanes(st, c);
-    float norm = kRowNegInf, inv = 1.f;
-    if (a.lse) norm = a.lse[row];
-    else {
-      for (int k = lane; k < a.K; k += 64)
+    float norm = a.lse ? a.lse[row] : kRowNegInf;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      xk[i] = id[i] >= 0 ? (float)xr[id[i]] : 0.f;
+      t[i] = id[i] >= 0 ? t[i] : kRowNegInf;
+    }
+    float inv = 1.f;
+    if (!a.lse) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) norm = fmaxf(norm, t[i] * itau);
+      for (int k = lane + 64 * kEach; k < a.K; k += 64)
         if (teacher_id(a, row, k) >= 0) norm = fmaxf(norm, teacher_value(a, row, k) * itau);
 #pragma unroll
       for (int m = 32; m >= 1; m >>= 1) norm = fmaxf(norm, __shfl_xor(norm, m, 64));
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) q[i] = teacher_weight(t[i], id[i], norm, itau);
+    if (!a.lse) {
       float s = 0.f;
-      for (int k = lane; k < a.K; k += 64)
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) s += q[i];
+      for (int k = lane + 64 * kEach; k < a.K; k += 64)
         s += teacher_weight(teacher_value(a, row, k), teacher_id(a, row, k), norm, itau);
 #pragma unroll
       for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
       inv = s == 0.f ? 0.f : 1.f / s;
     }
-    const T *xr = static_cast<const T *>(a.x) + row * a.xs;
-    const float logd = logf(st.d);
+    RowSum st;
+    st.merge(p.x, p.y, c);
+    for (int sp = lane + 64; sp < nsplit; sp += 64) st.merge(pr[sp].x, pr[sp].y, c);
+    merge_lanes(st, c);
+    const float d = sum_at_max(st.m, st.d, c), logd = logf(d);
     float loss = 0.f, Q = 0.f;
-    for (int k = lane; k < a.K; k += 64) {
-      const int id = teacher_id(a, row, k);
-      const float q = teacher_weight(teacher_value(a, row, k), id, norm, itau) * inv;
-      if (a.q) a.q[row * a.K + k] = q;
-      Q += q;
-      if (id >= 0) loss += loss_term(q, (float)xr[id], st.m, logd, itau);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int k = lane + 64 * i;
+      q[i] *= inv;
+      if (a.q && k < a.K) a.q[row * a.K + k] = q[i];
+      Q += q[i];
+      loss += loss_term(q[i], xk[i], st.m, logd, itau);
+    }
+    for (int k = lane + 64 * kEach; k < a.K; k += 64) {
+      const int at = teacher_id(a, row, k);
+      const float w = teacher_weight(teacher_value(a, row, k), at, norm, itau) * inv;
+      if (a.q) a.q[row * a.K + k] = w;
+      Q += w;
+      if (at >= 0) loss += loss_term(w, (float)xr[at], st.m, logd, itau);
     }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) {
@@ -243,7 +281,7 @@ __global__ __launch_bounds__(kThreads) void top_ce_combine_kernel(TopLogitsCeArg
     if (lane == 0) {
       __hip_atomic_store(a.loss + row, a.tau * a.tau * loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       a.stats[row] = st.m;
-      a.stats[a.N + row] = st.d;
+      a.stats[a.N + row] = d;
       a.stats[2 * (int64_t)a.N + row] = Q;
     }
   }
@@ -266,8 +304,8 @@ __global__ __launch_bounds__(kThreads) void top_ce_sum_kernel(const float *__res
 }
 
 // The gradient of the n elements at x to g.
-template <int B, bool NT, typename T>
-__device__ __forceinline__ void write_gradient(const GradRow &gradient, const T *x, T *g, int n) {
+template <int B, bool NT, typename T, typename G>
+__device__ __forceinline__ void write_gradient(const G &gradient, const T *x, T *g, int n) {
   constexpr int W = RowElem<T>::W;
   const int tid = threadIdx.x, off = (int)((reinterpret_cast<uintptr_t>(g) & 15) / sizeof(T));
   const int head = min(n, off ? W - off : 0), nvec = (n - head) / W, tail0 = head + nvec * W;
@@ -316,6 +354,7 @@ __global__ __launch_bounds__(kThreads) void top_ce_bwd_kernel(TopLogitsCeArgs a,
   const GradRow gradient(a.stats[row], a.stats[a.N + row], a.stats[2 * (int64_t)a.N + row], kLog2e / a.tau, coef);
   const T *xr = static_cast<const T *>(a.x) + row * a.xs + c0;
   T *gr = static_cast<T *>(a.grad) + row * a.gs + c0;
+  if (gradient.dead) return write_gradient<kThreads, NT>(ZeroRow(), xr, gr, n);
   write_gradient<kThreads, NT>(gradient, xr, gr, n);
   // the teacher's columns over what was just written
   __syncthreads();
@@ -394,7 +433,7 @@ __global__ __launch_bounds__(kStepThreads, 8) void top_ce_step_kernel(TopLogitsC
   }
   RowSum st = sum_elements<kStepThreads>(xr, a.V, c);
   const float m = group_reduce(st.m, part, true);
-  const float d = group_reduce(st.m == m ? st.d : st.d * ex2((st.m - m) * c), part, false);
+  const float d = sum_at_max(m, group_reduce(sum_at(st, m, c), part, false), c);
   const float logd = logf(d);
   float loss = 0.f;
 #pragma unroll
@@ -403,6 +442,7 @@ __global__ __launch_bounds__(kStepThreads, 8) void top_ce_step_kernel(TopLogitsC
   if (tid == 0) a.loss[n] = a.tau * a.tau * loss;
   const float coef = a.scale * a.tau;
   const GradRow gradient(m, d, Q, c, coef);
+  if (gradient.dead) return write_gradient<kStepThreads, NT>(ZeroRow(), xr, gr, a.V);
   write_gradient<kStepThreads, NT>(gradient, xr, gr, a.V);
   // the teacher's columns over what was just written
   __syncthreads();

@@ -220,8 +220,13 @@ __device__ __forceinline__ void sort_list(RowShared &sh, int n) {
   if (n <= 256) {
     const uint64_t mine = tid < n ? sh.list[tid] : 0;
     int above = 0;
-    if (tid < n)
-      for (int i = 0; i < n; ++i) above += sh.list[i] > mine;
+    if (tid < n) {
+      int i = 0;
+      for (; i + 8 <= n; i += 8)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) above += sh.list[i + u] > mine;
+      for (; i < n; ++i) above += sh.list[i] > mine;
+    }
     __syncthreads();
     if (tid < n) sh.list[above] = mine;
     __syncthreads();
@@ -373,30 +378,54 @@ __device__ uint64_t radix_threshold(const Row<T> &row, RowShared &sh, uint64_t f
   return ties >= in_bin / w ? (uint64_t)key << 32 : column_threshold(row, sh, floor, key, ties);
 }
 
-// A running maximum and sum of exponentials, (m, d = sum e^{(x - m) c ln 2}).
+// A running maximum m and sum d = sum 2^{x c - mc}, mc = m c rounded: one fma an
+// element for the exponent. What the rounding of mc does to d is taken out once, at
+// the end (sum_at_max).
+__device__ __forceinline__ float scaled(float m, float c) { return m == kRowNegInf ? 0.f : m * c; }
 struct RowSum {
-  float m = kRowNegInf, d = 0.f;
-  // elements with the largest of them, g (NaN left out)
+  float m = kRowNegInf, mc = 0.f, d = 0.f;
+  __device__ __forceinline__ void raise(float g, float c) {   // g > m
+    const float n = g * c;
+    if (m != kRowNegInf) d *= __builtin_amdgcn_exp2f(mc - n);
+    m = g;
+    mc = n;
+  }
+  // elements of which g is the largest (NaN left out); every lane of the wave calls
   template <int N>
   __device__ __forceinline__ void add(const float (&x)[N], float g, float c) {
-    if (g > m) {
-      d *= __builtin_amdgcn_exp2f((m - g) * c);   // 0 while m = -inf
-      m = g;
+    if (__ballot(g > m) != 0) {   // seldom after the first vectors
+      if (g > m) raise(g, c);
     }
-    const float base = m == kRowNegInf ? 0.f : m;
+    // four sums side by side: an add waits for the one before it
+    float s[N < 4 ? 1 : 4];
 #pragma unroll
-    for (int i = 0; i < N; ++i) d += __builtin_amdgcn_exp2f((x[i] - base) * c);
+    for (int i = 0; i < N; ++i) {
+      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -mc));
+      if (i < (int)(sizeof(s) / sizeof(float))) s[i] = e;
+      else s[i % (int)(sizeof(s) / sizeof(float))] += e;
+    }
+    if constexpr (N < 4) d += s[0];
+    else d += (s[0] + s[1]) + (s[2] + s[3]);
   }
   __device__ __forceinline__ void merge(float om, float od, float c) {
-    const float n = fmaxf(m, om);
-    if (n != kRowNegInf) {
-      d = d * __builtin_amdgcn_exp2f((m - n) * c) + od * __builtin_amdgcn_exp2f((om - n) * c);
-      m = n;
+    const float omc = scaled(om, c);
+    if (om > m) {
+      d = m == kRowNegInf ? d + od : d * __builtin_amdgcn_exp2f(mc - omc) + od;
+      m = om;
+      mc = omc;
     } else {
-      d += od;   // NaN stays
+      d += om == kRowNegInf ? od : od * __builtin_amdgcn_exp2f(omc - mc);   // od alone: 0 or NaN
     }
   }
 };
+// A part's sum at the whole's maximum m >= st.m.
+__device__ __forceinline__ float sum_at(const RowSum &st, float m, float c) {
+  return st.m == m || st.m == kRowNegInf ? st.d : st.d * __builtin_amdgcn_exp2f(st.mc - scaled(m, c));
+}
+// sum 2^{(x - m) c} from d = sum 2^{x c - mc}
+__device__ __forceinline__ float sum_at_max(float m, float d, float c) {
+  return m == kRowNegInf || m == -kRowNegInf ? d : d * __builtin_amdgcn_exp2f(-__builtin_fmaf(m, c, -scaled(m, c)));
+}
 
 // ---- the first elements in order ------------------------------------------------
 
@@ -406,36 +435,35 @@ struct RowSum {
 // element above a bound are found, and read again, without another pass.
 // With SUM the elements' exponentials are added too.
 constexpr int kGroups = 8;
-template <bool SUM, typename T>
+template <bool SUM, int AHEAD, typename T>
 __device__ __forceinline__ float scan_row(const Row<T> &row, RowShared &sh, int group, float c, RowSum &st) {
   constexpr int W = RowElem<T>::W;
   float *tops = reinterpret_cast<float *>(sh.bins) + threadIdx.x;
   const int nblocks = row.blocks();
   float tmax = fmaxf(row.edge, kRowNegInf), gmax = kRowNegInf;
   if constexpr (SUM) {
-    if (row.ecol >= 0) {
-      const float f[1] = {row.edge};
-      st.add(f, tmax, c);
-    }
+    const float f[1] = {row.edge};   // -inf adds nothing
+    st.add(f, tmax, c);
   }
-  i32x16 q = row.load_block(0);
+  i32x16 q[AHEAD + 1];
+#pragma unroll
+  for (int a = 0; a < AHEAD; ++a)
+    if (a < nblocks) q[a] = row.load_block(a);
   int g = 0, left = group;
 #pragma unroll 1
   for (int b = 0; b < nblocks; ++b) {
-    i32x16 next = q;
-    if (b + 1 < nblocks) next = row.load_block(b + 1);
+    if (b + AHEAD < nblocks) q[AHEAD] = row.load_block(b + AHEAD);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const i32x4 v = {q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]};
-      float f[W];
-      float m = f[0] = RowElem<T>::get(v, 0);
+      const i32x4 v = {q[0][4 * j], q[0][4 * j + 1], q[0][4 * j + 2], q[0][4 * j + 3]};
+      float f[W], m = kRowNegInf;
 #pragma unroll
-      for (int e = 1; e < W; ++e) m = fmaxf(m, f[e] = RowElem<T>::get(v, e));
-      m = fmaxf(m, kRowNegInf);
+      for (int e = 0; e < W; ++e) m = fmaxf(m, f[e] = RowElem<T>::get(v, e));
       gmax = fmaxf(gmax, m);
       if constexpr (SUM) st.add(f, m, c);
     }
-    q = next;
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) q[a] = q[a + 1];
     if (--left == 0 || b == nblocks - 1) {
       tops[g * kRowThreads] = gmax;
       tmax = fmaxf(tmax, gmax);
@@ -454,28 +482,37 @@ int row_group(int32_t V) {
   return (int)((((int64_t)V + block - 1) / block + kGroups - 1) / kGroups);
 }
 
-// f(x, col) of the elements that are >= least, by what scan_row left.
+// f(x, col) of the elements that are >= least, by what scan_row left: each thread
+// goes through its own groups that have one.
 template <typename T, typename F>
 __device__ __forceinline__ void scan_hits(const Row<T> &row, const RowShared &sh, int group, float least, F f) {
   constexpr int W = RowElem<T>::W;
   const float *tops = reinterpret_cast<const float *>(sh.bins) + threadIdx.x;
   const int nblocks = row.blocks(), ngroups = (nblocks + group - 1) / group;
   if (row.ecol >= 0 && row.edge >= least) f(row.edge, row.ecol);
-  for (int g = 0;; ++g) {
-    while (g < ngroups && !(tops[g * kRowThreads] >= least)) ++g;   // each lane to its own next one
-    if (g >= ngroups) break;
+  uint32_t groups = 0;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g)
+    if (g < ngroups && tops[g * kRowThreads] >= least) groups |= 1u << g;
+  while (groups) {
+    const int g = __builtin_ctz(groups);
+    groups &= groups - 1;
     for (int b = g * group; b < min(nblocks, (g + 1) * group); ++b) {
       const i32x16 q = row.load_block(b);
+      uint32_t hits = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int vi = (4 * b + j) * kRowThreads + (int)threadIdx.x;
-        if (vi >= row.nvec) continue;
         const i32x4 v = {q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]};
+        uint32_t h = 0;
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const float x = RowElem<T>::get(v, e);
-          if (x >= least) f(x, row.head + vi * W + e);
-        }
+        for (int e = 0; e < W; ++e) h |= RowElem<T>::get(v, e) >= least ? 1u << e : 0u;
+        if ((4 * b + j) * kRowThreads + (int)threadIdx.x < row.nvec) hits |= h << (j * W);
+      }
+      while (hits) {   // few: read once more instead of picked out of the registers
+        const int i = __builtin_ctz(hits);
+        hits &= hits - 1;
+        const int col = row.head + ((4 * b + i / W) * kRowThreads + (int)threadIdx.x) * W + i % W;
+        f((float)row.p[col], col);
       }
     }
   }

@@ -177,9 +177,8 @@ def top_logits_cross_entropy(student: torch.Tensor, values: torch.Tensor, ids: t
 def top_logits_loss_and_grad(student: torch.Tensor, values: torch.Tensor, ids: torch.Tensor,
                              lse: torch.Tensor | None = None, temperature: float = 1.0, scale: float = 1.0):
     """(loss, grad): top_logits_cross_entropy and ``scale`` times its gradient for
-    ``student``, in the student's dtype and shape, from one pass over the student's
-    logits (rows of up to 163 840 16-bit or 81 920 fp32 logits; longer rows are
-    read twice). For a training step whose loss scale is known:
+    ``student``, in the student's dtype and shape, in one pass over the rows. For a
+    training step whose loss scale is known:
 
         loss, grad = top_logits_loss_and_grad(logits, values, ids, lse, scale=1 / chunks)
         logits.backward(grad)

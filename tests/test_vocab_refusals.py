@@ -44,7 +44,7 @@ def _fwd(lib, step=False, **kw):
 
 COMMON = [dict(x=None), dict(rs=99), dict(n=0), dict(dtype=5), dict(k=0), dict(k=1025, vrs=1025, irs=1025),
           dict(t=0.0), dict(t=float("nan")), dict(ids=None), dict(irs=3), dict(ids=ctypes.c_void_p(68), i64=1),
-          dict(values=None), dict(vrs=3), dict(vd=7), dict(loss=None), dict(sum=None), dict(ws=None)]
+          dict(values=None), dict(vrs=3), dict(vd=7), dict(loss=None), dict(sum=None), dict(ws=None), dict(ws=ctypes.c_void_p(72))]
 
 
 @pytest.mark.parametrize("step", [False, True])
