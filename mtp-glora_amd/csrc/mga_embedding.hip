@@ -297,9 +297,10 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedArgs a, const 
 }
 
 // grid (chunk, slice of 256 columns): where a run begins in the chunk and goes on
-// behind it, the sum of its parts. Four waves take a quarter of the parts each.
+// behind it, the sum of its parts, a share of them a wave.
+constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64;
 template <typename TO, bool VEC, bool ADD>
-__global__ __launch_bounds__(kThreads) void embed_join_kernel(EmbedArgs a, const uint64_t *__restrict__ sorted,
+__global__ __launch_bounds__(kJoinThreads) void embed_join_kernel(EmbedArgs a, const uint64_t *__restrict__ sorted,
                                                               int32_t chunk, const float *__restrict__ part) {
   const int64_t n0 = (int64_t)blockIdx.x * chunk, n1 = n0 + chunk;
   if (n1 >= a.N) return;
@@ -315,9 +316,9 @@ __global__ __launch_bounds__(kThreads) void embed_join_kernel(EmbedArgs a, const
   const int64_t c0 = blockIdx.x, count = (lo - 1) / chunk - c0 + 1;   // slot 1 of c0, slot 0 of the others
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = (blockIdx.y * 64 + lane) * 4;
-  __shared__ f32x4 sums[kThreads / 64][64];
+  __shared__ f32x4 sums[kJoinWaves][64];
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  const int64_t per = (count + 3) / 4, from = wave * per, to = min(count, from + per);
+  const int64_t per = (count + kJoinWaves - 1) / kJoinWaves, from = min(count, wave * per), to = min(count, from + per);
   if (col < a.H) {
     auto slot = [&](int64_t i) {
       return *reinterpret_cast<const f32x4 *>(part + ((c0 + i) * 2 + (i == 0)) * a.part_rs + col);
@@ -343,7 +344,11 @@ __global__ __launch_bounds__(kThreads) void embed_join_kernel(EmbedArgs a, const
   if (wave || col >= a.H) return;
   float f[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) f[e] = (sums[0][lane][e] + sums[1][lane][e]) + (sums[2][lane][e] + sums[3][lane][e]);
+  for (int e = 0; e < 4; ++e) {
+    f[e] = sums[0][lane][e];
+#pragma unroll
+    for (int w = 1; w < kJoinWaves; ++w) f[e] += sums[w][lane][e];
+  }
   put_row<TO, VEC, ADD, 4>(a, id, col, f);
 }
 
@@ -352,7 +357,7 @@ namespace {
 // Sorted tokens a chunk: about a thousand workgroups over all slices.
 int chunk_of(int32_t N, int32_t H, int W) {
   const int64_t slices = ((int64_t)H + kThreads * W - 1) / (kThreads * W);
-  return (int)std::min<int64_t>(kMaxChunk, std::max<int64_t>(8, (int64_t)N * slices / 1024));
+  return (int)std::min<int64_t>(kMaxChunk, std::max<int64_t>(16, (int64_t)N * slices / 1024));
 }
 
 constexpr int64_t kCachedBytes = 200 << 20;   // of dW that are written into the last-level cache
@@ -392,7 +397,7 @@ void bwd_typed(EmbedArgs a, bool add, char *ws, hipStream_t st) {
   const dim3 grid(chunks, (a.H + kThreads * kW<T> - 1) / (kThreads * kW<T>)), join(chunks, (a.H + 255) / 256);
   auto run = [&](auto sum, auto joined) {
     hipLaunchKernelGGL(sum, grid, dim3(kThreads), 0, st, a, sorted, chunk, part);
-    if (chunks > 1) hipLaunchKernelGGL(joined, join, dim3(kThreads), 0, st, a, sorted, chunk, part);
+    if (chunks > 1) hipLaunchKernelGGL(joined, join, dim3(kJoinThreads), 0, st, a, sorted, chunk, part);
   };
   if (add) run(embed_sum_kernel<T, TO, VEC, true>, embed_join_kernel<TO, VEC, true>);
   else run(embed_sum_kernel<T, TO, VEC, false>, embed_join_kernel<TO, VEC, false>);

@@ -24,36 +24,88 @@ namespace mga {
 
 namespace {
 
+// 2^f for |f| <= 1 / 2 by the series of e^{f ln 2}: the rest is below 2^-47 of it.
+__device__ __forceinline__ double exp2_part(double f) {
+  double p = 4.44553827187081e-10;
+  p = __builtin_fma(p, f, 7.054911620801121e-09);
+  p = __builtin_fma(p, f, 1.0178086009239696e-07);
+  p = __builtin_fma(p, f, 1.3215486790144305e-06);
+  p = __builtin_fma(p, f, 1.5252733804059838e-05);
+  p = __builtin_fma(p, f, 0.00015403530393381606);
+  p = __builtin_fma(p, f, 0.0013333558146428441);
+  p = __builtin_fma(p, f, 0.009618129107628477);
+  p = __builtin_fma(p, f, 0.055504108664821576);
+  p = __builtin_fma(p, f, 0.2402265069591007);
+  p = __builtin_fma(p, f, 0.6931471805599453);
+  return __builtin_fma(p, f, 1.0);
+}
+
+constexpr double kTwo52 = 4503599627370496.0;   // added to a smaller number, leaves its nearest whole number in the low bits
+constexpr uint64_t kLow52 = (uint64_t(1) << 52) - 1;
+
 // round(2^s e^{(x - top) / T}) for x <= top; 0 for NaN and -inf.
 struct Weight {
-  float top;
   double topd, c;   // c = log2(e) / T
+  float top;
   int s;
-  __device__ __forceinline__ Weight(float m, float temperature, int bits)
-      : top(m), topd(m), c(1.4426950408889634074 / (double)temperature), s(bits) {}
+  __device__ __forceinline__ Weight(float m, float temperature, int bits) : top(m), s(bits) {
+    c = 1.4426950408889634074 / (double)temperature;
+    if (m == -kRowNegInf) {   // +inf counts as the largest number, and nothing beside it
+      top = 3.402823466e38f;
+      c = 1.0;
+    }
+    topd = (double)top;
+  }
   __device__ __forceinline__ uint64_t operator()(float x) const {
-    if (x == top) return uint64_t(1) << s;   // +inf among them
-    const double a = ((double)x - topd) * c;
-    if (!(a > (double)(-s - 2))) return 0;
-    const double n = __builtin_rint(a), t = (a - n) * 0.69314718055994530942;
-    // e^t, |t| <= ln(2) / 2, by its series: the rest is below 2^-47 of it
-    double p = 1.0 / 39916800;
-    p = __builtin_fma(p, t, 1.0 / 3628800);
-    p = __builtin_fma(p, t, 1.0 / 362880);
-    p = __builtin_fma(p, t, 1.0 / 40320);
-    p = __builtin_fma(p, t, 1.0 / 5040);
-    p = __builtin_fma(p, t, 1.0 / 720);
-    p = __builtin_fma(p, t, 1.0 / 120);
-    p = __builtin_fma(p, t, 1.0 / 24);
-    p = __builtin_fma(p, t, 1.0 / 6);
-    p = __builtin_fma(p, t, 0.5);
-    p = __builtin_fma(p, t, 1.0);
-    p = __builtin_fma(p, t, 1.0);
-    // 2^52 + p 2^{n + s}, rounded to a whole number by the addition
-    const double v = __builtin_amdgcn_ldexp(p, (int)n + s) + 4503599627370496.0;
-    return __builtin_bit_cast(uint64_t, v) & ((uint64_t(1) << 52) - 1);
+    constexpr double kMagic = 1.5 * kTwo52;
+    const float v = x > top ? top : x;              // NaN stays
+    // log2 of the weight; far below 2^-s (and NaN) at a value that rounds to 0
+    const double a = __builtin_fmax(((double)v - topd) * c, (double)(-s - 2));
+    const double m = a + kMagic, f = a - (m - kMagic);   // m: the nearest whole number in its low bits
+    const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, m) + (uint32_t)s;
+    const double w = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, exp2_part(f)) + ((uint64_t)n << 52));
+    return __builtin_bit_cast(uint64_t, w + kTwo52) & kLow52;
   }
 };
+
+// The same for whole rows. A double operation takes 16 cycles a wave here, four
+// times a float one, and they bound the pass: with 2^{i / 256} from LDS seven of
+// them are left of fourteen (32 003 weights a row: 21 -> 12 us).
+struct RowWeight {
+  double c, base;        // 768 + (x - top) c = x c + base: 43 bits of fraction in [512, 1024)
+  float low, top;        // x <= low has no weight
+  const double *roots;   // 2^{i / 256}
+  int s;
+  __device__ __forceinline__ RowWeight(const Weight &w, const double *table) : top(w.top), roots(table), s(w.s) {
+    // c so large that the number below top is 60 to 122 powers of two away: a larger one changes no weight
+    c = fmin(w.c, 1020054733.0 / fabs(w.topd));
+    base = 768.0 - w.topd * c;
+    const double l = w.topd - (s + 3) / c;
+    low = (float)l;
+    if ((double)low > l) low = rank_value((uint64_t)(value_key(low) - 1) << 32);   // the next one down
+  }
+  // x finite (or +inf, which counts as top)
+  __device__ __forceinline__ uint64_t operator()(float x) const {
+    const double m = __builtin_fma((double)fminf(fmaxf(x, low), top), c, base);
+    const uint64_t bits = __builtin_bit_cast(uint64_t, m);
+    const uint32_t hi = (uint32_t)(bits >> 32);   // 12 bits of exponent, 9 of whole part, 11 of fraction
+    const double f = m - __builtin_bit_cast(double, (uint64_t)(hi & ~7u) << 32);   // below 2^-8
+    double p = __builtin_fma(0.009618129107628477, f, 0.055504108664821576);
+    p = __builtin_fma(p, f, 0.2402265069591007);
+    p = __builtin_fma(p, f, 0.6931471805599453);
+    p = __builtin_fma(p, f, 1.0);
+    const uint32_t n = (hi >> 11 & 511u) - 256u + (uint32_t)s;
+    const double r = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, roots[hi >> 3 & 255u]) + ((uint64_t)n << 52));
+    return __builtin_bit_cast(uint64_t, __builtin_fma(r, p, kTwo52)) & kLow52;
+  }
+};
+__device__ __forceinline__ void make_roots(double *roots) {
+  if (threadIdx.x < 256) {
+    const int i = threadIdx.x - (threadIdx.x > 128 ? 256 : 0);
+    roots[threadIdx.x] = exp2_part(i / 256.0) * (threadIdx.x > 128 ? 2.0 : 1.0);
+  }
+  __syncthreads();
+}
 
 // What a running sum has to pass, as a whole number: the first sum >= this is the
 // first > u total. u outside [0, 1) and NaN: the first or the last kept token.
@@ -105,9 +157,11 @@ constexpr uint32_t kBelow = 0x80008000u;
 // Entries in descending order of the value.
 __device__ __forceinline__ int entry_at(int place) { return place < kHalf ? kHalf - 1 - place : place; }
 
-// Weight of a value that is at least `least`, computed.
+constexpr float kLeastNumber = -3.402823466e38f;
+
+// Weight of a value that is at least `least` (a number), computed.
 struct Computed {
-  Weight weight;
+  RowWeight weight;
   float least;
   __device__ __forceinline__ uint64_t operator()(float x) const { return x >= least ? weight(x) : 0; }
 };
@@ -117,28 +171,18 @@ struct Tabulated {
   Weight weight;
   float least;
   Window win;
-  TableShared *tab;
+  const TableShared *tab;
   __device__ __forceinline__ uint64_t operator()(float x) const {
     const uint32_t e = win.entries(__builtin_bit_cast(uint32_t, x) >> 16);
-    return e & 0x8000u ? (x >= least ? weight(x) : 0) : tab->weight[e & (kTable - 1)];
-  }
-  // Values below v have no weight from here on.
-  __device__ __forceinline__ void raise(float v) {
-    least = v;
-#pragma unroll
-    for (int j = 0; j < kPerThread; ++j) {
-      const int e = (int)threadIdx.x + j * kRowThreads;
-      if (win.value(e) < v) tab->weight[e] = 0;
-    }
-    __syncthreads();
+    return !(x >= least) ? 0 : e & 0x8000u ? weight(x) : tab->weight[e & (kTable - 1)];
   }
 };
 
 // The window for values up to weight.top; false where none will do.
 __device__ __forceinline__ bool find_window(const Weight &weight, Window *win) {
-  const double least = weight.topd - (weight.s + 2) / weight.c;   // nothing below it has a weight
+  const double least = (double)weight.top - (weight.s + 2) / weight.c;   // nothing below it has a weight
   const float big = fmaxf(fabsf((float)least), fabsf(weight.top));
-  const uint32_t octave = max((__builtin_bit_cast(uint32_t, big) >> 23) + 1, (uint32_t)kOctaves - 1);
+  const uint32_t octave = max((__builtin_bit_cast(uint32_t, big) >> 23) + 1, (uint32_t)kOctaves);   // zeros stay below it
   win->mag0 = ((octave + 1) << 7) - kHalf;
   return octave <= 254;   // no octave of infinities
 }
@@ -158,10 +202,40 @@ __device__ __forceinline__ void make_table(TableShared &tab, const Weight &weigh
   __syncthreads();
 }
 
+// The rank of the element that is number `ties` by column of the `there` <= kFewTies
+// ones that have this value: they are listed, and each counts those before it.
+constexpr uint32_t kFewTies = 256;
+__device__ __forceinline__ uint64_t tied_threshold(const Row<bf16_t> &row, RowShared &sh, float value, int there,
+                                                   int ties) {
+  uint64_t *list = sh.list;
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+  auto one = [&](float x, int col) {
+    if (x == value) list[atomicAdd(&sh.count, 1)] = (uint32_t)~col;
+  };
+  row.template each_vec<3>([&](const i32x4 &v, int col) {
+    if (col >= row.V) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) one(RowElem<bf16_t>::get(v, e), col + e);
+  }, [](int) {});
+  if (row.ecol >= 0) one(row.edge, row.ecol);
+  __syncthreads();
+  for (int i = threadIdx.x; i < there; i += kRowThreads) {
+    const uint64_t mine = list[i];
+    int above = 0;
+    for (int j = 0; j < there; ++j) above += list[j] > mine;
+    if (above == ties - 1) sh.found[0] = mine;
+  }
+  __syncthreads();
+  const uint64_t col = sh.found[0];
+  __syncthreads();
+  return (uint64_t)value_key(value) << 32 | col;
+}
+
 // Threshold of top_k and top_p by the histogram of the row's values (counted in
 // sh.list), and how many elements it leaves; what scan_row left stays. False where
 // a cut falls among the values below the window.
-__device__ bool table_threshold(const Row<bf16_t> &row, RowShared &sh, TableShared &tab, const Tabulated &t, bool by_k,
+__device__ __forceinline__ bool table_threshold(const Row<bf16_t> &row, RowShared &sh, TableShared &tab, const Tabulated &t, bool by_k,
                                 uint64_t top_k, bool by_p, float top_p, uint64_t *thr, uint64_t *kept) {
   const int tid = threadIdx.x;
   static_assert(sizeof(sh.list) >= kTable * sizeof(uint32_t), "the counts");
@@ -178,7 +252,7 @@ __device__ bool table_threshold(const Row<bf16_t> &row, RowShared &sh, TableShar
     atomicAdd((unsigned long long *)&tab.small_weight,
               (unsigned long long)t.weight(__builtin_bit_cast(float, bits << 16)));
   };
-  row.each_vec([&](const i32x4 &v, int col, int) {
+  row.template each_vec<3>([&](const i32x4 &v, int col) {
     if (col >= row.V) return;
     uint32_t e[4], below = 0;
 #pragma unroll
@@ -193,7 +267,7 @@ __device__ bool table_threshold(const Row<bf16_t> &row, RowShared &sh, TableShar
       tally(e[d] & 0xFFFFu);
       tally(e[d] >> 16);
     }
-  });
+  }, [](int) {});
   if (row.ecol >= 0) one(__builtin_bit_cast(uint32_t, row.edge) >> 16);
   __syncthreads();
   // a thread's entries, in descending order; the values below the window stand
@@ -267,10 +341,13 @@ __device__ bool table_threshold(const Row<bf16_t> &row, RowShared &sh, TableShar
     if (cut < 0) return false;
   }
   if (cut == kTable) return true;
-  const uint32_t key = value_key(t.win.value(entry_at(cut)));
+  const float value = t.win.value(entry_at(cut));
+  const uint64_t key = (uint64_t)value_key(value) << 32;
   const uint32_t there = count[entry_at(cut)];
   __syncthreads();   // the counts are over
-  *thr = ties >= there ? (uint64_t)key << 32 : column_threshold(row, sh, 0, key, ties);
+  if (ties >= there) *thr = key;
+  else *thr = there > kFewTies ? column_threshold(row, sh, 0, (uint32_t)(key >> 32), ties)
+                               : tied_threshold(row, sh, value, (int)there, (int)ties);
   return true;
 }
 
@@ -280,7 +357,7 @@ __device__ bool table_threshold(const Row<bf16_t> &row, RowShared &sh, TableShar
 // reaches its target, among the n <= kListCap ranks of sh.list: columns by two
 // digits of ten bits.
 template <typename WF>
-__device__ int pick_in_list(RowShared &sh, int n, const WF &weight, float u) {
+__device__ __forceinline__ int pick_in_list(RowShared &sh, int n, const WF &weight, float u) {
   constexpr int kEach = kListCap / kRowThreads;
   const int tid = threadIdx.x;
   __syncthreads();
@@ -352,10 +429,11 @@ __device__ __forceinline__ uint64_t vector_sum(const Tabulated &t, const i32x4 &
   uint32_t e[4], below = 0;
   uint64_t s = 0;
 #pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    below |= e[d] = t.win.entries((uint32_t)v[d]);
-    s += t.tab->weight[e[d] & (kTable - 1)] + t.tab->weight[e[d] >> 16 & (kTable - 1)];
-  }
+  for (int d = 0; d < 4; ++d) below |= e[d] = t.win.entries((uint32_t)v[d]);
+  // a random read of LDS by 64 lanes takes some 20 cycles, by few of them less
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (RowElem<T>::get(v, i) >= t.least) s += t.tab->weight[(e[i >> 1] >> (i & 1) * 16) & (kTable - 1)];
   if (below & kBelow) {
     s = 0;
 #pragma unroll 1
@@ -366,31 +444,34 @@ __device__ __forceinline__ uint64_t vector_sum(const Tabulated &t, const i32x4 &
 
 // The same among all elements of at least `thr`. `weight` is 0 for smaller values.
 template <typename T, typename WF>
-__device__ int pick_in_row(const Row<T> &row, RowShared &sh, uint64_t thr, const WF &weight, float u) {
+__device__ __forceinline__ int pick_in_row(const Row<T> &row, RowShared &sh, uint64_t thr, const WF &weight, float u) {
   constexpr int W = RowElem<T>::W;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // of the elements equal to least, the last column that counts
   const int last = (uint32_t)thr ? rank_col(thr) : row.V;
   auto kept = [&](float x, int col) { return x == weight.least && col > last ? uint64_t(0) : weight(x); };
+  const uint64_t tie = weight(weight.least);
   auto lane_sum = [&](const i32x4 &v, int col) {
-    uint64_t s = 0;
+    uint64_t s = vector_sum<T>(weight, v);   // 0 of the -inf past the row's end
     if (col + W - 1 > last) {
-      if (col < row.V) {
-#pragma unroll 1
-        for (int e = 0; e < W; ++e) s += kept(RowElem<T>::get(v, e), col + e);
-      }
-    } else {
-      s = vector_sum<T>(weight, v);
+      int out = 0;
+#pragma unroll
+      for (int e = 0; e < W; ++e) out += RowElem<T>::get(v, e) == weight.least && col + e > last;
+      s -= (uint64_t)out * tie;
     }
     return s;
   };
-  // in order of the columns: the elements before the vectors, (vector, wave)
-  // groups, the elements behind them
-  row.each_vec([&](const i32x4 &v, int col, int i) {
-    uint64_t s = lane_sum(v, col);
-    if (__ballot(s != 0) != 0) s = wave_scan(s);
-    if (lane == 63) sh.bins[i * kRowWaves + wave] = s;
-  });
+  // In order of the columns: the elements before the vectors, the (vector, wave)
+  // groups, the elements behind them; within a group its lanes, within a lane its
+  // elements.
+  int i = 0;
+  row.template each_vec<3>(
+      [&](const i32x4 &v, int col) {
+        const uint64_t s = last_lane(wave_scan(lane_sum(v, col)));
+        if (lane == 0) sh.bins[i * kRowWaves + wave] = s;
+        ++i;
+      },
+      [](int) {});
   const uint64_t mine = row.ecol >= 0 ? kept(row.edge, row.ecol) : 0;
   const uint64_t edges = wave_scan(mine);
   if (wave == 0 && lane == W - 1) sh.found[0] = edges;
@@ -398,7 +479,7 @@ __device__ int pick_in_row(const Row<T> &row, RowShared &sh, uint64_t thr, const
   __syncthreads();
   const uint64_t before = sh.found[0], behind = sh.found[1] - before;
   __syncthreads();
-  const int groups = row.blocks() * 4 * kRowWaves;
+  const int groups = row.blocks() * 4 * kRowWaves;   // at most kBins
   const int per = (groups + kRowThreads - 1) / kRowThreads, g0 = min(groups, tid * per), g1 = min(groups, g0 + per);
   uint64_t s = 0, total;
   for (int g = g0; g < g1; ++g) s += sh.bins[g];
@@ -432,10 +513,10 @@ __device__ int pick_in_row(const Row<T> &row, RowShared &sh, uint64_t thr, const
       if (upto >= want && upto - in < want) {
         uint64_t run = upto - in;
         int token = -1;
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
+#pragma unroll 1
+        for (int e = 0; e < W && token < 0; ++e) {
           run += kept(RowElem<T>::get(v, e), col + e);
-          if (token < 0 && run >= want) token = col + e;
+          if (run >= want) token = col + e;
         }
         sh.count = token;
       }
@@ -449,8 +530,9 @@ __device__ int pick_in_row(const Row<T> &row, RowShared &sh, uint64_t thr, const
 }
 
 // LDS of a type's kernel: the table for bf16.
-template <typename T> struct SampleShared : RowShared {};
-template <> struct SampleShared<bf16_t> : RowShared { TableShared tab; };
+struct SampleBase : RowShared { double roots[256]; };
+template <typename T> struct SampleShared : SampleBase {};
+template <> struct SampleShared<bf16_t> : SampleBase { TableShared tab; };
 
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict__ x, int64_t xs, int32_t V,
@@ -467,7 +549,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict
   Row<T> row;
   row.load(x + n * xs, V);
   RowSum none;
-  const float tmax = scan_row<false, 2>(row, sh, group, 0.f, none), top = block_max(tmax, sh);
+  const float tmax = scan_row<false, 5>(row, sh, group, 0.f, none), top = block_max(tmax, sh);
   if (top == kRowNegInf) {   // nothing to draw from
     if (tid == 0) token[n] = -1;
     return;
@@ -489,14 +571,20 @@ __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict
     if ((double)least < b) least = rank_value((uint64_t)(value_key(least) + 1) << 32);   // the next one up
   }
   const bool by_k = top_k > 0 && top_k < V, by_p = top_p < 1.f;
-  int t;
+  int t = -1;
   if (by_k && top_k <= kMaxTop) {
     top_list(row, sh, group, tmax, top_k);
     // thread i has the i-th element in order; the kept ones are the first ones
     const uint64_t r = tid < top_k ? sh.list[tid] : 0;
     const uint64_t w = tid < top_k && by_p ? weight(rank_value(r)) : 0;
     uint64_t total = 0, before = 0;
-    if (by_p) before = block_scan(w, sh, &total);
+    if (by_p && top_k <= 64) {   // the first wave has them
+      before = wave_scan(w);
+      total = __shfl(before, 63, 64);
+      before -= w;
+    } else if (by_p) {
+      before = block_scan(w, sh, &total);
+    }
     const bool keep = tid < top_k && (tid == 0 || ((!by_p || before < mass_needed(top_p, total)) && rank_value(r) >= least));
     t = pick_in_list(sh, __syncthreads_count(keep), weight, u);
   } else {
@@ -521,41 +609,40 @@ __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict
       thr = floor;
       listed = gather();
     }
-    auto threshold = [&]() {   // digit by digit
+    // bf16: by the table (up to kTable columns, their own weights are no more work)
+    bool tabulated = false, found = false;
+    Window win;
+    if constexpr (sizeof(SampleShared<T>) > sizeof(SampleBase)) {
+      if (listed > kListCap && top < -kRowNegInf && V > kTable && find_window(weight, &win)) {
+        tabulated = true;
+        make_table(sh.tab, weight, win);
+        found = !by_k && !by_p;
+        if (!found) {
+          const Tabulated tw{weight, kRowNegInf, win, &sh.tab};
+          found = table_threshold(row, sh, sh.tab, tw, by_k, top_k, by_p, top_p, &thr, &kept);
+          thr = max(thr, floor);
+          if (found && kept <= kListCap && thr >> 32 > 1) listed = gather();
+        }
+      }
+    }
+    const Computed row_weight{RowWeight(weight, sh.roots), kLeastNumber};
+    if (listed > kListCap && !(tabulated && found)) make_roots(sh.roots);
+    if (listed > kListCap && !found) {   // digit by digit
+      thr = 0;
       if (by_k)
         thr = radix_threshold<true>(row, sh, 0, [](float) { return uint64_t(1); },
                                     [&](uint64_t) { return (uint64_t)top_k; });
       if (by_p)
-        thr = radix_threshold<false>(row, sh, thr, weight, [&](uint64_t total) { return mass_needed(top_p, total); });
+        thr = radix_threshold<false>(row, sh, thr, row_weight, [&](uint64_t total) { return mass_needed(top_p, total); });
       thr = max(thr, floor);
-    };
-    bool done = listed <= kListCap;
-    if (done) t = pick_in_list(sh, listed, weight, u);
-    if constexpr (sizeof(SampleShared<T>) > sizeof(RowShared)) {
-      // up to kTable columns, their own weights are no more work than the table's
-      Window win;
-      if (!done && top < -kRowNegInf && V > kTable && find_window(weight, &win)) {
-        make_table(sh.tab, weight, win);
-        Tabulated tw{weight, kRowNegInf, win, &sh.tab};
-        bool found = true;
-        if (by_k || by_p) {
-          found = table_threshold(row, sh, sh.tab, tw, by_k, top_k, by_p, top_p, &thr, &kept);
-          if (!found) threshold();
-          thr = max(thr, floor);
-          if (found && kept <= kListCap && thr >> 32 > 1) listed = gather();
-        }
-        if (listed <= kListCap) {
-          t = pick_in_list(sh, listed, tw, u);
-        } else {
-          if (thr >> 32 > 1) tw.raise(rank_value(thr));
-          t = pick_in_row(row, sh, thr, tw, u);
-        }
-        done = true;
-      }
     }
-    if (!done) {
-      threshold();
-      t = pick_in_row(row, sh, thr, Computed{weight, thr >> 32 > 1 ? rank_value(thr) : kRowNegInf}, u);
+    const float low = thr >> 32 > 1 ? rank_value(thr) : kRowNegInf;
+    if (listed <= kListCap) {
+      t = pick_in_list(sh, listed, weight, u);
+    } else if (!tabulated) {
+      t = pick_in_row(row, sh, thr, Computed{row_weight.weight, fmaxf(low, kLeastNumber)}, u);
+    } else if constexpr (sizeof(SampleShared<T>) > sizeof(SampleBase)) {
+      t = pick_in_row(row, sh, thr, Tabulated{weight, low, win, &sh.tab}, u);
     }
   }
   if (tid == 0) token[n] = t;

@@ -24,12 +24,12 @@ __global__ __launch_bounds__(kRowThreads, 8) void top_logits_kernel(const T *__r
   const float c = itau * kLog2e;
   float tmax;
   if (lse) {
-    tmax = scan_row<true, 1>(row, sh, group, c, st);
+    tmax = scan_row<true, 2>(row, sh, group, c, st);
     const float m = block_max(st.m, sh);
     const float d = block_sum(sum_at(st, m, c), sh);
     if (threadIdx.x == 0) lse[n] = m == -kRowNegInf ? m : m * itau + logf(sum_at_max(m, d, c));
   } else {
-    tmax = scan_row<false, 1>(row, sh, group, c, st);
+    tmax = scan_row<false, 2>(row, sh, group, c, st);
   }
   top_list(row, sh, group, tmax, k);
   if ((int)threadIdx.x < k) {

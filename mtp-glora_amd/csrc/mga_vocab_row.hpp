@@ -109,36 +109,42 @@ struct Row {
   // blocks of four vectors a thread that hold the row's vectors
   __device__ __forceinline__ int blocks() const { return (nvec + 4 * kRowThreads - 1) / (4 * kRowThreads); }
 
-  // f(v, col, i): the i-th vector of every thread (all lanes take part; a thread
-  // without one has -inf and a column of at least V), in ascending order of i. The
-  // next block is on its way meanwhile.
-  template <typename F>
-  __device__ __forceinline__ void each_vec(F f) const {
+  // f(v, col): every thread's vectors in ascending order (all lanes take part; a
+  // thread without one has -inf and a column of at least V); last(b) behind the
+  // vectors of block b. K blocks are asked for before the first is used: a row is
+  // few blocks, and each wait for memory is about 2 600 cycles.
+  template <int K, typename F, typename L>
+  __device__ __forceinline__ void each_vec(F f, L last) const {
     const int n = blocks();
-    i32x16 q = load_block(0);
 #pragma unroll 1
-    for (int b = 0; b < n; ++b) {
-      i32x16 next = q;
-      if (b + 1 < n) next = load_block(b + 1);
+    for (int b0 = 0; b0 < n; b0 += K) {
+      i32x16 q[K];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = 4 * b + j, vi = i * kRowThreads + (int)threadIdx.x;
-        const i32x4 v = {q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]};
-        f(v, vi < nvec ? head + vi * W : V, i);
+      for (int k = 0; k < K; ++k)
+        if (b0 + k < n) q[k] = load_block(b0 + k);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (b0 + k >= n) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int vi = (4 * (b0 + k) + j) * kRowThreads + (int)threadIdx.x;
+          const i32x4 v = {q[k][4 * j], q[k][4 * j + 1], q[k][4 * j + 2], q[k][4 * j + 3]};
+          f(v, vi < nvec ? head + vi * W : V);
+        }
+        last(b0 + k);
       }
-      q = next;
     }
   }
 
   // f(x, col) of every element that there is.
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    each_vec([&](const i32x4 &v, int col, int) {
+    each_vec<1>([&](const i32x4 &v, int col) {
       if (col < V) {
 #pragma unroll
         for (int e = 0; e < W; ++e) f(RowElem<T>::get(v, e), col + e);
       }
-    });
+    }, [](int) {});
     if (ecol >= 0) f(edge, ecol);
   }
 };
@@ -157,36 +163,68 @@ struct RowShared : RowPart {
   int count;
 };
 
-template <typename F>
-__device__ __forceinline__ float block_reduce(float v, RowPart &sh, F op) {
+// A value of another lane, by data-parallel operands (no LDS crossbar): `old` where
+// there is none. kShr<n>: n lanes down in the row of 16; kLast15 / kLast31: the last
+// lane of the row / of the half before, to the rows of MASK.
+constexpr int kShr = 0x110, kLast15 = 0x142, kLast31 = 0x143;
+template <int CTRL, int MASK = 0xF>
+__device__ __forceinline__ uint32_t dpp(uint32_t old, uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, MASK, 0xF, false);
+}
+template <int CTRL, int MASK = 0xF>
+__device__ __forceinline__ uint64_t dpp_add(uint64_t v) {
+  return v + ((uint64_t)dpp<CTRL, MASK>(0u, (uint32_t)(v >> 32)) << 32 | dpp<CTRL, MASK>(0u, (uint32_t)v));
+}
+template <int CTRL, int MASK, typename F>
+__device__ __forceinline__ float dpp_op(float v, F op) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  return op(v, __builtin_bit_cast(float, dpp<CTRL, MASK>(b, b)));
+}
+
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {   // inclusive; all lanes active
+  v = dpp_add<kShr + 1>(v);
+  v = dpp_add<kShr + 2>(v);
+  v = dpp_add<kShr + 4>(v);
+  v = dpp_add<kShr + 8>(v);
+  v = dpp_add<kLast15, 0xA>(v);
+  return dpp_add<kLast31, 0xC>(v);
+}
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+__device__ __forceinline__ float block_max(float v, RowPart &sh) {
+  auto op = [](float a, float b) { return fmaxf(a, b); };
+  v = dpp_op<kShr + 1, 0xF>(v, op);
+  v = dpp_op<kShr + 2, 0xF>(v, op);
+  v = dpp_op<kShr + 4, 0xF>(v, op);
+  v = dpp_op<kShr + 8, 0xF>(v, op);
+  v = dpp_op<kLast15, 0xA>(v, op);
+  v = dpp_op<kLast31, 0xC>(v, op);
+  if ((threadIdx.x & 63) == 63) sh.fpart[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = sh.fpart[0];
 #pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v = op(v, __shfl_xor(v, m, 64));
+  for (int w = 1; w < kRowWaves; ++w) v = fmaxf(v, sh.fpart[w]);
+  __syncthreads();
+  return v;
+}
+__device__ __forceinline__ float block_sum(float v, RowPart &sh) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
   if ((threadIdx.x & 63) == 0) sh.fpart[threadIdx.x >> 6] = v;
   __syncthreads();
   v = sh.fpart[0];
 #pragma unroll
-  for (int w = 1; w < kRowWaves; ++w) v = op(v, sh.fpart[w]);
+  for (int w = 1; w < kRowWaves; ++w) v += sh.fpart[w];
   __syncthreads();
   return v;
 }
-__device__ __forceinline__ float block_max(float v, RowPart &sh) {
-  return block_reduce(v, sh, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float block_sum(float v, RowPart &sh) {
-  return block_reduce(v, sh, [](float a, float b) { return a + b; });
-}
 
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
-  const uint32_t lo = __shfl_up((uint32_t)v, d, 64), hi = __shfl_up((uint32_t)(v >> 32), d, 64);
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
+  const uint32_t lo = __shfl_xor((uint32_t)v, m, 64), hi = __shfl_xor((uint32_t)(v >> 32), m, 64);
   return (uint64_t)hi << 32 | lo;
-}
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {   // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t o = shfl_up64(v, d);
-    if ((int)(threadIdx.x & 63) >= d) v += o;
-  }
-  return v;
 }
 // Sum of v over the threads before this one and (*total) over all of them.
 __device__ __forceinline__ uint64_t block_scan(uint64_t v, RowShared &sh, uint64_t *total) {
@@ -206,35 +244,32 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, RowShared &sh, uint64
   return before + in - v;
 }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
-  const uint32_t lo = __shfl_xor((uint32_t)v, m, 64), hi = __shfl_xor((uint32_t)(v >> 32), m, 64);
-  return (uint64_t)hi << 32 | lo;
-}
-
 // sh.list[0, n) in descending order. Up to 256 entries by counting those above
-// each (n broadcast reads a thread); up to 1 024 by a bitonic network with an
-// entry a thread, whose steps within a wave need no barrier; more by one in LDS.
+// each, by all threads (360: 22 000 cycles, 16 000 by the network); up to 1 024 by a bitonic network with an entry a thread,
+// whose steps within a wave need no barrier; more by one in LDS. Uses sh.bins.
 __device__ __forceinline__ void sort_list(RowShared &sh, int n) {
   const int tid = threadIdx.x;
   __syncthreads();
   if (n <= 256) {
-    const uint64_t mine = tid < n ? sh.list[tid] : 0;
-    int above = 0;
-    if (tid < n) {
-      int i = 0;
-      for (; i + 8 <= n; i += 8)
+    const int wide = n <= 128 ? 128 : 256, mine = tid & (wide - 1), parts = kRowThreads / wide;
+    uint32_t *above = reinterpret_cast<uint32_t *>(sh.bins);
+    if (tid < wide) above[tid] = 0;
+    const uint64_t v = mine < n ? sh.list[mine] : 0;
+    const int per = (n + parts - 1) / parts, i0 = tid / wide * per, i1 = min(n, i0 + per);
+    int count = 0;
+    for (int i = i0; i < i1; i += 8)
 #pragma unroll
-        for (int u = 0; u < 8; ++u) above += sh.list[i + u] > mine;
-      for (; i < n; ++i) above += sh.list[i] > mine;
-    }
+      for (int u = 0; u < 8; ++u) count += i + u < i1 && sh.list[i + u] > v;
     __syncthreads();
-    if (tid < n) sh.list[above] = mine;
+    if (mine < n) atomicAdd(&above[mine], (uint32_t)count);
+    __syncthreads();
+    if (tid < n) sh.list[above[tid]] = v;
     __syncthreads();
     return;
   }
-  int size = 512;
+  int size = 1024;
   while (size < n) size <<= 1;
-  if (size <= kRowThreads) {
+  if (size == kRowThreads) {
     uint64_t v = tid < n ? sh.list[tid] : 0;
     for (int k = 2; k <= size; k <<= 1)
       for (int j = k >> 1; j > 0; j >>= 1) {
@@ -317,7 +352,7 @@ __device__ __forceinline__ void find_bin(RowShared &sh, const uint64_t *bins, in
 // The rank of the element that is number `ties` by column among those of `key` (and
 // of at least `floor`): more than that have the key. Uses sh.list.
 template <typename T>
-__device__ uint64_t column_threshold(const Row<T> &row, RowShared &sh, uint64_t floor, uint32_t key, uint64_t ties) {
+__device__ __forceinline__ uint64_t column_threshold(const Row<T> &row, RowShared &sh, uint64_t floor, uint32_t key, uint64_t ties) {
   uint32_t prefix = 0;
   uint64_t total;
   for (int shift = 20; shift > 0; shift -= 10) {
@@ -341,7 +376,7 @@ __device__ uint64_t column_threshold(const Row<T> &row, RowShared &sh, uint64_t 
 // number that depends on the value alone. Digits of the key from the top, 12
 // bits at first, then of the columns of the elements that share the last key.
 template <bool ONES, typename T, typename WF, typename NF>
-__device__ uint64_t radix_threshold(const Row<T> &row, RowShared &sh, uint64_t floor, WF weight, NF need) {
+__device__ __forceinline__ uint64_t radix_threshold(const Row<T> &row, RowShared &sh, uint64_t floor, WF weight, NF need) {
   uint64_t want = 0, total = 0;
   uint32_t prefix = 0;
   int shift = 32;
@@ -435,7 +470,7 @@ __device__ __forceinline__ float sum_at_max(float m, float d, float c) {
 // element above a bound are found, and read again, without another pass.
 // With SUM the elements' exponentials are added too.
 constexpr int kGroups = 8;
-template <bool SUM, int AHEAD, typename T>
+template <bool SUM, int K, typename T>
 __device__ __forceinline__ float scan_row(const Row<T> &row, RowShared &sh, int group, float c, RowSum &st) {
   constexpr int W = RowElem<T>::W;
   float *tops = reinterpret_cast<float *>(sh.bins) + threadIdx.x;
@@ -445,33 +480,23 @@ __device__ __forceinline__ float scan_row(const Row<T> &row, RowShared &sh, int 
     const float f[1] = {row.edge};   // -inf adds nothing
     st.add(f, tmax, c);
   }
-  i32x16 q[AHEAD + 1];
-#pragma unroll
-  for (int a = 0; a < AHEAD; ++a)
-    if (a < nblocks) q[a] = row.load_block(a);
   int g = 0, left = group;
-#pragma unroll 1
-  for (int b = 0; b < nblocks; ++b) {
-    if (b + AHEAD < nblocks) q[AHEAD] = row.load_block(b + AHEAD);
+  row.template each_vec<K>(
+      [&](const i32x4 &v, int) {
+        float f[W], m = kRowNegInf;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const i32x4 v = {q[0][4 * j], q[0][4 * j + 1], q[0][4 * j + 2], q[0][4 * j + 3]};
-      float f[W], m = kRowNegInf;
-#pragma unroll
-      for (int e = 0; e < W; ++e) m = fmaxf(m, f[e] = RowElem<T>::get(v, e));
-      gmax = fmaxf(gmax, m);
-      if constexpr (SUM) st.add(f, m, c);
-    }
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) q[a] = q[a + 1];
-    if (--left == 0 || b == nblocks - 1) {
-      tops[g * kRowThreads] = gmax;
-      tmax = fmaxf(tmax, gmax);
-      gmax = kRowNegInf;
-      left = group;
-      ++g;
-    }
-  }
+        for (int e = 0; e < W; ++e) m = fmaxf(m, f[e] = RowElem<T>::get(v, e));
+        gmax = fmaxf(gmax, m);
+        if constexpr (SUM) st.add(f, m, c);
+      },
+      [&](int b) {
+        if (--left != 0 && b != nblocks - 1) return;
+        tops[g * kRowThreads] = gmax;
+        tmax = fmaxf(tmax, gmax);
+        gmax = kRowNegInf;
+        left = group;
+        ++g;
+      });
   return tmax;
 }
 
@@ -526,7 +551,7 @@ __device__ __forceinline__ void scan_hits(const Row<T> &row, const RowShared &sh
 // ordinary rows few more: those are taken into LDS and put in order there. A row
 // with too many of them (equal values) has its threshold found digit by digit.
 template <typename T>
-__device__ void top_list(const Row<T> &row, RowShared &sh, int group, float tmax, int k) {
+__device__ __forceinline__ void top_list(const Row<T> &row, RowShared &sh, int group, float tmax, int k) {
   const int tid = threadIdx.x, lane = tid & 63;
   float v = tmax;
 #pragma unroll
