@@ -898,7 +898,7 @@ int64_t step_stats_at(int32_t n_rows, int32_t n_cols) {
 int check_embedding(const char *fn, const void *ids, int32_t ids64, int32_t n, int32_t n_rows, int32_t width,
                     int32_t dtype) {
   if (!elem_bytes(dtype)) return fail(MGA_ERR_INVALID, "%s: unknown dtype code %d", fn, dtype);
-  if (n < 0 || n_rows <= 0 || width <= 0)
+  if (n < 0 || n_rows <= 0 || width <= 0 || width > 1 << 23)
     return fail(MGA_ERR_INVALID, "%s: bad sizes (ids=%d rows=%d width=%d)", fn, n, n_rows, width);
   if (n > 0 && (!ids || reinterpret_cast<uintptr_t>(ids) % (ids64 ? 8 : 4)))
     return fail(MGA_ERR_INVALID, "%s: ids null or not aligned to their elements", fn);

@@ -103,26 +103,35 @@ __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(EmbedArgs a, int32_
   }
 }
 
-// Clears [V, H] (row stride rs) a row a wave at a time.
-template <typename TO, bool VEC, bool NT>
+// Clears [V, H] (row stride rs): kClear bytes a workgroup where the rows follow each
+// other, 16 KB at a time (1.24 GB: 204 us, 6.1 TB/s; past the cache or by workgroups
+// that go on to a next part 210 to 350 us), else a row a wave.
+constexpr int64_t kClear = 16 * 16 * kSortThreads;
+template <typename TO, bool VEC>
 __device__ __forceinline__ void clear_rows(TO *out, int64_t rs, int32_t V, int32_t H, int64_t block, int64_t blocks) {
+  const i32x4 zero = {0, 0, 0, 0};
+  if (VEC && rs == H) {
+    const int64_t n = (int64_t)V * H * (int64_t)sizeof(TO) / 16;
+    i32x4 *o = reinterpret_cast<i32x4 *>(out);
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      const int64_t i = (block * 16 + u) * kSortThreads + threadIdx.x;
+      if (i < n) o[i] = zero;
+    }
+    return;
+  }
   const int lane = threadIdx.x & 63;
   for (int64_t v = block * (kSortThreads / 64) + (threadIdx.x >> 6); v < V; v += blocks * (kSortThreads / 64)) {
     TO *o = out + v * rs;
     if constexpr (VEC) {
-      const i32x4 zero = {0, 0, 0, 0};
-#pragma unroll 4
-      for (int c = lane * kW<TO>; c < H; c += 64 * kW<TO>) {
-        if constexpr (NT) __builtin_nontemporal_store(zero, reinterpret_cast<i32x4 *>(o + c));
-        else *reinterpret_cast<i32x4 *>(o + c) = zero;
-      }
+      for (int c = lane * kW<TO>; c < H; c += 64 * kW<TO>) *reinterpret_cast<i32x4 *>(o + c) = zero;
     } else {
       for (int c = lane; c < H; c += 64) o[c] = (TO)0.f;
     }
   }
 }
 
-template <typename TO, bool VEC, bool NT>
+template <typename TO, bool VEC>
 __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a, int32_t tiles, bool clear,
                                                                   uint64_t *__restrict__ sorted) {
   __shared__ uint64_t key[kTile];
@@ -130,7 +139,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a, i
   const int tid = threadIdx.x;
   if ((int)blockIdx.x >= tiles) {
     if (clear)
-      clear_rows<TO, VEC, NT>(static_cast<TO *>(a.out), a.out_rs, a.V, a.H, blockIdx.x - tiles, gridDim.x - tiles);
+      clear_rows<TO, VEC>(static_cast<TO *>(a.out), a.out_rs, a.V, a.H, blockIdx.x - tiles, gridDim.x - tiles);
     return;
   }
   const int64_t n0 = (int64_t)blockIdx.x * kTile;
@@ -296,60 +305,72 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedArgs a, const 
   }
 }
 
-// grid (chunk, slice of 256 columns): where a run begins in the chunk and goes on
-// behind it, the sum of its parts, a share of them a wave.
-constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64;
+// grid (kLook chunks, slice of 256 columns): where a run begins in a chunk and goes on
+// behind it, the sum of its parts, shared by the waves. Most chunks have no such run:
+// a workgroup looks at several, since those that end at once cost their dispatch
+// (6 144 tokens x 2 560 and 5 120 x 4 096: four chunks 9.8 and 9.9 us, two 10.3 and
+// 13.0, eight 11.9 and 11.2, sixteen waves 16.7 and 18.9).
+constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64, kLook = 4;
 template <typename TO, bool VEC, bool ADD>
 __global__ __launch_bounds__(kJoinThreads) void embed_join_kernel(EmbedArgs a, const uint64_t *__restrict__ sorted,
-                                                              int32_t chunk, const float *__restrict__ part) {
-  const int64_t n0 = (int64_t)blockIdx.x * chunk, n1 = n0 + chunk;
-  if (n1 >= a.N) return;
-  const uint32_t id = id_at(sorted, n1);
-  if (id == kNoId || id_at(sorted, n1 - 1) != id) return;
-  if (n0 > 0 && id_at(sorted, n0) == id && id_at(sorted, n0 - 1) == id) return;   // began further back
-  int64_t lo = n1, hi = a.N;   // the run's end
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (id_at(sorted, mid) <= id) lo = mid + 1;
-    else hi = mid;
-  }
-  const int64_t c0 = blockIdx.x, count = (lo - 1) / chunk - c0 + 1;   // slot 1 of c0, slot 0 of the others
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = (blockIdx.y * 64 + lane) * 4;
+                                                                  int32_t chunk, const float *__restrict__ part) {
   __shared__ f32x4 sums[kJoinWaves][64];
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  const int64_t per = (count + kJoinWaves - 1) / kJoinWaves, from = min(count, wave * per), to = min(count, from + per);
-  if (col < a.H) {
-    auto slot = [&](int64_t i) {
-      return *reinterpret_cast<const f32x4 *>(part + ((c0 + i) * 2 + (i == 0)) * a.part_rs + col);
-    };
-    int64_t i = from;
-    for (; i + 8 <= to; i += 8) {
-      f32x4 f[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) f[u] = slot(i + u);
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] += f[u][e];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.y * 256 + lane * 4;
+  const int64_t chunks = ((int64_t)a.N + chunk - 1) / chunk, first = (int64_t)blockIdx.x * kLook;
+  auto goes_on = [&](int64_t c) {   // the run at the end of chunk c
+    const int64_t at = (c + 1) * chunk;
+    const uint32_t id = id_at(sorted, at);
+    if (id == kNoId || id_at(sorted, at - 1) != id) return false;
+    const int64_t n0 = c * chunk;
+    return !(n0 > 0 && id_at(sorted, n0) == id && id_at(sorted, n0 - 1) == id);   // began further back
+  };
+  uint64_t found = __ballot(lane < kLook && first + lane + 1 < chunks && goes_on(first + lane));
+  for (; found; found &= found - 1) {
+    const int64_t c0 = first + __builtin_ctzll(found);
+    const uint32_t id = id_at(sorted, (c0 + 1) * chunk);
+    int64_t lo = c0 + 1, hi = chunks;   // the last chunk that begins with the run: 64 probes a turn
+    while (hi - lo > 1) {
+      const int64_t step = (hi - lo + 63) / 64, c = lo + (lane + 1) * step;
+      lo += step * __popcll(__ballot(c < hi && id_at(sorted, c * chunk) == id));
+      hi = min(hi, lo + step);
     }
-    for (; i < to; ++i) {
-      const f32x4 f = slot(i);
+    const int64_t count = lo - c0 + 1;   // slot 1 of c0, slot 0 of the others
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (col < a.H) {
+      const int64_t per = (count + kJoinWaves - 1) / kJoinWaves, to = min(count, (wave + 1) * per);
+      auto slot = [&](int64_t i) {
+        return *reinterpret_cast<const f32x4 *>(part + ((c0 + i) * 2 + (i == 0)) * a.part_rs + col);
+      };
+      int64_t i = wave * per;
+      for (; i + 8 <= to; i += 8) {
+        f32x4 f[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += f[e];
+        for (int u = 0; u < 8; ++u) f[u] = slot(i + u);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += f[u][e];
+      }
+      for (; i < to; ++i) {
+        const f32x4 f = slot(i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += f[e];
+      }
     }
-  }
-  sums[wave][lane] = acc;
-  __syncthreads();
-  if (wave || col >= a.H) return;
-  float f[4];
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0 && col < a.H) {
+      float f[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    f[e] = sums[0][lane][e];
+      for (int e = 0; e < 4; ++e) {
+        f[e] = sums[0][lane][e];
 #pragma unroll
-    for (int w = 1; w < kJoinWaves; ++w) f[e] += sums[w][lane][e];
+        for (int w = 1; w < kJoinWaves; ++w) f[e] += sums[w][lane][e];
+      }
+      put_row<TO, VEC, ADD, 4>(a, id, col, f);
+    }
+    __syncthreads();
   }
-  put_row<TO, VEC, ADD, 4>(a, id, col, f);
 }
 
 namespace {
@@ -359,8 +380,6 @@ int chunk_of(int32_t N, int32_t H, int W) {
   const int64_t slices = ((int64_t)H + kThreads * W - 1) / (kThreads * W);
   return (int)std::min<int64_t>(kMaxChunk, std::max<int64_t>(16, (int64_t)N * slices / 1024));
 }
-
-constexpr int64_t kCachedBytes = 200 << 20;   // of dW that are written into the last-level cache
 
 template <typename T, bool VEC>
 void fwd_typed(const EmbedArgs &a, hipStream_t st) {
@@ -379,22 +398,23 @@ void bwd_typed(EmbedArgs a, bool add, char *ws, hipStream_t st) {
     ws += ((int64_t)a.N * 8 + 15) / 16 * 16;
   }
   float *part = reinterpret_cast<float *>(ws);
-  const int64_t rows = add ? 0 : ((int64_t)a.V + 15) / 16;
-  const unsigned clear = (unsigned)std::min<int64_t>(rows, 2048);
+  // workgroups that clear: one a part, or each for several rows
+  int64_t clear = 0;
+  if (!add) {
+    clear = ((int64_t)a.V * a.H * (int64_t)sizeof(TO) + kClear - 1) / kClear;
+    if (!VEC || a.out_rs != a.H) clear = std::min<int64_t>(((int64_t)a.V + 15) / 16, 4096);
+  }
   if (tiles + clear == 0) return;
-  if ((int64_t)a.V * a.H * (int64_t)sizeof(TO) > kCachedBytes)
-    hipLaunchKernelGGL((embed_sort_kernel<TO, VEC, true>), dim3(tiles + clear), dim3(kSortThreads), 0, st, a, tiles,
-                       !add, raw);
-  else
-    hipLaunchKernelGGL((embed_sort_kernel<TO, VEC, false>), dim3(tiles + clear), dim3(kSortThreads), 0, st, a, tiles,
-                       !add, raw);
+  hipLaunchKernelGGL((embed_sort_kernel<TO, VEC>), dim3((unsigned)(tiles + clear)), dim3(kSortThreads), 0, st, a, tiles,
+                     !add, raw);
   if (a.N == 0) return;
   if (tiles > 1)
     hipLaunchKernelGGL(embed_merge_kernel, dim3((a.N + kThreads - 1) / kThreads), dim3(kThreads), 0, st, raw, a.N,
                        tiles, sorted);
   const int chunk = chunk_of(a.N, a.H, kW<T>);
   const unsigned chunks = (a.N + chunk - 1) / chunk;
-  const dim3 grid(chunks, (a.H + kThreads * kW<T> - 1) / (kThreads * kW<T>)), join(chunks, (a.H + 255) / 256);
+  const dim3 grid(chunks, (a.H + kThreads * kW<T> - 1) / (kThreads * kW<T>));
+  const dim3 join((chunks + kLook - 1) / kLook, (a.H + 255) / 256);
   auto run = [&](auto sum, auto joined) {
     hipLaunchKernelGGL(sum, grid, dim3(kThreads), 0, st, a, sorted, chunk, part);
     if (chunks > 1) hipLaunchKernelGGL(joined, join, dim3(kJoinThreads), 0, st, a, sorted, chunk, part);

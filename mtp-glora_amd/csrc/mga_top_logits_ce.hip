@@ -11,10 +11,10 @@
 // The K columns are a few cache lines; all three kernels are bound by the rows of
 // x (read) and of the gradient (written).
 //
-// Forward: column ranges of the rows to (m, d), then a wave per row joins them,
-// forms q and the row's loss; the last workgroup adds the rows in a fixed order.
-// Backward: one more pass over x. Both in one (step): a workgroup holds the row in
-// registers between the sum and the gradient, so x is read once.
+// Forward of few rows: column ranges of the rows to (m, d), then a wave per row joins
+// them, forms q and the row's loss; the last workgroup adds the rows in a fixed order.
+// Of more: a workgroup a row, and a launch that adds them. Backward: one more pass
+// over x. Both in one (step): a workgroup a row, which reads it twice.
 #include "mga_internal.hpp"
 #include "mga_vocab_row.hpp"
 
@@ -366,92 +366,158 @@ __global__ __launch_bounds__(kThreads) void top_ce_bwd_kernel(TopLogitsCeArgs a,
   }
 }
 
-constexpr int kStepThreads = 512;
+// ---- loss and gradient in one kernel --------------------------------------------
 
-__device__ __forceinline__ float group_reduce(float v, float *part, bool is_max) {
+// Largest of two values each, and sums of three, over a workgroup of B threads.
+template <int B>
+__device__ __forceinline__ float2 block_max2(float2 v, float4 *part) {
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) {
-    const float o = __shfl_xor(v, m, 64);
-    v = is_max ? fmaxf(v, o) : v + o;
+    v.x = fmaxf(v.x, __shfl_xor(v.x, m, 64));
+    v.y = fmaxf(v.y, __shfl_xor(v.y, m, 64));
   }
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = {v.x, v.y, 0.f, 0.f};
   __syncthreads();
-  v = part[0];
+  v = {part[0].x, part[0].y};
 #pragma unroll
-  for (int w = 1; w < kStepThreads / 64; ++w) v = is_max ? fmaxf(v, part[w]) : v + part[w];
+  for (int w = 1; w < B / 64; ++w) v = {fmaxf(v.x, part[w].x), fmaxf(v.y, part[w].y)};
+  __syncthreads();
+  return v;
+}
+template <int B>
+__device__ __forceinline__ float3 block_sum3(float3 v, float4 *part) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) {
+    v.x += __shfl_xor(v.x, m, 64);
+    v.y += __shfl_xor(v.y, m, 64);
+    v.z += __shfl_xor(v.z, m, 64);
+  }
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = {v.x, v.y, v.z, 0.f};
+  __syncthreads();
+  v = {part[0].x, part[0].y, part[0].z};
+#pragma unroll
+  for (int w = 1; w < B / 64; ++w) v = {v.x + part[w].x, v.y + part[w].y, v.z + part[w].z};
   __syncthreads();
   return v;
 }
 
-// Loss and gradient of a row. The row's second reading follows its first at once
-// and comes from the caches; four workgroups share a compute unit, so that one's
-// arithmetic (the exponentials, twice) runs beside the others' memory. Holding the
-// row in registers instead leaves room for one workgroup a compute unit: 191 us
-// for 1 024 x 151 936 bf16.
+template <int B>
+struct StepShared {
+  int ids[kMaxTop];
+  float q[kMaxTop];
+  float4 part[B / 64];
+};
+
+// A teacher's row, entries tid, tid + B, .. a thread.
+template <int B>
+struct TeacherRow {
+  static constexpr int kEach = kMaxTop / B;
+  int id[kEach];
+  float t[kEach], x[kEach], q[kEach];   // values, the student's logits there, weights
+
+  template <typename T>
+  __device__ __forceinline__ void load(const TopLogitsCeArgs &a, int64_t n, const T *xr) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int k = threadIdx.x + i * B;
+      id[i] = k < a.K ? teacher_id(a, n, k) : -1;
+      t[i] = id[i] >= 0 ? teacher_value(a, n, k) : kRowNegInf;
+      x[i] = id[i] >= 0 ? (float)xr[id[i]] : 0.f;
+    }
+  }
+
+  // From this thread's part of the student's row: the row's loss and what its
+  // gradient has in common; the entries in LDS, or (SAVE) all that the backward
+  // reads in memory.
+  template <bool SAVE>
+  __device__ __forceinline__ GradRow finish(const TopLogitsCeArgs &a, int64_t n, const RowSum &st, float itau, float c,
+                                            StepShared<B> &sh) {
+    float top = kRowNegInf;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) top = fmaxf(top, t[i] * itau);
+    const float2 most = block_max2<B>({st.m, top}, sh.part);
+    const float m = most.x, norm = a.lse ? a.lse[n] : most.y;
+    float3 sums = {sum_at(st, m, c), 0.f, 0.f};   // d; of the weights; of their part of the loss
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      q[i] = teacher_weight(t[i], id[i], norm, itau);
+      sums.y += q[i];
+      sums.z += q[i] == 0.f ? 0.f : x[i] == kRowNegInf ? -kRowNegInf : q[i] * ((m - x[i]) * itau);
+    }
+    sums = block_sum3<B>(sums, sh.part);
+    const float d = sum_at_max(m, sums.x, c), inv = a.lse ? 1.f : sums.y == 0.f ? 0.f : 1.f / sums.y;
+    const float Q = sums.y * inv;
+    if (threadIdx.x == 0)
+      a.loss[n] = Q == 0.f ? 0.f : m == kRowNegInf ? -kRowNegInf : a.tau * a.tau * (sums.z * inv + Q * logf(d));
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int k = threadIdx.x + i * B;
+      q[i] *= inv;
+      if (k >= a.K) continue;
+      if constexpr (SAVE) {
+        if (a.q) a.q[n * a.K + k] = q[i];
+      } else {
+        sh.ids[k] = id[i];
+        sh.q[k] = q[i];
+      }
+    }
+    if (SAVE && threadIdx.x == 0) {
+      a.stats[n] = m;
+      a.stats[a.N + n] = d;
+      a.stats[2 * (int64_t)a.N + n] = Q;
+    }
+    return GradRow(m, d, Q, c, a.scale * a.tau);
+  }
+
+  // The teacher's columns over the gradient that was just written.
+  template <typename T>
+  __device__ __forceinline__ void patch(const TopLogitsCeArgs &a, const GradRow &gradient, T *gr,
+                                        const StepShared<B> &sh) const {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      float s;
+      if (id[i] >= 0 && owned_sum(sh.ids, sh.q, a.K, threadIdx.x + i * B, &s))
+        gr[id[i]] = (T)(gradient(x[i]) - a.scale * a.tau * s);
+    }
+  }
+};
+
+constexpr int kAloneThreads = 512;
+
+// The forward with a workgroup a row.
+template <typename T>
+__global__ __launch_bounds__(kAloneThreads, 8) void top_ce_row_kernel(TopLogitsCeArgs a) {
+  __shared__ StepShared<kAloneThreads> sh;
+  const int64_t n = blockIdx.x;
+  const float itau = 1.f / a.tau, c = itau * kLog2e;
+  const T *xr = static_cast<const T *>(a.x) + n * a.xs;
+  TeacherRow<kAloneThreads> teacher;
+  teacher.load(a, n, xr);
+  const RowSum st = sum_elements<kAloneThreads>(xr, a.V, c);
+  teacher.template finish<true>(a, n, st, itau, c, sh);
+}
+
+// A workgroup a row, whose second reading follows its first, from the end, and comes
+// from the caches; four workgroups share a compute unit, so that one's arithmetic
+// (the exponentials, twice) runs beside the others' memory. 1 024 x 151 936 bf16:
+// 160 us, 933 MB past the L2 at 5.8 TB/s. Holding the row in registers instead, so
+// that it is read once, leaves room for one workgroup a compute unit: 191 us, and
+// 231 us where that one takes the next row's vectors as it writes this one's.
 template <typename T, bool NT>
-__global__ __launch_bounds__(kStepThreads, 8) void top_ce_step_kernel(TopLogitsCeArgs a) {
-  constexpr int kEach = kMaxTop / kStepThreads;
-  __shared__ int ids[kMaxTop];
-  __shared__ float qs[kMaxTop];
-  __shared__ float part[kStepThreads / 64];
-  const int tid = threadIdx.x;
+__global__ __launch_bounds__(kAloneThreads, 8) void top_ce_step_kernel(TopLogitsCeArgs a) {
+  __shared__ StepShared<kAloneThreads> sh;
   const int64_t n = blockIdx.x;
   const float itau = 1.f / a.tau, c = itau * kLog2e;
   const T *xr = static_cast<const T *>(a.x) + n * a.xs;
   T *gr = static_cast<T *>(a.grad) + n * a.gs;
-  // the teacher's side, entries tid and tid + kStepThreads
-  int id[kEach];
-  float q[kEach], xk[kEach];
-  float norm = kRowNegInf;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int k = tid + i * kStepThreads;
-    id[i] = k < a.K ? teacher_id(a, n, k) : -1;
-    q[i] = id[i] >= 0 ? teacher_value(a, n, k) : kRowNegInf;
-    xk[i] = id[i] >= 0 ? (float)xr[id[i]] : 0.f;
-    norm = fmaxf(norm, q[i] * itau);
-  }
-  norm = a.lse ? a.lse[n] : group_reduce(norm, part, true);
-  float Q = 0.f;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) Q += q[i] = teacher_weight(q[i], id[i], norm, itau);
-  Q = group_reduce(Q, part, false);
-  if (!a.lse) {
-    const float inv = Q == 0.f ? 0.f : 1.f / Q;
-    Q = 0.f;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) Q += q[i] *= inv;
-    Q = group_reduce(Q, part, false);
-  }
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int k = tid + i * kStepThreads;
-    if (k < a.K) {
-      ids[k] = id[i];
-      qs[k] = q[i];
-    }
-  }
-  RowSum st = sum_elements<kStepThreads>(xr, a.V, c);
-  const float m = group_reduce(st.m, part, true);
-  const float d = sum_at_max(m, group_reduce(sum_at(st, m, c), part, false), c);
-  const float logd = logf(d);
-  float loss = 0.f;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) loss += loss_term(q[i], xk[i], m, logd, itau);
-  loss = group_reduce(loss, part, false);
-  if (tid == 0) a.loss[n] = a.tau * a.tau * loss;
-  const float coef = a.scale * a.tau;
-  const GradRow gradient(m, d, Q, c, coef);
-  if (gradient.dead) return write_gradient<kStepThreads, NT>(ZeroRow(), xr, gr, a.V);
-  write_gradient<kStepThreads, NT>(gradient, xr, gr, a.V);
-  // the teacher's columns over what was just written
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    float s;
-    if (id[i] >= 0 && owned_sum(ids, qs, a.K, tid + i * kStepThreads, &s))
-      gr[id[i]] = (T)(gradient(xk[i]) - coef * s);
-  }
+  TeacherRow<kAloneThreads> teacher;
+  teacher.load(a, n, xr);
+  const RowSum st = sum_elements<kAloneThreads>(xr, a.V, c);
+  const GradRow gradient = teacher.template finish<false>(a, n, st, itau, c, sh);
+  if (gradient.dead) return write_gradient<kAloneThreads, NT>(ZeroRow(), xr, gr, a.V);
+  write_gradient<kAloneThreads, NT>(gradient, xr, gr, a.V);
+  teacher.patch(a, gradient, gr, sh);
 }
 
 namespace {
@@ -471,8 +537,19 @@ constexpr int64_t kCachedBytes = 200 << 20;
 template <typename T>
 bool past_cache(const TopLogitsCeArgs &a) { return 2 * (int64_t)a.N * a.V * (int64_t)sizeof(T) > kCachedBytes; }
 
+// Rows from which a workgroup a row beats the column ranges and their joining. The
+// forward of 128 256 fp16, ranges against rows with their sum: 64 rows 16 and 18 us,
+// 96 rows 18.7 and 17.9, 333 rows 33 and 24. The step of 151 936 bf16: 64 rows 31 and
+// 35 us, 100 rows 39 and 36, 512 rows 109 and 89.
+constexpr int kRowsAlone = 96;
+
 template <typename T>
 void fwd_typed(const TopLogitsCeArgs &a, float *ws, hipStream_t st) {
+  if (a.N >= kRowsAlone) {
+    hipLaunchKernelGGL(top_ce_row_kernel<T>, dim3(a.N), dim3(kAloneThreads), 0, st, a);
+    hipLaunchKernelGGL(top_ce_sum_kernel, dim3(1), dim3(kThreads), 0, st, a.loss, a.N, a.sum);
+    return;
+  }
   int32_t ns, ch;
   split_plan(a.N, a.V, &ns, &ch);
   int *done = reinterpret_cast<int *>(ws);
@@ -490,19 +567,15 @@ void bwd_typed(const TopLogitsCeArgs &a, hipStream_t st) {
   else hipLaunchKernelGGL((top_ce_bwd_kernel<T, false>), grid, dim3(kThreads), 0, st, a, ch, ns);
 }
 
-// Rows from which a workgroup a row fills the chip: below, the column ranges of the
-// forward and the backward do.
-constexpr int kStepRows = 128;
-
 template <typename T>
 void step_typed(const TopLogitsCeArgs &a, float *ws, hipStream_t st) {
-  if (a.N < kStepRows) {
+  if (a.N < kRowsAlone) {
     fwd_typed<T>(a, ws, st);
     bwd_typed<T>(a, st);
     return;
   }
-  if (past_cache<T>(a)) hipLaunchKernelGGL((top_ce_step_kernel<T, true>), dim3(a.N), dim3(kStepThreads), 0, st, a);
-  else hipLaunchKernelGGL((top_ce_step_kernel<T, false>), dim3(a.N), dim3(kStepThreads), 0, st, a);
+  if (past_cache<T>(a)) hipLaunchKernelGGL((top_ce_step_kernel<T, true>), dim3(a.N), dim3(kAloneThreads), 0, st, a);
+  else hipLaunchKernelGGL((top_ce_step_kernel<T, false>), dim3(a.N), dim3(kAloneThreads), 0, st, a);
   hipLaunchKernelGGL(top_ce_sum_kernel, dim3(1), dim3(kThreads), 0, st, a.loss, a.N, a.sum);
 }
 

@@ -81,14 +81,20 @@ struct Row {
   int V, head, nvec, ecol;   // ecol: column of this thread's single element, or -1
   float edge;
 
+  // This thread's vector i. Its address is a uniform base and the lane's own 32-bit
+  // offset: one register a lane for all of them.
+  __device__ __forceinline__ i32x4 load_vec(int i) const {
+    const char *base = reinterpret_cast<const char *>(p + head);
+    const int at = i * kRowThreads;
+    i32x4 v = {RowElem<T>::kFill, RowElem<T>::kFill, RowElem<T>::kFill, RowElem<T>::kFill};
+    if ((int)threadIdx.x < nvec - at) v = *reinterpret_cast<const i32x4 *>(base + (int64_t)at * 16 + threadIdx.x * 16u);
+    return v;
+  }
   __device__ __forceinline__ i32x16 load_block(int b) const {
-    const i32x4 *vp = reinterpret_cast<const i32x4 *>(p + head) + threadIdx.x;
     i32x16 q;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int at = (b * 4 + j) * kRowThreads;
-      i32x4 v = {RowElem<T>::kFill, RowElem<T>::kFill, RowElem<T>::kFill, RowElem<T>::kFill};
-      if (at + (int)threadIdx.x < nvec) v = vp[at];
+      const i32x4 v = load_vec(4 * b + j);
       q[4 * j] = v[0]; q[4 * j + 1] = v[1]; q[4 * j + 2] = v[2]; q[4 * j + 3] = v[3];
     }
     return q;

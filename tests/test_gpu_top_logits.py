@@ -292,9 +292,11 @@ def test_refusals_and_empty(mga, dev):
 
 
 def test_gradient_past_the_cache(mga, dev):
-    """More bytes than the last-level cache holds: the gradient of a row is what it
-    is among fewer rows, bit for bit where a workgroup takes a row on both sides."""
-    x = logits(700, 151936, torch.bfloat16, dev, seed=12)
+    """More bytes than the last-level cache holds, and other kernels for fewer rows:
+    a row's gradients on both sides are within half a step and the sums' slack of
+    the exact one, so within eps |g| and twice the slack of each other."""
+    V = 151936
+    x = logits(700, V, torch.bfloat16, dev, seed=12)
     t = teacher(mga, x, 16, 1.0)
     xs = x.clone().requires_grad_()
     mga.top_logits_cross_entropy(xs, t.values, t.ids, t.lse).backward()
@@ -304,7 +306,8 @@ def test_gradient_past_the_cache(mga, dev):
         ys = x[few].clone().requires_grad_()
         mga.top_logits_cross_entropy(ys, t.values[few], t.ids[few], t.lse[few]).backward()
         _, h = mga.top_logits_loss_and_grad(x[few], t.values[few], t.ids[few], t.lse[few])
-        assert torch.equal(g[few], h)
-        # other column splits add the row's sum in another order
-        d = (xs.grad[few].float() - ys.grad.float()).abs()
-        assert bool((d <= 2.0 ** -7 * ys.grad.float().abs() + 1e-30).all())
+        q = torch.zeros(200, V, device=dev).scatter_(1, t.ids[few].long(), (t.values[few].float() - t.lse[few][:, None]).exp())
+        slack = 2 * chain(V) * (torch.softmax(x[few].float(), -1) * q.sum(-1, keepdim=True) + q)
+        for a, b in ((g[few], h), (xs.grad[few], ys.grad), (g[few], xs.grad[few])):
+            d = (a.float() - b.float()).abs()
+            assert bool((d <= 2.0 ** -7 * torch.maximum(a.abs(), b.abs()).float() + slack + 1e-30).all())
