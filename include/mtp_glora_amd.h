@@ -432,7 +432,7 @@ int mga_soft_ce_bwd(const void *student, int64_t student_row_stride,
  * null) the row's log sum_j exp(x_j / temperature) in fp32 (-inf for a row of
  * -inf alone, NaN where the row holds a NaN). Rows of n_cols <= 1 048 576
  * logits, row r at logits + r * row_stride elements, columns contiguous;
- * 1 <= k <= min(n_cols, 1024); temperature positive and finite.
+ * 1 <= k <= min(n_cols, 1024); temperature within 2^-60 to 2^60.
  * No counterpart in the reference, which keeps a teacher's whole rows
  * (mtp_glora/core/mtp.py:121-126): what is kept of them here feeds
  * mga_top_logits_ce_*.

@@ -861,9 +861,10 @@ int check_matrix(const char *fn, const char *name, const void *p, int64_t rs, in
   return MGA_OK;
 }
 
-int check_positive(const char *fn, const char *name, float v) {
-  if (v > 0.f && v < __builtin_huge_valf()) return MGA_OK;
-  return fail(MGA_ERR_INVALID, "%s: %s must be positive and finite (got %g)", fn, name, (double)v);
+// Its square and its reciprocal times log2(e) are ordinary fp32 numbers.
+int check_temperature(const char *fn, float v) {
+  if (v >= 0x1p-60f && v <= 0x1p60f) return MGA_OK;
+  return fail(MGA_ERR_INVALID, "%s: temperature must be within 2^-60 to 2^60 (got %g)", fn, (double)v);
 }
 
 int check_top_k(const char *fn, int32_t k) {
@@ -874,7 +875,7 @@ int check_top_k(const char *fn, int32_t k) {
 int check_top_ce(const char *fn, const mga::TopLogitsCeArgs &a, int32_t dtype) {
   int rc = check_matrix(fn, "student", a.x, a.xs, a.N, a.V, dtype);
   if (rc == MGA_OK) rc = check_top_k(fn, a.K);
-  if (rc == MGA_OK) rc = check_positive(fn, "temperature", a.tau);
+  if (rc == MGA_OK) rc = check_temperature(fn, a.tau);
   if (rc != MGA_OK) return rc;
   if (!a.ids || a.ids_rs < a.K) return fail(MGA_ERR_INVALID, "%s: ids null or with a row stride below k", fn);
   if (reinterpret_cast<uintptr_t>(a.ids) % (a.ids64 ? 8 : 4))
@@ -914,7 +915,7 @@ int mga_top_logits(const void *logits, int64_t row_stride, int32_t n_rows, int32
   const char *fn = "mga_top_logits";
   int rc = check_matrix(fn, "logits", logits, row_stride, n_rows, n_cols, dtype);
   if (rc == MGA_OK) rc = check_top_k(fn, k);
-  if (rc == MGA_OK) rc = check_positive(fn, "temperature", temperature);
+  if (rc == MGA_OK) rc = check_temperature(fn, temperature);
   if (rc != MGA_OK) return rc;
   if (k > n_cols || n_cols > kMaxVocab)
     return fail(MGA_ERR_INVALID, "%s: k=%d of %d columns (at most %d)", fn, k, n_cols, kMaxVocab);

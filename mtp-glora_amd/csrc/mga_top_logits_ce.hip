@@ -136,7 +136,12 @@ struct GradRow {
   float mc, c, a;
   bool dead;
   __device__ __forceinline__ GradRow(float m, float d, float Q, float c_, float coef)
-      : mc(scaled(m, c_)), c(c_), a(d == 0.f ? 0.f : sum_at_max(m, coef * Q / d, c_)), dead(Q == 0.f) {}
+      : mc(scaled(m, c_)), c(c_), a(d == 0.f ? 0.f : sum_at_max(m, coef * Q / d, c_)), dead(Q == 0.f) {
+    if (far(m, c_)) {   // a where x is m and 0 elsewhere: m c and x c exact, |m c| up to 2^60
+      c = ldexpf(1.f, 60 - __builtin_amdgcn_frexp_expf(m));
+      mc = m * c;
+    }
+  }
   __device__ __forceinline__ float operator()(float x) const { return a * ex2(__builtin_fmaf(x, c, -mc)); }
 };
 struct ZeroRow {
@@ -164,9 +169,10 @@ __global__ __launch_bounds__(kThreads) void top_ce_partial_kernel(const T *__res
                                                                   float *__restrict__ part, int *__restrict__ done) {
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x / nsplit;
-  const int sp = blockIdx.x - row * nsplit, c0 = sp * chunk, c1 = min(V, c0 + chunk);
+  const int sp = blockIdx.x - row * nsplit, c0 = sp * chunk, n = min(V, c0 + chunk) - c0;
   if (blockIdx.x == 0 && tid == 0) *done = 0;   // for the combine kernel
-  RowSum st = sum_elements<kThreads>(x + row * xs + c0, c1 - c0, c);
+  const T *xr = x + row * xs + c0;
+  RowSum st = sum_elements<kThreads>(xr, n, c);
   merge_lanes(st, c);
   __shared__ float wm[kThreads / 64], wd[kThreads / 64];
   if ((tid & 63) == 0) {
@@ -174,11 +180,26 @@ __global__ __launch_bounds__(kThreads) void top_ce_partial_kernel(const T *__res
     wd[tid >> 6] = st.d;
   }
   __syncthreads();
-  if (tid == 0) {
+  float m = wm[0];
 #pragma unroll
-    for (int w = 1; w < kThreads / 64; ++w) st.merge(wm[w], wd[w], c);
-    part[2 * blockIdx.x] = st.m;
-    part[2 * blockIdx.x + 1] = st.d;
+  for (int w = 1; w < kThreads / 64; ++w) m = fmaxf(m, wm[w]);
+  if (far(m, c)) {
+    float s = count_equal<kThreads>(xr, n, m);
+#pragma unroll
+    for (int i = 32; i >= 1; i >>= 1) s += __shfl_xor(s, i, 64);
+    __syncthreads();
+    if ((tid & 63) == 0) {
+      wm[tid >> 6] = m;
+      wd[tid >> 6] = s;
+    }
+    __syncthreads();
+  }
+  if (tid == 0) {
+    float d = 0.f;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) d += wd[w] * part_weight(wm[w], m, c);
+    part[2 * blockIdx.x] = m;
+    part[2 * blockIdx.x + 1] = d;
   }
 }
 
@@ -426,18 +447,19 @@ struct TeacherRow {
     }
   }
 
-  // From this thread's part of the student's row: the row's loss and what its
+  // From this thread's part of the student's row xr: the row's loss and what its
   // gradient has in common; the entries in LDS, or (SAVE) all that the backward
   // reads in memory.
-  template <bool SAVE>
-  __device__ __forceinline__ GradRow finish(const TopLogitsCeArgs &a, int64_t n, const RowSum &st, float itau, float c,
-                                            StepShared<B> &sh) {
+  template <bool SAVE, typename T>
+  __device__ __forceinline__ GradRow finish(const TopLogitsCeArgs &a, int64_t n, const T *xr, const RowSum &st,
+                                            float itau, float c, StepShared<B> &sh) {
     float top = kRowNegInf;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) top = fmaxf(top, t[i] * itau);
     const float2 most = block_max2<B>({st.m, top}, sh.part);
     const float m = most.x, norm = a.lse ? a.lse[n] : most.y;
-    float3 sums = {sum_at(st, m, c), 0.f, 0.f};   // d; of the weights; of their part of the loss
+    // d; of the weights; of their part of the loss
+    float3 sums = {far(m, c) ? count_equal<B>(xr, a.V, m) : sum_at(st, m, c), 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       q[i] = teacher_weight(t[i], id[i], norm, itau);
@@ -495,7 +517,7 @@ __global__ __launch_bounds__(kAloneThreads, 8) void top_ce_row_kernel(TopLogitsC
   TeacherRow<kAloneThreads> teacher;
   teacher.load(a, n, xr);
   const RowSum st = sum_elements<kAloneThreads>(xr, a.V, c);
-  teacher.template finish<true>(a, n, st, itau, c, sh);
+  teacher.template finish<true>(a, n, xr, st, itau, c, sh);
 }
 
 // A workgroup a row, whose second reading follows its first, from the end, and comes
@@ -514,7 +536,7 @@ __global__ __launch_bounds__(kAloneThreads, 8) void top_ce_step_kernel(TopLogits
   TeacherRow<kAloneThreads> teacher;
   teacher.load(a, n, xr);
   const RowSum st = sum_elements<kAloneThreads>(xr, a.V, c);
-  const GradRow gradient = teacher.template finish<false>(a, n, st, itau, c, sh);
+  const GradRow gradient = teacher.template finish<false>(a, n, xr, st, itau, c, sh);
   if (gradient.dead) return write_gradient<kAloneThreads, NT>(ZeroRow(), xr, gr, a.V);
   write_gradient<kAloneThreads, NT>(gradient, xr, gr, a.V);
   teacher.patch(a, gradient, gr, sh);

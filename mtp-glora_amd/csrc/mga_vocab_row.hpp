@@ -421,13 +421,24 @@ __device__ __forceinline__ uint64_t radix_threshold(const Row<T> &row, RowShared
 
 // A running maximum m and sum d = sum 2^{x c - mc}, mc = m c rounded: one fma an
 // element for the exponent. What the rounding of mc does to d is taken out once, at
-// the end (sum_at_max).
-__device__ __forceinline__ float scaled(float m, float c) { return m == kRowNegInf ? 0.f : m * c; }
+// the end (sum_at_max): a factor of at most 2^32 while |m c| < 2^30. Further out
+// (a row masked with the type's lowest value) two different elements are at least 64
+// octaves apart, and d is the number of those that equal m: counted when the maximum
+// of the row is known (count_equal); until then mc = 0, and d is 0 below zero and
+// of no use above.
+constexpr float kFar = 1073741824.f;
+__device__ __forceinline__ bool far(float m, float c) { return m != kRowNegInf && !(fabsf(m * c) < kFar); }
+__device__ __forceinline__ float scaled(float m, float c) { return fabsf(m * c) < kFar ? m * c : 0.f; }
+// What a sum at the maximum `part` counts at the maximum `whole`.
+__device__ __forceinline__ float part_weight(float part, float whole, float c) {
+  if (part == whole || part == kRowNegInf) return 1.f;   // a sum at -inf: 0, or NaN
+  return far(part, c) || far(whole, c) ? 0.f : __builtin_amdgcn_exp2f(scaled(part, c) - scaled(whole, c));
+}
 struct RowSum {
   float m = kRowNegInf, mc = 0.f, d = 0.f;
   __device__ __forceinline__ void raise(float g, float c) {   // g > m
-    const float n = g * c;
-    if (m != kRowNegInf) d *= __builtin_amdgcn_exp2f(mc - n);
+    const float n = scaled(g, c);
+    if (d != 0.f) d *= __builtin_amdgcn_exp2f(mc - n);
     m = g;
     mc = n;
   }
@@ -449,23 +460,31 @@ struct RowSum {
     else d += (s[0] + s[1]) + (s[2] + s[3]);
   }
   __device__ __forceinline__ void merge(float om, float od, float c) {
-    const float omc = scaled(om, c);
     if (om > m) {
-      d = m == kRowNegInf ? d + od : d * __builtin_amdgcn_exp2f(mc - omc) + od;
+      d = d * part_weight(m, om, c) + od;
       m = om;
-      mc = omc;
+      mc = scaled(om, c);
     } else {
-      d += om == kRowNegInf ? od : od * __builtin_amdgcn_exp2f(omc - mc);   // od alone: 0 or NaN
+      d += od * part_weight(om, m, c);
     }
   }
 };
 // A part's sum at the whole's maximum m >= st.m.
-__device__ __forceinline__ float sum_at(const RowSum &st, float m, float c) {
-  return st.m == m || st.m == kRowNegInf ? st.d : st.d * __builtin_amdgcn_exp2f(st.mc - scaled(m, c));
-}
+__device__ __forceinline__ float sum_at(const RowSum &st, float m, float c) { return st.d * part_weight(st.m, m, c); }
 // sum 2^{(x - m) c} from d = sum 2^{x c - mc}
 __device__ __forceinline__ float sum_at_max(float m, float d, float c) {
-  return m == kRowNegInf || m == -kRowNegInf ? d : d * __builtin_amdgcn_exp2f(-__builtin_fmaf(m, c, -scaled(m, c)));
+  return m == kRowNegInf || far(m, c) ? d : d * __builtin_amdgcn_exp2f(-__builtin_fmaf(m, c, -scaled(m, c)));
+}
+// This thread's part of d of n elements whose maximum m is far: how many equal it. NaN
+// where there is one, and for m = +inf.
+template <int B, typename T>
+__device__ __forceinline__ float count_equal(const T *p, int n, float m) {
+  float s = m - m;
+  for (int i = threadIdx.x; i < n; i += B) {
+    const float x = (float)p[i];
+    s += x == m ? 1.f : x == x ? 0.f : x;
+  }
+  return s;
 }
 
 // ---- the first elements in order ------------------------------------------------

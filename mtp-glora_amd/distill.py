@@ -52,8 +52,8 @@ def _like(name: str, t: torch.Tensor, lead, device) -> None:
 
 def _temperature(t) -> float:
     t = float(t)
-    if not 0.0 < t < float("inf"):
-        raise ValueError(f"temperature must be positive and finite (got {t})")
+    if not 2.0 ** -60 <= t <= 2.0 ** 60:
+        raise ValueError(f"temperature must be within 2^-60 to 2^60 (got {t})")
     return t
 
 

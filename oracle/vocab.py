@@ -58,12 +58,14 @@ def top_ce(x, values, ids, lse=None, temperature=1.0, grad_output=1.0):
         if not live.any():
             continue
         y = x[r] / temperature
-        norm = logsumexp(y)
+        m = y.max()
         at = np.asarray(ids[r])[live]
-        with np.errstate(invalid="ignore"):
-            terms = np.where(y[at] == -np.inf, np.inf, q[r][live] * (norm - y[at]))
+        with np.errstate(invalid="ignore", divide="ignore"):
+            # not logsumexp(y) - y: m + log d is m where m is large
+            e = np.exp(y - m) if m > -np.inf else np.zeros(V)
+            terms = np.where(y[at] == -np.inf, np.inf, q[r][live] * ((m - y[at]) + np.log(e.sum())))
+            p = e / e.sum() if m > -np.inf else e
         loss[r] = temperature ** 2 * terms.sum()
-        p = np.exp(y - norm) if norm > -np.inf else np.zeros(V)
         g = q[r].sum() * p
         np.subtract.at(g, at, q[r][live])
         grad[r] = grad_output * temperature * g

@@ -213,6 +213,43 @@ def test_padding_duplicates_and_masks(mga, dev, dtype):
     assert bool(mga.top_logits_cross_entropy(y, values[2:3], ids[2:3]).isnan())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tau", [1.0, 4.0, 2.0 ** -20])
+def test_rows_far_from_zero(mga, dev, dtype, tau):
+    """Rows masked with the type's lowest value, all of them too, and rows of other
+    values whose quotient by the temperature is far past fp32's whole numbers: the
+    sums there are exact (equal elements count 1, others nothing)."""
+    V, k = 5003, 6
+    print(f"case {dtype} {tau}", flush=True)
+    low = torch.finfo(dtype).min if tau >= 1 else max(torch.finfo(dtype).min, -1e30)
+    x = logits(9, V, dtype, dev, seed=13)
+    x[0] = low                              # nothing left: uniform
+    x[1, :V // 2] = low                     # masked from the start,
+    x[2, V // 2:] = low                     # to the end,
+    x[3, 0::2] = low                        # and between
+    x[4] = low
+    x[4, 77] = low / 2
+    x[5, 1000::1000] = -low                 # the largest value, five times
+    x[6] = max(-1e12, low / 4) * (1 + torch.randint(0, 64, (V,), device=dev) * 2.0 ** -6)
+    x[7] = 7e8 if dtype != torch.float16 else 6e4   # next to where counting begins (at tau = 1)
+    x[7, 5::7] = float(x[7, 0]) * (1 + 2.0 ** -7)
+    x[8] = -x[7]
+    t = check_top(mga, x, k, tau)
+    ids = t.ids.clone()
+    ids[4, 1:] = -1
+    ids[5, 5:] = -1
+    values = torch.randn(9, k, device=dev).to(dtype) * min(tau, 1.0)
+    for i in range(9):
+        check_ce(mga, x[i:i + 1], values[i:i + 1], ids[i:i + 1], None, tau)
+    check_ce(mga, x.repeat(12, 1), values.repeat(12, 1), ids.repeat(12, 1), None, tau)
+    # NaN in such a row
+    y = x[:1].clone()
+    y[0, 7] = float("nan")
+    for z in (y, y.repeat(100, 1)):
+        loss, g = mga.top_logits_loss_and_grad(z, values[:1].expand(len(z), k), ids[:1].expand(len(z), k))
+        assert bool(loss.isnan()) and bool(g.isnan().all())
+
+
 @pytest.mark.parametrize("V", [5003, 170003])   # in registers, read twice
 def test_strides_and_types(mga, dev, V):
     """Student rows off a 16-byte boundary, columns that are not contiguous, strided

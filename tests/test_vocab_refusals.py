@@ -24,7 +24,8 @@ def _top(lib, **kw):
 
 @pytest.mark.parametrize("kw", [dict(x=None), dict(rs=99), dict(n=0), dict(v=0), dict(dtype=3), dict(k=0), dict(k=101),
                                 dict(v=2000, rs=2000, k=1025), dict(v=(1 << 20) + 1, rs=1 << 21), dict(t=0.0),
-                                dict(t=-1.0), dict(t=float("inf")), dict(t=float("nan")), dict(values=None),
+                                dict(t=-1.0), dict(t=float("inf")), dict(t=float("nan")), dict(t=1e-30),
+                                dict(values=None),
                                 dict(ids=None), dict(x=ctypes.c_void_p(65)), dict(x=ctypes.c_void_p(66), dtype=1)])
 def test_top_logits(mga, kw):
     refused(mga, _top(mga.load_library(), **kw))
@@ -44,7 +45,8 @@ def _fwd(lib, step=False, **kw):
 
 COMMON = [dict(x=None), dict(rs=99), dict(n=0), dict(dtype=5), dict(k=0), dict(k=1025, vrs=1025, irs=1025),
           dict(t=0.0), dict(t=float("nan")), dict(ids=None), dict(irs=3), dict(ids=ctypes.c_void_p(68), i64=1),
-          dict(values=None), dict(vrs=3), dict(vd=7), dict(loss=None), dict(sum=None), dict(ws=None), dict(ws=ctypes.c_void_p(72))]
+          dict(values=None), dict(vrs=3), dict(vd=7), dict(loss=None), dict(sum=None), dict(ws=None),
+          dict(ws=ctypes.c_void_p(72)), dict(t=1e-30), dict(t=1e30)]
 
 
 @pytest.mark.parametrize("step", [False, True])
@@ -113,7 +115,7 @@ def test_cpu_tensors(mga):
                  lambda: mga.embedding_grad(torch.zeros(2, 3, 4), ids, 5)):
         with pytest.raises(RuntimeError, match="GPU tensor"):
             call()
-    for t in (0.0, -1.0, float("nan"), float("inf")):
+    for t in (0.0, -1.0, float("nan"), float("inf"), 1e-30, 1e30):
         with pytest.raises(ValueError, match="temperature"):
             mga.top_logits_cross_entropy(x, torch.zeros(2, 3), ids, None, t)
 
