@@ -19,6 +19,7 @@
 // by the package's own Python function, with the same exception types.
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -94,6 +95,19 @@ bool same(const Tensor &a, const Tensor &b) { return a.scalar_type() == b.scalar
 void *stream(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 bool aligned16(const Tensor &t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+// A captured backward joins the stream of the leaf's gradient accumulator. An eager
+// graph that still lives has bound it to the default stream, which no capture may
+// touch: torch's engine then ends the process. Refused while it can be said.
+void check_capture(const char *fn, const Tensor &leaf) {
+  if (!at::GradMode::is_enabled() || !leaf.requires_grad() || !leaf.is_leaf() ||
+      c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None)
+    return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  const auto stream = node ? node->stream() : std::nullopt;
+  TORCH_CHECK(!stream || stream->id() != 0, fn, ": under graph capture, while an eager graph of the same leaf lives on "
+              "the default stream; release that graph first");
+}
 
 // [1, H, S, D] with unit stride on D and 16-byte aligned rows
 bool rows4(const Tensor &t) {
@@ -613,6 +627,7 @@ std::optional<Tensor> top_logits_ce(const Tensor &x, const Tensor &values, const
                                     const std::optional<Tensor> &lse, double tau) {
   if (!top_ce_operands(x, values, ids, lse)) return std::nullopt;
   const at::DeviceGuard guard(x.device());
+  check_capture("top_logits_cross_entropy", x);
   return TopLogitsCE::apply(x, values.detach(), ids, lse ? std::optional<Tensor>(lse->detach()) : lse, tau);
 }
 
@@ -715,6 +730,7 @@ std::optional<Tensor> embedding(const Tensor &ids, const Tensor &w, double scale
       w.size(0) > INT32_MAX || w.size(1) > INT32_MAX)
     return std::nullopt;
   const at::DeviceGuard guard(w.device());
+  check_capture("scaled_embedding", w);
   return Embedding::apply(ids, w, scale, padding_idx);
 }
 

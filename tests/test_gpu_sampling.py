@@ -105,6 +105,24 @@ def test_equal_and_masked_values(mga, dev, dtype):
         check(mga, x, uniform(8, dev, 20 + i), **s)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_far_from_zero(mga, dev, dtype):
+    """Rows masked with the type's lowest value, all of them too, and rows whose
+    largest logit is the type's largest."""
+    V, low = 5003, torch.finfo(dtype).min
+    x = logits(6, V, dtype, dev, seed=9)
+    x[0] = low                              # nothing left: uniform
+    x[1, :V // 2] = low
+    x[2, 0::2] = low
+    x[3] = low
+    x[3, 77] = low / 2
+    x[4, 1000::1000] = -low
+    x[5] = low / 4 * (1 + torch.randint(0, 4, (V,), device=dev) / 4)
+    for i, s in enumerate(SETTINGS):
+        print(f"case {dtype} {s}", flush=True)
+        check(mga, x, uniform(6, dev, i + 20), **s)
+
+
 def test_borders(mga, dev):
     """Four equal tokens: half of their weight is two of them, just above is three;
     quarters of the uniform fall to the next token."""
