@@ -3,9 +3,10 @@
 //
 // One workgroup takes a row in one pass (mga_vocab_row.hpp): the running maximum
 // and sum, and the largest element of each run of vectors, from which the few
-// vectors that hold a candidate are known and read again. Bound by the read where
-// two workgroups share a compute unit; the exponentials alone (152 a thread, 16
-// cycles a wave each) are half of the row's time there.
+// vectors that hold a candidate are known and read again. Two workgroups share a
+// compute unit, one's exponentials (152 a thread, 16 cycles a wave each: half of a
+// row's time) beside the other's loads. 1 024 x 151 936 bf16, k = 64: 79 us, 3.9
+// TB/s, where a copy moves 5.2.
 #include "mga_internal.hpp"
 #include "mga_vocab_row.hpp"
 
@@ -48,7 +49,9 @@ static void top_logits_typed(const void *x, int64_t xs, int32_t N, int32_t V, in
 
 void launch_top_logits(const void *x, int64_t xs, int32_t N, int32_t V, int dtype, int32_t k, float tau, void *values,
                        int32_t *ids, float *lse, hipStream_t st) {
-  auto run = dtype == kDtF32 ? top_logits_typed<float> : dtype == kDtF16 ? top_logits_typed<f16_t> : top_logits_typed<bf16_t>;
+  auto run = dtype == kDtF32   ? top_logits_typed<float>
+             : dtype == kDtF16 ? top_logits_typed<f16_t>
+                               : top_logits_typed<bf16_t>;
   run(x, xs, N, V, k, 1.f / tau, values, ids, lse, st);
 }
 

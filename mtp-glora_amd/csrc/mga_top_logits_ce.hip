@@ -87,7 +87,8 @@ __device__ __forceinline__ RowSum sum_elements(const T *p, int n, float c) {
     st.add(f, fmaxf(x, kRowNegInf), c);
   };
   constexpr int fill = RowElem<T>::kFill;
-  vectors_up<B>(reinterpret_cast<const i32x4 *>(p + head), nvec, i32x4{fill, fill, fill, fill}, [&](const i32x4 &v) {
+  const i32x4 none = {fill, fill, fill, fill};
+  vectors_up<B>(reinterpret_cast<const i32x4 *>(p + head), nvec, none, [&](const i32x4 &v) {
     float f[W], g = kRowNegInf;
 #pragma unroll
     for (int e = 0; e < W; ++e) g = fmaxf(g, f[e] = RowElem<T>::get(v, e));

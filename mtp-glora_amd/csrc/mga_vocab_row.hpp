@@ -21,7 +21,6 @@ namespace mga {
 
 constexpr int kRowThreads = 1024;
 constexpr int kRowWaves = kRowThreads / 64;
-constexpr int kRowMaxCols = 1 << 20;       // columns' width in rank_of
 constexpr int kListCap = 4096;             // candidates that are put in order in LDS
 constexpr int kMaxTop = 1024;              // most elements that are asked for in order
 constexpr float kRowNegInf = -__builtin_huge_valf();
@@ -251,8 +250,9 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, RowShared &sh, uint64
 }
 
 // sh.list[0, n) in descending order. Up to 256 entries by counting those above
-// each, by all threads (360: 22 000 cycles, 16 000 by the network); up to 1 024 by a bitonic network with an entry a thread,
-// whose steps within a wave need no barrier; more by one in LDS. Uses sh.bins.
+// each, by all threads (360 of them: 22 000 cycles, 16 000 by the network); up to
+// 1 024 by a bitonic network with an entry a thread, whose steps within a wave need
+// no barrier; more by one in LDS. Uses sh.bins.
 __device__ __forceinline__ void sort_list(RowShared &sh, int n) {
   const int tid = threadIdx.x;
   __syncthreads();
@@ -358,7 +358,8 @@ __device__ __forceinline__ void find_bin(RowShared &sh, const uint64_t *bins, in
 // The rank of the element that is number `ties` by column among those of `key` (and
 // of at least `floor`): more than that have the key. Uses sh.list.
 template <typename T>
-__device__ __forceinline__ uint64_t column_threshold(const Row<T> &row, RowShared &sh, uint64_t floor, uint32_t key, uint64_t ties) {
+__device__ __forceinline__ uint64_t column_threshold(const Row<T> &row, RowShared &sh, uint64_t floor, uint32_t key,
+                                                     uint64_t ties) {
   uint32_t prefix = 0;
   uint64_t total;
   for (int shift = 20; shift > 0; shift -= 10) {
@@ -382,7 +383,8 @@ __device__ __forceinline__ uint64_t column_threshold(const Row<T> &row, RowShare
 // number that depends on the value alone. Digits of the key from the top, 12
 // bits at first, then of the columns of the elements that share the last key.
 template <bool ONES, typename T, typename WF, typename NF>
-__device__ __forceinline__ uint64_t radix_threshold(const Row<T> &row, RowShared &sh, uint64_t floor, WF weight, NF need) {
+__device__ __forceinline__ uint64_t radix_threshold(const Row<T> &row, RowShared &sh, uint64_t floor, WF weight,
+                                                    NF need) {
   uint64_t want = 0, total = 0;
   uint32_t prefix = 0;
   int shift = 32;

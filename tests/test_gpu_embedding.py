@@ -192,6 +192,37 @@ def test_gradient_past_the_cache(mga, dev):
     assert not g.any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,H", [(511, 5000, 3), (512, 9, 520), (513, 9, 520), (512, 1, 1), (300, 70000, 8),
+                                   (40, 3, 70001), (1, 9000, 1), (200, 16500, 8192)])
+def test_few_tokens(mga, dev, dtype, n, V, H):
+    """About the number of tokens up to which one launch takes them all, with tables
+    on both sides of the size to which it does; both types of ids, written into rows
+    that lie apart, and added to, where rows without a token keep every bit."""
+    print(f"case {n} {V} {H} {dtype}", flush=True)
+    ids = tokens(n, V, dev, seed=9).int()
+    ids[::11] = -1
+    rows = torch.unique(ids[ids >= 0].long())
+    i = np.where(ids.cpu().numpy() < 0, -1, np.searchsorted(rows.cpu().numpy(), ids.cpu().numpy()))
+    dy = table(n, H, dtype, dev, seed=8)
+    want, bound = vo.embedding_grad(f64(dy), i, len(rows), 2.0), grad_bound(f64(dy), i, len(rows), 2.0)
+    buf = torch.full((V, H + 8), 7.0, device=dev, dtype=dtype)
+    out = buf[:, :H]
+    for given in (ids, ids.long()):
+        out.fill_(float("nan"))
+        mga.embedding_grad(dy, given, V, 2.0, out=out)
+        close(out[rows], want, bound, dtype)
+        assert bool((buf[:, H:] == 7).all())
+        out[rows] = 0
+        assert not out.any()
+    out.fill_(float("nan"))
+    out[rows] = 1.0
+    mga.embedding_grad(dy, ids, V, 2.0, out=out, accumulate=True)
+    close(out[rows], want + 1, bound + torch.finfo(dtype).eps * (np.abs(want) + 1), dtype)
+    out[rows] = float("nan")
+    assert bool(out.isnan().all())
+
+
 def test_layer(mga, dev):
     base = torch.nn.Embedding(30, 24, padding_idx=3, device=dev)
     layer = mga.ScaledEmbedding.wrap(base, 4.0)
