@@ -612,7 +612,9 @@ struct TopLogitsCE : public Function<TopLogitsCE> {
     const at::DeviceGuard guard(x.device());
     const Rows rx = *rows_of(x), ri = *rows_of(ids);
     const float *stats = s[2].data_ptr<float>();
-    const Tensor go = grad[0].detach().reshape({1}).to(x.device(), at::kFloat).contiguous();
+    // of a scalar: one value, contiguous as it is
+    const Tensor &g0 = grad[0];
+    const Tensor go = g0.scalar_type() == at::kFloat && g0.device() == x.device() ? g0 : g0.detach().to(x.device(), at::kFloat);
     Tensor gx = at::empty(x.sizes(), x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
     check_rc("mga_top_logits_ce_bwd",
              g.mga_top_logits_ce_bwd(rx.data, rx.stride, ri.data, ri.stride, ids.scalar_type() == at::kLong,
