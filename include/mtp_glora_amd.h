@@ -432,7 +432,7 @@ int mga_soft_ce_bwd(const void *student, int64_t student_row_stride,
  * null) the row's log sum_j exp(x_j / temperature) in fp32 (-inf for a row of
  * -inf alone, NaN where the row holds a NaN). Rows of n_cols <= 1 048 576
  * logits, row r at logits + r * row_stride elements, columns contiguous;
- * 1 <= k <= min(n_cols, 1024); temperature within 2^-60 to 2^60.
+ * 1 <= k <= min(n_cols, 1024); temperature within 2^-60 to 2^60; n_rows < 2^22.
  * No counterpart in the reference, which keeps a teacher's whole rows
  * (mtp_glora/core/mtp.py:121-126): what is kept of them here feeds
  * mga_top_logits_ce_*.
@@ -456,8 +456,8 @@ int mga_top_logits(const void *logits, int64_t row_stride, int32_t n_rows, int32
  * whatever its logits are; a student logit of -inf at an entry of q > 0 gives an
  * infinite loss; NaN and +inf among other rows' student logits give NaN. An id
  * may stand in a row more than once: its q add up.
- * 1 <= k <= 1024. workspace: mga_top_logits_ce_workspace_floats fp32 values,
- * 16-byte aligned.
+ * 1 <= k <= 1024, n_rows < 2^22. workspace: mga_top_logits_ce_workspace_floats fp32
+ * values, 16-byte aligned.
  * Stands beside mga_soft_ce_* (loss.py:259-330), which reads whole teacher rows.
  */
 int64_t mga_top_logits_ce_workspace_floats(int32_t n_rows, int32_t n_cols);
@@ -471,7 +471,7 @@ int mga_top_logits_ce_fwd(const void *student, int64_t student_row_stride, const
  * Its backward for the student (the teacher gets none):
  *   grad[r, j] = grad_output * tau * (Q p_j - sum over k with id_k = j of q_k),
  * in the student's dtype, one rounding; grad_output: one fp32 value in device
- * memory.
+ * memory. grad may not overlap student.
  */
 int mga_top_logits_ce_bwd(const void *student, int64_t student_row_stride, const void *ids, int64_t ids_row_stride,
                           int32_t ids_are_int64, const float *q, const float *stats, int32_t n_rows, int32_t n_cols,
@@ -481,7 +481,7 @@ int mga_top_logits_ce_bwd(const void *student, int64_t student_row_stride, const
 /*
  * Loss and gradient in one call, with an upstream gradient that the host knows:
  * loss_sum as mga_top_logits_ce_fwd, grad as mga_top_logits_ce_bwd with
- * grad_output = scale. With 128 rows and more a row's second reading follows its
+ * grad_output = scale. With 96 rows and more a row's second reading follows its
  * first and comes from the caches; fewer are taken as by the two calls. grad may
  * not overlap student.
  * workspace: mga_top_logits_ce_step_workspace_floats fp32 values, 16-byte aligned.
@@ -505,12 +505,14 @@ int mga_top_logits_ce_step(const void *student, int64_t student_row_stride, cons
  *     of those the tokens with w >= min_p (min_p <= 0: all; the largest stays),
  *   and the token is the first, by ascending column, at which the running sum of
  *   the weights that are left exceeds u times their total.
- * Weights are computed in 64 bits and held in whole multiples of 2^-45 (2^-42 at
- * the largest n_cols) of the largest, whose sums are exact. NaN and -inf logits are never drawn; a row with no
- * other gives -1; u < 0 or NaN draws as 0, u >= 1 the last token that is left.
+ * Weights are computed in 64 bits and held in whole multiples of 2^-45 (from
+ * 131 073 columns 2^-44, at the largest n_cols 2^-42) of the largest, whose sums
+ * are exact. NaN and -inf logits are never drawn; a row with no other gives -1;
+ * u < 0 or NaN draws as 0, u >= 1 the last token that is left.
  * temperature, top_k, top_p and min_p: one value a row in device memory, or
- * null for the *_all value. n_cols <= 1 048 576. No counterpart in the reference
- * (its sampler head is trained, never run; mtp_glora/core/mtp.py:28-144).
+ * null for the *_all value. n_cols <= 1 048 576, n_rows < 2^22. No counterpart in
+ * the reference (its sampler head is trained, never run;
+ * mtp_glora/core/mtp.py:28-144).
  */
 int mga_sample(const void *logits, int64_t row_stride, int32_t n_rows, int32_t n_cols, int32_t dtype,
                const float *uniform, const float *temperature, float temperature_all, const int32_t *top_k,
@@ -520,7 +522,8 @@ int mga_sample(const void *logits, int64_t row_stride, int32_t n_rows, int32_t n
 /*
  * Scaled embedding lookup: out[n, :] = T(scale * weight[ids[n], :]) for n_ids ids
  * (int64 if ids_are_int64 else int32) of a [n_rows, width] table, T = rounding to
- * the dtype; zeros for an id outside the table. The lookup at the start of
+ * the dtype; zeros for an id outside the table. n_ids times the 1 024s of columns
+ * (rounded up) < 2^26, width < 2^23; out may not overlap weight. The lookup at the start of
  * Qwen3Model.forward (mtp_glora/models/modeling_qwen3.py:436); the table is the one
  * that resize_token_embeddings grows (:616).
  */
@@ -530,7 +533,8 @@ int mga_embedding_fwd(const void *ids, int32_t ids_are_int64, int32_t n_ids, con
 
 /*
  * Its gradient: grad_weight[v, :] = T(scale * sum over n with ids[n] = v of
- * grad_out[n, :]), summed in fp32 in ascending order of n; ids equal to
+ * grad_out[n, :]), summed in fp32 in a fixed order (parts of ascending n, added in
+ * their order); n_ids < 2^30; grad_weight may not overlap grad_out; ids equal to
  * padding_idx (-1: none) or outside the table count nowhere. The whole of
  * grad_weight [n_rows, width] is written, or, with accumulate, the sums are added
  * to it (one rounding) and rows without a token are left as they are.

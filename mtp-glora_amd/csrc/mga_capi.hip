@@ -861,6 +861,19 @@ int check_matrix(const char *fn, const char *name, const void *p, int64_t rs, in
   return MGA_OK;
 }
 
+// Do rows [p_rows, cols] at p and rows [q_rows, cols] at q share a byte's range?
+bool overlap(const void *p, int64_t prs, const void *q, int64_t qrs, int64_t p_rows, int64_t q_rows, int64_t cols, int peb,
+             int qeb) {
+  const uintptr_t p0 = reinterpret_cast<uintptr_t>(p), q0 = reinterpret_cast<uintptr_t>(q);
+  return p0 < q0 + (uintptr_t)((q_rows - 1) * qrs + cols) * qeb && q0 < p0 + (uintptr_t)((p_rows - 1) * prs + cols) * peb;
+}
+
+// Rows that are a workgroup each: a launch has fewer than 2^32 threads.
+int check_row_count(const char *fn, int32_t n_rows) {
+  if (n_rows < 1 << 22) return MGA_OK;
+  return fail(MGA_ERR_INVALID, "%s: %d rows (fewer than %d)", fn, n_rows, 1 << 22);
+}
+
 // Its square and its reciprocal times log2(e) are ordinary fp32 numbers.
 int check_temperature(const char *fn, float v) {
   if (v >= 0x1p-60f && v <= 0x1p60f) return MGA_OK;
@@ -875,6 +888,7 @@ int check_top_k(const char *fn, int32_t k) {
 int check_top_ce(const char *fn, const mga::TopLogitsCeArgs &a, int32_t dtype) {
   int rc = check_matrix(fn, "student", a.x, a.xs, a.N, a.V, dtype);
   if (rc == MGA_OK) rc = check_top_k(fn, a.K);
+  if (rc == MGA_OK) rc = check_row_count(fn, a.N);
   if (rc == MGA_OK) rc = check_temperature(fn, a.tau);
   if (rc != MGA_OK) return rc;
   if (!a.ids || a.ids_rs < a.K) return fail(MGA_ERR_INVALID, "%s: ids null or with a row stride below k", fn);
@@ -914,6 +928,7 @@ int mga_top_logits(const void *logits, int64_t row_stride, int32_t n_rows, int32
                    float temperature, void *values, int32_t *ids, float *lse, void *stream) {
   const char *fn = "mga_top_logits";
   int rc = check_matrix(fn, "logits", logits, row_stride, n_rows, n_cols, dtype);
+  if (rc == MGA_OK) rc = check_row_count(fn, n_rows);
   if (rc == MGA_OK) rc = check_top_k(fn, k);
   if (rc == MGA_OK) rc = check_temperature(fn, temperature);
   if (rc != MGA_OK) return rc;
@@ -963,6 +978,9 @@ int mga_top_logits_ce_bwd(const void *student, int64_t student_row_stride, const
   if (rc == MGA_OK) rc = check_matrix(fn, "grad", grad, grad_row_stride, n_rows, n_cols, dtype);
   if (rc != MGA_OK) return rc;
   if (!q || !stats || !grad_output) return fail(MGA_ERR_INVALID, "%s: null q, stats or grad_output", fn);
+  if (overlap(student, student_row_stride, grad, grad_row_stride, n_rows, n_rows, n_cols, elem_bytes(dtype),
+              elem_bytes(dtype)))
+    return fail(MGA_ERR_INVALID, "%s: grad overlaps student", fn);
   mga::launch_top_ce_bwd(a, dtype, (hipStream_t)stream);
   return check_launch(fn);
 }
@@ -982,10 +1000,9 @@ int mga_top_logits_ce_step(const void *student, int64_t student_row_stride, cons
   if (rc == MGA_OK) rc = check_teacher(fn, a, workspace);
   if (rc == MGA_OK) rc = check_matrix(fn, "grad", grad, grad_row_stride, n_rows, n_cols, dtype);
   if (rc != MGA_OK) return rc;
-  const uintptr_t eb = elem_bytes(dtype), x0 = reinterpret_cast<uintptr_t>(student), g0 = reinterpret_cast<uintptr_t>(grad);
-  const uintptr_t x1 = x0 + ((uintptr_t)(n_rows - 1) * student_row_stride + n_cols) * eb;
-  const uintptr_t g1 = g0 + ((uintptr_t)(n_rows - 1) * grad_row_stride + n_cols) * eb;
-  if (x0 < g1 && g0 < x1) return fail(MGA_ERR_INVALID, "%s: grad overlaps student", fn);
+  if (overlap(student, student_row_stride, grad, grad_row_stride, n_rows, n_rows, n_cols, elem_bytes(dtype),
+              elem_bytes(dtype)))
+    return fail(MGA_ERR_INVALID, "%s: grad overlaps student", fn);
   mga::launch_top_ce_step(a, dtype, workspace, (hipStream_t)stream);
   return check_launch(fn);
 }
@@ -995,7 +1012,8 @@ int mga_sample(const void *logits, int64_t row_stride, int32_t n_rows, int32_t n
                int32_t top_k_all, const float *top_p, float top_p_all, const float *min_p, float min_p_all,
                int64_t *token, void *stream) {
   const char *fn = "mga_sample";
-  const int rc = check_matrix(fn, "logits", logits, row_stride, n_rows, n_cols, dtype);
+  int rc = check_matrix(fn, "logits", logits, row_stride, n_rows, n_cols, dtype);
+  if (rc == MGA_OK) rc = check_row_count(fn, n_rows);
   if (rc != MGA_OK) return rc;
   if (n_cols > kMaxVocab) return fail(MGA_ERR_INVALID, "%s: %d columns (at most %d)", fn, n_cols, kMaxVocab);
   if (!uniform || !token) return fail(MGA_ERR_INVALID, "%s: null uniform or token", fn);
@@ -1014,9 +1032,11 @@ int mga_embedding_fwd(const void *ids, int32_t ids_are_int64, int32_t n_ids, con
   if (rc != MGA_OK || n_ids == 0) return rc;
   rc = check_matrix(fn, "out", out, out_row_stride, n_ids, width, dtype);
   if (rc != MGA_OK) return rc;
-  if ((int64_t)n_ids * (width / 1024 + 1) >= int64_t(1) << 32)
+  if ((int64_t)n_ids * ((width + 1023) / 1024) >= int64_t(1) << 26)
     return fail(MGA_ERR_INVALID, "%s: %d ids of width %d are too many", fn, n_ids, width);
   const int eb = elem_bytes(dtype);
+  if (overlap(weight, weight_row_stride, out, out_row_stride, n_rows, n_ids, width, eb, eb))
+    return fail(MGA_ERR_INVALID, "%s: out overlaps weight", fn);
   const mga::EmbedArgs a{ids, weight, weight_row_stride, nullptr, 0, out, out_row_stride, scale, -1, 0, n_ids, n_rows,
                          width, ids_are_int64 != 0};
   mga::launch_embed_fwd(a, dtype, (int64_t)width * eb % 16 == 0 && vec_rows(weight, weight_row_stride, eb) &&
@@ -1045,6 +1065,9 @@ int mga_embedding_bwd(const void *grad_out, int64_t grad_out_row_stride, const v
     return fail(MGA_ERR_INVALID, "%s: workspace null, not 16-byte aligned or smaller than %lld bytes", fn,
                 (long long)mga::embed_workspace_bytes(n_ids, width));
   const int eb = elem_bytes(dtype), ob = elem_bytes(grad_weight_dtype);
+  if (n_ids >= 1 << 30) return fail(MGA_ERR_INVALID, "%s: %d ids (fewer than %d)", fn, n_ids, 1 << 30);
+  if (n_ids > 0 && overlap(grad_out, grad_out_row_stride, grad_weight, grad_weight_row_stride, n_ids, n_rows, width, eb, ob))
+    return fail(MGA_ERR_INVALID, "%s: grad_weight overlaps grad_out", fn);
   const mga::EmbedArgs a{ids, nullptr, 0, grad_out, grad_out_row_stride, grad_weight, grad_weight_row_stride, scale,
                          padding_idx, 0, n_ids, n_rows, width, ids_are_int64 != 0};
   const bool vec = (int64_t)width * eb % 16 == 0 && (n_ids == 0 || vec_rows(grad_out, grad_out_row_stride, eb)) &&

@@ -8,7 +8,7 @@
 //
 // Neighbouring borders of that sum lie 2^-17 of it apart in a row of 151 936
 // about equal tokens, so the weights e^{(x - max) / T} are taken in 64 bits and
-// held as whole numbers of 2^-s of the largest (s = 45 at that width): their sums
+// held as whole numbers of 2^-s of the largest (s = 44 at that width): their sums
 // are exact and the same in whatever order they are formed.
 //
 // One workgroup a row (mga_vocab_row.hpp). Rows with 1 <= top_k <= 1024, or whose

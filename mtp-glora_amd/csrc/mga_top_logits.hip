@@ -28,7 +28,7 @@ __global__ __launch_bounds__(kRowThreads, 8) void top_logits_kernel(const T *__r
     tmax = scan_row<true, 2>(row, sh, group, c, st);
     const float m = block_max(st.m, sh);
     const float d = block_sum(far(m, c) ? count_equal<kRowThreads>(x + n * xs, V, m) : sum_at(st, m, c), sh);
-    if (threadIdx.x == 0) lse[n] = m == -kRowNegInf ? m : m * itau + logf(sum_at_max(m, d, c));
+    if (threadIdx.x == 0) lse[n] = m * itau + logf(sum_at_max(m, d, c));
   } else {
     tmax = scan_row<false, 2>(row, sh, group, c, st);
   }

@@ -185,7 +185,7 @@ __global__ __launch_bounds__(kThreads) void top_ce_partial_kernel(const T *__res
 #pragma unroll
   for (int w = 1; w < kThreads / 64; ++w) m = fmaxf(m, wm[w]);
   if (far(m, c)) {
-    float s = count_equal<kThreads>(xr, n, m);
+    float s = count_equal<kThreads>(xr, n, m) + (m - m);   // NaN for +inf
 #pragma unroll
     for (int i = 32; i >= 1; i >>= 1) s += __shfl_xor(s, i, 64);
     __syncthreads();
@@ -459,8 +459,8 @@ struct TeacherRow {
     for (int i = 0; i < kEach; ++i) top = fmaxf(top, t[i] * itau);
     const float2 most = block_max2<B>({st.m, top}, sh.part);
     const float m = most.x, norm = a.lse ? a.lse[n] : most.y;
-    // d; of the weights; of their part of the loss
-    float3 sums = {far(m, c) ? count_equal<B>(xr, a.V, m) : sum_at(st, m, c), 0.f, 0.f};
+    // d (NaN for m = +inf); of the weights; of their part of the loss
+    float3 sums = {far(m, c) ? count_equal<B>(xr, a.V, m) + (m - m) : sum_at(st, m, c), 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       q[i] = teacher_weight(t[i], id[i], norm, itau);

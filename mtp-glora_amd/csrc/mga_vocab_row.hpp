@@ -478,10 +478,10 @@ __device__ __forceinline__ float sum_at_max(float m, float d, float c) {
   return m == kRowNegInf || far(m, c) ? d : d * __builtin_amdgcn_exp2f(-__builtin_fmaf(m, c, -scaled(m, c)));
 }
 // This thread's part of d of n elements whose maximum m is far: how many equal it. NaN
-// where there is one, and for m = +inf.
+// where there is one.
 template <int B, typename T>
 __device__ __forceinline__ float count_equal(const T *p, int n, float m) {
-  float s = m - m;
+  float s = 0.f;
   for (int i = threadIdx.x; i < n; i += B) {
     const float x = (float)p[i];
     s += x == m ? 1.f : x == x ? 0.f : x;

@@ -19,6 +19,7 @@ from .ops import _dev, _stream, dtype_code
 
 MAX_TOP = 1024          # most logits kept of a row
 MAX_VOCAB = 1 << 20     # longest row that is put in order
+INT32_MAX = (1 << 31) - 1
 
 
 class TopLogits(NamedTuple):
@@ -32,6 +33,8 @@ def row_view(name: str, t: torch.Tensor) -> torch.Tensor:
     _dev(name, t)
     if t.dim() < 1 or t.shape[-1] == 0:
         raise ValueError(f"{name}: expected [..., V] with V > 0, got {tuple(t.shape)}")
+    if max(t.shape[-1], t.shape[:-1].numel()) > INT32_MAX:
+        raise ValueError(f"{name}: {tuple(t.shape)} has more than {INT32_MAX} rows or columns")
     v = t.detach().reshape(-1, t.shape[-1])
     if v.stride(1) != 1 or (v.shape[0] > 1 and v.stride(0) < v.shape[1]):
         v = v.contiguous()

@@ -12,6 +12,7 @@ import torch
 from torch import nn
 
 from . import _lib
+from .distill import INT32_MAX
 from .ops import _dev, _stream, dtype_code
 
 
@@ -21,6 +22,8 @@ def _check(ids: torch.Tensor, device) -> torch.Tensor:
         raise TypeError(f"ids: int32 or int64 required (got {ids.dtype})")
     if ids.device != device:
         raise ValueError(f"ids are on {ids.device}, the table on {device}")
+    if ids.numel() > INT32_MAX:
+        raise ValueError(f"{ids.numel()} ids; at most {INT32_MAX}")
     return ids.detach().reshape(-1).contiguous()
 
 
@@ -40,7 +43,7 @@ def embedding_grad(grad_out: torch.Tensor, ids: torch.Tensor, num_embeddings: in
                    accumulate: bool = False) -> torch.Tensor:
     """Gradient [num_embeddings, H] of scaled_embedding for its table:
     row v is scale times the sum of ``grad_out`` [..., H] over the tokens with id v,
-    added in fp32 in the order of the tokens; ids equal to ``padding_idx`` or
+    added in fp32 in a fixed order; ids equal to ``padding_idx`` or
     outside the table count nowhere. ``out`` (the gradients' dtype or fp32) receives
     it; with ``accumulate`` the sums are added to ``out``, whose other rows are
     neither read nor written: the chunks of a sequence can share one buffer."""
@@ -49,7 +52,7 @@ def embedding_grad(grad_out: torch.Tensor, ids: torch.Tensor, num_embeddings: in
         raise ValueError(f"grad_out {tuple(grad_out.shape)} does not fit ids {tuple(ids.shape)}")
     code, H, V = dtype_code(grad_out.dtype), grad_out.shape[-1], int(num_embeddings)
     i = _check(ids, grad_out.device)
-    if V <= 0 or H <= 0:
+    if not (0 < V <= INT32_MAX and 0 < H <= INT32_MAX):
         raise ValueError(f"bad table size [{V}, {H}]")
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
@@ -109,7 +112,7 @@ def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
     table. Differentiable in ``weight`` (a dense gradient, embedding_grad);
     ``padding_idx`` is looked up like any other id and has no gradient."""
     _dev("weight", weight)
-    if weight.dim() != 2 or weight.numel() == 0:
+    if weight.dim() != 2 or weight.numel() == 0 or max(weight.shape) > INT32_MAX:
         raise ValueError(f"weight: expected [V, H], got {tuple(weight.shape)}")
     dtype_code(weight.dtype)
     if padding_idx is not None:

@@ -97,6 +97,27 @@ def test_strides(mga, dev, dtype, off):
     check_top(mga, x[0].expand(3, 9001), 4)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinities_with_nan(mga, dev, dtype):
+    """A NaN makes the log-sum-exp NaN, beside +inf too; +inf in the student's row makes
+    loss and gradient NaN."""
+    x = logits(4, 3001, dtype, dev, seed=21)
+    x[0, 5], x[0, 9] = float("inf"), float("nan")
+    x[1, 5:8] = float("inf")
+    x[2, :] = float("inf")
+    x[2, 7] = float("nan")
+    t = check_top(mga, x, 4)
+    assert t.lse.isnan().tolist() == [True, False, True, False]
+    v = torch.zeros(4, 4, device=dev)
+    for n in (1, 100):
+        y, vals, ids = x[1:2].repeat(n, 1), v[:1].repeat(n, 1), t.ids[3:].repeat(n, 1)
+        loss, g = mga.top_logits_loss_and_grad(y, vals, ids)
+        ys = y.clone().requires_grad_()
+        total = mga.top_logits_cross_entropy(ys, vals, ids)
+        total.backward()
+        assert bool(loss.isnan()) and bool(total.isnan()) and bool(g.isnan().all()) and bool(ys.grad.isnan().all())
+
+
 def test_no_rows_and_refusals(mga, dev):
     x = torch.randn(2, 50, device=dev)
     r = mga.top_logits(x[:0], 4)

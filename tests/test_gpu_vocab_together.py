@@ -213,6 +213,19 @@ def test_broadcast_inputs(mga, dev, dtype):
         assert bool(((got[0].float() - parts.float().sum(0)).abs() <= bound).all())
 
 
+def test_sizes_past_32_bits_are_refused(mga, dev):
+    n = 1 << 31
+    x, ids = torch.zeros(1, 1, device=dev).expand(n, 1), torch.zeros(1, dtype=torch.int32, device=dev).expand(n)
+    top = torch.zeros(1, 1, device=dev).expand(n, 1), torch.zeros(1, 1, dtype=torch.int32, device=dev).expand(n, 1)
+    w = torch.zeros(3, 1, device=dev)
+    for call in (lambda: mga.top_logits(x, 1), lambda: mga.sample_tokens(x, x[:, 0]),
+                 lambda: mga.top_logits_cross_entropy(x, *top), lambda: mga.top_logits_loss_and_grad(x, *top),
+                 lambda: mga.scaled_embedding(ids, w), lambda: mga.embedding_grad(x, ids, 3),
+                 lambda: mga.embedding_grad(w, ids[:3], n), lambda: mga.scaled_embedding(ids[:3], x)):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_past_2_31_elements(mga, dev):
     """The last rows of tensors of more than 2^31 elements are the same rows alone."""
     V, n = 151936, 14200

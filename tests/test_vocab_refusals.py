@@ -100,6 +100,24 @@ def test_embedding_bwd(mga, kw):
                                        a["dtype"], a["dw"], a["wrs"], a["wd"], 0, a["ws"], a["wn"], None))
 
 
+def test_too_many_rows(mga):
+    lib, n = mga.load_library(), 1 << 22
+    refused(mga, _top(lib, n=n), b"rows")
+    for step in (False, True):
+        refused(mga, _fwd(lib, step, n=n, grad=ctypes.c_void_p(1 << 40)), b"rows")
+    refused(mga, lib.mga_sample(P, 10, n, 10, 0, P, None, 1.0, None, 0, None, 1.0, None, 0.0, P, None), b"rows")
+    far = ctypes.c_void_p(1 << 40)
+    refused(mga, lib.mga_embedding_fwd(P, 0, 1 << 26, P, 8, 10, 8, 1.0, 0, far, 8, None), b"too many")
+    refused(mga, lib.mga_embedding_bwd(P, 8, P, 0, 1 << 30, 1.0, -1, 10, 8, 0, far, 8, 0, 0, P, 1 << 40, None), b"ids")
+
+
+def test_overlaps(mga):
+    lib, at = mga.load_library(), ctypes.c_void_p(64 + 2 * (199 - 4))
+    refused(mga, lib.mga_top_logits_ce_bwd(P, 100, P, 4, 0, P, P, 2, 100, 4, 1.0, 0, P, at, 100, None), b"overlaps")
+    refused(mga, lib.mga_embedding_fwd(P, 0, 3, P, 8, 25, 8, 1.0, 0, at, 8, None), b"overlaps")
+    refused(mga, lib.mga_embedding_bwd(P, 8, P, 0, 25, 1.0, -1, 10, 8, 0, at, 8, 0, 0, P, 1 << 20, None), b"overlaps")
+
+
 def test_workspace_sizes_of_no_work(mga):
     lib = mga.load_library()
     assert lib.mga_embedding_workspace_bytes(0, 8) == 0
