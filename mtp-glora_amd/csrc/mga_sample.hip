@@ -18,7 +18,7 @@
 // take few values, so their weights are tabulated and a histogram of the values
 // gives the thresholds. 256 rows of 151 936 bf16, a workgroup and a compute unit
 // each: the largest logit 17 us (4.5 TB/s), top-k 40 26, temperature alone 49,
-// top-p 0.95 with thousands left 77, of which the histogram's and the table's reads
+// top-p 0.95 with thousands left 67, of which the histogram's and the table's reads
 // of LDS at random bound the last two passes.
 #include "mga_internal.hpp"
 #include "mga_vocab_row.hpp"
@@ -79,17 +79,22 @@ struct RowWeight {
   double c, base;        // 768 + (x - top) c = x c + base: 43 bits of fraction in [512, 1024)
   float low, top;        // x <= low has no weight
   const double *roots;   // 2^{i / 256}
-  int s;
+  int s, rough;
   __device__ __forceinline__ RowWeight(const Weight &w, const double *table) : top(w.top), roots(table), s(w.s) {
     // c so large that the number below top is 60 to 122 powers of two away: a larger one changes no weight
     c = fmin(w.c, 1020054733.0 / fabs(w.topd));
     base = 768.0 - w.topd * c;
+    // top c + base is 768 where base has its 43 bits, else next to it
+    rough = __builtin_amdgcn_readfirstlane(!(fabs(base) < 1024.0));
     const double l = w.topd - (s + 3) / c;
     low = (float)l;
     if ((double)low > l) low = rank_value((uint64_t)(value_key(low) - 1) << 32);   // the next one down
   }
-  // x finite (or +inf, which counts as top)
-  __device__ __forceinline__ uint64_t operator()(float x) const {
+  // x finite (or +inf, which counts as top). The weight of top is 2^s itself: a share of
+  // equal largest elements that is a whole number of them stays one.
+  __device__ __forceinline__ uint64_t operator()(float x) const { return x >= top ? uint64_t(1) << s : fine(x); }
+  // The same unless rough.
+  __device__ __forceinline__ uint64_t fine(float x) const {
     const double m = __builtin_fma((double)fminf(fmaxf(x, low), top), c, base);
     const uint64_t bits = __builtin_bit_cast(uint64_t, m);
     const uint32_t hi = (uint32_t)(bits >> 32);   // 12 bits of exponent, 9 of whole part, 11 of fraction
@@ -237,11 +242,12 @@ __device__ __forceinline__ uint64_t tied_threshold(const Row<bf16_t> &row, RowSh
 }
 
 // Threshold of top_k and top_p by the histogram of the row's values (counted in
-// sh.list), and how many elements it leaves; what scan_row left stays. False where
-// a cut falls among the values below the window.
+// sh.list), and how many elements it leaves; what scan_row left stays. More than
+// kListCap: its key alone, and how many elements of that key count (quota). False
+// where a cut falls among the values below the window.
 __device__ __forceinline__ bool table_threshold(const Row<bf16_t> &row, RowShared &sh, TableShared &tab,
                                                 const Tabulated &t, bool by_k, uint64_t top_k, bool by_p, float top_p,
-                                                uint64_t *thr, uint64_t *kept) {
+                                                uint64_t *thr, uint64_t *kept, uint64_t *quota) {
   const int tid = threadIdx.x;
   static_assert(sizeof(sh.list) >= kTable * sizeof(uint32_t), "the counts");
   uint32_t *count = reinterpret_cast<uint32_t *>(sh.list);
@@ -350,7 +356,9 @@ __device__ __forceinline__ bool table_threshold(const Row<bf16_t> &row, RowShare
   const uint64_t key = (uint64_t)value_key(value) << 32;
   const uint32_t there = count[entry_at(cut)];
   __syncthreads();   // the counts are over
-  if (ties >= there) *thr = key;
+  *thr = key;
+  if (ties >= there) return true;
+  if (*kept > kListCap) *quota = ties;
   else *thr = there > kFewTies ? column_threshold(row, sh, 0, (uint32_t)(key >> 32), ties)
                                : tied_threshold(row, sh, value, (int)there, (int)ties);
   return true;
@@ -425,8 +433,16 @@ __device__ __forceinline__ int pick_in_list(RowShared &sh, int n, const WF &weig
 template <typename T>
 __device__ __forceinline__ uint64_t vector_sum(const Computed &weight, const i32x4 &v) {
   uint64_t s = 0;
+  if (weight.weight.rough) {   // of the whole row
+#pragma unroll 1
+    for (int e = 0; e < RowElem<T>::W; ++e) s += weight(RowElem<T>::get(v, e));
+    return s;
+  }
 #pragma unroll
-  for (int e = 0; e < RowElem<T>::W; ++e) s += weight(RowElem<T>::get(v, e));
+  for (int e = 0; e < RowElem<T>::W; ++e) {   // 96 rows of 32 003 fp32: 18.3 us, with the comparison to top 19.4
+    const float x = RowElem<T>::get(v, e);
+    s += x >= weight.least ? weight.weight.fine(x) : 0;
+  }
   return s;
 }
 template <typename T>
@@ -447,47 +463,70 @@ __device__ __forceinline__ uint64_t vector_sum(const Tabulated &t, const i32x4 &
   return s;
 }
 
-// The same among all elements of at least `thr`. `weight` is 0 for smaller values.
+// The same among all elements of at least weight.least (`weight` is 0 for smaller
+// ones), of those equal to it the first `quota` by column (~0: all).
 template <typename T, typename WF>
-__device__ __forceinline__ int pick_in_row(const Row<T> &row, RowShared &sh, uint64_t thr, const WF &weight, float u) {
+__device__ __forceinline__ int pick_in_row(const Row<T> &row, RowShared &sh, uint64_t quota, const WF &weight, float u) {
   constexpr int W = RowElem<T>::W;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  // of the elements equal to least, the last column that counts
-  const int last = (uint32_t)thr ? rank_col(thr) : row.V;
-  auto kept = [&](float x, int col) { return x == weight.least && col > last ? uint64_t(0) : weight(x); };
+  const bool some = quota != ~uint64_t(0);
   const uint64_t tie = weight(weight.least);
-  auto lane_sum = [&](const i32x4 &v, int col) {
-    uint64_t s = vector_sum<T>(weight, v);   // 0 of the -inf past the row's end
-    if (col + W - 1 > last) {
-      int out = 0;
-#pragma unroll
-      for (int e = 0; e < W; ++e) out += RowElem<T>::get(v, e) == weight.least && col + e > last;
-      s -= (uint64_t)out * tie;
-    }
-    return s;
+  uint32_t *tied = reinterpret_cast<uint32_t *>(sh.list);   // a group's elements equal to the least
+  // the weight of the `n` of them, behind `before` others, that do not count
+  auto over = [&](uint64_t before, uint64_t n) {
+    return (before + n <= quota ? 0 : before >= quota ? n : before + n - quota) * tie;
   };
   // In order of the columns: the elements before the vectors, the (vector, wave)
   // groups, the elements behind them; within a group its lanes, within a lane its
   // elements.
   int i = 0;
   row.template each_vec<3>(
-      [&](const i32x4 &v, int col) {
-        const uint64_t s = last_lane(wave_scan(lane_sum(v, col)));
-        if (lane == 0) sh.bins[i * kRowWaves + wave] = s;
+      [&](const i32x4 &v, int) {
+        const uint64_t s = last_lane(wave_scan(vector_sum<T>(weight, v)));   // 0 of the -inf past the row's end
+        uint32_t c = 0;
+        if (some) {
+#pragma unroll
+          for (int e = 0; e < W; ++e) c += __popcll(__ballot(RowElem<T>::get(v, e) == weight.least));
+        }
+        if (lane == 0) {
+          sh.bins[i * kRowWaves + wave] = s;
+          tied[i * kRowWaves + wave] = c;
+        }
         ++i;
       },
       [](int) {});
-  const uint64_t mine = row.ecol >= 0 ? kept(row.edge, row.ecol) : 0;
+  const uint64_t edge_ties = __ballot(some && row.ecol >= 0 && row.edge == weight.least);   // of the first wave
+  if (tid == 0) sh.found[0] = __popcll(edge_ties & ((uint64_t(1) << W) - 1));
+  __syncthreads();
+  const uint64_t first_ties = sh.found[0];
+  const int groups = row.blocks() * 4 * kRowWaves;   // at most kBins
+  const int per = (groups + kRowThreads - 1) / kRowThreads, g0 = min(groups, tid * per), g1 = min(groups, g0 + per);
+  uint64_t ties = 0, all_ties = 0, s = 0, total;
+  if (some) {
+    for (int g = g0; g < g1; ++g) ties += tied[g];
+    ties = first_ties + block_scan(ties, sh, &all_ties);
+  }
+  uint64_t run = ties;
+  for (int g = g0; g < g1; ++g) {
+    uint64_t w = sh.bins[g];
+    if (some) {
+      sh.bins[g] = w -= over(run, tied[g]);
+      run += tied[g];
+    }
+    s += w;
+  }
+  uint64_t mine = row.ecol >= 0 ? weight(row.edge) : 0;
+  if (edge_ties >> lane & 1) {
+    const int below = __popcll(edge_ties & lanes_below());
+    mine -= over(lane < W ? below : all_ties + below, 1);
+  }
   const uint64_t edges = wave_scan(mine);
+  __syncthreads();
   if (wave == 0 && lane == W - 1) sh.found[0] = edges;
   if (wave == 0 && lane == 2 * W - 1) sh.found[1] = edges;
   __syncthreads();
   const uint64_t before = sh.found[0], behind = sh.found[1] - before;
   __syncthreads();
-  const int groups = row.blocks() * 4 * kRowWaves;   // at most kBins
-  const int per = (groups + kRowThreads - 1) / kRowThreads, g0 = min(groups, tid * per), g1 = min(groups, g0 + per);
-  uint64_t s = 0, total;
-  for (int g = g0; g < g1; ++g) s += sh.bins[g];
   uint64_t at = before + block_scan(s, sh, &total);
   const uint64_t target = target_of(u, before + total + behind);
   if (tid == 0) sh.count = -1;
@@ -498,30 +537,39 @@ __device__ __forceinline__ int pick_in_row(const Row<T> &row, RowShared &sh, uin
         if (at + sh.bins[g] >= target) {
           sh.count = g;
           sh.found[0] = target - at;   // to be reached within the group
+          sh.found[1] = ties;          // equal to the least before it
           break;
         }
         at += sh.bins[g];
+        if (some) ties += tied[g];
       }
     __syncthreads();
     const int g = sh.count;
     const uint64_t want = sh.found[0];
+    ties = sh.found[1];
     __syncthreads();
     if (wave == (g & (kRowWaves - 1))) {
       const int vi = (g / kRowWaves) * kRowThreads + tid;
       i32x4 v = {RowElem<T>::kFill, RowElem<T>::kFill, RowElem<T>::kFill, RowElem<T>::kFill};
-      int col = row.V;
-      if (vi < row.nvec) {
-        v = reinterpret_cast<const i32x4 *>(row.p + row.head)[vi];
-        col = row.head + vi * W;
+      if (vi < row.nvec) v = reinterpret_cast<const i32x4 *>(row.p + row.head)[vi];
+      uint64_t in = vector_sum<T>(weight, v);
+      if (some) {
+        uint64_t c = 0;
+#pragma unroll
+        for (int e = 0; e < W; ++e) c += RowElem<T>::get(v, e) == weight.least;
+        ties += wave_scan(c) - c;
+        in -= over(ties, c);
       }
-      const uint64_t in = lane_sum(v, col), upto = wave_scan(in);
+      const uint64_t upto = wave_scan(in);
       if (upto >= want && upto - in < want) {
-        uint64_t run = upto - in;
+        uint64_t sum = upto - in;
         int token = -1;
 #pragma unroll 1
         for (int e = 0; e < W && token < 0; ++e) {
-          run += kept(RowElem<T>::get(v, e), col + e);
-          if (run >= want) token = col + e;
+          const float x = RowElem<T>::get(v, e);
+          sum += weight(x);
+          if (some && x == weight.least) sum -= over(ties++, 1);
+          if (sum >= want) token = row.head + vi * W + e;
         }
         sh.count = token;
       }
@@ -594,7 +642,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict
     const bool keep = tid < top_k && (tid == 0 || in);
     t = pick_in_list(sh, __syncthreads_count(keep), weight, u);
   } else {
-    uint64_t thr = 0, kept = by_k ? (uint64_t)top_k : (uint64_t)V;
+    uint64_t thr = 0, quota = ~uint64_t(0), kept = by_k ? (uint64_t)top_k : (uint64_t)V;
     const uint64_t floor = least > kRowNegInf ? (uint64_t)value_key(least) << 32 : 0;
     // the elements of at least thr into the list; how many there are
     auto gather = [&]() {
@@ -609,6 +657,11 @@ __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict
       });
       __syncthreads();
       return sh.count;
+    };
+    auto raise = [&]() {
+      if (floor <= thr) return;
+      thr = floor;
+      quota = ~uint64_t(0);
     };
     int listed = kListCap + 1;
     if (floor && !by_k && !by_p) {   // min_p alone: mostly few
@@ -625,8 +678,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict
         found = !by_k && !by_p;
         if (!found) {
           const Tabulated tw{weight, kRowNegInf, win, &sh.tab};
-          found = table_threshold(row, sh, sh.tab, tw, by_k, top_k, by_p, top_p, &thr, &kept);
-          thr = max(thr, floor);
+          found = table_threshold(row, sh, sh.tab, tw, by_k, top_k, by_p, top_p, &thr, &kept, &quota);
+          raise();
           if (found && kept <= kListCap && thr >> 32 > 1) listed = gather();
         }
       }
@@ -635,20 +688,26 @@ __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict
     if (listed > kListCap && !(tabulated && found)) make_roots(sh.roots);
     if (listed > kListCap && !found) {   // digit by digit
       thr = 0;
+      quota = ~uint64_t(0);
       if (by_k)
         thr = radix_threshold<true>(row, sh, 0, [](float) { return uint64_t(1); },
-                                    [&](uint64_t) { return (uint64_t)top_k; });
+                                    [&](uint64_t) { return (uint64_t)top_k; }, &quota);
+      if (by_k && by_p && quota != ~uint64_t(0)) {   // top_p counts among them
+        thr = column_threshold(row, sh, 0, (uint32_t)(thr >> 32), quota);
+        quota = ~uint64_t(0);
+      }
       if (by_p)
-        thr = radix_threshold<false>(row, sh, thr, row_weight, [&](uint64_t total) { return mass_needed(top_p, total); });
-      thr = max(thr, floor);
+        thr = radix_threshold<false>(row, sh, thr, row_weight,
+                                     [&](uint64_t total) { return mass_needed(top_p, total); }, &quota);
+      raise();
     }
     const float low = thr >> 32 > 1 ? rank_value(thr) : kRowNegInf;
     if (listed <= kListCap) {
       t = pick_in_list(sh, listed, weight, u);
     } else if (!tabulated) {
-      t = pick_in_row(row, sh, thr, Computed{row_weight.weight, fmaxf(low, kLeastNumber)}, u);
+      t = pick_in_row(row, sh, quota, Computed{row_weight.weight, fmaxf(low, kLeastNumber)}, u);
     } else if constexpr (sizeof(SampleShared<T>) > sizeof(SampleBase)) {
-      t = pick_in_row(row, sh, thr, Tabulated{weight, low, win, &sh.tab}, u);
+      t = pick_in_row(row, sh, quota, Tabulated{weight, low, win, &sh.tab}, u);
     }
   }
   if (tid == 0) token[n] = t;

@@ -379,12 +379,13 @@ __device__ __forceinline__ uint64_t column_threshold(const Row<T> &row, RowShare
 }
 
 // The largest rank such that the elements of at least that rank (among those of
-// at least `floor`) weigh need(total) or more. weight(x) is 1 (ONES) or a whole
+// at least `floor`) weigh need(total) or more; with `quota` its key alone, and how
+// many elements of that key count, by column (~0: all). weight(x) is 1 (ONES) or a whole
 // number that depends on the value alone. Digits of the key from the top, 12
 // bits at first, then of the columns of the elements that share the last key.
 template <bool ONES, typename T, typename WF, typename NF>
 __device__ __forceinline__ uint64_t radix_threshold(const Row<T> &row, RowShared &sh, uint64_t floor, WF weight,
-                                                    NF need) {
+                                                    NF need, uint64_t *quota = nullptr) {
   uint64_t want = 0, total = 0;
   uint32_t prefix = 0;
   int shift = 32;
@@ -418,7 +419,10 @@ __device__ __forceinline__ uint64_t radix_threshold(const Row<T> &row, RowShared
   // elements of this key that are needed, of those there are
   const uint64_t w = ONES ? 1 : weight(rank_value((uint64_t)key << 32));
   const uint64_t ties = (want + w - 1) / w;
-  return ties >= in_bin / w ? (uint64_t)key << 32 : column_threshold(row, sh, floor, key, ties);
+  if (ties >= in_bin / w) return (uint64_t)key << 32;
+  if (!quota) return column_threshold(row, sh, floor, key, ties);
+  *quota = ties;
+  return (uint64_t)key << 32;
 }
 
 // A running maximum m and sum d = sum 2^{x c - mc}, mc = m c rounded: one fma an

@@ -123,6 +123,43 @@ def test_rows_far_from_zero(mga, dev, dtype):
         check(mga, x, uniform(6, dev, i + 20), **s)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("off", [0, 3])
+def test_ties_at_the_threshold(mga, dev, dtype, off):
+    """Rows of few values, of which a filter keeps a part of the last one's elements,
+    more than are listed: those of the lowest columns, at the row's ends too."""
+    V = 30011
+    g = torch.Generator(device=dev).manual_seed(31)
+    x = torch.randint(0, 3, (24, V + 8), generator=g, device=dev).to(dtype)[:, off:off + V]
+    x[1] = 1.0
+    u = torch.cat([uniform(20, dev, 32), torch.tensor([0.0, 0.999, 0.99999, 1.0], device=dev)])
+    for s in (dict(top_k=15000), dict(top_k=29990), dict(top_k=4097), dict(top_p=0.95), dict(top_p=0.9999),
+              dict(top_k=25000, top_p=0.99), dict(top_k=12000, min_p=0.3), dict(top_p=0.8, min_p=0.01)):
+        print(f"case {dtype} {off} {s}", flush=True)
+        check(mga, x, u, **s)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_whole_shares_of_equal_logits(mga, dev, dtype):
+    """Half of an even number of equal largest logits is a whole number of them, at any
+    value of theirs: top_p = 0.5 and u = 0.5 lie on borders between tokens, where only
+    exact weights decide."""
+    V = 12006
+    for top in (1.0, 37.25, 150.5, 3e4, -2e4, torch.finfo(dtype).min / 4, torch.finfo(dtype).max):
+        print(f"case {dtype} {top}", flush=True)
+        x = torch.full((6, V), top, device=dev, dtype=dtype)
+        x[1, ::2] = float("-inf")
+        x[1, 0] = x[1, 1]
+        x[1, 1] = float("-inf")
+        x[2, 5000:] = float("-inf")
+        x[3, 2::3] = torch.finfo(dtype).min if top > 0 else float("-inf")
+        x[4, 100:] = float("-inf")
+        x[5, 2:] = float("-inf")
+        for s in (dict(top_p=0.5), dict(top_p=0.25), dict(top_p=0.5, temperature=0.3), dict(), dict(top_k=5000, top_p=0.5)):
+            for u in (0.25, 0.5, 0.9999999):
+                check(mga, x, torch.full((6,), u, device=dev), **s)
+
+
 def test_borders(mga, dev):
     """Four equal tokens: half of their weight is two of them, just above is three;
     quarters of the uniform fall to the next token."""
