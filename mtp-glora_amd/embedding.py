@@ -110,7 +110,9 @@ def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
     """``scale * weight[ids]`` [..., H] for ids [...] (int32 or int64) of a table
     ``weight`` [V, H], rounded once to its dtype; zeros for an id outside the
     table. Differentiable in ``weight`` (a dense gradient, embedding_grad);
-    ``padding_idx`` is looked up like any other id and has no gradient."""
+    ``padding_idx`` is looked up like any other id and has no gradient. Under graph
+    capture refused while an eager graph of the same leaf lives (its backward would
+    join the default stream); embedding_grad needs no graph."""
     _dev("weight", weight)
     if weight.dim() != 2 or weight.numel() == 0 or max(weight.shape) > INT32_MAX:
         raise ValueError(f"weight: expected [V, H], got {tuple(weight.shape)}")

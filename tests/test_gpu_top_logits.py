@@ -272,7 +272,7 @@ def test_rows_far_from_zero(mga, dev, dtype, tau):
         assert bool(loss.isnan()) and bool(g.isnan().all())
 
 
-@pytest.mark.parametrize("V", [5003, 170003])   # in registers, read twice
+@pytest.mark.parametrize("V", [5003, 170003])
 def test_strides_and_types(mga, dev, V):
     """Student rows off a 16-byte boundary, columns that are not contiguous, strided
     teachers, int64 ids, values of another type than the student."""
@@ -365,7 +365,8 @@ def test_gradient_past_the_cache(mga, dev):
         ys = x[few].clone().requires_grad_()
         mga.top_logits_cross_entropy(ys, t.values[few], t.ids[few], t.lse[few]).backward()
         _, h = mga.top_logits_loss_and_grad(x[few], t.values[few], t.ids[few], t.lse[few])
-        q = torch.zeros(200, V, device=dev).scatter_(1, t.ids[few].long(), (t.values[few].float() - t.lse[few][:, None]).exp())
+        kept = (t.values[few].float() - t.lse[few][:, None]).exp()
+        q = torch.zeros(200, V, device=dev).scatter_(1, t.ids[few].long(), kept)
         slack = 2 * chain(V) * (torch.softmax(x[few].float(), -1) * q.sum(-1, keepdim=True) + q)
         for a, b in ((g[few], h), (xs.grad[few], ys.grad), (g[few], xs.grad[few])):
             d = (a.float() - b.float()).abs()
