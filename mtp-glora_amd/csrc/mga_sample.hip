@@ -692,13 +692,16 @@ __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict
       if (by_k)
         thr = radix_threshold<true>(row, sh, 0, [](float) { return uint64_t(1); },
                                     [&](uint64_t) { return (uint64_t)top_k; }, &quota);
-      if (by_k && by_p && quota != ~uint64_t(0)) {   // top_p counts among them
-        thr = column_threshold(row, sh, 0, (uint32_t)(thr >> 32), quota);
-        quota = ~uint64_t(0);
+      if (by_p) {
+        // top_p counts among the first `quota` of top_k's key; where its own cut has that
+        // key (and leaves them all: its quota is none), the smaller quota holds
+        const uint64_t floor_k =
+            quota != ~uint64_t(0) ? column_threshold(row, sh, 0, (uint32_t)(thr >> 32), quota) : thr;
+        uint64_t quota_p = ~uint64_t(0);
+        thr = radix_threshold<false>(row, sh, floor_k, row_weight,
+                                     [&](uint64_t total) { return mass_needed(top_p, total); }, &quota_p);
+        quota = thr < floor_k ? min(quota, quota_p) : quota_p;
       }
-      if (by_p)
-        thr = radix_threshold<false>(row, sh, thr, row_weight,
-                                     [&](uint64_t total) { return mass_needed(top_p, total); }, &quota);
       raise();
     }
     const float low = thr >> 32 > 1 ? rank_value(thr) : kRowNegInf;

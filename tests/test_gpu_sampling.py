@@ -221,3 +221,22 @@ def test_refusals_and_empty(mga, dev):
         mga.sample_tokens(x, u, torch.ones(3))
     with pytest.raises(ValueError, match="at most"):
         mga.sample_tokens(torch.zeros(1, (1 << 20) + 1, device=dev, dtype=torch.float16), u[:1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [8011, 30011])
+def test_top_p_among_the_ties_of_top_k(mga, dev, dtype, V):
+    """The border of top_k falls among equal logits, and top_p (below 1, yet so near it
+    that the mass it needs is that of all of those elements, or of all but a few) leaves
+    none of the others of that value in. 8 011 columns: no table for bf16 either."""
+    g = torch.Generator(device=dev).manual_seed(41)
+    x = torch.randint(0, 3, (6, V), generator=g, device=dev).to(dtype)
+    x[0], x[1] = 1.0, -3.0
+    x[2, ::2] = 5.0
+    x[3, V // 3:] = -float("inf")
+    u = torch.tensor([0.0, 0.3, 0.9, 0.999999, 0.99, 0.6], device=dev)
+    for k in (1025, 2000, V // 2 + 7, V - 5):
+        for p in (0.99, 0.9999, 0.99999994):
+            for m in (0.0, 0.3):
+                print(f"case {dtype} {V} {k} {p} {m}", flush=True)
+                check(mga, x, u, top_k=k, top_p=p, min_p=m)
