@@ -502,7 +502,8 @@ int mga_top_logits_ce_step(const void *student, int64_t student_row_stride, cons
  *     the first top_k tokens (top_k <= 0 or >= n_cols: all),
  *     of those the shortest leading run with at least top_p of their weight
  *     (top_p >= 1: all; at least the first),
- *     of those the tokens with w >= min_p (min_p <= 0: all; the largest stays),
+ *     of those the tokens with w >= min_p (min_p <= 0: all; above 1: as 1, the
+ *     largest stay),
  *   and the token is the first, by ascending column, at which the running sum of
  *   the weights that are left exceeds u times their total.
  * Weights are computed in 64 bits and held in whole multiples of 2^-45 (from

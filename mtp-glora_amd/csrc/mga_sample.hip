@@ -47,24 +47,22 @@ __device__ __forceinline__ double exp2_part(double f) {
 constexpr double kTwo52 = 4503599627370496.0;
 constexpr uint64_t kLow52 = (uint64_t(1) << 52) - 1;
 
-// round(2^s e^{(x - top) / T}) for x <= top; 0 for NaN and -inf.
+// round(2^s e^{(x - top) / T}) for x <= top; 0 for NaN and -inf. Where top is +inf it
+// counts as 2^128, 2^104 above the largest number: that and all others have weight 0.
 struct Weight {
   double topd, c;   // c = log2(e) / T
   float top;
   int s;
   __device__ __forceinline__ Weight(float m, float temperature, int bits) : top(m), s(bits) {
-    c = 1.4426950408889634074 / (double)temperature;
-    if (m == -kRowNegInf) {   // +inf counts as the largest number, and nothing beside it
-      top = 3.402823466e38f;
-      c = 1.0;
-    }
-    topd = (double)top;
+    const bool inf = m == -kRowNegInf;
+    c = inf ? 1.0 : 1.4426950408889634074 / (double)temperature;
+    topd = inf ? 0x1p128 : (double)m;
   }
   __device__ __forceinline__ uint64_t operator()(float x) const {
     constexpr double kMagic = 1.5 * kTwo52;
-    const float v = x > top ? top : x;              // NaN stays
+    const double v = (double)x > topd ? topd : (double)x;   // NaN stays
     // log2 of the weight; far below 2^-s (and NaN) at a value that rounds to 0
-    const double a = __builtin_fmax(((double)v - topd) * c, (double)(-s - 2));
+    const double a = __builtin_fmax((v - topd) * c, (double)(-s - 2));
     const double m = a + kMagic, f = a - (m - kMagic);   // m: the nearest whole number in its low bits
     const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, m) + (uint32_t)s;
     const double w = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, exp2_part(f)) + ((uint64_t)n << 52));
@@ -81,7 +79,8 @@ struct RowWeight {
   const double *roots;   // 2^{i / 256}
   int s, rough;
   __device__ __forceinline__ RowWeight(const Weight &w, const double *table) : top(w.top), roots(table), s(w.s) {
-    // c so large that the number below top is 60 to 122 powers of two away: a larger one changes no weight
+    // c so large that the number below top is 60 to 122 powers of two away: a larger one
+    // changes no weight (+inf: the largest number is 60 away)
     c = fmin(w.c, 1020054733.0 / fabs(w.topd));
     base = 768.0 - w.topd * c;
     // top c + base is 768 where base has its 43 bits, else next to it
@@ -90,8 +89,8 @@ struct RowWeight {
     low = (float)l;
     if ((double)low > l) low = rank_value((uint64_t)(value_key(low) - 1) << 32);   // the next one down
   }
-  // x finite (or +inf, which counts as top). The weight of top is 2^s itself: a share of
-  // equal largest elements that is a whole number of them stays one.
+  // x finite or +inf. The weight of top is 2^s itself: a share of equal largest elements
+  // that is a whole number of them stays one.
   __device__ __forceinline__ uint64_t operator()(float x) const { return x >= top ? uint64_t(1) << s : fine(x); }
   // The same unless rough.
   __device__ __forceinline__ uint64_t fine(float x) const {
@@ -619,7 +618,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict
   // least value that min_p leaves: w >= min_p as (x - top) / T >= ln(min_p)
   float least = kRowNegInf;
   if (min_p > 0.f) {
-    const double b = min_p < 1.f ? (double)top + (double)temperature * log((double)min_p) : (double)top;
+    const bool below = min_p < 1.f && top < -kRowNegInf;
+    const double b = below ? (double)top + (double)temperature * log((double)min_p) : (double)top;
     least = (float)b;
     if ((double)least < b) least = rank_value((uint64_t)(value_key(least) + 1) << 32);   // the next one up
   }

@@ -33,9 +33,10 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     In the order of the logits (descending, the lower id first among equals) and
     with w = exp((x - max) / temperature): ``top_k`` keeps the first k tokens (0:
     all), ``top_p`` of those the shortest leading run that holds at least top_p of
-    their weight (1: all), ``min_p`` the tokens with w >= min_p. The token is the
-    first, by ascending id, at which the running sum of the kept weights exceeds
-    uniform times their total. ``temperature`` 0 takes the largest logit, the lowest id among
+    their weight (1: all), ``min_p`` the tokens with w >= min_p (above 1: as 1). With
+    +inf among the logits those have w = 1 and all others 0. The token is the first,
+    by ascending id, at which the running sum of the kept weights exceeds uniform
+    times their total. ``temperature`` 0 takes the largest logit, the lowest id among
     equals. Each setting is a number or a tensor with one value a row and is taken
     in fp32 (top_k: int32). -inf and NaN logits are never drawn; a row with nothing
     else gives -1. Sums are exact: the same inputs give the same tokens on every

@@ -95,7 +95,7 @@ def sample_row(row, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         n = max(1, int((before < np.longdouble(np.float64(top_p)) * w.sum()).sum()))
     at, w = at[:n], w[:n]
     if min_p > 0:
-        n = max(1, int((w >= np.float64(min_p)).sum()))
+        n = max(1, int((w >= min(np.float64(min_p), 1.0)).sum()))
         at, w = at[:n], w[:n]
     by = np.argsort(at)
     at, c = at[by], np.cumsum(w[by])

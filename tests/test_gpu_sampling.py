@@ -240,3 +240,24 @@ def test_top_p_among_the_ties_of_top_k(mga, dev, dtype, V):
             for m in (0.0, 0.3):
                 print(f"case {dtype} {V} {k} {p} {m}", flush=True)
                 check(mga, x, u, top_k=k, top_p=p, min_p=m)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [300, 9001])
+def test_infinity_beside_the_largest_number(mga, dev, dtype, V):
+    """+inf alone is drawn, at any temperature, also where the type's largest number
+    stands beside it."""
+    x = logits(3, V, dtype, dev, seed=43)
+    x[0, 3::5] = torch.finfo(dtype).max
+    x[0, 7::50] = float("inf")
+    x[1] = torch.finfo(dtype).max
+    x[1, V - 2:] = float("inf")
+    x[2, :] = float("inf")
+    x[2, :5] = torch.finfo(dtype).max
+    for s in SETTINGS + [dict(top_k=5, top_p=0.5), dict(top_p=0.75), dict(temperature=1e30, top_p=0.9)]:
+        for t in (s.get("temperature", 1.0), float("inf")):
+            for u in (0.0, 0.35, 0.999999):
+                print(f"case {dtype} {V} {s} {t} {u}", flush=True)
+                check(mga, x, torch.full((3,), u, device=dev), **dict(s, temperature=t))
+    for m in (0.05, 1.0, 2.0):
+        check(mga, x, torch.full((3,), 0.9, device=dev), float("inf"), 40, 1.0, m)
