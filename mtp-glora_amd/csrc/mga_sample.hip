@@ -702,6 +702,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_kernel(const T *__restrict
                                      [&](uint64_t total) { return mass_needed(top_p, total); }, &quota_p);
         quota = thr < floor_k ? min(quota, quota_p) : quota_p;
       }
+      // a cut among -inf or NaN leaves all that has a weight
+      if (thr >> 32 <= value_key(kRowNegInf)) quota = ~uint64_t(0);
       raise();
     }
     const float low = thr >> 32 > 1 ? rank_value(thr) : kRowNegInf;

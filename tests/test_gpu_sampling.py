@@ -261,3 +261,23 @@ def test_infinity_beside_the_largest_number(mga, dev, dtype, V):
                 check(mga, x, torch.full((3,), u, device=dev), **dict(s, temperature=t))
     for m in (0.05, 1.0, 2.0):
         check(mga, x, torch.full((3,), 0.9, device=dev), float("inf"), 40, 1.0, m)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hole", [-float("inf"), float("nan")])
+def test_top_k_among_logits_without_weight(mga, dev, dtype, hole):
+    """The border of top_k falls among -inf or NaN: no logit is cut, the row's numbers
+    may all be the type's lowest."""
+    V, n = 32003, 20000
+    g = torch.Generator(device=dev).manual_seed(47)
+    x = torch.full((3, V), hole, device=dev, dtype=dtype)
+    at = torch.randperm(V, generator=g, device=dev)[:n]
+    x[0, at] = torch.finfo(dtype).min
+    x[1, at] = torch.finfo(dtype).min
+    x[1, at[::2]] = torch.finfo(dtype).min / 2
+    x[2, at] = logits(1, n, dtype, dev, seed=48)[0]
+    for u in (0.1, 0.5, 0.9, 0.999999):
+        for s in (dict(top_k=25000), dict(top_k=n), dict(top_k=n + 1), dict(top_k=V - 1),
+                  dict(top_k=25000, top_p=0.9999), dict(top_k=25000, min_p=0.5)):
+            print(f"case {dtype} {hole} {u} {s}", flush=True)
+            check(mga, x, torch.full((3,), u, device=dev), **s)
