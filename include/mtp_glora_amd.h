@@ -456,8 +456,8 @@ int mga_top_logits(const void *logits, int64_t row_stride, int32_t n_rows, int32
  * whatever its logits are; a student logit of -inf at an entry of q > 0 gives an
  * infinite loss; NaN and +inf among other rows' student logits give NaN. An id
  * may stand in a row more than once: its q add up.
- * 1 <= k <= 1024, n_rows < 2^22. workspace: mga_top_logits_ce_workspace_floats fp32
- * values, 16-byte aligned.
+ * 1 <= k <= 1024, n_rows < 2^22, n_cols <= 2^30. workspace:
+ * mga_top_logits_ce_workspace_floats fp32 values, 16-byte aligned.
  * Stands beside mga_soft_ce_* (loss.py:259-330), which reads whole teacher rows.
  */
 int64_t mga_top_logits_ce_workspace_floats(int32_t n_rows, int32_t n_cols);

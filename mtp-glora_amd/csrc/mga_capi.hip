@@ -846,7 +846,7 @@ int mga_soft_ce_bwd(const void *student, int64_t student_row_stride, const void 
 
 namespace {
 
-constexpr int32_t kMaxVocab = 1 << 20, kMaxTopLogits = 1024;
+constexpr int32_t kMaxVocab = 1 << 20, kMaxCeVocab = 1 << 30, kMaxTopLogits = 1024;
 
 // A [n_rows, n_cols] operand of 16-bit or fp32 elements.
 int check_matrix(const char *fn, const char *name, const void *p, int64_t rs, int32_t n_rows, int32_t n_cols,
@@ -891,6 +891,8 @@ int check_top_ce(const char *fn, const mga::TopLogitsCeArgs &a, int32_t dtype) {
   if (rc == MGA_OK) rc = check_row_count(fn, a.N);
   if (rc == MGA_OK) rc = check_temperature(fn, a.tau);
   if (rc != MGA_OK) return rc;
+  // the column behind a range or a turn of the workgroup is a 32-bit number too
+  if (a.V > kMaxCeVocab) return fail(MGA_ERR_INVALID, "%s: %d columns (at most %d)", fn, a.V, kMaxCeVocab);
   if (!a.ids || a.ids_rs < a.K) return fail(MGA_ERR_INVALID, "%s: ids null or with a row stride below k", fn);
   if (reinterpret_cast<uintptr_t>(a.ids) % (a.ids64 ? 8 : 4))
     return fail(MGA_ERR_INVALID, "%s: ids are not aligned to their elements", fn);

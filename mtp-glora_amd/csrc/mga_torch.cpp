@@ -534,7 +534,7 @@ std::optional<Rows> rows_of(const Tensor &t) {
   return r;
 }
 
-constexpr int64_t kMaxTop = 1024, kMaxVocab = 1 << 20;
+constexpr int64_t kMaxTop = 1024, kMaxVocab = 1 << 20, kMaxCeVocab = 1 << 30;
 
 std::optional<std::tuple<Tensor, Tensor, Tensor>> top_logits(const Tensor &x, int64_t k, double temperature) {
   if (!eager() || !plain(x) || dtype_code(x.scalar_type()) < 0) return std::nullopt;
@@ -575,7 +575,7 @@ std::optional<TopCe> top_ce_operands(const Tensor &x, const Tensor &values, cons
   const auto lead = x.sizes().slice(0, x.dim() - 1);
   if (values.sizes().slice(0, x.dim() - 1) != lead || values.size(-1) > kMaxTop) return std::nullopt;
   const auto rx = rows_of(x), rv = rows_of(values), ri = rows_of(ids);
-  if (!rx || !rv || !ri) return std::nullopt;
+  if (!rx || !rv || !ri || rx->cols > kMaxCeVocab) return std::nullopt;
   if (lse) {
     if (!plain(*lse) || lse->device() != x.device() || lse->scalar_type() != at::kFloat || lse->sizes() != lead ||
         !lse->is_contiguous())

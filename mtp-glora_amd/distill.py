@@ -19,6 +19,7 @@ from .ops import _dev, _stream, dtype_code
 
 MAX_TOP = 1024          # most logits kept of a row
 MAX_VOCAB = 1 << 20     # longest row that is put in order
+MAX_CE_VOCAB = 1 << 30  # longest row of the loss
 INT32_MAX = (1 << 31) - 1
 
 
@@ -94,6 +95,13 @@ class _Teacher(NamedTuple):
     lse: torch.Tensor | None
 
 
+def _student(t: torch.Tensor) -> torch.Tensor:
+    x = row_view("student", t)
+    if x.shape[1] > MAX_CE_VOCAB:
+        raise ValueError(f"{x.shape[1]} columns; at most {MAX_CE_VOCAB}")
+    return x
+
+
 def _teacher(student: torch.Tensor, values: torch.Tensor, ids: torch.Tensor, lse) -> _Teacher:
     lead = student.shape[:-1]
     _like("values", values, lead, student.device)
@@ -126,7 +134,7 @@ class TopLogitsCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, student, values, ids, lse, temperature):
-        x = row_view("student", student)
+        x = _student(student)
         code = dtype_code(x.dtype)
         t = _teacher(student, values, ids, lse)
         N, V = x.shape
@@ -171,7 +179,7 @@ def top_logits_cross_entropy(student: torch.Tensor, values: torch.Tensor, ids: t
     id outside [0, V) is padding; a row with no entry left has loss and gradient
     zero. ``values`` may have another dtype than the student. Differentiable in
     ``student``; the teacher gets no gradient. With k = V kept and temperature 1
-    this is StableSoftCrossEntropy. Under graph capture refused while an eager
+    this is StableSoftCrossEntropy. k <= 1024, V <= 2^30. Under graph capture refused while an eager
     graph of the same leaf lives; top_logits_loss_and_grad needs no graph."""
     temperature = _temperature(temperature)
     r = _lib.native("top_logits_ce", student, values, ids, lse, temperature)
@@ -192,7 +200,7 @@ def top_logits_loss_and_grad(student: torch.Tensor, values: torch.Tensor, ids: t
     r = _lib.native("top_logits_step", student, values, ids, lse, temperature, scale)
     if r is not None:
         return r
-    x = row_view("student", student)
+    x = _student(student)
     code = dtype_code(x.dtype)
     t = _teacher(student, values, ids, lse)
     N, V = x.shape

@@ -147,3 +147,13 @@ def test_layer_keeps_the_parameter(mga):
     assert own.weight.dtype == torch.bfloat16 and list(own.state_dict()) == ["weight"]
     with pytest.raises(NotImplementedError):
         mga.ScaledEmbedding.wrap(torch.nn.Embedding(6, 4, max_norm=1.0))
+
+
+def test_columns_next_to_2_31(mga):
+    """The loss's last column range would end past 2^31, its 32-bit length be that of a
+    whole range: elements behind the row, which the backward writes."""
+    lib, far = mga.load_library(), ctypes.c_void_p(1 << 40)
+    for v in ((1 << 30) + 1, 2147383647, (1 << 31) - 1):
+        for step in (False, True):
+            refused(mga, _fwd(lib, step, n=1, v=v, rs=v, gs=v, grad=far), b"columns")
+        refused(mga, lib.mga_top_logits_ce_bwd(P, v, P, 4, 0, P, P, 1, v, 4, 1.0, 0, P, far, v, None), b"columns")
