@@ -511,7 +511,8 @@ std::optional<Tensor> soft_ce(const Tensor &x, const Tensor &t) {
 
 // ---- vocabulary rows -----------------------------------------------------------------
 
-// Rows of a [..., cols] tensor with unit stride on the last dimension.
+// Rows of a [..., cols] tensor with unit stride on the last dimension; of every
+// contiguous one with elements.
 struct Rows {
   int64_t n = 1, stride = 0;
   int32_t cols = 0;
@@ -520,7 +521,8 @@ struct Rows {
 std::optional<Rows> rows_of(const Tensor &t) {
   Rows r;
   const int64_t d = t.dim();
-  if (d < 1 || t.numel() == 0 || t.stride(d - 1) != 1 || t.size(d - 1) > INT32_MAX) return std::nullopt;
+  if (d < 1 || t.numel() == 0 || t.size(d - 1) > INT32_MAX) return std::nullopt;
+  if (t.size(d - 1) > 1 && t.stride(d - 1) != 1) return std::nullopt;   // one column may carry any stride
   r.cols = (int32_t)t.size(d - 1);
   for (int64_t i = d - 2; i >= 0; --i) {
     if (t.size(i) == 1) continue;

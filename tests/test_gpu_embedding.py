@@ -232,3 +232,23 @@ def test_layer(mga, dev):
     (ga,) = torch.autograd.grad(a.square().sum(), layer.weight)
     (gb,) = torch.autograd.grad(b.square().sum(), base.weight)
     torch.testing.assert_close(ga, gb, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 2, 700])
+def test_gradients_of_one_column(mga, dev, dtype, n):
+    """A table of one column: gradients whose last dimension carries a stride that is
+    none (0 of an expanded one, a far one of a slice), of one token too."""
+    V = 3
+    w = table(V, 1, dtype, dev).requires_grad_()
+    ids = torch.arange(n, device=dev) % 2
+    i = ids.cpu().numpy()
+    for t in (ids, ids[None], ids[:, None]):
+        w.grad = None
+        mga.scaled_embedding(t, w, 2.0).sum().backward()
+        close(w.grad, vo.embedding_grad(np.ones((n, 1)), i, V, 2.0), 0.0, dtype)
+    wide = table(n, 10, dtype, dev, seed=3)
+    for dy in (wide[:, 3:4], wide[:, ::7][:, 1:], wide[:, :1], wide[:1, :1].expand(n, 1)):
+        w.grad = None
+        mga.scaled_embedding(ids, w, 2.0).backward(dy)
+        close(w.grad, vo.embedding_grad(f64(dy), i, V, 2.0), grad_bound(f64(dy), i, V, 2.0), dtype)
