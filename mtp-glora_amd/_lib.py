@@ -183,5 +183,12 @@ def native(name: str, t, *args):
     return getattr(_torch_module or load_torch_module(), name)(t, *args)
 
 
+def check_capture(fn: str, leaf) -> None:
+    """Refuse a differentiable call of ``fn`` under graph capture while an eager graph
+    of ``leaf`` lives: its captured backward would end the process."""
+    if getattr(leaf, "is_cuda", False):
+        (_torch_module or load_torch_module()).check_capture(fn, leaf)
+
+
 def version() -> int:
     return int(load().mga_version())

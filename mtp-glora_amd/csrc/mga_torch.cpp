@@ -99,10 +99,10 @@ bool aligned16(const Tensor &t) { return reinterpret_cast<uintptr_t>(t.data_ptr(
 // A captured backward joins the stream of the leaf's gradient accumulator. An eager
 // graph that still lives has bound it to the default stream, which no capture may
 // touch: torch's engine then ends the process. Refused while it can be said.
-void check_capture(const char *fn, const Tensor &leaf) {
-  if (!at::GradMode::is_enabled() || !leaf.requires_grad() || !leaf.is_leaf() ||
-      c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None)
-    return;
+void check_capture(const std::string &fn, const Tensor &leaf) {
+  if (!leaf.is_cuda() || !at::GradMode::is_enabled() || !leaf.requires_grad() || !leaf.is_leaf()) return;
+  const at::DeviceGuard guard(leaf.device());
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
   const auto stream = node ? node->stream() : std::nullopt;
   TORCH_CHECK(!stream || stream->id() != 0, fn, ": under graph capture, while an eager graph of the same leaf lives on "
@@ -754,4 +754,5 @@ PYBIND11_MODULE(_mga_torch, m) {
   MGA_DEF(top_logits_step);
   MGA_DEF(sample);
   MGA_DEF(embedding);
+  MGA_DEF(check_capture);
 }

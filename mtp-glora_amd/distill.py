@@ -132,6 +132,11 @@ def _common(x: torch.Tensor, t: _Teacher):
 class TopLogitsCrossEntropy(torch.autograd.Function):
     """``apply(student, values, ids, lse, temperature)``; see top_logits_cross_entropy."""
 
+    @classmethod
+    def apply(cls, student, *args):
+        _lib.check_capture("top_logits_cross_entropy", student)
+        return super().apply(student, *args)
+
     @staticmethod
     def forward(ctx, student, values, ids, lse, temperature):
         x = _student(student)

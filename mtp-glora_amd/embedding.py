@@ -122,7 +122,10 @@ def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
             raise ValueError(f"padding_idx {padding_idx} outside a table of {weight.shape[0]} rows")
         padding_idx = int(padding_idx) % weight.shape[0]
     r = _lib.native("embedding", ids, weight, float(scale), -1 if padding_idx is None else padding_idx)
-    return r if r is not None else _Embedding.apply(ids, weight, float(scale), padding_idx)
+    if r is not None:
+        return r
+    _lib.check_capture("scaled_embedding", weight)
+    return _Embedding.apply(ids, weight, float(scale), padding_idx)
 
 
 class ScaledEmbedding(nn.Embedding):

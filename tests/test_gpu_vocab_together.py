@@ -264,3 +264,40 @@ def test_past_2_31_elements(mga, dev):
     dw = mga.embedding_grad(e, ids, V, out=w)
     assert dw is w and torch.equal(dw[-500:], mga.embedding_grad(e, ids - (V - 500), 500))
     assert not dw[:-500].any()
+
+
+def test_capture_refused_in_every_form(mga, dev):
+    """While an eager graph of the leaf lives, a differentiable call under capture is
+    refused also where the operands are not those that the native forms take; nothing
+    of it is refused without a gradient, outside a capture or after that graph is gone."""
+    n, V, H = 20, 2003, 64
+    x, t, u, w, dy = inputs(n, V, H, torch.bfloat16, dev, seed=17)
+    top = mga.top_logits(t, 8)
+    ids = torch.randint(V, (2 * n,), device=dev)[::2]
+    lse = torch.stack([top.lse, top.lse], 1)[:, 0]
+    xs, ws = x.requires_grad_(), w.requires_grad_()
+    wide = torch.stack([x, x], -1)[..., 0].detach().requires_grad_()
+    calls = [("scaled_embedding", ws, lambda: mga.scaled_embedding(ids, ws, 2.0)),
+             ("top_logits_cross_entropy", xs, lambda: mga.top_logits_cross_entropy(xs, top.values, top.ids, lse)),
+             ("top_logits_cross_entropy", xs, lambda: mga.TopLogitsCrossEntropy.apply(xs, *top, 1.0)),
+             ("top_logits_cross_entropy", wide, lambda: mga.top_logits_cross_entropy(wide, *top))]
+    for name, leaf, call in calls:
+        want = call().detach()
+        eager = call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = u * 2
+            with pytest.raises(RuntimeError, match=name + ": under graph capture"):
+                call()
+            with torch.no_grad():
+                e = call()
+        graph.replay()
+        assert torch.equal(y, u * 2) and torch.equal(e, want) and torch.equal(call(), want)
+        del eager
+        graph, out = capture(lambda: [call().detach()])
+        for _ in range(3):
+            scribble(out)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], want)
