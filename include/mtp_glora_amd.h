@@ -453,8 +453,8 @@ int mga_top_logits(const void *logits, int64_t row_stride, int32_t n_rows, int32
  * loss_sum: the row losses added in a fixed order. q [n_rows, k] (null: not kept)
  * and stats [3, n_rows] = (max x, sum exp((x - max) / tau), Q) are what the
  * backward reads. A row without an entry of q > 0 has loss and gradient 0,
- * whatever its logits are; a student logit of -inf at an entry of q > 0 gives an
- * infinite loss; NaN and +inf among other rows' student logits give NaN. An id
+ * whatever its logits are; in the others NaN and +inf among the student logits give
+ * NaN, else a logit of -inf at an entry of q > 0 an infinite loss. An id
  * may stand in a row more than once: its q add up.
  * 1 <= k <= 1024, n_rows < 2^22, n_cols <= 2^30. workspace:
  * mga_top_logits_ce_workspace_floats fp32 values, 16-byte aligned.

@@ -127,7 +127,7 @@ __device__ __forceinline__ float teacher_weight(float t, int id, float norm, flo
 
 __device__ __forceinline__ float loss_term(float q, float x, float m, float logd, float itau) {
   if (q == 0.f) return 0.f;
-  if (x == kRowNegInf) return -kRowNegInf;   // all of the row among them (m = -inf)
+  if (x == kRowNegInf && logd == logd) return -kRowNegInf;   // all of the row among them (m = -inf)
   return q * ((m - x) * itau + logd);
 }
 
@@ -471,7 +471,7 @@ struct TeacherRow {
     const float d = sum_at_max(m, sums.x, c), inv = a.lse ? 1.f : sums.y == 0.f ? 0.f : 1.f / sums.y;
     const float Q = sums.y * inv;
     if (threadIdx.x == 0)
-      a.loss[n] = Q == 0.f ? 0.f : m == kRowNegInf ? -kRowNegInf : a.tau * a.tau * (sums.z * inv + Q * logf(d));
+      a.loss[n] = Q == 0.f ? 0.f : m == kRowNegInf && d == d ? -kRowNegInf : a.tau * a.tau * (sums.z * inv + Q * logf(d));
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int k = threadIdx.x + i * B;

@@ -371,3 +371,25 @@ def test_gradient_past_the_cache(mga, dev):
         for a, b in ((g[few], h), (xs.grad[few], ys.grad), (g[few], xs.grad[few])):
             d = (a.float() - b.float()).abs()
             assert bool((d <= 2.0 ** -7 * torch.maximum(a.abs(), b.abs()).float() + slack + 1e-30).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 100])
+def test_student_rows_of_nan(mga, dev, dtype, n):
+    """NaN in a row that counts gives NaN, for few rows and many: in a row of nothing
+    else, beside -inf alone, and where the teacher wants a masked logit."""
+    V, k = 3001, 4
+    x = torch.full((3, V), float("nan"), device=dev, dtype=dtype)
+    x[1, 5:] = -float("inf")
+    x[2] = logits(1, V, dtype, dev, seed=31)[0]
+    x[2, 1], x[2, 9] = float("nan"), -float("inf")
+    ids = torch.full((3, k), 9, dtype=torch.int32, device=dev)
+    values = torch.zeros(3, k, device=dev)
+    for r in range(3):
+        xs = x[r:r + 1].repeat(n, 1).requires_grad_()
+        args = values[r:r + 1].repeat(n, 1), ids[r:r + 1].repeat(n, 1)
+        loss, g = mga.top_logits_loss_and_grad(xs.detach(), *args)
+        total = mga.top_logits_cross_entropy(xs, *args)
+        total.backward()
+        assert bool(loss.isnan()) and bool(total.isnan()), (r, float(loss), float(total.detach()))
+        assert bool(g.isnan().all()) and bool(xs.grad.isnan().all()), r
