@@ -4,7 +4,7 @@
 //   q_k = e^{t_k / tau - lse}, or the softmax of t / tau over the row's K;
 //   Q = sum_k q_k; p = softmax(x / tau);
 //   row loss = tau^2 (Q log sum_j e^{x_j / tau} - sum_k q_k x_{id_k} / tau)
-//            = tau^2 sum_k q_k ((m - x_{id_k}) / tau + log d),
+//            = sum_k q_k (tau (m - x_{id_k}) + tau^2 log d),
 //              m = max x, d = sum_j e^{(x_j - m) / tau} (no difference of large
 //              numbers where student and teacher agree);
 //   grad_j = go tau (Q p_j - sum_{k: id_k = j} q_k).
@@ -118,17 +118,25 @@ __device__ __forceinline__ int teacher_id(const TopLogitsCeArgs &a, int64_t row,
   const int64_t id = a.ids64 ? static_cast<const int64_t *>(a.ids)[at] : static_cast<const int32_t *>(a.ids)[at];
   return id >= 0 && id < a.V ? (int)id : -1;
 }
-// q of a teacher value before the division by its sum (no lse) or as it is (lse)
-__device__ __forceinline__ float teacher_weight(float t, int id, float norm, float itau) {
-  const float s = t * itau;
-  if (id < 0 || s == kRowNegInf || norm == kRowNegInf) return 0.f;
-  return ex2((s - norm) * kLog2e);
-}
+// q of a teacher value before the division by its sum (no lse; norm: the largest value)
+// or as it is (lse). Without lse the values' difference is taken before the quotient by
+// tau: a value's own may be past fp32 (the type's lowest at tau < 1).
+struct TeacherWeight {
+  float before, behind;
+  __device__ __forceinline__ TeacherWeight(const TopLogitsCeArgs &a, float itau)
+      : before(a.lse ? itau : 1.f), behind(a.lse ? kLog2e : itau * kLog2e) {}
+  __device__ __forceinline__ float operator()(float t, int id, float norm) const {
+    const float s = t * before;
+    if (id < 0 || s == kRowNegInf || norm == kRowNegInf) return 0.f;
+    return ex2((s - norm) * behind);
+  }
+};
 
-__device__ __forceinline__ float loss_term(float q, float x, float m, float logd, float itau) {
+// tau^2 q ((m - x) / tau + log d); tau2logd: tau^2 log d
+__device__ __forceinline__ float loss_term(float q, float x, float m, float tau, float tau2logd) {
   if (q == 0.f) return 0.f;
-  if (x == kRowNegInf && logd == logd) return -kRowNegInf;   // all of the row among them (m = -inf)
-  return q * ((m - x) * itau + logd);
+  if (x == kRowNegInf && tau2logd == tau2logd) return -kRowNegInf;   // all of the row among them (m = -inf)
+  return q * ((m - x) * tau + tau2logd);
 }
 
 // What the gradient's elements of a row have in common: a 2^{x c - mc}; zeros,
@@ -233,6 +241,7 @@ __global__ __launch_bounds__(kThreads) void top_ce_combine_kernel(TopLogitsCeArg
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   const float itau = 1.f / a.tau, c = itau * kLog2e;
+  const TeacherWeight weight(a, itau);
   if (row < a.N) {
     const T *xr = static_cast<const T *>(a.x) + row * a.xs;
     const float2 *pr = reinterpret_cast<const float2 *>(part) + row * nsplit;
@@ -256,20 +265,20 @@ __global__ __launch_bounds__(kThreads) void top_ce_combine_kernel(TopLogitsCeArg
     float inv = 1.f;
     if (!a.lse) {
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) norm = fmaxf(norm, t[i] * itau);
+      for (int i = 0; i < kEach; ++i) norm = fmaxf(norm, t[i]);
       for (int k = lane + 64 * kEach; k < a.K; k += 64)
-        if (teacher_id(a, row, k) >= 0) norm = fmaxf(norm, teacher_value(a, row, k) * itau);
+        if (teacher_id(a, row, k) >= 0) norm = fmaxf(norm, teacher_value(a, row, k));
 #pragma unroll
       for (int m = 32; m >= 1; m >>= 1) norm = fmaxf(norm, __shfl_xor(norm, m, 64));
     }
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) q[i] = teacher_weight(t[i], id[i], norm, itau);
+    for (int i = 0; i < kEach; ++i) q[i] = weight(t[i], id[i], norm);
     if (!a.lse) {
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < kEach; ++i) s += q[i];
       for (int k = lane + 64 * kEach; k < a.K; k += 64)
-        s += teacher_weight(teacher_value(a, row, k), teacher_id(a, row, k), norm, itau);
+        s += weight(teacher_value(a, row, k), teacher_id(a, row, k), norm);
 #pragma unroll
       for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
       inv = s == 0.f ? 0.f : 1.f / s;
@@ -278,7 +287,7 @@ __global__ __launch_bounds__(kThreads) void top_ce_combine_kernel(TopLogitsCeArg
     st.merge(p.x, p.y, c);
     for (int sp = lane + 64; sp < nsplit; sp += 64) st.merge(pr[sp].x, pr[sp].y, c);
     merge_lanes(st, c);
-    const float d = sum_at_max(st.m, st.d, c), logd = logf(d);
+    const float d = sum_at_max(st.m, st.d, c), tau2logd = a.tau * a.tau * logf(d);
     float loss = 0.f, Q = 0.f;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -286,14 +295,14 @@ __global__ __launch_bounds__(kThreads) void top_ce_combine_kernel(TopLogitsCeArg
       q[i] *= inv;
       if (a.q && k < a.K) a.q[row * a.K + k] = q[i];
       Q += q[i];
-      loss += loss_term(q[i], xk[i], st.m, logd, itau);
+      loss += loss_term(q[i], xk[i], st.m, a.tau, tau2logd);
     }
     for (int k = lane + 64 * kEach; k < a.K; k += 64) {
       const int at = teacher_id(a, row, k);
-      const float w = teacher_weight(teacher_value(a, row, k), at, norm, itau) * inv;
+      const float w = weight(teacher_value(a, row, k), at, norm) * inv;
       if (a.q) a.q[row * a.K + k] = w;
       Q += w;
-      if (at >= 0) loss += loss_term(w, (float)xr[at], st.m, logd, itau);
+      if (at >= 0) loss += loss_term(w, (float)xr[at], st.m, a.tau, tau2logd);
     }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) {
@@ -301,7 +310,7 @@ __global__ __launch_bounds__(kThreads) void top_ce_combine_kernel(TopLogitsCeArg
       Q += __shfl_xor(Q, m, 64);
     }
     if (lane == 0) {
-      __hip_atomic_store(a.loss + row, a.tau * a.tau * loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(a.loss + row, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       a.stats[row] = st.m;
       a.stats[a.N + row] = d;
       a.stats[2 * (int64_t)a.N + row] = Q;
@@ -456,22 +465,23 @@ struct TeacherRow {
                                             float itau, float c, StepShared<B> &sh) {
     float top = kRowNegInf;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) top = fmaxf(top, t[i] * itau);
+    for (int i = 0; i < kEach; ++i) top = fmaxf(top, t[i]);
     const float2 most = block_max2<B>({st.m, top}, sh.part);
     const float m = most.x, norm = a.lse ? a.lse[n] : most.y;
+    const TeacherWeight weight(a, itau);
     // d (NaN for m = +inf); of the weights; of their part of the loss
     float3 sums = {far(m, c) ? count_equal<B>(xr, a.V, m) + (m - m) : sum_at(st, m, c), 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      q[i] = teacher_weight(t[i], id[i], norm, itau);
+      q[i] = weight(t[i], id[i], norm);
       sums.y += q[i];
-      sums.z += q[i] == 0.f ? 0.f : x[i] == kRowNegInf ? -kRowNegInf : q[i] * ((m - x[i]) * itau);
+      sums.z += q[i] == 0.f ? 0.f : x[i] == kRowNegInf ? -kRowNegInf : q[i] * ((m - x[i]) * a.tau);
     }
     sums = block_sum3<B>(sums, sh.part);
     const float d = sum_at_max(m, sums.x, c), inv = a.lse ? 1.f : sums.y == 0.f ? 0.f : 1.f / sums.y;
     const float Q = sums.y * inv;
     if (threadIdx.x == 0)
-      a.loss[n] = Q == 0.f ? 0.f : m == kRowNegInf && d == d ? -kRowNegInf : a.tau * a.tau * (sums.z * inv + Q * logf(d));
+      a.loss[n] = Q == 0.f ? 0.f : m == kRowNegInf && d == d ? -kRowNegInf : sums.z * inv + a.tau * a.tau * Q * logf(d);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int k = threadIdx.x + i * B;

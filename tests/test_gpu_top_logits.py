@@ -393,3 +393,34 @@ def test_student_rows_of_nan(mga, dev, dtype, n):
         total.backward()
         assert bool(loss.isnan()) and bool(total.isnan()), (r, float(loss), float(total.detach()))
         assert bool(g.isnan().all()) and bool(xs.grad.isnan().all()), r
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 100])
+def test_quotients_by_the_temperature_past_fp32(mga, dev, dtype, n):
+    """Teacher and student logits of the type's lowest value at temperature 1 / 2: a
+    teacher's row of equal values has equal weights whatever the value, and a student's
+    masked logit that the teacher wants a finite loss."""
+    V, k, tau = 3001, 5, 0.5
+    low = torch.finfo(dtype).min
+    x = logits(n, V, dtype, dev, seed=33)
+    ids = torch.arange(k, device=dev, dtype=torch.int32).expand(n, k) * 7
+    zero = torch.zeros(n, k, device=dev, dtype=dtype)
+    want = check_ce(mga, x, zero, ids, None, tau)
+    for value in (low, -low):
+        for got, w in zip(check_ce_calls(mga, x, torch.full_like(zero, value), ids, tau), want):
+            assert torch.equal(got, w)
+    part = torch.full_like(zero, low)
+    part[:, 2] = low / 2                    # the only one with a weight
+    for got, w in zip(check_ce_calls(mga, x, part, ids, tau), check_ce_calls(mga, x, zero[:, :1], ids[:, 2:3], tau)):
+        assert torch.equal(got, w)
+    x[0, 7], x[0, 14] = low, low / 2
+    check_ce(mga, x, zero, ids, None, tau)
+
+
+def check_ce_calls(mga, x, values, ids, tau, go=0.375):
+    """What check_ce returns, without an oracle."""
+    xs = x.detach().clone().requires_grad_()
+    total = mga.top_logits_cross_entropy(xs, values, ids, None, tau)
+    (total * go).backward()
+    return total, xs.grad, mga.top_logits_loss_and_grad(x, values, ids, None, tau, scale=go)[1]
