@@ -190,5 +190,10 @@ def check_capture(fn: str, leaf) -> None:
         (_torch_module or load_torch_module()).check_capture(fn, leaf)
 
 
+def once(fn: str, grad):
+    """``grad`` of ``fn``'s backward, not to be differentiated again (refused there)."""
+    return (_torch_module or load_torch_module()).once(fn, grad)
+
+
 def version() -> int:
     return int(load().mga_version())

@@ -22,6 +22,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
@@ -107,6 +108,14 @@ void check_capture(const std::string &fn, const Tensor &leaf) {
   const auto stream = node ? node->stream() : std::nullopt;
   TORCH_CHECK(!stream || stream->id() != 0, fn, ": under graph capture, while an eager graph of the same leaf lives on "
               "the default stream; release that graph first");
+}
+
+// A gradient that is asked for with a graph of its own: differentiating it again is
+// refused where that happens, since the backward leaves no graph.
+Tensor once(const std::string &fn, const Tensor &g) {
+  if (!at::GradMode::is_enabled()) return g;
+  const auto refuse = std::make_shared<torch::autograd::DelayedError>(fn + ": no second derivatives", 1);
+  return (*refuse)({g.detach().set_requires_grad(true)})[0];
 }
 
 // [1, H, S, D] with unit stride on D and 16-byte aligned rows
@@ -623,7 +632,7 @@ struct TopLogitsCE : public Function<TopLogitsCE> {
                                      stats + 3 * rx.n, stats, (int32_t)rx.n, rx.cols, ri.cols,
                                      (float)ctx->saved_data["tau"].toDouble(), dtype_code(x.scalar_type()),
                                      go.data_ptr<float>(), gx.data_ptr(), rx.cols, stream(x)));
-    return {gx, Tensor(), Tensor(), Tensor(), Tensor()};
+    return {once("top_logits_cross_entropy", gx), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -722,7 +731,8 @@ struct Embedding : public Function<Embedding> {
                                  (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["pad"].toInt(), (int32_t)V,
                                  H, dtype_code(dy.scalar_type()), dw.data_ptr(), H, dtype_code(dy.scalar_type()), 0,
                                  ws.data_ptr(), wn, stream(dy)));
-    return {Tensor(), dw, Tensor(), Tensor()};
+    // linear in the output's gradient, of nothing else
+    return {Tensor(), grad[0].requires_grad() ? once("scaled_embedding", dw) : dw, Tensor(), Tensor()};
   }
 };
 
@@ -755,4 +765,5 @@ PYBIND11_MODULE(_mga_torch, m) {
   MGA_DEF(sample);
   MGA_DEF(embedding);
   MGA_DEF(check_capture);
+  MGA_DEF(once);
 }

@@ -168,7 +168,7 @@ class TopLogitsCrossEntropy(torch.autograd.Function):
                 _lib.call("mga_top_logits_ce_bwd", x.data_ptr(), row_stride(x), ids.data_ptr(), row_stride(ids),
                           int(ids.dtype == torch.int64), q.data_ptr(), stats.data_ptr(), N, V, ids.shape[1],
                           temperature, dtype_code(x.dtype), go.data_ptr(), grad.data_ptr(), V, _stream(x))
-        return grad.view(shape), None, None, None, None
+        return _lib.once("top_logits_cross_entropy", grad.view(shape)), None, None, None, None
 
 
 def top_logits_cross_entropy(student: torch.Tensor, values: torch.Tensor, ids: torch.Tensor,
@@ -183,7 +183,7 @@ def top_logits_cross_entropy(student: torch.Tensor, values: torch.Tensor, ids: t
     what was not kept then carries the rest), else renormalised over the kept. An
     id outside [0, V) is padding; a row with no entry left has loss and gradient
     zero. ``values`` may have another dtype than the student. Differentiable in
-    ``student``; the teacher gets no gradient. With k = V kept and temperature 1
+    ``student``, once; the teacher gets no gradient. With k = V kept and temperature 1
     this is StableSoftCrossEntropy. k <= 1024, V <= 2^30. Under graph capture refused while an eager
     graph of the same leaf lives; top_logits_loss_and_grad needs no graph."""
     temperature = _temperature(temperature)

@@ -102,14 +102,15 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_out):
         (ids,), (V, scale, padding_idx) = ctx.saved_tensors, ctx.meta
-        return None, embedding_grad(grad_out, ids, V, scale, padding_idx), None, None
+        grad = embedding_grad(grad_out, ids, V, scale, padding_idx)
+        return None, _lib.once("scaled_embedding", grad) if grad_out.requires_grad else grad, None, None
 
 
 def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
                      padding_idx: int | None = None) -> torch.Tensor:
     """``scale * weight[ids]`` [..., H] for ids [...] (int32 or int64) of a table
     ``weight`` [V, H], rounded once to its dtype; zeros for an id outside the
-    table. Differentiable in ``weight`` (a dense gradient, embedding_grad);
+    table. Differentiable in ``weight``, once (a dense gradient, embedding_grad);
     ``padding_idx`` is looked up like any other id and has no gradient. Under graph
     capture refused while an eager graph of the same leaf lives (its backward would
     join the default stream); embedding_grad needs no graph."""

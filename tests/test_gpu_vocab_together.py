@@ -6,6 +6,7 @@ Equality is bit for bit where the same kernels run on the same values."""
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from oracle import vocab as vo
 from test_gpu_embedding import close, grad_bound
@@ -301,3 +302,47 @@ def test_capture_refused_in_every_form(mga, dev):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out[0], want)
+
+
+@pytest.mark.parametrize("form", ["native", "python"])
+def test_second_derivatives_are_refused(mga, dev, monkeypatch, form):
+    """A gradient with a graph of its own has the ordinary values; to differentiate it
+    again is refused instead of leaving its part out, also beside other terms. What
+    does not go through a second derivative of these operators is not refused."""
+    if form == "python":
+        monkeypatch.setattr(mga._lib, "native", lambda *args: None)
+    n, V, H = 12, 301, 16
+    x, t, u, w, dy = inputs(n, V, H, torch.float32, dev, seed=19)
+    top = mga.top_logits(t, 5)
+    ids = torch.arange(n, device=dev) % 7
+    xs, ws = x.requires_grad_(), w.requires_grad_()
+    (want,) = torch.autograd.grad(mga.top_logits_cross_entropy(xs, *top), xs)
+    (g,) = torch.autograd.grad(mga.top_logits_cross_entropy(xs, *top), xs, create_graph=True)
+    assert torch.equal(g, want) and g.requires_grad
+    with pytest.raises(RuntimeError, match="top_logits_cross_entropy: no second derivatives"):
+        g.square().sum().backward()
+    (g,) = torch.autograd.grad(mga.top_logits_cross_entropy(xs, *top) + xs.pow(3).sum(), xs, create_graph=True)
+    with pytest.raises(RuntimeError, match="top_logits_cross_entropy: no second derivatives"):
+        g.sum().backward()
+    e = mga.scaled_embedding(ids, ws, 3.0)
+    (want,) = torch.autograd.grad(e.square().sum(), ws, retain_graph=True)
+    (g,) = torch.autograd.grad(e.square().sum(), ws, create_graph=True)
+    assert torch.equal(g, want)
+    with pytest.raises(RuntimeError, match="scaled_embedding: no second derivatives"):
+        g.sum().backward()
+    e = mga.scaled_embedding(ids, ws, 3.0)
+    (g,) = torch.autograd.grad(e, ws, dy, create_graph=True)   # of a constant: no graph behind it
+    assert not g.requires_grad
+    ws.grad = None
+    e = mga.scaled_embedding(ids, ws, 3.0)                      # a penalty on the gradient of what was looked up
+    (g,) = torch.autograd.grad(e.pow(3).sum(), e, create_graph=True)
+    g.square().sum().backward()                                 # of 9 e^4
+    de = 36 * f64(e) ** 3
+    got = f64(ws.grad)
+    want = vo.embedding_grad(de, ids.cpu().numpy(), V, 3.0)
+    # the powers' roundings (some 8 of 2^-24) beside the sum's
+    bound = grad_bound(de, ids.cpu().numpy(), V, 3.0) + 2.0 ** -20 * vo.embedding_grad(abs(de), ids.cpu().numpy(), V, 3.0)
+    assert (np.abs(got - want) <= bound + 1e-30).all()
+    for leaf, call in ((xs, lambda a: mga.top_logits_cross_entropy(a, *top)), (ws, lambda a: mga.scaled_embedding(ids, a))):
+        with forward_ad.dual_level(), pytest.raises(RuntimeError):
+            call(forward_ad.make_dual(leaf.detach(), torch.ones_like(leaf)))
