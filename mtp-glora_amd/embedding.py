@@ -140,14 +140,22 @@ class ScaledEmbedding(nn.Embedding):
 
     @classmethod
     def wrap(cls, base: nn.Embedding, scale: float = 1.0) -> "ScaledEmbedding":
-        """The layer of ``base``'s own parameter (shared, not copied)."""
+        """The layer of ``base``'s own parameter (shared, not copied), in its place: with
+        its hooks (shared too: their handles remove them here), training flag and other
+        attributes. A layer whose class or instance has a ``forward`` of its own, or
+        whose weight is no plain parameter, is refused."""
         if base.max_norm is not None or base.scale_grad_by_freq or base.sparse:
             raise NotImplementedError("max_norm, scale_grad_by_freq and sparse gradients are not supported")
+        if type(base).forward is not nn.Embedding.forward or "forward" in vars(base):
+            raise NotImplementedError(f"{type(base).__name__} has a forward of its own")
+        if not isinstance(base._parameters.get("weight"), nn.Parameter):
+            raise NotImplementedError("the weight is not a parameter of the layer itself")
         m = cls.__new__(cls)
         nn.Module.__init__(m)
-        m.num_embeddings, m.embedding_dim, m.padding_idx = base.num_embeddings, base.embedding_dim, base.padding_idx
-        m.max_norm, m.norm_type, m.scale_grad_by_freq, m.sparse = None, base.norm_type, False, False
-        m.weight, m.scale = base.weight, float(scale)
+        vars(m).update(vars(base))
+        for own in ("_parameters", "_buffers", "_modules", "_non_persistent_buffers_set"):
+            vars(m)[own] = vars(base)[own].copy()
+        m.scale = float(scale)
         return m
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:

@@ -252,3 +252,16 @@ def test_gradients_of_one_column(mga, dev, dtype, n):
         w.grad = None
         mga.scaled_embedding(ids, w, 2.0).backward(dy)
         close(w.grad, vo.embedding_grad(f64(dy), i, V, 2.0), grad_bound(f64(dy), i, V, 2.0), dtype)
+
+
+def test_layer_of_a_frozen_model(mga, dev):
+    """The hook by which a frozen model's inputs come to require gradients goes on
+    working, and its handle removes it."""
+    base = torch.nn.Embedding(30, 24, device=dev).requires_grad_(False)
+    handle = base.register_forward_hook(lambda m, args, out: out.requires_grad_())
+    layer = mga.ScaledEmbedding.wrap(base, 4.0)
+    ids = torch.arange(30, device=dev)
+    out = layer(ids)
+    assert out.requires_grad and torch.equal(out, base.weight * 4.0)
+    handle.remove()
+    assert not layer(ids).requires_grad

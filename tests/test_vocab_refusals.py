@@ -157,3 +157,42 @@ def test_columns_next_to_2_31(mga):
         for step in (False, True):
             refused(mga, _fwd(lib, step, n=1, v=v, rs=v, gs=v, grad=far), b"columns")
         refused(mga, lib.mga_top_logits_ce_bwd(P, v, P, 4, 0, P, P, 1, v, 4, 1.0, 0, P, far, v, None), b"columns")
+
+
+def test_layer_keeps_what_the_base_carries(mga):
+    base = torch.nn.Embedding(6, 4).eval()
+    base.note = "mine"
+    seen = []
+    handles = [base.register_forward_pre_hook(lambda m, args: seen.append("pre")),
+               base.register_forward_hook(lambda m, args, out: seen.append("post")),
+               base.register_full_backward_hook(lambda m, gi, go: None),
+               base._register_state_dict_hook(lambda m, sd, prefix, meta: sd.update(extra=1) or sd)]
+    layer = mga.ScaledEmbedding.wrap(base, 3.0)
+    assert not layer.training and layer.note == "mine" and "extra" in layer.state_dict()
+    assert len(layer._forward_hooks) == len(layer._backward_hooks) == 1
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        layer(torch.zeros(2, dtype=torch.long))
+    assert seen == ["pre"]
+    for h in handles:
+        h.remove()
+    assert not layer._forward_hooks and not layer._forward_pre_hooks and not layer._backward_hooks
+    layer.weight = torch.nn.Parameter(torch.zeros(6, 4))   # of the layer alone
+    assert layer.weight is not base.weight
+
+
+def test_layers_that_are_not_wrapped(mga):
+    class Scaled(torch.nn.Embedding):
+        def forward(self, ids):
+            return super().forward(ids) * 2
+
+    class Named(torch.nn.Embedding):
+        pass
+
+    patched = torch.nn.Embedding(6, 4)
+    patched.forward = lambda ids: None
+    normed = torch.nn.utils.parametrizations.weight_norm(torch.nn.Embedding(6, 4))
+    for base, text in ((Scaled(6, 4), "forward of its own"), (patched, "forward of its own"),
+                       (mga.ScaledEmbedding(6, 4, scale=2.0), "forward of its own"), (normed, "parameter")):
+        with pytest.raises(NotImplementedError, match=text):
+            mga.ScaledEmbedding.wrap(base)
+    assert mga.ScaledEmbedding.wrap(Named(6, 4)).num_embeddings == 6
