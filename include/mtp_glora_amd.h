@@ -524,7 +524,7 @@ int mga_sample(const void *logits, int64_t row_stride, int32_t n_rows, int32_t n
  * Scaled embedding lookup: out[n, :] = T(scale * weight[ids[n], :]) for n_ids ids
  * (int64 if ids_are_int64 else int32) of a [n_rows, width] table, T = rounding to
  * the dtype; zeros for an id outside the table. n_ids times the 1 024s of columns
- * (rounded up) < 2^26, width < 2^23; out may not overlap weight. The lookup at the start of
+ * (rounded up) <= 2^26 - 4, width <= 2^23; out may not overlap weight. The lookup at the start of
  * Qwen3Model.forward (mtp_glora/models/modeling_qwen3.py:436); the table is the one
  * that resize_token_embeddings grows (:616).
  */
@@ -535,7 +535,7 @@ int mga_embedding_fwd(const void *ids, int32_t ids_are_int64, int32_t n_ids, con
 /*
  * Its gradient: grad_weight[v, :] = T(scale * sum over n with ids[n] = v of
  * grad_out[n, :]), summed in fp32 in a fixed order (parts of ascending n, added in
- * their order); n_ids < 2^30; grad_weight may not overlap grad_out; ids equal to
+ * their order); n_ids <= 2^26; grad_weight may not overlap grad_out; ids equal to
  * padding_idx (-1: none) or outside the table count nowhere. The whole of
  * grad_weight [n_rows, width] is written, or, with accumulate, the sums are added
  * to it (one rounding) and rows without a token are left as they are.

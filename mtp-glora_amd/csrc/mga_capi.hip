@@ -848,6 +848,10 @@ namespace {
 
 constexpr int32_t kMaxVocab = 1 << 20, kMaxCeVocab = 1 << 30, kMaxTopLogits = 1024;
 
+// Sorted tiles of 8 192 ids are merged in time that grows with the square of their
+// number: 2^23 ids 65 ms, so 2^26 four seconds and 2^30 a quarter of an hour.
+constexpr int32_t kMaxGradIds = 1 << 26;
+
 // A [n_rows, n_cols] operand of 16-bit or fp32 elements.
 int check_matrix(const char *fn, const char *name, const void *p, int64_t rs, int32_t n_rows, int32_t n_cols,
                  int32_t dtype) {
@@ -1034,7 +1038,8 @@ int mga_embedding_fwd(const void *ids, int32_t ids_are_int64, int32_t n_ids, con
   if (rc != MGA_OK || n_ids == 0) return rc;
   rc = check_matrix(fn, "out", out, out_row_stride, n_ids, width, dtype);
   if (rc != MGA_OK) return rc;
-  if ((int64_t)n_ids * ((width + 1023) / 1024) >= int64_t(1) << 26)
+  // four waves a workgroup, a launch of fewer than 2^32 threads
+  if ((int64_t)n_ids * ((width + 1023) / 1024) > (int64_t(1) << 26) - 4)
     return fail(MGA_ERR_INVALID, "%s: %d ids of width %d are too many", fn, n_ids, width);
   const int eb = elem_bytes(dtype);
   if (overlap(weight, weight_row_stride, out, out_row_stride, n_rows, n_ids, width, eb, eb))
@@ -1067,7 +1072,7 @@ int mga_embedding_bwd(const void *grad_out, int64_t grad_out_row_stride, const v
     return fail(MGA_ERR_INVALID, "%s: workspace null, not 16-byte aligned or smaller than %lld bytes", fn,
                 (long long)mga::embed_workspace_bytes(n_ids, width));
   const int eb = elem_bytes(dtype), ob = elem_bytes(grad_weight_dtype);
-  if (n_ids >= 1 << 30) return fail(MGA_ERR_INVALID, "%s: %d ids (fewer than %d)", fn, n_ids, 1 << 30);
+  if (n_ids > kMaxGradIds) return fail(MGA_ERR_INVALID, "%s: %d ids (at most %d)", fn, n_ids, kMaxGradIds);
   if (n_ids > 0 && overlap(grad_out, grad_out_row_stride, grad_weight, grad_weight_row_stride, n_ids, n_rows, width, eb, ob))
     return fail(MGA_ERR_INVALID, "%s: grad_weight overlaps grad_out", fn);
   const mga::EmbedArgs a{ids, nullptr, 0, grad_out, grad_out_row_stride, grad_weight, grad_weight_row_stride, scale,

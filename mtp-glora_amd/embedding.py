@@ -46,7 +46,8 @@ def embedding_grad(grad_out: torch.Tensor, ids: torch.Tensor, num_embeddings: in
     added in fp32 in a fixed order; ids equal to ``padding_idx`` or
     outside the table count nowhere. ``out`` (the gradients' dtype or fp32) receives
     it; with ``accumulate`` the sums are added to ``out``, whose other rows are
-    neither read nor written: the chunks of a sequence can share one buffer."""
+    neither read nor written: the chunks of a sequence can share one buffer. At most
+    2^26 ids."""
     _dev("grad_out", grad_out)
     if grad_out.dim() < 1 or grad_out.shape[:-1] != ids.shape:
         raise ValueError(f"grad_out {tuple(grad_out.shape)} does not fit ids {tuple(ids.shape)}")

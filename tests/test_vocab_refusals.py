@@ -196,3 +196,13 @@ def test_layers_that_are_not_wrapped(mga):
         with pytest.raises(NotImplementedError, match=text):
             mga.ScaledEmbedding.wrap(base)
     assert mga.ScaledEmbedding.wrap(Named(6, 4)).num_embeddings == 6
+
+
+def test_launches_of_2_32_threads(mga):
+    """The smallest numbers of ids that are refused, and those that would make a launch
+    of exactly 2^32 threads (in the backward behind others that were queued)."""
+    lib, far = mga.load_library(), ctypes.c_void_p(1 << 44)
+    for n, h in (((1 << 26) - 3, 8), ((1 << 26) - 1, 1024), ((1 << 25) - 1, 1025), ((1 << 26) // 3, 3000)):
+        refused(mga, lib.mga_embedding_fwd(P, 0, n, P, h, 10, h, 1.0, 0, far, h, None), b"too many")
+    for n in ((1 << 26) + 1, (1 << 30) - 63, (1 << 30) - 1):
+        refused(mga, lib.mga_embedding_bwd(P, 8, P, 0, n, 1.0, -1, 10, 8, 0, far, 8, 0, 0, P, 1 << 40, None), b"ids")
