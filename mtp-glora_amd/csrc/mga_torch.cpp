@@ -574,7 +574,7 @@ struct TopCe {
 };
 std::optional<TopCe> top_ce_operands(const Tensor &x, const Tensor &values, const Tensor &ids,
                                      const std::optional<Tensor> &lse) {
-  if (!eager()) return std::nullopt;
+  if (!eager() || x.dim() < 1) return std::nullopt;
   for (const Tensor *t : {&x, &values, &ids})
     if (!plain(*t) || t->device() != x.device() || t->dim() != x.dim()) return std::nullopt;
   TopCe o;

@@ -424,3 +424,11 @@ def check_ce_calls(mga, x, values, ids, tau, go=0.375):
     total = mga.top_logits_cross_entropy(xs, values, ids, None, tau)
     (total * go).backward()
     return total, xs.grad, mga.top_logits_loss_and_grad(x, values, ids, None, tau, scale=go)[1]
+
+
+def test_logits_without_a_dimension_are_refused(mga, dev):
+    x, i = torch.zeros((), device=dev), torch.zeros((), dtype=torch.int32, device=dev)
+    for call in (lambda: mga.top_logits_cross_entropy(x, x, i), lambda: mga.top_logits_loss_and_grad(x, x, i),
+                 lambda: mga.top_logits(x, 1), lambda: mga.sample_tokens(x, x)):
+        with pytest.raises(ValueError):
+            call()
