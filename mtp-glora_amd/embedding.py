@@ -69,6 +69,7 @@ def embedding_grad(grad_out: torch.Tensor, ids: torch.Tensor, num_embeddings: in
             raise ValueError("out: rows must be contiguous and must not overlap")
         if out.requires_grad and torch.is_grad_enabled():
             raise ValueError("out must not require a gradient")
+        torch.autograd.graph.increment_version(out)   # a graph that saved it sees the write
     dy = _rows2(grad_out, H)
     n = i.numel()
     nb = int(_lib.load().mga_embedding_workspace_bytes(n, H))

@@ -265,3 +265,18 @@ def test_layer_of_a_frozen_model(mga, dev):
     assert out.requires_grad and torch.equal(out, base.weight * 4.0)
     handle.remove()
     assert not layer(ids).requires_grad
+
+
+def test_out_counts_as_written(mga, dev):
+    """A graph that saved ``out`` before it was written refuses its backward."""
+    ids, dy = torch.arange(4, device=dev), torch.ones(4, 8, device=dev)
+    for accumulate in (False, True):
+        out, w = torch.ones(6, 8, device=dev), torch.ones(6, 8, device=dev, requires_grad=True)
+        y = (out * w).sum()
+        mga.embedding_grad(dy, ids, 6, out=out, accumulate=accumulate)
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    with torch.inference_mode():
+        out = torch.zeros(6, 8, device=dev)
+        mga.embedding_grad(dy, ids, 6, out=out)
+    assert float(out.sum()) == 32
