@@ -25,3 +25,10 @@ def dev():
     if not torch.cuda.is_available():
         raise RuntimeError("GPU tests need a visible GPU")
     return torch.device("cuda:0")
+
+
+@pytest.fixture(autouse=True)
+def seeded():
+    """Every test begins with the same generators, so that a failure repeats."""
+    import torch
+    torch.manual_seed(20240)
