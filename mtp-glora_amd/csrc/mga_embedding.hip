@@ -379,8 +379,10 @@ __global__ __launch_bounds__(kJoinThreads) void embed_join_kernel(EmbedArgs a, c
 // waves in order. The others: clear those of `rows` rows that no token has. 323
 // tokens, half of one id, new and added to: 1 024 x 256 fp32 5.8 and 5.5 us, sorted
 // 15.6 and 17.1; 32 003 x 2 560 fp16 27 and 8, sorted 34 and 20; all 512 of one id
-// 35 and 16, sorted 33 and 18. A table of 1.2 GB is cleared faster beside the sort
-// (tiles of 256 KB that look no row up): 218 against 237 us.
+// 35 and 16, sorted 33 and 18. A large table is cleared faster beside the sort (parts
+// of 256 KB that look no row up); 323 tokens x 4 096 bf16, few against sorted: 131 MB 29
+// and 32 us, 213 MB 49 and 50, 262 MB 59 and 59, 426 MB 91 and 87, 1.2 GB 233 and 221
+// (64 tokens: even at 524 MB; 512: 33 MB 23 and 27, 131 MB 34 and 31).
 constexpr int kFew = 512, kFewThreads = 512, kFewWaves = kFewThreads / 64, kFewRows = 4096;
 constexpr int64_t kFewClear = 64 << 10, kFewTable = 256 << 20;   // bytes a workgroup clears; of the table
 template <typename T, typename TO, bool VEC, bool ADD>

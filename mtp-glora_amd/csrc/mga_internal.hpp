@@ -224,7 +224,7 @@ struct TopLogitsCeArgs {
 int64_t top_ce_workspace_floats(int32_t N, int32_t V);
 void launch_top_ce_fwd(const TopLogitsCeArgs &a, int dtype, float *ws, hipStream_t stream);
 void launch_top_ce_bwd(const TopLogitsCeArgs &a, int dtype, hipStream_t stream);
-// loss and gradient; q and stats are written too where the rows do not fit registers
+// loss and gradient; of fewer than 96 rows by the two above, which write q and stats too
 void launch_top_ce_step(const TopLogitsCeArgs &a, int dtype, float *ws, hipStream_t stream);
 
 // Scaled embedding and its gradient (mga_embedding.hip).

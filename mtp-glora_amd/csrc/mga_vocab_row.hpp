@@ -117,7 +117,9 @@ struct Row {
   // f(v, col): every thread's vectors in ascending order (all lanes take part; a
   // thread without one has -inf and a column of at least V); last(b) behind the
   // vectors of block b. K blocks are asked for before the first is used: a row is
-  // few blocks, and each wait for memory is about 2 600 cycles.
+  // few blocks, and each wait for memory is about 2 600 cycles. K = 5 is the whole of a
+  // 16-bit row of up to 163 840 columns, in 80 registers a lane: for kernels that have
+  // the compute unit to themselves anyway.
   template <int K, typename F, typename L>
   __device__ __forceinline__ void each_vec(F f, L last) const {
     const int n = blocks();
@@ -580,7 +582,12 @@ __device__ __forceinline__ void scan_hits(const Row<T> &row, const RowShared &sh
 // Each wave puts its threads' largest in order; with j = ceil(k / 16) the least of
 // the 16 waves' j-th ones has at least 16 j >= k elements at or above it, and for
 // ordinary rows few more: those are taken into LDS and put in order there. A row
-// with too many of them (equal values) has its threshold found digit by digit.
+// with too many of them (equal values) has its threshold found digit by digit. So
+// has any row where k comes near the 1 024 threads (the least of all their largest lets
+// some 4 % through), and one of 16-bit elements and 4 097 to about 7 700 columns, of which
+// some waves hold no vector. 1 024 x 151 936 bf16, a call by itself: k = 64 89 us, 256 114,
+// 512 139, 896 226, 1 024 427; 256 rows, k = 64: of 6 000 columns 23 us, of 8 192 14, of
+// 3 000 (all in the list) 46.
 template <typename T>
 __device__ __forceinline__ void top_list(const Row<T> &row, RowShared &sh, int group, float tmax, int k) {
   const int tid = threadIdx.x, lane = tid & 63;
