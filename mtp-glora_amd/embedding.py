@@ -157,6 +157,7 @@ class ScaledEmbedding(nn.Embedding):
         vars(m).update(vars(base))
         for own in ("_parameters", "_buffers", "_modules", "_non_persistent_buffers_set"):
             vars(m)[own] = vars(base)[own].copy()
+        vars(m).pop("_compiled_call_impl", None)   # the base's own forward, compiled
         m.scale = float(scale)
         return m
 

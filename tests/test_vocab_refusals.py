@@ -206,3 +206,11 @@ def test_launches_of_2_32_threads(mga):
         refused(mga, lib.mga_embedding_fwd(P, 0, n, P, h, 10, h, 1.0, 0, far, h, None), b"too many")
     for n in ((1 << 26) + 1, (1 << 30) - 63, (1 << 30) - 1):
         refused(mga, lib.mga_embedding_bwd(P, 8, P, 0, n, 1.0, -1, 10, 8, 0, far, 8, 0, 0, P, 1 << 40, None), b"ids")
+
+
+def test_layer_does_not_keep_a_compiled_forward(mga):
+    base = torch.nn.Embedding(6, 4)
+    base._compiled_call_impl = lambda ids: "base"   # as Module.compile() leaves it
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        mga.ScaledEmbedding.wrap(base, 3.0)(torch.zeros(2, dtype=torch.long))
+    assert base(torch.zeros(2, dtype=torch.long)) == "base"
