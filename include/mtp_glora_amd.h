@@ -393,7 +393,7 @@ int mga_gated_lora_bwd(const void *grad_y, int64_t gy_rs, const void *x, int64_t
  *   row_loss[r] = -(sum e^{t - mt} x) / dt + mx + log dx,
  *   stats = [mx[n_rows], dx[n_rows], mt[n_rows], dt[n_rows]] (fp32).
  * The caller sums row_loss (StableSoftCrossEntropy.forward returns that sum).
- * workspace: mga_soft_ce_workspace_floats(n_rows, n_cols) fp32 values.
+ * n_cols <= 2^30. workspace: mga_soft_ce_workspace_floats(n_rows, n_cols) fp32 values.
  * Replaces stable_soft_ce_forward_kernel_{auto,manual}
  * (mtp_glora/core/loss.py:63-179) as launched by
  * StableSoftCrossEntropy.forward (loss.py:259-296).

@@ -787,11 +787,15 @@ int check_rows(const char *fn, const char *name, const void *p, int64_t rs, int3
   return MGA_OK;
 }
 
+// A loss's column behind a range or a turn of the workgroup is a 32-bit number too.
+constexpr int32_t kMaxLossCols = 1 << 30;
+
 int check_soft_ce(const char *fn, const void *x, int64_t xs, const void *t, int64_t ts, int32_t n_rows,
                   int32_t n_cols, int32_t dtype, bool *vec) {
   const int eb = elem_bytes(dtype);
   if (!eb) return fail(MGA_ERR_INVALID, "%s: unknown dtype code %d", fn, dtype);
   if (n_rows <= 0 || n_cols <= 0) return fail(MGA_ERR_INVALID, "%s: bad sizes (rows=%d cols=%d)", fn, n_rows, n_cols);
+  if (n_cols > kMaxLossCols) return fail(MGA_ERR_INVALID, "%s: %d columns (at most %d)", fn, n_cols, kMaxLossCols);
   int rc = check_rows(fn, "student", x, xs, n_cols, eb, vec);
   if (rc == MGA_OK) rc = check_rows(fn, "teacher", t, ts, n_cols, eb, vec);
   return rc;
@@ -846,7 +850,7 @@ int mga_soft_ce_bwd(const void *student, int64_t student_row_stride, const void 
 
 namespace {
 
-constexpr int32_t kMaxVocab = 1 << 20, kMaxCeVocab = 1 << 30, kMaxTopLogits = 1024;
+constexpr int32_t kMaxVocab = 1 << 20, kMaxTopLogits = 1024;
 
 // Sorted tiles of 8 192 ids are merged in time that grows with the square of their
 // number: 2^23 ids 65 ms, so 2^26 four seconds and 2^30 a quarter of an hour.
@@ -895,8 +899,7 @@ int check_top_ce(const char *fn, const mga::TopLogitsCeArgs &a, int32_t dtype) {
   if (rc == MGA_OK) rc = check_row_count(fn, a.N);
   if (rc == MGA_OK) rc = check_temperature(fn, a.tau);
   if (rc != MGA_OK) return rc;
-  // the column behind a range or a turn of the workgroup is a 32-bit number too
-  if (a.V > kMaxCeVocab) return fail(MGA_ERR_INVALID, "%s: %d columns (at most %d)", fn, a.V, kMaxCeVocab);
+  if (a.V > kMaxLossCols) return fail(MGA_ERR_INVALID, "%s: %d columns (at most %d)", fn, a.V, kMaxLossCols);
   if (!a.ids || a.ids_rs < a.K) return fail(MGA_ERR_INVALID, "%s: ids null or with a row stride below k", fn);
   if (reinterpret_cast<uintptr_t>(a.ids) % (a.ids64 ? 8 : 4))
     return fail(MGA_ERR_INVALID, "%s: ids are not aligned to their elements", fn);

@@ -184,8 +184,9 @@ def top_logits_cross_entropy(student: torch.Tensor, values: torch.Tensor, ids: t
     id outside [0, V) is padding; a row with no entry left has loss and gradient
     zero. ``values`` may have another dtype than the student. Differentiable in
     ``student``, once; the teacher gets no gradient. With k = V kept and temperature 1
-    this is StableSoftCrossEntropy. k <= 1024, V <= 2^30. Under graph capture refused while an eager
-    graph of the same leaf lives; top_logits_loss_and_grad needs no graph."""
+    this is StableSoftCrossEntropy. k <= 1024, V <= 2^30. Under graph capture refused
+    while an eager graph of the same leaf lives; top_logits_loss_and_grad needs no
+    graph."""
     temperature = _temperature(temperature)
     r = _lib.native("top_logits_ce", student, values, ids, lse, temperature)
     return r if r is not None else TopLogitsCrossEntropy.apply(student, values, ids, lse, temperature)

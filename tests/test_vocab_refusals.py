@@ -214,3 +214,11 @@ def test_layer_does_not_keep_a_compiled_forward(mga):
     with pytest.raises(RuntimeError, match="GPU tensor"):
         mga.ScaledEmbedding.wrap(base, 3.0)(torch.zeros(2, dtype=torch.long))
     assert base(torch.zeros(2, dtype=torch.long)) == "base"
+
+
+def test_soft_ce_columns_next_to_2_31(mga):
+    lib, far = mga.load_library(), ctypes.c_void_p(1 << 40)
+    for v in ((1 << 30) + 1, 2147383647, (1 << 31) - 1):
+        refused(mga, lib.mga_soft_ce_fwd(P, v, P, v, 1, v, 0, P, P, P, None), b"columns")
+        refused(mga, lib.mga_soft_ce_loss(P, v, P, v, 1, v, 0, P, P, P, P, None), b"columns")
+        refused(mga, lib.mga_soft_ce_bwd(P, v, P, v, 1, v, 0, P, P, far, v, None), b"columns")
