@@ -548,6 +548,57 @@ int mga_embedding_bwd(const void *grad_out, int64_t grad_out_row_stride, const v
                       void *grad_weight, int64_t grad_weight_row_stride, int32_t grad_weight_dtype,
                       int32_t accumulate, void *workspace, int64_t workspace_bytes, void *stream);
 
+/*
+ * New tokens' keys and values into a paged 8-bit cache, normalised and rotated on the
+ * way. A cache of num_pages pages of page_size (16, 32, 64 or 128) tokens:
+ *   k_pages [num_pages, Hkv, page_size, head_dim], v_pages [num_pages, Hkv, head_dim,
+ *   page_size], one e4m3 byte each, 16-byte aligned; k_scale, v_scale [num_pages, Hkv].
+ * n_seqs sequences: cu_tokens [n_seqs + 1] (ascending from 0) bounds each one's new
+ * tokens among the n_tokens rows, lengths [n_seqs] holds its tokens in the cache, and row b of
+ * block_table [n_seqs, table_width] its pages in order. Token i of sequence b goes
+ * to position lengths[b] + i; positions without a page (past the table, an id
+ * outside [0, num_pages)) are not stored. No two sequences may write to one page.
+ *   k: y = x rsqrt(mean x^2 + eps) k_weight (k_weight null: y = x), then
+ *      r = y cos + rotate_half(y) sin (cos null: r = y), in fp32; v: r = x.
+ *   scale of a (page, head): the least power of two (2^-100 .. 2^119) of which 448 hold
+ *      |r| of its rows; where the first row written is not the page's row 0, at least the
+ *      old scale, and if it grows the rows before are rounded again.
+ *   code = e4m3(r / scale), to nearest even; NaN and infinities become NaN codes and
+ *      count in no scale.
+ * query (null: none) likewise with q_weight into query_out, rounded once to the dtype;
+ * its rows behind cu_tokens[n_seqs] are zeros. cos, sin [n_tokens, head_dim] in the dtype, or fp32
+ * with cos_sin_f32. Rows behind a sequence's end in its last page, and all other pages,
+ * stay as they are. n_seqs <= 4096; head_dim 64 or 128. Beside mga_kv_append and
+ * mga_qk_norm_rope_stage_fwd (mtp_glora/models/modeling_qwen3.py:274-284).
+ */
+int mga_paged_append(const void *key, int64_t k_stride_s, int64_t k_stride_h, const void *value, int64_t v_stride_s,
+                     int64_t v_stride_h, const void *query, int64_t q_stride_s, int64_t q_stride_h, const void *q_weight,
+                     const void *k_weight, const void *cos, const void *sin, int64_t cos_sin_stride, int32_t cos_sin_f32,
+                     float eps, int32_t n_tokens, int32_t n_seqs, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t dtype,
+                     void *k_pages, void *v_pages, float *k_scale, float *v_scale, int32_t num_pages, int32_t page_size,
+                     const int32_t *block_table, int64_t table_row_stride, int32_t table_width, const int32_t *cu_tokens,
+                     const int32_t *lengths, void *query_out, int64_t qo_stride_s, int64_t qo_stride_h, void *stream);
+
+/*
+ * Attention of the new tokens over that cache, themselves included (append first):
+ *   o_i = sum_j softmax_j(scale q_i . k_j) v_j over the positions j <= lengths[b] + i
+ * of the token's sequence that have a page; zeros where there is none. What a row may
+ * not see does not reach it, NaN included. Scores, sums and outputs in fp32; P
+ * is rounded to bf16 (bf16 queries), or kept to 16 (fp16) or 24 bits (fp32).
+ * q, out: [n_tokens, Hq, head_dim], rows 16-byte aligned; Hq / Hkv <= 32. Rows of
+ * out behind cu_tokens[n_seqs]: zeros with zero_rest, else left as they are. workspace:
+ * mga_paged_attn_workspace_bytes bytes, 16-byte aligned, one for each call in flight. Sums run in a fixed
+ * order. Beside mga_attn_fwd ([tf]integrations/flex_attention.py:262-368).
+ */
+int64_t mga_paged_attn_workspace_bytes(int32_t n_tokens, int32_t n_seqs, int32_t Hq, int32_t Hkv, int32_t head_dim,
+                                       int32_t dtype);
+int mga_paged_attn(const void *q, int64_t q_stride_s, int64_t q_stride_h, const void *k_pages, const void *v_pages,
+                   const float *k_scale, const float *v_scale, int32_t num_pages, int32_t page_size,
+                   const int32_t *block_table, int64_t table_row_stride, int32_t table_width, const int32_t *cu_tokens,
+                   const int32_t *lengths, int32_t n_tokens, int32_t n_seqs, int32_t Hq, int32_t Hkv, int32_t head_dim,
+                   int32_t dtype, float scale, void *out, int64_t o_stride_s, int64_t o_stride_h, int32_t zero_rest,
+                   void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,9 @@ The package mirrors the reference's operator boundaries for this path:
   cross-entropy against whole rows
 * ``sample_tokens``             - tokens from logits with temperature, top-k,
   top-p and min-p, from given random numbers
+* ``PagedKVCache`` / ``paged_append`` / ``paged_attention`` - decoding: a paged 8-bit
+  cache of several sequences, filled with the rotation on the way, and the attention
+  of new tokens over it
 * ``scaled_embedding`` / ``ScaledEmbedding`` / ``embedding_grad`` - the lookup at
   the start of a chunk and its gradient by sorted tokens
 
@@ -38,6 +41,7 @@ from .embedding import ScaledEmbedding, embedding_grad, scaled_embedding
 from .lora import GatedLoRALinear, apply_lora_to_model, gated_lora_linear
 from .loss import StableSoftCrossEntropy
 from .manager import StreamingKVCacheManager
+from .paged import KVPages, PagedKVCache, paged_append, paged_attention
 from .rope import qk_norm_rope, qwen3_attention_forward
 from .sampling import sample_tokens
 
@@ -46,7 +50,8 @@ __all__ = [
     "mtp_attention", "mtp_attention_forward", "register", "ops", "StableSoftCrossEntropy",
     "qk_norm_rope", "qwen3_attention_forward", "GatedLoRALinear", "apply_lora_to_model", "gated_lora_linear",
     "TopLogits", "TopLogitsCrossEntropy", "top_logits", "top_logits_cross_entropy", "top_logits_loss_and_grad",
-    "sample_tokens", "ScaledEmbedding", "scaled_embedding", "embedding_grad",
+    "sample_tokens", "ScaledEmbedding", "scaled_embedding", "embedding_grad", "PagedKVCache", "KVPages",
+    "paged_append", "paged_attention",
 ]
 
 

@@ -10,6 +10,7 @@
 #include "../../include/mtp_glora_amd.h"
 #include "mga_common.hpp"
 #include "mga_internal.hpp"
+#include "mga_paged.hpp"
 
 static_assert(MGA_BWD_DQ == mga::kBwdDq && MGA_BWD_DKDV == mga::kBwdDkDv, "pass flags");
 static_assert(MGA_DTYPE_BF16 == mga::kDtBf16 && MGA_DTYPE_F32 == mga::kDtF32 && MGA_DTYPE_F16 == mga::kDtF16,
@@ -1083,6 +1084,135 @@ int mga_embedding_bwd(const void *grad_out, int64_t grad_out_row_stride, const v
   const bool vec = (int64_t)width * eb % 16 == 0 && (n_ids == 0 || vec_rows(grad_out, grad_out_row_stride, eb)) &&
                    vec_rows(grad_weight, grad_weight_row_stride, ob);
   mga::launch_embed_bwd(a, dtype, grad_weight_dtype, vec, accumulate != 0, workspace, (hipStream_t)stream);
+  return check_launch(fn);
+}
+
+namespace {
+
+struct PagedCall {
+  const void *k_pages, *v_pages;
+  const float *k_scale, *v_scale;
+  int32_t num_pages, page_size;
+  const int32_t *table; int64_t table_rs; int32_t width;
+  const int32_t *cu, *lengths;
+  int32_t T, B, Hq, Hkv, D, dtype;
+};
+
+int check_paged(const char *fn, const PagedCall &c) {
+  if (c.T < 0 || c.B <= 0 || c.B > mga::kMaxSeqs)
+    return fail(MGA_ERR_INVALID, "%s: bad sizes (tokens=%d sequences=%d, at most %d)", fn, c.T, c.B, mga::kMaxSeqs);
+  if (c.D != 64 && c.D != 128) return fail(MGA_ERR_INVALID, "%s: head_dim must be 64 or 128 (got %d)", fn, c.D);
+  if (c.Hq <= 0 || c.Hkv <= 0 || c.Hq % c.Hkv)
+    return fail(MGA_ERR_INVALID, "%s: Hq (%d) must be a positive multiple of Hkv (%d)", fn, c.Hq, c.Hkv);
+  if (!elem_bytes(c.dtype)) return fail(MGA_ERR_INVALID, "%s: unknown dtype code %d", fn, c.dtype);
+  if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128)
+    return fail(MGA_ERR_INVALID, "%s: page_size must be 16, 32, 64 or 128 (got %d)", fn, c.page_size);
+  if (c.num_pages <= 0 || c.width <= 0)
+    return fail(MGA_ERR_INVALID, "%s: bad sizes (pages=%d table width=%d)", fn, c.num_pages, c.width);
+  if (c.table_rs < c.width)
+    return fail(MGA_ERR_INVALID, "%s: block_table row stride %lld < %d", fn, (long long)c.table_rs, c.width);
+  // positions are 32-bit numbers
+  if ((int64_t)c.width * c.page_size + c.T > (int64_t(1) << 30))
+    return fail(MGA_ERR_INVALID, "%s: sequences of %lld tokens are too long", fn, (long long)c.width * c.page_size + c.T);
+  if (!c.k_pages || !c.v_pages || !aligned16(c.k_pages) || !aligned16(c.v_pages))
+    return fail(MGA_ERR_INVALID, "%s: pages null or not 16-byte aligned", fn);
+  if (!c.k_scale || !c.v_scale || !c.table || !c.cu || !c.lengths)
+    return fail(MGA_ERR_INVALID, "%s: null scale, block_table, cu_tokens or lengths", fn);
+  return MGA_OK;
+}
+
+int paged_shift(int page_size) { return page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7; }
+
+// rows of a [tokens, heads, head_dim] operand; *vec stays set where every row is 16-byte aligned
+int check_token_rows(const char *fn, const char *name, const void *p, int64_t ss, int64_t hs, int eb, bool *vec) {
+  if (!p) return fail(MGA_ERR_INVALID, "%s: %s is null", fn, name);
+  if (ss < 0 || hs < 0) return fail(MGA_ERR_INVALID, "%s: %s has negative strides", fn, name);
+  if (reinterpret_cast<uintptr_t>(p) % eb) return fail(MGA_ERR_INVALID, "%s: %s is not aligned to its elements", fn, name);
+  *vec = *vec && aligned16(p) && ss * eb % 16 == 0 && hs * eb % 16 == 0;
+  return MGA_OK;
+}
+
+}  // namespace
+
+int mga_paged_append(const void *key, int64_t k_stride_s, int64_t k_stride_h, const void *value, int64_t v_stride_s,
+                     int64_t v_stride_h, const void *query, int64_t q_stride_s, int64_t q_stride_h, const void *q_weight,
+                     const void *k_weight, const void *cos, const void *sin, int64_t cos_sin_stride, int32_t cos_sin_f32,
+                     float eps, int32_t n_tokens, int32_t n_seqs, int32_t Hq, int32_t Hkv, int32_t head_dim, int32_t dtype,
+                     void *k_pages, void *v_pages, float *k_scale, float *v_scale, int32_t num_pages, int32_t page_size,
+                     const int32_t *block_table, int64_t table_row_stride, int32_t table_width, const int32_t *cu_tokens,
+                     const int32_t *lengths, void *query_out, int64_t qo_stride_s, int64_t qo_stride_h, void *stream) {
+  const char *fn = "mga_paged_append";
+  int rc = check_paged(fn, {k_pages, v_pages, k_scale, v_scale, num_pages, page_size, block_table, table_row_stride,
+                            table_width, cu_tokens, lengths, n_tokens, n_seqs, query ? Hq : Hkv, Hkv, head_dim, dtype});
+  if (rc != MGA_OK || n_tokens == 0) return rc;
+  const int eb = elem_bytes(dtype);
+  bool vec = true;
+  if ((rc = check_token_rows(fn, "key", key, k_stride_s, k_stride_h, eb, &vec)) != MGA_OK ||
+      (rc = check_token_rows(fn, "value", value, v_stride_s, v_stride_h, eb, &vec)) != MGA_OK)
+    return rc;
+  if (query) {
+    if ((rc = check_token_rows(fn, "query", query, q_stride_s, q_stride_h, eb, &vec)) != MGA_OK ||
+        (rc = check_token_rows(fn, "query_out", query_out, qo_stride_s, qo_stride_h, eb, &vec)) != MGA_OK)
+      return rc;
+  }
+  if ((cos == nullptr) != (sin == nullptr)) return fail(MGA_ERR_INVALID, "%s: one of cos and sin is null", fn);
+  const int ceb = cos_sin_f32 ? 4 : eb;
+  if (cos && ((rc = check_token_rows(fn, "cos", cos, cos_sin_stride, 0, ceb, &vec)) != MGA_OK ||
+              (rc = check_token_rows(fn, "sin", sin, cos_sin_stride, 0, ceb, &vec)) != MGA_OK))
+    return rc;
+  for (const void *w : {q_weight, k_weight})
+    if (w && (rc = check_token_rows(fn, "norm weight", w, 0, 0, eb, &vec)) != MGA_OK) return rc;
+  if (!(eps >= 0.f)) return fail(MGA_ERR_INVALID, "%s: eps must not be negative (got %g)", fn, (double)eps);
+  const mga::PagedAppendArgs a{key, k_stride_s, k_stride_h, value, v_stride_s, v_stride_h, query, q_stride_s, q_stride_h,
+                               query_out, qo_stride_s, qo_stride_h, q_weight, k_weight, cos, sin, cos_sin_stride,
+                               (uint8_t *)k_pages, (uint8_t *)v_pages, k_scale, v_scale, block_table, table_row_stride,
+                               cu_tokens, lengths, eps, n_tokens, n_seqs, Hq, Hkv, num_pages, paged_shift(page_size),
+                               table_width, vec, cos_sin_f32 != 0};
+  // a launch of fewer than 2^32 threads
+  if (mga::paged_append_blocks(a) >= (int64_t(1) << 24))
+    return fail(MGA_ERR_INVALID, "%s: %d tokens of %d sequences are too many", fn, n_tokens, n_seqs);
+  mga::launch_paged_append(a, head_dim, dtype, (hipStream_t)stream);
+  return check_launch(fn);
+}
+
+int64_t mga_paged_attn_workspace_bytes(int32_t n_tokens, int32_t n_seqs, int32_t Hq, int32_t Hkv, int32_t head_dim,
+                                       int32_t dtype) {
+  if (n_tokens <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0) return 0;
+  return mga::paged_attn_ws_bytes(n_tokens, n_seqs, Hq, Hkv, head_dim, dtype);
+}
+
+int mga_paged_attn(const void *q, int64_t q_stride_s, int64_t q_stride_h, const void *k_pages, const void *v_pages,
+                   const float *k_scale, const float *v_scale, int32_t num_pages, int32_t page_size,
+                   const int32_t *block_table, int64_t table_row_stride, int32_t table_width, const int32_t *cu_tokens,
+                   const int32_t *lengths, int32_t n_tokens, int32_t n_seqs, int32_t Hq, int32_t Hkv, int32_t head_dim,
+                   int32_t dtype, float scale, void *out, int64_t o_stride_s, int64_t o_stride_h, int32_t zero_rest,
+                   void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *fn = "mga_paged_attn";
+  int rc = check_paged(fn, {k_pages, v_pages, k_scale, v_scale, num_pages, page_size, block_table, table_row_stride,
+                            table_width, cu_tokens, lengths, n_tokens, n_seqs, Hq, Hkv, head_dim, dtype});
+  if (rc != MGA_OK || n_tokens == 0) return rc;
+  if (Hq / Hkv > 32) return fail(MGA_ERR_INVALID, "%s: %d query heads a KV head (at most 32)", fn, Hq / Hkv);
+  if (!(scale > 0.f) || !(scale < __builtin_huge_valf()))
+    return fail(MGA_ERR_INVALID, "%s: scale must be positive and finite (got %g)", fn, (double)scale);
+  const int eb = elem_bytes(dtype);
+  bool vec = true;
+  if ((rc = check_token_rows(fn, "q", q, q_stride_s, q_stride_h, eb, &vec)) != MGA_OK ||
+      (rc = check_token_rows(fn, "out", out, o_stride_s, o_stride_h, eb, &vec)) != MGA_OK)
+    return rc;
+  if (!vec) return fail(MGA_ERR_INVALID, "%s: rows of q and out must be 16-byte aligned", fn);
+  float *ws = nullptr;
+  const int64_t need = mga::paged_attn_ws_bytes(n_tokens, n_seqs, Hq, Hkv, head_dim, dtype);
+  if (!workspace) return fail(MGA_ERR_INVALID, "%s: null workspace", fn);
+  if ((rc = check_attn_ws(fn, workspace, workspace_bytes, need, &ws)) != MGA_OK) return rc;
+  const mga::PagedAttnArgs a{q, q_stride_s, q_stride_h, (const uint8_t *)k_pages, (const uint8_t *)v_pages, k_scale,
+                             v_scale, block_table, table_row_stride, cu_tokens, lengths, out, o_stride_s, o_stride_h, ws,
+                             scale * mga::kLog2e, n_tokens, n_seqs, Hq, Hkv, num_pages, paged_shift(page_size),
+                             table_width, zero_rest != 0};
+  // the list of steps is counted in 32 bits
+  if (mga::paged_attn_steps(a, dtype) >= (int64_t(1) << 31))
+    return fail(MGA_ERR_INVALID, "%s: %d tokens over sequences of %lld are too many", fn, n_tokens,
+                (long long)table_width * page_size);
+  mga::launch_paged_attn(a, head_dim, dtype, (hipStream_t)stream);
   return check_launch(fn);
 }
 

@@ -258,6 +258,42 @@ struct SampleParams {
 void launch_sample(const void *x, int64_t xs, int32_t N, int32_t V, int dtype, const float *uniform,
                    const SampleParams &prm, int64_t *token, hipStream_t stream);
 
+// Paged 8-bit cache (mga_paged.hpp): appending with norm and rotation
+// (mga_paged_append.hip), attention over it (mga_paged_attn.hip).
+struct PagedAppendArgs {
+  const void *k; int64_t k_ss, k_hs;   // [T, Hkv, D]
+  const void *v; int64_t v_ss, v_hs;
+  const void *q; int64_t q_ss, q_hs;   // [T, Hq, D], or null
+  void *qo; int64_t qo_ss, qo_hs;
+  const void *qw, *kw;                 // norm weights [D], or null
+  const void *cos, *sin; int64_t cs_ss;   // [T, D], or null
+  uint8_t *kp, *vp;                    // pages
+  float *ks, *vs;                      // [num_pages, Hkv]
+  const int32_t *table; int64_t table_rs;   // [B, width]
+  const int32_t *cu, *lengths;         // [B + 1], [B]
+  float eps;
+  int32_t T, B, Hq, Hkv, num_pages, pshift, width;
+  bool vec, cs32;                      // 16-byte loads of every operand; cos / sin in fp32
+};
+int64_t paged_append_blocks(const PagedAppendArgs &a);   // at most
+void launch_paged_append(const PagedAppendArgs &a, int head_dim, int dtype, hipStream_t stream);
+struct PagedAttnArgs {
+  const void *q; int64_t q_ss, q_hs;   // [T, Hq, D]
+  const uint8_t *kp, *vp;
+  const float *ks, *vs;
+  const int32_t *table; int64_t table_rs;
+  const int32_t *cu, *lengths;
+  void *out; int64_t o_ss, o_hs;
+  float *ws;
+  float scale_log2;
+  int32_t T, B, Hq, Hkv, num_pages, pshift, width;
+  bool zero_rest;                      // rows behind the last sequence: zeros, else left as they are
+};
+int64_t paged_attn_ws_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int head_dim, int dtype);
+// an upper bound of the 64-key steps of a call
+int64_t paged_attn_steps(const PagedAttnArgs &a, int dtype);
+void launch_paged_attn(const PagedAttnArgs &a, int head_dim, int dtype, hipStream_t stream);
+
 // Compute units of the current device (queried once per device).
 int device_cu_count();
 

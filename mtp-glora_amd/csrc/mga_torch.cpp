@@ -41,7 +41,8 @@ using torch::autograd::variable_list;
   X(mga_gated_lora_fwd) X(mga_gated_lora_bwd) X(mga_soft_ce_workspace_floats) X(mga_soft_ce_loss)     \
   X(mga_soft_ce_bwd) X(mga_top_logits) X(mga_top_logits_ce_workspace_floats) X(mga_top_logits_ce_fwd)  \
   X(mga_top_logits_ce_bwd) X(mga_top_logits_ce_step_workspace_floats) X(mga_top_logits_ce_step)          \
-  X(mga_sample) X(mga_embedding_fwd) X(mga_embedding_workspace_bytes) X(mga_embedding_bwd)
+  X(mga_sample) X(mga_embedding_fwd) X(mga_embedding_workspace_bytes) X(mga_embedding_bwd) \
+  X(mga_paged_append) X(mga_paged_attn_workspace_bytes) X(mga_paged_attn)
 struct Api {
 #define X(f) decltype(&::f) f = nullptr;
   MGA_API(X)
@@ -748,6 +749,108 @@ std::optional<Tensor> embedding(const Tensor &ids, const Tensor &w, double scale
   return Embedding::apply(ids, w, scale, padding_idx);
 }
 
+// ---- paged cache -----------------------------------------------------------------------
+
+// [tokens, heads, D] rows with unit stride on D
+bool rows3(const Tensor &t, int64_t D, const Tensor &like) {
+  return plain(t) && t.dim() == 3 && t.size(2) == D && t.stride(2) == 1 && t.stride(0) >= 0 && t.stride(1) >= 0 &&
+         t.device() == like.device() && t.size(0) <= INT32_MAX;
+}
+
+bool aligned_rows3(const Tensor &t) {
+  const int64_t eb = t.element_size();
+  return t.stride(0) * eb % 16 == 0 && t.stride(1) * eb % 16 == 0 && aligned16(t);
+}
+
+struct Paged {
+  int32_t n, Hkv, ps, D, B, width;
+};
+
+// Pages and batch of their plain form, contiguous.
+std::optional<Paged> paged_operands(const Tensor &k, const Tensor &v, const Tensor &ks, const Tensor &vs,
+                                    const Tensor &table, const Tensor &cu, const Tensor &lengths) {
+  if (!eager()) return std::nullopt;
+  for (const Tensor *t : {&k, &v, &ks, &vs})
+    if (!plain(*t) || !t->is_contiguous() || t->device() != k.device()) return std::nullopt;
+  for (const Tensor *t : {&table, &cu, &lengths})
+    if (!int32_on(*t, k)) return std::nullopt;
+  if (k.dim() != 4 || v.dim() != 4 || k.scalar_type() != at::kFloat8_e4m3fn || v.scalar_type() != at::kFloat8_e4m3fn ||
+      ks.scalar_type() != at::kFloat || vs.scalar_type() != at::kFloat || table.dim() != 2 || table.numel() == 0)
+    return std::nullopt;
+  for (int64_t s : k.sizes())
+    if (s <= 0 || s > INT32_MAX) return std::nullopt;
+  const int64_t B = table.size(0);
+  if (v.sizes() != at::IntArrayRef{k.size(0), k.size(1), k.size(3), k.size(2)} || ks.sizes() != k.sizes().slice(0, 2) ||
+      vs.sizes() != k.sizes().slice(0, 2) || cu.sizes() != at::IntArrayRef{B + 1} || lengths.sizes() != at::IntArrayRef{B} ||
+      B > INT32_MAX || table.size(1) > INT32_MAX)
+    return std::nullopt;
+  return Paged{(int32_t)k.size(0), (int32_t)k.size(1), (int32_t)k.size(2), (int32_t)k.size(3), (int32_t)B,
+               (int32_t)table.size(1)};
+}
+
+// one tensor with a query, none without
+std::optional<std::vector<Tensor>> paged_append(const Tensor &key, const Tensor &value, const Tensor &kp, const Tensor &vp,
+                                                const Tensor &ks, const Tensor &vs, const Tensor &table, const Tensor &cu,
+                                                const Tensor &lengths, const std::optional<Tensor> &query,
+                                                const std::optional<Tensor> &cos, const std::optional<Tensor> &sin,
+                                                const std::optional<Tensor> &qw, const std::optional<Tensor> &kw,
+                                                double eps) {
+  const auto p = paged_operands(kp, vp, ks, vs, table, cu, lengths);
+  if (!p || !rows3(key, p->D, kp) || !rows3(value, p->D, kp) || dtype_code(key.scalar_type()) < 0 ||
+      value.sizes() != key.sizes() || key.size(1) != p->Hkv || !same(key, value) || key.size(0) == 0)
+    return std::nullopt;
+  const int64_t T = key.size(0);
+  if (query && (!rows3(*query, p->D, kp) || !same(*query, key) || query->size(0) != T || query->size(1) == 0))
+    return std::nullopt;
+  if (cos.has_value() != sin.has_value()) return std::nullopt;
+  if (cos) {
+    for (const Tensor *t : {&*cos, &*sin})
+      if (!plain(*t) || t->dim() != 2 || t->size(0) != T || t->size(1) != p->D || t->stride(1) != 1 || t->stride(0) < 0 ||
+          t->strides() != cos->strides() || !same(*t, *cos) || t->device() != kp.device() ||
+          (t->scalar_type() != key.scalar_type() && t->scalar_type() != at::kFloat))
+        return std::nullopt;
+  }
+  for (const auto *w : {&qw, &kw})
+    if (*w && (!plain(**w) || !(*w)->is_contiguous() || (*w)->dim() != 1 || (*w)->size(0) != p->D || !same(**w, key)))
+      return std::nullopt;
+  const at::DeviceGuard guard(kp.device());
+  std::vector<Tensor> out;
+  if (query) out.push_back(at::empty(query->sizes(), query->options().requires_grad(false)));
+  for (const Tensor *t : {&kp, &vp, &ks, &vs}) t->unsafeGetTensorImpl()->bump_version();
+  auto ptr = [](const std::optional<Tensor> &t) { return t ? t->data_ptr() : nullptr; };
+  auto st = [](const std::optional<Tensor> &t, int i) { return t ? t->stride(i) : 0; };
+  check_rc("mga_paged_append",
+           g.mga_paged_append(key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+                              value.stride(1), ptr(query), st(query, 0), st(query, 1), ptr(qw), ptr(kw), ptr(cos), ptr(sin),
+                              st(cos, 0), cos && cos->scalar_type() == at::kFloat, (float)eps, (int32_t)T, p->B,
+                              query ? (int32_t)query->size(1) : 0, p->Hkv, p->D, dtype_code(key.scalar_type()),
+                              kp.data_ptr(), vp.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), p->n, p->ps,
+                              table.data_ptr<int32_t>(), p->width, p->width, cu.data_ptr<int32_t>(),
+                              lengths.data_ptr<int32_t>(), query ? out[0].data_ptr() : nullptr, query ? out[0].stride(0) : 0,
+                              query ? out[0].stride(1) : 0, stream(kp)));
+  return out;
+}
+
+std::optional<Tensor> paged_attention(const Tensor &q, const Tensor &kp, const Tensor &vp, const Tensor &ks,
+                                      const Tensor &vs, const Tensor &table, const Tensor &cu, const Tensor &lengths,
+                                      double scaling, const std::optional<Tensor> &given) {
+  const auto p = paged_operands(kp, vp, ks, vs, table, cu, lengths);
+  if (!p || given || !rows3(q, p->D, kp) || dtype_code(q.scalar_type()) < 0 || q.numel() == 0 || !aligned_rows3(q) ||
+      q.size(1) > INT32_MAX || q.size(1) % p->Hkv)
+    return std::nullopt;
+  const at::DeviceGuard guard(kp.device());
+  const int32_t T = (int32_t)q.size(0), Hq = (int32_t)q.size(1), code = dtype_code(q.scalar_type());
+  Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
+  const int64_t wn = g.mga_paged_attn_workspace_bytes(T, p->B, Hq, p->Hkv, p->D, code);
+  Tensor ws = bytes(wn, q);
+  check_rc("mga_paged_attn",
+           g.mga_paged_attn(q.data_ptr(), q.stride(0), q.stride(1), kp.data_ptr(), vp.data_ptr(), ks.data_ptr<float>(),
+                            vs.data_ptr<float>(), p->n, p->ps, table.data_ptr<int32_t>(), p->width, p->width,
+                            cu.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), T, p->B, Hq, p->Hkv, p->D, code,
+                            (float)scaling, out.data_ptr(), out.stride(0), out.stride(1), 1, ws.data_ptr(), wn, stream(q)));
+  return out;
+}
+
 }  // namespace
 
 #define MGA_DEF(f) m.def(#f, torch::wrap_pybind_function_no_gil(f))
@@ -764,6 +867,8 @@ PYBIND11_MODULE(_mga_torch, m) {
   MGA_DEF(top_logits_step);
   MGA_DEF(sample);
   MGA_DEF(embedding);
+  MGA_DEF(paged_append);
+  MGA_DEF(paged_attention);
   MGA_DEF(check_capture);
   MGA_DEF(once);
 }

@@ -37,6 +37,7 @@ import torch
 from . import _lib
 from .cache import StreamingKVCache
 from .ops import _dev, _stream, dtype_code
+from .paged import PagedKVCache
 
 
 def _heads(name: str, t: torch.Tensor):
@@ -291,7 +292,9 @@ def qwen3_attention_forward(self, hidden_states: torch.Tensor, position_embeddin
     ``Qwen3Attention.forward = qwen3_attention_forward``. Takes the reference's
     arguments (gate_mask, past_key_value, cache_position) and transformers'
     ``past_key_values`` keyword; modules without the reference's fused
-    ``forward_qkv_proj`` use q_proj / k_proj / v_proj."""
+    ``forward_qkv_proj`` use q_proj / k_proj / v_proj. With a ``PagedKVCache`` the
+    packed tokens [1, T] of its batch are appended and attend over their own
+    sequences, without a mask, under torch.no_grad()."""
     if past_key_value is None:
         past_key_value = kwargs.pop("past_key_values", None)
     else:
@@ -306,6 +309,19 @@ def qwen3_attention_forward(self, hidden_states: torch.Tensor, position_embeddin
     if self.q_norm.variance_epsilon != self.k_norm.variance_epsilon:
         raise ValueError("q_norm and k_norm epsilons differ")
     cos, sin = position_embeddings
+    if isinstance(past_key_value, PagedKVCache):
+        # the packed tokens of the batch that the cache was given: one launch
+        # stores them, the attention needs no mask
+        if hidden_states.shape[0] != 1:
+            raise ValueError("a paged cache takes one packed row of tokens")
+        if self.sliding_window is not None:
+            raise NotImplementedError("paged_attention has no sliding window")
+        query = past_key_value.append(self.layer_idx, k.view(hidden_shape)[0], v.view(hidden_shape)[0],
+                                      query=q.view(hidden_shape)[0], cos=cos[0], sin=sin[0],
+                                      q_weight=self.q_norm.weight, k_weight=self.k_norm.weight,
+                                      eps=self.q_norm.variance_epsilon)
+        attn_output = past_key_value.attend(self.layer_idx, query, self.scaling).reshape(*input_shape, -1)
+        return (self.o_proj(attn_output, gate_mask) if gate_mask is not None else self.o_proj(attn_output)), None
     if isinstance(past_key_value, StreamingKVCache):
         # keys and values go straight into the cache rows [P, P + S): the
         # update below finds them in place and copies nothing
