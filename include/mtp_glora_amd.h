@@ -559,13 +559,13 @@ int mga_embedding_bwd(const void *grad_out, int64_t grad_out_row_stride, const v
  * to position lengths[b] + i; positions without a page (past the table, an id
  * outside [0, num_pages)) are not stored. No two sequences may write to one page.
  *   k: y = x rsqrt(mean x^2 + eps) k_weight (k_weight null: y = x), then
- *      r = y cos + rotate_half(y) sin (cos null: r = y), in fp32; v: r = x.
+ *      r = y cos + rotate_half(y) sin (cos null: r = y), in fp64; v: r = x.
  *   scale of a (page, head): the least power of two (2^-100 .. 2^119) of which 448 hold
  *      |r| of its rows; where the first row written is not the page's row 0, at least the
  *      old scale, and if it grows the rows before are rounded again.
  *   code = e4m3(r / scale), to nearest even; NaN and infinities become NaN codes and
  *      count in no scale.
- * query (null: none) likewise with q_weight into query_out, rounded once to the dtype;
+ * query (null: none) likewise in fp32 with q_weight into query_out, rounded once to the dtype;
  * its rows behind cu_tokens[n_seqs] are zeros. cos, sin [n_tokens, head_dim] in the dtype, or fp32
  * with cos_sin_f32. Rows behind a sequence's end in its last page, and all other pages,
  * stay as they are. n_seqs <= 4096; head_dim 64 or 128. Beside mga_kv_append and
@@ -598,6 +598,30 @@ int mga_paged_attn(const void *q, int64_t q_stride_s, int64_t q_stride_h, const 
                    const int32_t *lengths, int32_t n_tokens, int32_t n_seqs, int32_t Hq, int32_t Hkv, int32_t head_dim,
                    int32_t dtype, float scale, void *out, int64_t o_stride_s, int64_t o_stride_h, int32_t zero_rest,
                    void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Logits shaped before a token is drawn (mga_sample): for row r and column v
+ *   y = x; if v is among the first lengths[r] of the row's tokens (prompt and output):
+ *     y = x > 0 ? x / repetition : x * repetition;
+ *   with c = how often v is among tokens prompt_lengths[r] .. lengths[r] - 1 (output):
+ *     y -= frequency * c + (c > 0 ? presence : 0);
+ *   y += the sum of bias[r, i] over bias_ids[r, i] = v, added in the order of i;
+ *   y = -inf where bit v % 32 of allowed[r, v / 32] is 0, whatever x is;
+ * in fp32, rounded once to the dtype. tokens [n_rows, n_tokens] int64 if tokens_are_int64
+ * else int32 (n_tokens 0: none), bias_ids and bias [n_rows, n_bias] (n_bias 0: none),
+ * allowed [n_rows, ceil(n_cols / 32)] (null: all): a row stride of 0 shares a row. Ids outside
+ * [0, n_cols) do not count. lengths null: n_tokens; prompt_lengths null: 0.
+ * repetition, frequency, presence: one value a row in device memory, or null for the
+ * *_all value; a repetition that is not positive counts as 1. out may be logits itself (the same
+ * rows), else may not overlap it. n_cols <= 2^30, n_rows < 2^22. No counterpart in the reference.
+ */
+int mga_adjust_logits(const void *logits, int64_t row_stride, int32_t n_rows, int32_t n_cols, int32_t dtype,
+                      const void *tokens, int32_t tokens_are_int64, int64_t tokens_row_stride, int32_t n_tokens,
+                      const int32_t *lengths, const int32_t *prompt_lengths, const float *repetition, float repetition_all,
+                      const float *frequency, float frequency_all, const float *presence, float presence_all,
+                      const void *bias_ids, int32_t bias_ids_are_int64, int64_t bias_ids_row_stride, const float *bias,
+                      int64_t bias_row_stride, int32_t n_bias, const int32_t *allowed, int64_t allowed_row_stride,
+                      void *out, int64_t out_row_stride, void *stream);
 
 #ifdef __cplusplus
 }

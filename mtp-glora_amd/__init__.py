@@ -21,6 +21,8 @@ The package mirrors the reference's operator boundaries for this path:
   cross-entropy against whole rows
 * ``sample_tokens``             - tokens from logits with temperature, top-k,
   top-p and min-p, from given random numbers
+* ``adjust_logits``             - penalties for repeated tokens, biases and masks of
+  allowed tokens, before sample_tokens
 * ``PagedKVCache`` / ``paged_append`` / ``paged_attention`` - decoding: a paged 8-bit
   cache of several sequences, filled with the rotation on the way, and the attention
   of new tokens over it
@@ -43,7 +45,7 @@ from .loss import StableSoftCrossEntropy
 from .manager import StreamingKVCacheManager
 from .paged import KVPages, PagedKVCache, paged_append, paged_attention
 from .rope import qk_norm_rope, qwen3_attention_forward
-from .sampling import sample_tokens
+from .sampling import adjust_logits, sample_tokens
 
 __all__ = [
     "StreamingKVCache", "StreamingKVCacheManager", "MTPBlockMask", "build_mtp_block_mask",
@@ -51,7 +53,7 @@ __all__ = [
     "qk_norm_rope", "qwen3_attention_forward", "GatedLoRALinear", "apply_lora_to_model", "gated_lora_linear",
     "TopLogits", "TopLogitsCrossEntropy", "top_logits", "top_logits_cross_entropy", "top_logits_loss_and_grad",
     "sample_tokens", "ScaledEmbedding", "scaled_embedding", "embedding_grad", "PagedKVCache", "KVPages",
-    "paged_append", "paged_attention",
+    "paged_append", "paged_attention", "adjust_logits",
 ]
 
 

@@ -93,6 +93,8 @@ SIGNATURES = {
     "mga_embedding_fwd": [_P, _I32, _I32, _P, _I64, _I32, _I32, _F32, _I32, _P, _I64, _P],
     "mga_embedding_workspace_bytes": [_I32, _I32],
     "mga_embedding_bwd": [_P, _I64, _P, _I32, _I32, _F32, _I64, _I32, _I32, _I32, _P, _I64, _I32, _I32, _P, _I64, _P],
+    "mga_adjust_logits": [_P, _I64, _I32, _I32, _I32, _P, _I32, _I64, _I32, _P, _P, _P, _F32, _P, _F32, _P, _F32,
+                          _P, _I32, _I64, _P, _I64, _I32, _P, _I64, _P, _I64, _P],
     "mga_paged_append": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I32, _F32,
                          _I32, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _I32, _I32, _P, _I64, _I32, _P, _P,
                          _P, _I64, _I64, _P],

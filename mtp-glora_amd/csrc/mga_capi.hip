@@ -1216,4 +1216,49 @@ int mga_paged_attn(const void *q, int64_t q_stride_s, int64_t q_stride_h, const 
   return check_launch(fn);
 }
 
+int mga_adjust_logits(const void *logits, int64_t row_stride, int32_t n_rows, int32_t n_cols, int32_t dtype,
+                      const void *tokens, int32_t tokens_are_int64, int64_t tokens_row_stride, int32_t n_tokens,
+                      const int32_t *lengths, const int32_t *prompt_lengths, const float *repetition, float repetition_all,
+                      const float *frequency, float frequency_all, const float *presence, float presence_all,
+                      const void *bias_ids, int32_t bias_ids_are_int64, int64_t bias_ids_row_stride, const float *bias,
+                      int64_t bias_row_stride, int32_t n_bias, const int32_t *allowed, int64_t allowed_row_stride,
+                      void *out, int64_t out_row_stride, void *stream) {
+  const char *fn = "mga_adjust_logits";
+  int rc = check_matrix(fn, "logits", logits, row_stride, n_rows, n_cols, dtype);
+  if (rc == MGA_OK) rc = check_row_count(fn, n_rows);
+  if (rc == MGA_OK) rc = check_matrix(fn, "out", out, out_row_stride, n_rows, n_cols, dtype);
+  if (rc != MGA_OK) return rc;
+  if (n_cols > (1 << 30)) return fail(MGA_ERR_INVALID, "%s: %d columns (at most 2^30)", fn, n_cols);
+  if (n_tokens < 0 || n_bias < 0)
+    return fail(MGA_ERR_INVALID, "%s: bad sizes (tokens=%d biases=%d)", fn, n_tokens, n_bias);
+  // rows of a list, one for all rows with a stride of 0
+  const auto list = [&](const char *name, const void *p, int64_t rs, int32_t n, int eb) {
+    if (n == 0) return (int)MGA_OK;
+    if (!p || reinterpret_cast<uintptr_t>(p) % eb)
+      return fail(MGA_ERR_INVALID, "%s: %s null or not aligned to its elements", fn, name);
+    if (rs != 0 && rs < n) return fail(MGA_ERR_INVALID, "%s: %s row stride %lld < %d", fn, name, (long long)rs, n);
+    return (int)MGA_OK;
+  };
+  if ((rc = list("tokens", tokens, tokens_row_stride, n_tokens, tokens_are_int64 ? 8 : 4)) != MGA_OK ||
+      (rc = list("bias_ids", bias_ids, bias_ids_row_stride, n_bias, bias_ids_are_int64 ? 8 : 4)) != MGA_OK ||
+      (rc = list("bias", bias, bias_row_stride, n_bias, 4)) != MGA_OK ||
+      (rc = list("allowed", allowed, allowed_row_stride, allowed ? (n_cols + 31) / 32 : 0, 4)) != MGA_OK)
+    return rc;
+  if (!repetition && !(repetition_all > 0.f && repetition_all < __builtin_huge_valf()))
+    return fail(MGA_ERR_INVALID, "%s: repetition must be positive and finite (got %g)", fn, (double)repetition_all);
+  const int eb = elem_bytes(dtype);
+  const bool same = logits == out && (row_stride == out_row_stride || n_rows == 1);
+  if (!same && overlap(logits, row_stride, out, out_row_stride, n_rows, n_rows, n_cols, eb, eb))
+    return fail(MGA_ERR_INVALID, "%s: out overlaps logits", fn);
+  // a launch of fewer than 2^32 threads
+  if (mga::adjust_blocks(n_rows, n_cols) >= (int64_t(1) << 24))
+    return fail(MGA_ERR_INVALID, "%s: %d rows of %d columns are too many", fn, n_rows, n_cols);
+  const mga::AdjustArgs a{logits, row_stride, out, out_row_stride, tokens, tokens_row_stride, lengths, prompt_lengths,
+                          repetition, frequency, presence, bias_ids, bias_ids_row_stride, bias, bias_row_stride, allowed,
+                          allowed_row_stride, repetition_all, frequency_all, presence_all, n_rows, n_cols, n_tokens, n_bias,
+                          tokens_are_int64 != 0, bias_ids_are_int64 != 0};
+  mga::launch_adjust_logits(a, dtype, (hipStream_t)stream);
+  return check_launch(fn);
+}
+
 }  // extern "C"

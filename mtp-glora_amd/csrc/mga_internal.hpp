@@ -258,6 +258,23 @@ struct SampleParams {
 void launch_sample(const void *x, int64_t xs, int32_t N, int32_t V, int dtype, const float *uniform,
                    const SampleParams &prm, int64_t *token, hipStream_t stream);
 
+// Penalties, biases and masks of logits (mga_adjust_logits.hip).
+struct AdjustArgs {
+  const void *x; int64_t xs;           // [N, V]
+  void *out; int64_t os;
+  const void *tokens; int64_t tokens_rs;   // [N, L], int64 (tokens64) or int32
+  const int32_t *lengths, *prompts;    // [N], or null (L, 0)
+  const float *repetition, *frequency, *presence;   // [N], or null (the *_all values)
+  const void *bias_ids; int64_t bias_ids_rs;   // [N, K], int64 (bias64) or int32
+  const float *bias; int64_t bias_rs;
+  const int32_t *allowed; int64_t allowed_rs;   // [N, ceil(V / 32)], or null
+  float repetition_all, frequency_all, presence_all;
+  int32_t N, V, L, K;
+  bool tokens64, bias64;
+};
+int64_t adjust_blocks(int32_t N, int32_t V);   // at most
+void launch_adjust_logits(const AdjustArgs &a, int dtype, hipStream_t stream);
+
 // Paged 8-bit cache (mga_paged.hpp): appending with norm and rotation
 // (mga_paged_append.hip), attention over it (mga_paged_attn.hip).
 struct PagedAppendArgs {

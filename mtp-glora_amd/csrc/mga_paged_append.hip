@@ -3,9 +3,10 @@
 //
 //   y = x * rsqrt(mean(x^2) + eps) * w            (where norm weights are given)
 //   r = y * cos + rotate_half(y) * sin            (where cos / sin are given)
-// in fp32 from the projections' values; the query rows are rounded once to their
-// type. Keys and values are rounded once to e4m3 under the scale of their (page,
-// head): the least power of two of which 448 hold every value the page has taken
+// from the projections' values; the query rows in fp32, rounded once to their type.
+// Keys are prepared in fp64 (half the rate of fp32, in a kernel that memory bounds): an
+// fp32 value next to the middle between two codes takes the wrong one about once in 2^20
+// values. Keys and values are rounded once to e4m3 under the scale of their (page, head): the least power of two of which 448 hold every value the page has taken
 // since a row 0 was written. Where new rows make it grow, the rows kept from before
 // are rounded again under the new scale (a shift of their exponents: exact unless a
 // code falls below e4m3's normal range).
@@ -63,37 +64,49 @@ __device__ __forceinline__ void load_row(const T *row, int j, bool vec, float *x
   load8f(row + D / 2 + 8 * j, vec, x + 8);
 }
 
-template <typename T, int D>
-__device__ __forceinline__ void norm_rotate(const PagedAppendArgs &a, const void *weight, const void *cos, const void *sin,
-                                            bool cs32, int64_t tok, int j, float *x) {
+__device__ __forceinline__ float inv_root(float x) { return rsqrtf(x); }
+__device__ __forceinline__ double inv_root(double x) { return 1.0 / sqrt(x); }
+
+// y = x * rsqrt(mean(x^2) + eps) * w, then y * cos + rotate_half(y) * sin, in F.
+template <typename T, int D, typename F>
+__device__ __forceinline__ void norm_rotate(const PagedAppendArgs &a, const void *weight, int64_t tok, int j, F *x) {
   constexpr int LR = D / 16;
   if (weight) {
-    float w[16], s = 0.f;
+    float w[16];
+    F s = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s += x[i] * x[i];
     for (int m = 1; m < LR; m <<= 1) s += __shfl_xor(s, m, 64);
     load_row<T, D>((const T *)weight, j, a.vec, w);
-    // the sum of finite values may be infinite in fp32: such a row is all zeros, as by the formula in fp32
-    const float rs = rsqrtf(s * (1.f / D) + a.eps);
+    const F rs = inv_root(s * (F)(1.f / D) + (F)a.eps);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = x[i] * rs * w[i];
+    for (int i = 0; i < 16; ++i) x[i] = x[i] * rs * (F)w[i];
   }
-  if (cos) {
+  if (a.cos) {
     float c[16], s[16];
-    if (cs32) {
-      load_row<float, D>((const float *)cos + tok * a.cs_ss, j, a.vec, c);
-      load_row<float, D>((const float *)sin + tok * a.cs_ss, j, a.vec, s);
+    if (a.cs32) {
+      load_row<float, D>((const float *)a.cos + tok * a.cs_ss, j, a.vec, c);
+      load_row<float, D>((const float *)a.sin + tok * a.cs_ss, j, a.vec, s);
     } else {
-      load_row<T, D>((const T *)cos + tok * a.cs_ss, j, a.vec, c);
-      load_row<T, D>((const T *)sin + tok * a.cs_ss, j, a.vec, s);
+      load_row<T, D>((const T *)a.cos + tok * a.cs_ss, j, a.vec, c);
+      load_row<T, D>((const T *)a.sin + tok * a.cs_ss, j, a.vec, s);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float lo = x[i], hi = x[i + 8];
-      x[i] = lo * c[i] - hi * s[i];
-      x[i + 8] = hi * c[i + 8] + lo * s[i + 8];
+      const F lo = x[i], hi = x[i + 8];
+      x[i] = lo * (F)c[i] - hi * (F)s[i];
+      x[i + 8] = hi * (F)c[i + 8] + lo * (F)s[i + 8];
     }
   }
+}
+
+// fp32 next to d on the side of d: what is rounded to e4m3 from it is what d would be.
+__device__ __forceinline__ float beside(double d) {
+  const float f = (float)d;
+  const double r = (double)f;
+  const int bits = __builtin_bit_cast(int, f);
+  const bool more = fabs(d) > fabs(r), less = fabs(d) < fabs(r);
+  return fabsf(f) < __builtin_huge_valf() ? __builtin_bit_cast(float, bits + (more ? 1 : less ? -1 : 0)) : f;
 }
 
 __device__ __forceinline__ void store8f(bf16_t *p, bool vec, const float *x) {
@@ -167,7 +180,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, in
       for (int i = 0; i < 16; ++i) x[i] = 0.f;
       if (live) {
         load_row<T, D>((const T *)a.q + tok * a.q_ss + h * a.q_hs, j, a.vec, x);
-        norm_rotate<T, D>(a, a.qw, a.cos, a.sin, a.cs32, tok, j, x);
+        norm_rotate<T, D>(a, a.qw, tok, j, x);
       }
       T *o = (T *)a.qo + tok * a.qo_ss + h * a.qo_hs;
       store8f(o + 8 * j, a.vec, x);
@@ -212,7 +225,14 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, in
     if (r < r1) {
       const int64_t tok = tok0 + (r - r0);
       load_row<T, D>(src + tok * ss + head * hs, j, a.vec, x[p]);
-      if (!is_v) norm_rotate<T, D>(a, a.kw, a.cos, a.sin, a.cs32, tok, j, x[p]);
+      if (!is_v && (a.kw || a.cos)) {
+        double y[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] = x[p][i];
+        norm_rotate<T, D>(a, a.kw, tok, j, y);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[p][i] = beside(y[i]);
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float v = fabsf(x[p][i]);

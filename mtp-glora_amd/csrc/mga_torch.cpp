@@ -42,7 +42,8 @@ using torch::autograd::variable_list;
   X(mga_soft_ce_bwd) X(mga_top_logits) X(mga_top_logits_ce_workspace_floats) X(mga_top_logits_ce_fwd)  \
   X(mga_top_logits_ce_bwd) X(mga_top_logits_ce_step_workspace_floats) X(mga_top_logits_ce_step)          \
   X(mga_sample) X(mga_embedding_fwd) X(mga_embedding_workspace_bytes) X(mga_embedding_bwd) \
-  X(mga_paged_append) X(mga_paged_attn_workspace_bytes) X(mga_paged_attn)
+  X(mga_paged_append) X(mga_paged_attn_workspace_bytes) X(mga_paged_attn) \
+  X(mga_adjust_logits)
 struct Api {
 #define X(f) decltype(&::f) f = nullptr;
   MGA_API(X)
@@ -694,6 +695,64 @@ std::optional<Tensor> sample(const Tensor &x, const Tensor &u, const std::option
   return token;
 }
 
+// A list with the rows of x, or (shared) one for all of them.
+struct RowList {
+  const void *data = nullptr;
+  int64_t stride = 0;
+  int32_t n = 0;
+  bool wide = false;
+};
+std::optional<RowList> row_list(const std::optional<Tensor> &t, const Tensor &x, bool shared) {
+  RowList r;
+  if (!t) return r;
+  if (!plain(*t) || t->device() != x.device() || t->dim() < 1 || !t->is_contiguous() || t->numel() == 0 ||
+      t->size(-1) > INT32_MAX)
+    return std::nullopt;
+  const bool one = t->dim() == 1 && x.dim() > 1;
+  if (!(one && shared) && t->sizes().slice(0, t->dim() - 1) != x.sizes().slice(0, x.dim() - 1)) return std::nullopt;
+  r.data = t->data_ptr();
+  r.n = (int32_t)t->size(-1);
+  r.stride = one ? 0 : r.n;
+  r.wide = t->scalar_type() == at::kLong;
+  return r;
+}
+
+std::optional<Tensor> adjust_logits(const Tensor &x, const std::optional<Tensor> &tokens, const std::optional<Tensor> &lengths,
+                                    const std::optional<Tensor> &prompts, const std::optional<Tensor> &repetition,
+                                    const std::optional<Tensor> &frequency, const std::optional<Tensor> &presence,
+                                    double repetition_all, double frequency_all, double presence_all,
+                                    const std::optional<Tensor> &bias_ids, const std::optional<Tensor> &bias,
+                                    const std::optional<Tensor> &allowed, const std::optional<Tensor> &given) {
+  if (!eager() || !plain(x) || dtype_code(x.scalar_type()) < 0 || given) return std::nullopt;
+  const auto r = rows_of(x);
+  if (!r) return std::nullopt;
+  const auto tok = row_list(tokens, x, false), bid = row_list(bias_ids, x, true), val = row_list(bias, x, true),
+             ok = row_list(allowed, x, true);
+  if (!tok || !bid || !val || !ok || bid->n != val->n || (!tokens && (lengths || prompts))) return std::nullopt;
+  for (const auto *t : {&tokens, &bias_ids})
+    if (*t && (*t)->scalar_type() != at::kInt && (*t)->scalar_type() != at::kLong) return std::nullopt;
+  if ((bias && bias->scalar_type() != at::kFloat) ||
+      (allowed && (allowed->scalar_type() != at::kInt || ok->n != (r->cols + 31) / 32)))
+    return std::nullopt;
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  for (const auto *t : {&lengths, &prompts})
+    if (*t && (!int32_on(**t, x) || (*t)->sizes() != lead)) return std::nullopt;
+  if (!setting(repetition, x, r->n, at::kFloat) || !setting(frequency, x, r->n, at::kFloat) ||
+      !setting(presence, x, r->n, at::kFloat))
+    return std::nullopt;
+  const at::DeviceGuard guard(x.device());
+  Tensor out = at::empty(x.sizes(), x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+  auto f32 = [](const std::optional<Tensor> &t) { return t ? t->data_ptr<float>() : nullptr; };
+  auto i32 = [](const std::optional<Tensor> &t) { return t ? t->data_ptr<int32_t>() : nullptr; };
+  check_rc("mga_adjust_logits",
+           g.mga_adjust_logits(r->data, r->stride, (int32_t)r->n, r->cols, dtype_code(x.scalar_type()), tok->data, tok->wide,
+                               tok->stride, tok->n, i32(lengths), i32(prompts), f32(repetition), (float)repetition_all,
+                               f32(frequency), (float)frequency_all, f32(presence), (float)presence_all, bid->data,
+                               bid->wide, bid->stride, (const float *)val->data, val->stride, bid->n,
+                               (const int32_t *)ok->data, ok->stride, out.data_ptr(), r->cols, stream(x)));
+  return out;
+}
+
 // ---- embedding -----------------------------------------------------------------------
 
 struct Embedding : public Function<Embedding> {
@@ -866,6 +925,7 @@ PYBIND11_MODULE(_mga_torch, m) {
   MGA_DEF(top_logits_ce);
   MGA_DEF(top_logits_step);
   MGA_DEF(sample);
+  MGA_DEF(adjust_logits);
   MGA_DEF(embedding);
   MGA_DEF(paged_append);
   MGA_DEF(paged_attention);

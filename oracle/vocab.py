@@ -116,3 +116,41 @@ def embedding_grad(dy, ids, V, scale, padding_idx=None):
     ok = (ids >= 0) & (ids < V) & (ids != (-1 if padding_idx is None else padding_idx))
     np.add.at(out, ids[ok], dy.reshape(len(ids), -1)[ok])
     return scale * out
+
+
+def adjust(x, tokens=None, lengths=None, prompts=None, repetition=1.0, frequency=0.0, presence=0.0, bias_ids=None, bias=None,
+           allowed=None):
+    """Rows x [N, V] with penalties, biases and mask (mga_adjust_logits), and the sum of the
+    magnitudes that went into each value."""
+    x = np.asarray(x, np.float64)
+    N, V = x.shape
+    each = lambda v: np.broadcast_to(np.asarray(v, np.float64), (N,))   # noqa: E731
+    rep, freq, pres = each(repetition), each(frequency), each(presence)
+    y, mag = x.copy(), np.abs(x)
+    for r in range(N):
+        if tokens is not None:
+            n = len(tokens[r]) if lengths is None else min(max(int(lengths[r]), 0), len(tokens[r]))
+            m = 0 if prompts is None else min(max(int(prompts[r]), 0), n)
+            seen = {int(t) for t in tokens[r][:n] if 0 <= t < V}
+            count = {}
+            for t in tokens[r][m:n]:
+                if 0 <= t < V:
+                    count[int(t)] = count.get(int(t), 0) + 1
+            f = rep[r] if rep[r] > 0 else 1.0
+            for t in seen:
+                y[r, t] = y[r, t] / f if y[r, t] > 0 else y[r, t] * f
+                mag[r, t] = abs(y[r, t])
+                if t in count:
+                    y[r, t] -= freq[r] * count[t] + pres[r]
+                    mag[r, t] += abs(freq[r]) * count[t] + abs(pres[r])
+        if bias_ids is not None:
+            for t, b in zip(np.broadcast_to(bias_ids, (N, np.shape(bias_ids)[-1]))[r],
+                            np.broadcast_to(bias, (N, np.shape(bias)[-1]))[r]):
+                if 0 <= t < V:
+                    y[r, int(t)] += float(b)
+                    mag[r, int(t)] += abs(float(b))
+        if allowed is not None:
+            words = np.broadcast_to(allowed, (N, np.shape(allowed)[-1]))[r].astype(np.int64)
+            v = np.arange(V)
+            y[r][(words[v // 32] >> (v % 32)) & 1 == 0] = -np.inf
+    return y, mag
