@@ -587,11 +587,11 @@ int mga_paged_append(const void *key, int64_t k_stride_s, int64_t k_stride_h, co
  * is rounded to bf16 (bf16 queries), or kept to 16 (fp16) or 24 bits (fp32).
  * q, out: [n_tokens, Hq, head_dim], rows 16-byte aligned; Hq / Hkv <= 32. Rows of
  * out behind cu_tokens[n_seqs]: zeros with zero_rest, else left as they are. workspace:
- * mga_paged_attn_workspace_bytes bytes, 16-byte aligned, one for each call in flight. Sums run in a fixed
- * order. Beside mga_attn_fwd ([tf]integrations/flex_attention.py:262-368).
+ * mga_paged_attn_workspace_bytes bytes (0: may be null), 16-byte aligned, one for each call in flight. Sums
+ * run in a fixed order. Beside mga_attn_fwd ([tf]integrations/flex_attention.py:262-368).
  */
 int64_t mga_paged_attn_workspace_bytes(int32_t n_tokens, int32_t n_seqs, int32_t Hq, int32_t Hkv, int32_t head_dim,
-                                       int32_t dtype);
+                                       int32_t page_size, int32_t table_width, int32_t dtype);
 int mga_paged_attn(const void *q, int64_t q_stride_s, int64_t q_stride_h, const void *k_pages, const void *v_pages,
                    const float *k_scale, const float *v_scale, int32_t num_pages, int32_t page_size,
                    const int32_t *block_table, int64_t table_row_stride, int32_t table_width, const int32_t *cu_tokens,

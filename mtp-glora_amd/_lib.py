@@ -98,7 +98,7 @@ SIGNATURES = {
     "mga_paged_append": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I32, _F32,
                          _I32, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _I32, _I32, _P, _I64, _I32, _P, _P,
                          _P, _I64, _I64, _P],
-    "mga_paged_attn_workspace_bytes": [_I32, _I32, _I32, _I32, _I32, _I32],
+    "mga_paged_attn_workspace_bytes": [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32],
     "mga_paged_attn": [_P, _I64, _I64, _P, _P, _P, _P, _I32, _I32, _P, _I64, _I32, _P, _P,
                        _I32, _I32, _I32, _I32, _I32, _I32, _F32, _P, _I64, _I64, _I32, _P, _I64, _P],
 }

@@ -1176,9 +1176,10 @@ int mga_paged_append(const void *key, int64_t k_stride_s, int64_t k_stride_h, co
 }
 
 int64_t mga_paged_attn_workspace_bytes(int32_t n_tokens, int32_t n_seqs, int32_t Hq, int32_t Hkv, int32_t head_dim,
-                                       int32_t dtype) {
-  if (n_tokens <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0) return 0;
-  return mga::paged_attn_ws_bytes(n_tokens, n_seqs, Hq, Hkv, head_dim, dtype);
+                                       int32_t page_size, int32_t table_width, int32_t dtype) {
+  if (n_tokens <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0 || page_size <= 0 || table_width <= 0)
+    return 0;
+  return mga::paged_attn_ws_bytes(n_tokens, n_seqs, Hq, Hkv, head_dim, (int64_t)page_size * table_width, dtype);
 }
 
 int mga_paged_attn(const void *q, int64_t q_stride_s, int64_t q_stride_h, const void *k_pages, const void *v_pages,
@@ -1201,8 +1202,8 @@ int mga_paged_attn(const void *q, int64_t q_stride_s, int64_t q_stride_h, const 
     return rc;
   if (!vec) return fail(MGA_ERR_INVALID, "%s: rows of q and out must be 16-byte aligned", fn);
   float *ws = nullptr;
-  const int64_t need = mga::paged_attn_ws_bytes(n_tokens, n_seqs, Hq, Hkv, head_dim, dtype);
-  if (!workspace) return fail(MGA_ERR_INVALID, "%s: null workspace", fn);
+  const int64_t need = mga::paged_attn_ws_bytes(n_tokens, n_seqs, Hq, Hkv, head_dim, (int64_t)page_size * table_width, dtype);
+  if (need && !workspace) return fail(MGA_ERR_INVALID, "%s: null workspace", fn);
   if ((rc = check_attn_ws(fn, workspace, workspace_bytes, need, &ws)) != MGA_OK) return rc;
   const mga::PagedAttnArgs a{q, q_stride_s, q_stride_h, (const uint8_t *)k_pages, (const uint8_t *)v_pages, k_scale,
                              v_scale, block_table, table_row_stride, cu_tokens, lengths, out, o_stride_s, o_stride_h, ws,

@@ -306,7 +306,8 @@ struct PagedAttnArgs {
   int32_t T, B, Hq, Hkv, num_pages, pshift, width;
   bool zero_rest;                      // rows behind the last sequence: zeros, else left as they are
 };
-int64_t paged_attn_ws_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int head_dim, int dtype);
+// keys: the most that a sequence's row of the table holds
+int64_t paged_attn_ws_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int head_dim, int64_t keys, int dtype);
 // an upper bound of the 64-key steps of a call
 int64_t paged_attn_steps(const PagedAttnArgs &a, int dtype);
 void launch_paged_attn(const PagedAttnArgs &a, int head_dim, int dtype, hipStream_t stream);

@@ -900,13 +900,14 @@ std::optional<Tensor> paged_attention(const Tensor &q, const Tensor &kp, const T
   const at::DeviceGuard guard(kp.device());
   const int32_t T = (int32_t)q.size(0), Hq = (int32_t)q.size(1), code = dtype_code(q.scalar_type());
   Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
-  const int64_t wn = g.mga_paged_attn_workspace_bytes(T, p->B, Hq, p->Hkv, p->D, code);
-  Tensor ws = bytes(wn, q);
+  const int64_t wn = g.mga_paged_attn_workspace_bytes(T, p->B, Hq, p->Hkv, p->D, p->ps, p->width, code);
+  Tensor ws;
+  if (wn) ws = bytes(wn, q);
   check_rc("mga_paged_attn",
            g.mga_paged_attn(q.data_ptr(), q.stride(0), q.stride(1), kp.data_ptr(), vp.data_ptr(), ks.data_ptr<float>(),
                             vs.data_ptr<float>(), p->n, p->ps, table.data_ptr<int32_t>(), p->width, p->width,
                             cu.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), T, p->B, Hq, p->Hkv, p->D, code,
-                            (float)scaling, out.data_ptr(), out.stride(0), out.stride(1), 1, ws.data_ptr(), wn, stream(q)));
+                            (float)scaling, out.data_ptr(), out.stride(0), out.stride(1), 1, wn ? ws.data_ptr() : nullptr, wn, stream(q)));
   return out;
 }
 

@@ -210,12 +210,12 @@ def paged_attention(query: torch.Tensor, pages, block_table: torch.Tensor, cu_to
     if T == 0:
         return out
     with torch.cuda.device(p.k.device):
-        nb = int(_lib.load().mga_paged_attn_workspace_bytes(T, table.shape[0], Hq, Hkv, D, code))
+        nb = int(_lib.load().mga_paged_attn_workspace_bytes(T, table.shape[0], Hq, Hkv, D, ps, table.shape[1], code))
         ws = torch.empty(nb, device=q.device, dtype=torch.uint8)
         _lib.call("mga_paged_attn", q.data_ptr(), q.stride(0), q.stride(1), p.k.data_ptr(), p.v.data_ptr(),
                   p.k_scale.data_ptr(), p.v_scale.data_ptr(), n, ps, table.data_ptr(), table.stride(0), table.shape[1],
                   cu.data_ptr(), lens.data_ptr(), T, table.shape[0], Hq, Hkv, D, code, float(scaling), out.data_ptr(),
-                  out.stride(0), out.stride(1), int(fresh), ws.data_ptr(), nb, _stream(q))
+                  out.stride(0), out.stride(1), int(fresh), ws.data_ptr() if nb else None, nb, _stream(q))
     return out
 
 

@@ -19,6 +19,9 @@ PAGED = [dict(T=-1), dict(B=0), dict(B=4097), dict(D=96), dict(Hq=3), dict(Hkv=0
          dict(kp=ctypes.c_void_p(72)), dict(ks=None), dict(vs=None), dict(table=None), dict(cu=None), dict(lens=None)]
 
 
+LONG = dict(width=1000, trs=1000)   # sequences that need a workspace
+
+
 def _args(**kw):
     a = dict(k=P, ss=256, hs=128, v=P, q=P, qw=None, kw=None, cos=None, sin=None, cs=128, c32=0, eps=1e-6, T=2, B=1, Hq=4,
              Hkv=2, D=128, dtype=0, kp=P, vp=P, ks=P, vs=P, n=4, ps=64, table=P, trs=4, width=4, cu=P, lens=P, qo=P,
@@ -52,8 +55,8 @@ def test_append(mga, kw):
 
 @pytest.mark.parametrize("kw", PAGED + [dict(q=None), dict(out=None), dict(q=ctypes.c_void_p(72)), dict(ss=100),
                                         dict(hs=-128), dict(out=ctypes.c_void_p(66)), dict(Hq=66), dict(scale=0.0),
-                                        dict(scale=float("inf")), dict(scale=float("nan")), dict(ws=None), dict(nb=100),
-                                        dict(ws=ctypes.c_void_p(72)), dict(T=1 << 28, width=1 << 22, trs=1 << 22)])
+                                        dict(scale=float("inf")), dict(scale=float("nan")), LONG | dict(ws=None), LONG | dict(nb=100),
+                                        LONG | dict(ws=ctypes.c_void_p(72)), dict(T=1 << 28, width=1 << 22, trs=1 << 22)])
 def test_attend(mga, kw):
     refused(mga, _attend(mga.load_library(), **kw))
 
@@ -61,8 +64,8 @@ def test_attend(mga, kw):
 def test_no_tokens(mga):
     lib = mga.load_library()
     assert _append(lib, T=0) == 0 and _attend(lib, T=0) == 0
-    assert lib.mga_paged_attn_workspace_bytes(0, 1, 4, 2, 128, 0) == 0
-    assert lib.mga_paged_attn_workspace_bytes(1, 1, 4, 2, 128, 0) > 0
+    assert lib.mga_paged_attn_workspace_bytes(0, 1, 4, 2, 128, 64, 4, 0) == 0
+    assert lib.mga_paged_attn_workspace_bytes(1, 1, 4, 2, 128, 64, 1000, 0) > 0
 
 
 def test_cpu_tensors(mga):
