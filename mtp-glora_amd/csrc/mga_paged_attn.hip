@@ -134,21 +134,28 @@ __device__ __forceinline__ int tile_slot(const SeqSpan &q, int b, int t, int tms
 }
 __host__ __device__ __forceinline__ int tile_slots(int T, int B, int tmshift) { return (T >> tmshift) + B; }
 
-// The tile of a slot; false: none. All lanes of the wave take part.
+// The tile of a slot; false: none. All lanes of the wave take part. The lanes' loads find the
+// sequence and hold what is needed of it.
 __device__ __forceinline__ bool tile_of_slot(const PagedAttnArgs &a, int slot, int tmshift, int G, Tile &x) {
-  int b = 0;
   for (int i0 = 0; i0 < a.B; i0 += 64) {
-    const int i = i0 + (threadIdx.x & 63) + 1;
-    b += __popcll(__ballot(i <= a.B && (min(max(a.cu[min(i, a.B)], 0), a.T) >> tmshift) + i <= slot));
+    const int i = min(i0 + (int)(threadIdx.x & 63), a.B - 1);
+    const SeqSpan q = seq_span(a.cu, a.lengths, i, a.T, a.width << a.pshift);
+    // the sequences whose slots end at or before this one
+    const uint64_t done = __ballot((min(max(a.cu[i + 1], 0), a.T) >> tmshift) + i + 1 <= slot);
+    if (~done) {
+      const int at = __ffsll((unsigned long long)~done) - 1;
+      x.b = i0 + at;
+      x.q.first = __builtin_amdgcn_readlane(q.first, at);
+      x.q.n = __builtin_amdgcn_readlane(q.n, at);
+      x.q.len = __builtin_amdgcn_readlane(q.len, at);
+      const SeqTiles st{x.q.n, x.q.len, tmshift};
+      const int t = slot - tile_slot(x.q, x.b, 0, tmshift);
+      if (x.b >= a.B || t < 0 || t >= st.tiles()) return false;
+      x.set(st, t, G);
+      return true;
+    }
   }
-  x.b = __builtin_amdgcn_readfirstlane(b);
-  if (x.b >= a.B) return false;
-  x.q = seq_span(a.cu, a.lengths, x.b, a.T, a.width << a.pshift);
-  const SeqTiles st{x.q.n, x.q.len, tmshift};
-  const int t = slot - tile_slot(x.q, x.b, 0, tmshift);
-  if (t < 0 || t >= st.tiles()) return false;
-  x.set(st, t, G);
-  return true;
+  return false;
 }
 
 // A row of a tile in q and out.
@@ -157,6 +164,9 @@ __device__ __forceinline__ T *row_of(const Tile &x, int G, int r, const void *ba
   const int tk = r / G;
   return (T *)base + (int64_t)(x.q.first + x.tok0 + tk) * ss + (int64_t)(x.h * G + r - tk * G) * hs;
 }
+
+// s_waitcnt's operand: at most n vector memory operations in flight.
+constexpr int wait_vm(int n) { return (n & 15) | (n >> 4) << 14 | 7 << 4 | 15 << 8; }
 
 // 16 bytes at a wave-uniform address plus a lane offset; the address stays in scalar registers.
 __device__ __forceinline__ i32x4 load16(const uint8_t *base, uint32_t off) {
@@ -169,22 +179,136 @@ __device__ __forceinline__ i32x4 load16(const uint8_t *base, uint32_t off) {
 
 // ---- the steps of one wave ------------------------------------------------------
 
+// The K and V loads of a wave's steps, whatever tiles they belong to, one step ahead of their
+// use. The lanes hold the pages (page * Hkv + head, -1: none), places and scales of the next steps:
+// 64 steps of one page each, or 64 / 2^pps of 2^pps pages each.
 // UNI: pages of 64 tokens or more, so that a step lies in one page: its id and scales are
-// wave-uniform (read for 64 steps at a time, one a lane), and the loads take a scalar base with
-// a lane offset that never changes.
+// wave-uniform, and the loads take a scalar base with a lane offset that never changes.
+template <int HD, bool UNI>
+struct Stream {
+  static constexpr int ND = HD / 16, KL = HD / 64;
+  const PagedAttnArgs &a;
+  const int n;   // steps
+  const int lane, col, g, kg, PS, pps, hold;
+  const uint32_t koff, voff;
+  int tph = -1, tp = 0;
+  float tks = 0.f, tvs = 0.f;
+  i32x4 kc[4][KL], vc[ND];   // 16 channels of keys 16 kg + 4 t + col % 4; 16 keys of channels 16 d + col
+  float ksc = 0.f, vsc = 0.f;
+  int vph = -1;
+
+  __device__ __forceinline__ Stream(const PagedAttnArgs &a_, int n_)
+      : a(a_), n(n_), lane(threadIdx.x & 63), col(lane & 15), g(lane >> 4), kg(col >> 2), PS(1 << a_.pshift),
+        pps(UNI ? 0 : 6 - a_.pshift), hold(64 >> pps), koff((16 * kg + (col & 3)) * HD + 16 * g),
+        voff(col * PS + 16 * g) {}
+
+  // step p of sequence b and head h: the page of this lane's part of it
+  __device__ __forceinline__ int page_of(int b, int h, int p) const {
+    const int at = UNI ? p >> (a.pshift - 6) : (p << pps) + (lane & ((1 << pps) - 1));
+    const int id = a.table[(int64_t)b * a.table_rs + min(at, a.width - 1)];
+    return at < a.width && (uint32_t)id < (uint32_t)a.num_pages ? id * a.Hkv + h : -1;
+  }
+  __device__ __forceinline__ void scales() {
+    tks = a.ks[max(tph, 0)];
+    tvs = a.vs[max(tph, 0)];
+  }
+  // what lane group `grp` needs of a held value at step i
+  template <typename V>
+  __device__ __forceinline__ V held(V v, int i, int grp) const {
+    if constexpr (UNI)
+      return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i & 63));
+    else
+      return __shfl(v, ((i & (hold - 1)) << pps) + (grp >> (2 - pps)), 64);
+  }
+  // a held value that a step's lanes share
+  __device__ __forceinline__ int step_of(int v, int i) const {
+    return __builtin_amdgcn_readlane(v, (i & (hold - 1)) << pps);
+  }
+  // Step i's loads. Past the last step they still issue (a branch around them would make the
+  // compiler wait for all loads where its paths meet), for a few bytes of page 0.
+  __device__ __forceinline__ void load_k(int i) {
+    const int64_t ph = max(held(tph, i, kg), 0);
+    if constexpr (UNI) {
+      const uint8_t *base = a.kp + (ph * PS + ((step_of(tp, i) * 64) & (PS - 1))) * HD;
+      const uint32_t off = i < n ? koff : 0;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < KL; ++j) kc[t][j] = load16(base + (4 * t * HD + 64 * j), off);
+    } else {
+      const uint8_t *base = a.kp + (ph * PS + ((16 * kg) & (PS - 1)) + (col & 3)) * HD + 16 * g;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < KL; ++j) kc[t][j] = *reinterpret_cast<const i32x4 *>(base + 4 * t * HD + 64 * j);
+    }
+    __builtin_amdgcn_sched_barrier(0);   // keys before values, here and in the loop
+  }
+  __device__ __forceinline__ void load_v(int i) {
+    vph = held(tph, i, g);
+    const int64_t ph = max(vph, 0);
+    if constexpr (UNI) {
+      const uint8_t *base = a.vp + ph * HD * PS + ((step_of(tp, i) * 64) & (PS - 1));
+      const uint32_t off = i < n ? voff : 0;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) vc[d] = load16(base + 16 * d * PS, off);
+    } else {
+      const uint8_t *base = a.vp + (ph * HD + col) * PS + ((16 * g) & (PS - 1));
+#pragma unroll
+      for (int d = 0; d < ND; ++d) vc[d] = *reinterpret_cast<const i32x4 *>(base + 16 * d * PS);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // find(lane's step, tp) -> tph, for the steps from i0 on
+  template <typename F>
+  __device__ __forceinline__ void find_steps(int i0, F find) {
+    const int i = i0 + (lane >> pps);
+    tph = -1;
+    if (i < n) tph = find(i, tp);
+  }
+  template <typename F>
+  __device__ __forceinline__ void start(F find) {
+    find_steps(0, find);
+    scales();
+    load_k(0);
+    load_v(0);
+    __builtin_amdgcn_s_waitcnt(wait_vm(4 * KL + ND));   // the scales
+    ksc = held(tks, 0, kg);
+    vsc = held(tvs, 0, g);
+  }
+  template <typename F>
+  __device__ __forceinline__ void next_k(int i, F find) {
+    if ((i & (hold - 1)) == 0 && i < n) {
+      find_steps(i, find);
+      scales();
+      // wait here, once for all these steps: left to the reads of a lane, the wait would be in
+      // every step and drain the tiles in flight
+      __builtin_amdgcn_s_waitcnt(wait_vm(0));
+    }
+    load_k(i);
+    ksc = held(tks, i, kg);
+  }
+  __device__ __forceinline__ void next_v(int i) {
+    load_v(i);
+    vsc = held(tvs, i, g);
+  }
+};
+
+// One tile's queries and results.
 template <int HD, int NT, typename T, bool UNI>
-struct Steps {
-  static constexpr int NQ = Parts<T>::n, KS = HD / 32, ND = HD / 16, KL = HD / 64;
+struct Rows {
+  static constexpr int NQ = Parts<T>::n, KS = HD / 32, ND = HD / 16;
   const PagedAttnArgs &a;
   const Tile &x;
-  const int lane, col, g;
+  const int col, g;
   bf16x8 qf[NT][NQ][KS];
   int lim[NT];          // each row's last key
   f32x4 o[NT][ND];
   float m[NT], l[NT];   // l: this lane's part of the row sum
+  int nan_from;         // the first edge step with a NaN among its values
 
-  __device__ __forceinline__ Steps(const PagedAttnArgs &a_, const Tile &x_, int G)
-      : a(a_), x(x_), lane(threadIdx.x & 63), col(lane & 15), g(lane >> 4) {
+  __device__ __forceinline__ Rows(const PagedAttnArgs &a_, const Tile &x_, int G)
+      : a(a_), x(x_), col(threadIdx.x & 15), g((threadIdx.x & 63) >> 4), nan_from(x_.steps) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = nt * 16 + col;
@@ -223,201 +347,93 @@ struct Steps {
     }
   }
 
-  // steps p0, p0 + stride, .. below p1
-  __device__ __forceinline__ void run(int p0, int p1, int stride) {
-    if (p0 >= p1) return;
-    const int n = (p1 - p0 + stride - 1) / stride;
-    const int PS = 1 << a.pshift, kg = col >> 2;
-    const int32_t *trow = a.table + (int64_t)x.b * a.table_rs;
-    const int first_lim = x.q.len + x.tok0;   // the last key that the tile's first token sees
-    const int end_key = x.q.len + x.q.n;
-
-    auto page_at = [&](int i) {   // -1: none
-      const int id = i < a.width ? trow[i] : -1;
-      return (uint32_t)id < (uint32_t)a.num_pages ? id : -1;
-    };
-    // UNI: lane i holds what step 64 k + i needs
-    int tpage = -1;
-    float tks = 0.f, tvs = 0.f;
-    auto refill = [&](int i0) {
-      const int i = i0 + lane;
-      tpage = i < n ? page_at((p0 + i * stride) >> (a.pshift - 6)) : -1;
-      const int64_t ph = (int64_t)max(tpage, 0) * a.Hkv + x.h;
-      tks = a.ks[ph];
-      tvs = a.vs[ph];
-      // wait here, once in 64 steps: left to the reads of a lane, the wait would be in every step
-      // and drain the tiles in flight
-      __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));   // vmcnt(0) only
-    };
-    // else: the ids of the lane's key group (K) and of its value group, two steps ahead
-    int kid[2] = {-1, -1}, vid[2] = {-1, -1};
-    auto ids = [&](int i, int at) {
-      const int k0 = (p0 + i * stride) * 64;
-      kid[at] = i < n ? page_at((k0 + 16 * kg) >> a.pshift) : -1;
-      vid[at] = i < n ? page_at((k0 + 16 * g) >> a.pshift) : -1;
-    };
-
-    i32x4 kc[4][KL], vc[ND];
-    float ksc = 0.f, vsc = 0.f;
-    int vpage = -1;
-    const uint32_t koff = (uint32_t)((16 * kg + (col & 3)) * HD + 16 * g), voff = (uint32_t)(col * PS + 16 * g);
-    // Step i's loads. Past the last step they still issue (a branch around them would make the
-    // compiler wait for all loads where its paths meet), for a few bytes of page 0.
-    auto load_k = [&](int i) {
-      const int p = p0 + i * stride;
-      if constexpr (UNI) {
-        const int page = max(__builtin_amdgcn_readlane(tpage, i & 63), 0);
-        const uint8_t *base = a.kp + (((int64_t)page * a.Hkv + x.h) * PS + ((p * 64) & (PS - 1))) * HD;
-        ksc = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, tks), i & 63));
-        const uint32_t off = i < n ? koff : 0;
+  // Step p of the tile, the stream's step i; the stream's loads go on to its next one.
+  template <typename F>
+  __device__ __forceinline__ void step(Stream<HD, UNI> &st, int i, int p, F find) {
+    f32x4 s[NT][4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int j = 0; j < KL; ++j) kc[t][j] = load16(base + (4 * t * HD + 64 * j), off);
-      } else {
-        const int64_t ph = (int64_t)max(kid[0], 0) * a.Hkv + x.h;
-        const uint8_t *base = a.kp + (ph * PS + ((p * 64 + 16 * kg) & (PS - 1)) + (col & 3)) * HD + 16 * g;
-        ksc = a.ks[ph];
+      for (int t = 0; t < 4; ++t) s[nt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // four independent sums a turn; the fences keep the compiler from converting the whole step
+    // first, which would take 64 registers each for K and V
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+    for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-          for (int j = 0; j < KL; ++j) kc[t][j] = *reinterpret_cast<const i32x4 *>(base + 4 * t * HD + 64 * j);
-      }
-      __builtin_amdgcn_sched_barrier(0);   // keys before values, here and in the loop
-    };
-    auto load_v = [&](int i, int at) {   // at: the lane that holds step i's page
-      const int p = p0 + i * stride;
-      if constexpr (UNI) {
-        vpage = __builtin_amdgcn_readlane(tpage, at);
-        const uint8_t *base = a.vp + ((int64_t)max(vpage, 0) * a.Hkv + x.h) * HD * PS + ((p * 64) & (PS - 1));
-        vsc = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, tvs), at));
-        const uint32_t off = i < n ? voff : 0;
+      for (int t = 0; t < 4; ++t) {
+        const i32x4 c = st.kc[t][ks >> 1];
+        const bf16x8 kf = decode8(c[2 * (ks & 1)], c[2 * (ks & 1) + 1], st.ksc);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) vc[d] = load16(base + 16 * d * PS, off);
-      } else {
-        vpage = vid[0];
-        const int64_t ph = (int64_t)max(vpage, 0) * a.Hkv + x.h;
-        const uint8_t *base = a.vp + (ph * HD + col) * PS + ((p * 64 + 16 * g) & (PS - 1));
-        vsc = a.vs[ph];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) vc[d] = *reinterpret_cast<const i32x4 *>(base + 16 * d * PS);
+          for (int q = 0; q < NQ; ++q) s[nt][t] = mfma16(kf, qf[nt][q][ks], s[nt][t]);
       }
       __builtin_amdgcn_sched_barrier(0);
-    };
-
-    if constexpr (UNI) {
-      refill(0);
-    } else {
-      ids(0, 0);
-      ids(1, 1);
     }
-    int nan_from = n;
-    load_k(0);
-    load_v(0, 0);
-    for (int i = 0; i < n; ++i) {
-      const int p = p0 + i * stride;
-      f32x4 s[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) s[nt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      // four independent sums a turn; the fences keep the compiler from converting the whole
-      // step first, which would take 64 registers each for K and V
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const i32x4 c = kc[t][ks >> 1];
-          const bf16x8 kf = decode8(c[2 * (ks & 1)], c[2 * (ks & 1) + 1], ksc);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) s[nt][t] = mfma16(kf, qf[nt][q][ks], s[nt][t]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      const int vnow = vpage;
-      if constexpr (UNI) {
-        if (((i + 1) & 63) == 0) refill(i + 1);
-      } else {
-        kid[0] = kid[1];
-        vid[0] = vid[1];
-        ids(i + 2, 1);
-      }
-      load_k(i + 1);
+    st.next_k(i + 1, find);
 
-      // this lane's keys: key0 + 4 t + r
-      const int key0 = p * 64 + 16 * g;
-      const bool edge = p * 64 + 63 > first_lim || (UNI ? vnow < 0 : (bool)__any(vnow < 0));
-      bf16x8 pf[NT][NQ][2];
+    // this lane's keys: key0 + 4 t + r
+    const int key0 = p * 64 + 16 * g;
+    const bool edge = p * 64 + 63 > x.q.len + x.tok0 || (UNI ? st.vph < 0 : (bool)__any(st.vph < 0));
+    bf16x8 pf[NT][NQ][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (edge) {
-          const int last = vnow < 0 ? -1 : lim[nt];
+    for (int nt = 0; nt < NT; ++nt) {
+      if (edge) {
+        const int last = st.vph < 0 ? -1 : lim[nt];
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[nt][t][r] = key0 + 4 * t + r <= last ? s[nt][t][r] : kNegInf;
-        }
-        float e[16], sum = 0.f;
+          for (int r = 0; r < 4; ++r) s[nt][t][r] = key0 + 4 * t + r <= last ? s[nt][t][r] : kNegInf;
+      }
+      float e[16], sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        e[k] = __builtin_amdgcn_exp2f(fmaf(s[nt][k >> 2][k & 3], a.scale_log2, -m[nt]));
+        sum += e[k];
+      }
+      if (__any(!(sum <= 0x1p20f))) {
+        float mx = kNegInf;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, s[nt][k >> 2][k & 3]);
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float now = fmaxf(m[nt], mx * a.scale_log2);
+        const float off = now == kNegInf ? 0.f : now;
+        const float alpha = __builtin_amdgcn_exp2f(m[nt] - off);   // 0 from -inf
+        l[nt] *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[nt][d] *= alpha;
+        m[nt] = now;
+        sum = 0.f;
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          e[k] = __builtin_amdgcn_exp2f(fmaf(s[nt][k >> 2][k & 3], a.scale_log2, -m[nt]));
+          e[k] = __builtin_amdgcn_exp2f(fmaf(s[nt][k >> 2][k & 3], a.scale_log2, -off));
           sum += e[k];
         }
-        if (__any(!(sum <= 0x1p20f))) {
-          float mx = kNegInf;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) mx = fmaxf(mx, s[nt][k >> 2][k & 3]);
-          mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-          mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-          const float now = fmaxf(m[nt], mx * a.scale_log2);
-          const float off = now == kNegInf ? 0.f : now;
-          const float alpha = __builtin_amdgcn_exp2f(m[nt] - off);   // 0 from -inf
-          l[nt] *= alpha;
-#pragma unroll
-          for (int d = 0; d < ND; ++d) o[nt][d] *= alpha;
-          m[nt] = now;
-          sum = 0.f;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            e[k] = __builtin_amdgcn_exp2f(fmaf(s[nt][k >> 2][k & 3], a.scale_log2, -off));
-            sum += e[k];
-          }
-        }
-        l[nt] += sum;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          bf16x8 part[NQ];
-          split8<NQ>(e + 8 * c, part);
-#pragma unroll
-          for (int q = 0; q < NQ; ++q) pf[nt][q][c] = part[q];
-        }
       }
-
-      if (edge && cut_values(vc, vnow < 0 ? 0 : end_key - key0)) nan_from = min(nan_from, i);
+      l[nt] += sum;
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < 2; ++c) {
+        bf16x8 part[NQ];
+        split8<NQ>(e + 8 * c, part);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const bf16x8 vf = decode8(vc[d][2 * c], vc[d][2 * c + 1], vsc);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) o[nt][d] = mfma16(vf, pf[nt][q][c], o[nt][d]);
-          if (d % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-        }
-      load_v(i + 1, (i + 1) & 63);
+        for (int q = 0; q < NQ; ++q) pf[nt][q][c] = part[q];
+      }
     }
 
-    // NaNs that were taken out of an edge step's values (rare)
-    for (int i = nan_from; i < n; ++i) {
-      const int p = p0 + i * stride;
-      if constexpr (UNI) refill(i);
-      else ids(i, 0);
-      load_v(i, 0);
-      if (p * 64 + 63 > first_lim || __any(vpage < 0)) put_nan(vc, p * 64 + 16 * g, vpage);
-    }
+    if (edge && cut_values(st.vc, st.vph < 0 ? 0 : x.q.len + x.q.n - key0)) nan_from = min(nan_from, p);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const bf16x8 vf = decode8(st.vc[d][2 * c], st.vc[d][2 * c + 1], st.vsc);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) o[nt][d] = mfma16(vf, pf[nt][q][c], o[nt][d]);
+        if (d % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    st.next_v(i + 1);
   }
 
   // Of an edge step's values: zeros from row `valid` on and for NaN, whose product with a
@@ -435,24 +451,35 @@ struct Steps {
     return __any(nan);
   }
 
-  // The NaNs of an edge step's values count for the rows that see them, and only for those: an
-  // output becomes NaN where a product of the NaNs' places with the mask is not 0.
-  __device__ __forceinline__ void put_nan(const i32x4 *vc, int key0, int vnow) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      bf16x8 sees[2];
-#pragma unroll
-      for (int k = 0; k < 16; ++k) sees[k >> 3][k & 7] = (bf16_t)(key0 + k <= lim[nt] && vnow >= 0 ? 1.f : 0.f);
+  // The NaNs taken out of the edge steps below p1 count for the rows that see them, and only for
+  // those: an output becomes NaN where a product of the NaNs' places with the mask is not 0. Rare; the
+  // values are read again.
+  __device__ __forceinline__ void put_nan(const Stream<HD, UNI> &st, int p1, int stride) {
+    for (int p = nan_from; p < p1; p += stride) {
+      const int key0 = p * 64 + 16 * g, at = key0 >> a.pshift;
+      const int id = at < a.width ? a.table[(int64_t)x.b * a.table_rs + at] : -1;
+      const bool there = (uint32_t)id < (uint32_t)a.num_pages;
+      if (p * 64 + 63 <= x.q.len + x.tok0 && !__any(!there)) continue;
+      const uint8_t *base =
+          a.vp + (((int64_t)(there ? id : 0) * a.Hkv + x.h) * HD + col) * st.PS + (key0 & (st.PS - 1));
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
+        const i32x4 c = *reinterpret_cast<const i32x4 *>(base + 16 * d * st.PS);
         uint32_t one[4];   // 1.0 (0x38) where the code is NaN
 #pragma unroll
-        for (int k = 0; k < 4; ++k) one[k] = (nan_bits((uint32_t)vc[d][k]) >> 7) * 0x38u;
-        f32x4 hit = {0.f, 0.f, 0.f, 0.f};
-        hit = mfma16(decode8(one[0], one[1], 1.f), sees[0], hit);
-        hit = mfma16(decode8(one[2], one[3], 1.f), sees[1], hit);
+        for (int k = 0; k < 4; ++k)
+          one[k] = (nan_bits((uint32_t)c[k] & first_bytes(x.q.len + x.q.n - key0 - 4 * k)) >> 7) * 0x38u;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[nt][d][r] = hit[r] > 0.f ? __builtin_nanf("") : o[nt][d][r];
+        for (int nt = 0; nt < NT; ++nt) {
+          bf16x8 sees[2];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) sees[k >> 3][k & 7] = (bf16_t)(key0 + k <= lim[nt] && there ? 1.f : 0.f);
+          f32x4 hit = {0.f, 0.f, 0.f, 0.f};
+          hit = mfma16(decode8(one[0], one[1], 1.f), sees[0], hit);
+          hit = mfma16(decode8(one[2], one[3], 1.f), sees[1], hit);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[nt][d][r] = hit[r] > 0.f ? __builtin_nanf("") : o[nt][d][r];
+        }
       }
     }
   }
@@ -476,20 +503,35 @@ __device__ __forceinline__ void zero_rest(const PagedAttnArgs &a) {
 
 // ---- equal shares of all steps, a wave each ----------------------------------------
 
-constexpr int kMinShare = 1;
-
 // Workgroups a CU: what the registers of a wave allow.
-constexpr int share_occupancy(int NT, int parts) { return parts == 1 || (NT == 1 && parts == 2) ? 2 : 1; }
+constexpr int share_occupancy(int NT, int parts) { return NT == 1 && parts < 3 ? 2 : 1; }
 
 // Partial results of a worker's first (0) and last (1) tile: rows of HD values, then (max, sum) pairs.
 __host__ __device__ __forceinline__ int64_t slot_floats(int rows, int HD) { return (int64_t)rows * (HD + 2); }
 
-struct JoinNote {   // of a tile: the worker that begins it, how many go through it, the first one's slot
-  int worker, n, slot, pad;
+struct JoinNote {   // of a tile: the workers that begin and end it, the first one's slot
+  int first, last, slot, pad;
 };
 
-// Inclusive sums of the sequences' steps (all heads) in LDS; returns the total.
-__device__ __forceinline__ int scan_steps(const PagedAttnArgs &a, int tmshift, int32_t *pre, int32_t *wave_sum) {
+// Where the share of workgroup wg (its waves' shares in their order) begins in `total` steps: equal
+// shares, or, with two workgroups a CU and steps enough, kOld : kYoung for the one that a CU takes first
+// and the other: a CU serves its older waves first, and with equal shares they end in 5/6 of the others' time.
+constexpr int kOld = 11, kYoung = 9;
+__device__ __forceinline__ int64_t share_begin(int me, int workers, int total, bool uneven) {
+  if (!uneven) {
+    const int w = min(workers, total);   // no share is empty
+    return me >= w ? total : (int64_t)me * total / w;
+  }
+  // blocks reach the XCDs in turn: an XCD's first half are the older ones
+  const int per = workers >> 3, x = me / per, in = me - x * per, half = per >> 1;
+  const int64_t cum = (int64_t)x * half * (kOld + kYoung) + (in <= half ? in * kOld : half * kOld + (in - half) * kYoung);
+  return cum * total / ((int64_t)(workers >> 1) * (kOld + kYoung));
+}
+
+// Inclusive sums of the sequences' steps (all heads) and the sequences themselves in LDS;
+// returns the total.
+__device__ __forceinline__ int scan_steps(const PagedAttnArgs &a, int tmshift, int32_t *pre, SeqSpan *seqs,
+                                          int32_t *wave_sum) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   int carry = 0;
   for (int b0 = 0; b0 < a.B; b0 += 256) {
@@ -498,6 +540,7 @@ __device__ __forceinline__ int scan_steps(const PagedAttnArgs &a, int tmshift, i
     if (b < a.B) {
       const SeqSpan q = seq_span(a.cu, a.lengths, b, a.T, a.width << a.pshift);
       s = (int)(SeqTiles{q.n, q.len, tmshift}.all() * a.Hkv);
+      seqs[b] = q;
     }
     for (int m = 1; m < 64; m <<= 1) {
       const int o = __shfl_up(s, m, 64);
@@ -516,127 +559,182 @@ __device__ __forceinline__ int scan_steps(const PagedAttnArgs &a, int tmshift, i
   return carry;
 }
 
-// The tile that holds step u, and u's place in it.
-__device__ __forceinline__ int locate(const PagedAttnArgs &a, int tmshift, int G, const int32_t *pre, int u, Tile &x) {
-  int b = 0;
-  for (int i0 = 0; i0 < a.B; i0 += 64) {
-    const int i = i0 + (threadIdx.x & 63);
-    b += __popcll(__ballot(i < a.B && pre[min(i, a.B - 1)] <= u));
+// The tile that holds step u (u differs from lane to lane) and u's place in it.
+struct Place {
+  int b, h, t, p;
+};
+__device__ __forceinline__ Place locate(const PagedAttnArgs &a, int tmshift, const int32_t *pre, const SeqSpan *seqs,
+                                        int u) {
+  Place r;
+  int lo = 0, hi = a.B - 1;
+  while (lo < hi) {   // the first sequence that ends behind u
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] > u) hi = mid;
+    else lo = mid + 1;
   }
-  x.b = __builtin_amdgcn_readfirstlane(min(b, a.B - 1));
-  const int rest = u - (x.b ? __builtin_amdgcn_readfirstlane(pre[x.b - 1]) : 0);
-  x.q = seq_span(a.cu, a.lengths, x.b, a.T, a.width << a.pshift);
-  const SeqTiles st{x.q.n, x.q.len, tmshift};
-  const int each = (int)st.all();
-  x.h = rest / each;
-  const int in = rest - x.h * each;
-  int lo = 0, hi = st.tiles() - 1;
+  r.b = lo;
+  const SeqSpan q = seqs[lo];
+  const SeqTiles st{q.n, q.len, tmshift};
+  const int rest = u - (lo ? pre[lo - 1] : 0), each = max((int)st.all(), 1);
+  r.h = rest / each;
+  const int in = rest - r.h * each;
+  lo = 0;
+  hi = st.tiles() - 1;
   while (lo < hi) {   // the last tile that begins at or before `in`
     const int mid = (lo + hi + 1) >> 1;
     if (st.before(mid) <= in) lo = mid;
     else hi = mid - 1;
   }
-  x.set(st, lo, G);
-  return in - (int)st.before(lo);
+  r.t = lo;
+  r.p = in - (int)st.before(lo);
+  return r;
 }
 
 template <int HD, int NT, typename T, bool UNI>
 __global__ __launch_bounds__(256, share_occupancy(NT, Parts<T>::n)) void paged_share_kernel(PagedAttnArgs a, int tmshift, int G) {
   constexpr int ND = HD / 16, ROWS = 16 * NT;
   __shared__ int32_t pre[kMaxSeqs];
+  __shared__ SeqSpan seqs[kMaxSeqs];
   __shared__ int32_t wave_sum[4];
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int workers = gridDim.x * 4;
   const int me = xcd_swizzle(blockIdx.x, gridDim.x) * 4 + wave_id();
-  const int total = scan_steps(a, tmshift, pre, wave_sum);
-  const int share = max((total + workers - 1) / workers, kMinShare);
-  const int u0 = (int)min((int64_t)me * share, (int64_t)total), u1 = (int)min((int64_t)u0 + share, (int64_t)total);
+  const int total = scan_steps(a, tmshift, pre, seqs, wave_sum);
+  const bool uneven = share_occupancy(NT, Parts<T>::n) == 2 && workers % 64 == 0 && total >= 4 * workers;
+  const int u0 = (int)share_begin(me, workers, total, uneven), u1 = (int)share_begin(me + 1, workers, total, uneven);
   JoinNote *notes = reinterpret_cast<JoinNote *>(a.ws + (int64_t)workers * 2 * slot_floats(ROWS, HD));
 
-  for (int u = u0; u < u1;) {
-    Tile x;
-    const int p0 = locate(a, tmshift, G, pre, u, x), p1 = min(x.steps, p0 + u1 - u);
-    const bool whole = p0 == 0 && p1 == x.steps;
-    const int slot = 2 * me + (u > u0 ? 1 : 0);
-    if (p0 == 0 && lane == 0)
-      notes[tile_slot(x.q, x.b, x.t, tmshift) * a.Hkv + x.h] =
-          JoinNote{me, whole ? 0 : (u + x.steps - 1) / share - me + 1, slot, 0};
-    Steps<HD, NT, T, UNI> st(a, x, G);
-    st.run(p0, p1, 1);
-    float *pp = a.ws + slot * slot_floats(ROWS, HD);
+  if (u0 < u1) {
+    Stream<HD, UNI> st(a, u1 - u0);
+    int tb = 0, th = 0, tt = 0;   // a lane holds the tile of its step, too
+    auto find = [&](int i, int &p) {
+      const Place pl = locate(a, tmshift, pre, seqs, u0 + i);
+      tb = pl.b;
+      th = pl.h;
+      tt = pl.t;
+      p = pl.p;
+      return st.page_of(pl.b, pl.h, pl.p);
+    };
+    st.start(find);
+    int nb = st.step_of(tb, 0), nh = st.step_of(th, 0), nt_ = st.step_of(tt, 0), np = st.step_of(st.tp, 0);
+    for (int i = 0; i < st.n;) {
+      Tile x;
+      x.b = nb;
+      x.h = nh;
+      x.q.first = __builtin_amdgcn_readfirstlane(seqs[nb].first);
+      x.q.n = __builtin_amdgcn_readfirstlane(seqs[nb].n);
+      x.q.len = __builtin_amdgcn_readfirstlane(seqs[nb].len);
+      x.set(SeqTiles{x.q.n, x.q.len, tmshift}, nt_, G);
+      const int p0 = np, p1 = min(x.steps, p0 + st.n - i), slot = 2 * me + (i > 0 ? 1 : 0);
+      const bool whole = p0 == 0 && p1 == x.steps;
+      JoinNote &note = notes[tile_slot(x.q, x.b, x.t, tmshift) * a.Hkv + x.h];
+      if (st.lane == 0) {
+        if (p0 == 0) note.first = me, note.slot = slot;
+        if (p1 == x.steps) note.last = me;
+      }
+      Rows<HD, NT, T, UNI> rows(a, x, G);
+      for (int p = p0; p < p1; ++p, ++i) rows.step(st, i, p, find);
+      // the next tile, whose first step's page is held by now
+      nb = st.step_of(tb, i);
+      nh = st.step_of(th, i);
+      nt_ = st.step_of(tt, i);
+      np = st.step_of(st.tp, i);
+      if (rows.nan_from < p1) rows.put_nan(st, p1, 1);
+      float *pp = a.ws + slot * slot_floats(ROWS, HD);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const float sum = st.row_sum(nt);
-      const int r = nt * 16 + col;
-      if (r < x.rows) {
-        if (whole) {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;   // no visible key: zeros
-          T *op = row_of<T>(x, G, r, a.out, a.o_ss, a.o_hs) + 4 * g;
+      for (int nt = 0; nt < NT; ++nt) {
+        const float sum = rows.row_sum(nt);
+        const int r = nt * 16 + col;
+        if (r < x.rows) {
+          if (whole) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;   // no visible key: zeros
+            T *op = row_of<T>(x, G, r, a.out, a.o_ss, a.o_hs) + 4 * g;
 #pragma unroll
-          for (int d = 0; d < ND; ++d) {
-            const f32x4 v = st.o[nt][d] * inv;
-            store4(op + 16 * d, v[0], v[1], v[2], v[3]);
-          }
-        } else {
+            for (int d = 0; d < ND; ++d) {
+              const f32x4 v = rows.o[nt][d] * inv;
+              store4(op + 16 * d, v[0], v[1], v[2], v[3]);
+            }
+          } else {
 #pragma unroll
-          for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4 *>(pp + r * HD + 16 * d + 4 * g) = st.o[nt][d];
-          if (g == 0) {
-            pp[ROWS * HD + 2 * r] = st.m[nt];
-            pp[ROWS * HD + 2 * r + 1] = sum;
+            for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4 *>(pp + r * HD + 16 * d + 4 * g) = rows.o[nt][d];
+            if (g == 0) {
+              pp[ROWS * HD + 2 * r] = rows.m[nt];
+              pp[ROWS * HD + 2 * r + 1] = sum;
+            }
           }
         }
       }
     }
-    u += p1 - p0;
   }
   zero_rest<HD, T>(a);
 }
 
-// The partial results of a tile that more than one worker went through, joined in a fixed
-// order: a workgroup a row, its waves a quarter of every 64 parts each.
-template <int HD, int NT, typename T>
+// The partial results of the tiles that more than one worker went through, joined in a fixed order.
+// WPR waves take a row's parts, groups of HD / 4 lanes a part each (4 channels a lane), U of them in
+// flight before their maximum is known: 1 where there are rows enough to fill the chip, else 4.
+template <int HD, int NT, typename T, int WPR>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int tmshift, int G, int workers) {
-  constexpr int ROWS = 16 * NT, C = HD / 64;
-  __shared__ float acc4[4][HD];
-  const int lane = threadIdx.x & 63, w = wave_id();
-  const int slot = blockIdx.x / a.Hkv, h = blockIdx.x - slot * a.Hkv, r = blockIdx.y;
+  constexpr int ROWS = 16 * NT, TPP = HD / 4, PG = 64 / TPP, U = 8;
+  __shared__ f32x4 accs[4][64];
+  const int lane = threadIdx.x & 63, w = wave_id(), sub = w % WPR, pg = sub * PG + lane / TPP, c = lane % TPP;
+  const int slot = blockIdx.x / a.Hkv;
   const JoinNote *notes = reinterpret_cast<const JoinNote *>(a.ws + (int64_t)workers * 2 * slot_floats(ROWS, HD));
-  JoinNote n = notes[blockIdx.x];   // of a slot without a tile: anything, and not used
+  const JoinNote n = notes[blockIdx.x];   // of a slot without a tile: anything, and not used
   Tile x;
-  x.h = h;
-  if (!tile_of_slot(a, slot, tmshift, G, x) || n.n == 0 || r >= x.rows) return;
-  auto part = [&](int i) { return a.ws + (int64_t)(i == 0 ? n.slot : 2 * (n.worker + i)) * slot_floats(ROWS, HD); };
-  float m = kNegInf;
-  for (int i = lane; i < n.n; i += 64) m = fmaxf(m, part(i)[ROWS * HD + 2 * r]);
-  for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
-  const float off = m == kNegInf ? 0.f : m;
-  float l = 0.f, acc[C];
+  x.h = blockIdx.x - slot * a.Hkv;
+  if (!tile_of_slot(a, slot, tmshift, G, x) || n.first == n.last) return;
+  const int parts = n.last - n.first + 1;
+  auto part = [&](int i) { return a.ws + (int64_t)(i == 0 ? n.slot : 2 * (n.first + i)) * slot_floats(ROWS, HD); };
+  for (int r0 = blockIdx.y * (4 / WPR); r0 < x.rows; r0 += gridDim.y * (4 / WPR)) {
+    const int r = min(r0 + w / WPR, x.rows - 1);   // past the last row: the same once more, not stored
+    float m = kNegInf, l = 0.f;   // l: of this lane's parts
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+      const int k = min(64, parts - i0);
+      float pm = kNegInf, pl = 0.f;
+      if (lane < k) {
+        const float *pp = part(i0 + lane) + ROWS * HD + 2 * r;
+        pm = pp[0];
+        pl = pp[1];
+      }
+      f32x4 v[U];
+      auto load = [&](int j0) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) acc[c] = 0.f;
-  for (int i0 = 0; i0 < n.n; i0 += 64) {
-    float f = 0.f;
-    if (i0 + lane < n.n) {
-      const float *pp = part(i0 + lane) + ROWS * HD + 2 * r;
-      f = __builtin_amdgcn_exp2f(pp[0] - off);
-      l += f * pp[1];
+        for (int u = 0; u < U; ++u)
+          v[u] = *reinterpret_cast<const f32x4 *>(part(i0 + min(j0 + u * PG * WPR + pg, k - 1)) + r * HD + 4 * c);
+      };
+      load(0);
+      float mx = pm;
+      for (int s = 32; s; s >>= 1) mx = fmaxf(mx, __shfl_xor(mx, s, 64));
+      const float now = fmaxf(m, mx), off = now == kNegInf ? 0.f : now, alpha = __builtin_amdgcn_exp2f(m - off);
+      const float f = __builtin_amdgcn_exp2f(pm - off);
+      l = l * alpha + pl * f;
+      acc *= alpha;
+      m = now;
+      for (int j0 = 0; j0 < k; j0 += U * PG * WPR) {
+        if (j0) load(j0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int j = j0 + u * PG * WPR + pg;
+          const float fj = __shfl(f, min(j, 63), 64);
+          acc += v[u] * (j < k ? fj : 0.f);
+        }
+      }
     }
-    const int k1 = min(16 * (w + 1), n.n - i0);
-#pragma unroll 8
-    for (int k = 16 * w; k < k1; ++k) {
-      const float fk = __shfl(f, k, 64);
-      const float *pp = part(i0 + k) + r * HD + lane * C;
+    for (int s = 32; s; s >>= 1) l += __shfl_xor(l, s, 64);
+    // the groups of the row's waves
+    accs[w][lane] = acc;
+    __syncthreads();
+    if (sub == 0 && lane < TPP && r0 + w / WPR < x.rows) {
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < C; ++c) acc[c] += fk * pp[c];
+      for (int v = 0; v < WPR; ++v)
+#pragma unroll
+        for (int i = 0; i < PG; ++i) sum += accs[w + v][i * TPP + lane];
+      const float inv = l == 0.f ? 0.f : 1.f / l;   // no visible key: zeros
+      store4(row_of<T>(x, G, r, a.out, a.o_ss, a.o_hs) + 4 * lane, sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
     }
-  }
-  for (int k = 32; k; k >>= 1) l += __shfl_xor(l, k, 64);
-#pragma unroll
-  for (int c = 0; c < C; ++c) acc4[w][lane * C + c] = acc[c];
-  __syncthreads();
-  const int d = threadIdx.x;
-  if (d < HD) {
-    const float v = (acc4[0][d] + acc4[1][d]) + (acc4[2][d] + acc4[3][d]);
-    row_of<T>(x, G, r, a.out, a.o_ss, a.o_hs)[d] = (T)(l == 0.f ? 0.f : v * (1.f / l));
+    __syncthreads();
   }
 }
 
@@ -653,19 +751,28 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttnArgs a, in
   Tile x;
   x.h = blockIdx.x - slot * a.Hkv;
   if (tile_of_slot(a, slot, tmshift, G, x)) {
-    Steps<HD, NT, T, UNI> st(a, x, G);
-    st.run(w, x.steps, NW);
+    Rows<HD, NT, T, UNI> rows(a, x, G);
+    Stream<HD, UNI> st(a, (x.steps - w + NW - 1) / NW);   // 0 or less: none
+    if (st.n > 0) {
+      auto find = [&](int i, int &p) {
+        p = w + i * NW;
+        return st.page_of(x.b, x.h, p);
+      };
+      st.start(find);
+      for (int i = 0; i < st.n; ++i) rows.step(st, i, w + i * NW, find);
+      if (rows.nan_from < x.steps) rows.put_nan(st, x.steps, NW);
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       if (nt * 16 >= x.rows) break;
-      const float sum = st.row_sum(nt);
+      const float sum = rows.row_sum(nt);
       if (nt) __syncthreads();   // om and ml are free again
       if (g == 0) {
-        ml[w][0][col] = st.m[nt];
+        ml[w][0][col] = rows.m[nt];
         ml[w][1][col] = sum;
       }
 #pragma unroll
-      for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4 *>(&om[w][col][16 * d + 4 * g]) = st.o[nt][d];
+      for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4 *>(&om[w][col][16 * d + 4 * g]) = rows.o[nt][d];
       __syncthreads();
       // 4 channels a thread
       for (int i = tid; i < 16 * HD / 4; i += 64 * NW) {
@@ -698,7 +805,7 @@ struct Shape {
 };
 
 // Keys up to which a sequence is one workgroup's.
-constexpr int kShortKeys = 4096;
+constexpr int kShortKeys = 1024;
 
 // The narrowest tile that holds an average sequence's query rows: a wide one's empty
 // columns cost matrix work only, a narrow one reads the cache once more a tile.
@@ -717,8 +824,12 @@ void launch3(const PagedAttnArgs &a, const Shape &s, hipStream_t stream) {
     paged_tile_kernel<HD, NT, T, UNI, NW><<<tiles, 64 * NW, 0, stream>>>(a, s.tmshift, G);
   } else {
     paged_share_kernel<HD, NT, T, UNI><<<s.nwg, 256, 0, stream>>>(a, s.tmshift, G);
-    const int rows = std::min(1 << s.tmshift, a.T) * G;
-    paged_join_kernel<HD, NT, T><<<dim3(tiles, rows), 256, 0, stream>>>(a, s.tmshift, G, s.nwg * 4);
+    // for the rows of an average sequence's tile
+    const int rows = std::min(1 << s.tmshift, (a.T + a.B - 1) / a.B) * G;
+    if ((int64_t)tiles * rows >= 8 * device_cu_count())
+      paged_join_kernel<HD, NT, T, 1><<<dim3(tiles, (rows + 3) / 4), 256, 0, stream>>>(a, s.tmshift, G, s.nwg * 4);
+    else
+      paged_join_kernel<HD, NT, T, 4><<<dim3(tiles, rows), 256, 0, stream>>>(a, s.tmshift, G, s.nwg * 4);
   }
 }
 
