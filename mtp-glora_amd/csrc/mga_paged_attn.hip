@@ -106,10 +106,10 @@ struct SeqTiles {
   }
 };
 
-// Tokens of a tile: the largest power of two (at most 64) of which a tile holds the query heads.
-inline int tm_shift(int rows, int G) {
+// Tokens of a tile: the largest power of two (at most 2^most) of which a tile holds the query heads.
+inline int tm_shift(int rows, int G, int most = 6) {
   int s = 0;
-  while (((2 << s) * G <= rows) && s < 6) ++s;
+  while (((2 << s) * G <= rows) && s < most) ++s;
   return s;
 }
 
@@ -513,19 +513,12 @@ struct JoinNote {   // of a tile: the workers that begin and end it, the first o
   int first, last, slot, pad;
 };
 
-// Where the share of workgroup wg (its waves' shares in their order) begins in `total` steps: equal
-// shares, or, with two workgroups a CU and steps enough, kOld : kYoung for the one that a CU takes first
-// and the other: a CU serves its older waves first, and with equal shares they end in 5/6 of the others' time.
-constexpr int kOld = 11, kYoung = 9;
-__device__ __forceinline__ int64_t share_begin(int me, int workers, int total, bool uneven) {
-  if (!uneven) {
-    const int w = min(workers, total);   // no share is empty
-    return me >= w ? total : (int64_t)me * total / w;
-  }
-  // blocks reach the XCDs in turn: an XCD's first half are the older ones
-  const int per = workers >> 3, x = me / per, in = me - x * per, half = per >> 1;
-  const int64_t cum = (int64_t)x * half * (kOld + kYoung) + (in <= half ? in * kOld : half * kOld + (in - half) * kYoung);
-  return cum * total / ((int64_t)(workers >> 1) * (kOld + kYoung));
+// Where worker me's share begins: shares differ by one step at most and none is empty. (A CU serves
+// its older workgroup first, which ends in 5/6 of the other's time; shares of 11 : 9 for the two were
+// within 2% either way.)
+__device__ __forceinline__ int share_begin(int me, int workers, int total) {
+  const int w = min(workers, total);
+  return me >= w ? total : (int)((int64_t)me * total / w);
 }
 
 // Inclusive sums of the sequences' steps (all heads) and the sequences themselves in LDS;
@@ -600,8 +593,7 @@ __global__ __launch_bounds__(256, share_occupancy(NT, Parts<T>::n)) void paged_s
   const int workers = gridDim.x * 4;
   const int me = xcd_swizzle(blockIdx.x, gridDim.x) * 4 + wave_id();
   const int total = scan_steps(a, tmshift, pre, seqs, wave_sum);
-  const bool uneven = share_occupancy(NT, Parts<T>::n) == 2 && workers % 64 == 0 && total >= 4 * workers;
-  const int u0 = (int)share_begin(me, workers, total, uneven), u1 = (int)share_begin(me + 1, workers, total, uneven);
+  const int u0 = share_begin(me, workers, total), u1 = share_begin(me + 1, workers, total);
   JoinNote *notes = reinterpret_cast<JoinNote *>(a.ws + (int64_t)workers * 2 * slot_floats(ROWS, HD));
 
   if (u0 < u1) {
@@ -797,7 +789,237 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttnArgs a, in
   zero_rest<HD, T>(a);
 }
 
-enum Mode { kShares, kTiles };
+// ---- prompts: 128 query rows a workgroup ----------------------------------------------
+
+// Four waves of 32 rows share the keys and values, which are converted once for all of them: step
+// j + 1's codes go from registers to bf16 tiles in LDS (rows XOR-swizzled, mga_common.hpp) and step
+// j + 2's are loaded while step j is computed, one barrier a step. S^T = K Q^T and O^T += V^T P^T by
+// v_mfma_f32_32x32x16_bf16; key m of a 32-key tile is read from row 16 (m / 16) + 8 (m / 4 % 2)
+// + 4 (m / 8 % 2) + m % 4, so that a lane's scores are those of 8 consecutive keys twice and meet V rows of 16
+// bytes as they lie. Bounded by the matrix unit and the softmax's vector work beside it.
+constexpr int kPromptRows = 128;
+
+template <int HD, typename T>
+__global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_kernel(PagedAttnArgs a, int tmshift, int G, int slots) {
+  constexpr int NQ = Parts<T>::n, KS = HD / 16, DT = HD / 32;
+  constexpr int NL = HD / 64;            // 16-byte loads a thread and step, for keys and for values
+  constexpr int VR = 256 / HD;           // threads a value row
+  __shared__ __attribute__((aligned(16))) bf16_t kt[2][64 * HD];
+  __shared__ __attribute__((aligned(16))) bf16_t vt[2][HD * 64];
+  __shared__ int there[2][4];            // whether a 16-key group has a page
+  __shared__ int nan_step;               // the first edge step with a NaN among its values
+  const int tid = threadIdx.x, lane = tid & 63, w = wave_id(), l32 = lane & 31, hi = lane >> 5;
+  const int PS = 1 << a.pshift;
+  Tile x;
+  x.h = blockIdx.x % a.Hkv;
+  const int slot = slots - 1 - (int)blockIdx.x / a.Hkv;   // long tiles first
+  if (tile_of_slot(a, slot, tmshift, G, x)) {
+    const int row = w * 32 + l32, first_lim = x.q.len + x.tok0, end_key = x.q.len + x.q.n;
+    const int lim = row < x.rows ? first_lim + row / G : -1;
+    // of the wave's rows: the last key of the first and of the last one
+    const int wave_first = w * 32 < x.rows ? first_lim + w * 32 / G : -1;
+    const int wave_last = w * 32 < x.rows ? first_lim + min(w * 32 + 31, x.rows - 1) / G : -1;
+    bf16x8 qf[NQ][KS];
+    {
+      const T *qp = row_of<const T>(x, G, row, a.q, a.q_ss, a.q_hs);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int c = 16 * ks + 8 * hi;
+        if constexpr (NQ == 1) {
+          qf[0][ks] = row < x.rows ? load8(qp + c) : bf16x8{};
+        } else {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = 0.f;
+          if (row < x.rows) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = (float)qp[c + i];
+          }
+          bf16x8 part[NQ];
+          split8<NQ>(v, part);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) qf[n][ks] = part[n];
+        }
+      }
+    }
+    f32x16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = zero16();
+    float m = kNegInf, l = 0.f;
+
+    // this thread's part of a step: NL * 16 bytes of key row kr, and of value row vr
+    const int kr = tid >> 2, kpart = tid & 3, vr = tid / VR, vpart = tid % VR;
+    const int32_t *trow = a.table + (int64_t)x.b * a.table_rs;
+    int kid = 0, vid[NL];   // pages of the step after the one in registers, not checked yet
+    auto ids = [&](int p) {
+      kid = trow[min((p * 64 + kr) >> a.pshift, a.width - 1)];
+#pragma unroll
+      for (int i = 0; i < NL; ++i) vid[i] = trow[min((p * 64 + 16 * (vpart * NL + i)) >> a.pshift, a.width - 1)];
+    };
+    auto checked = [&](int id, int key) {
+      return (uint32_t)id < (uint32_t)a.num_pages && (key >> a.pshift) < a.width ? id : -1;
+    };
+    i32x4 kc[NL], vc[NL];
+    float ksc, vsc[NL];
+    int kpage, vpage[NL];
+    auto load = [&](int p) {
+      kpage = checked(kid, p * 64 + kr);
+      const int64_t kph = (int64_t)max(kpage, 0) * a.Hkv + x.h;
+      const uint8_t *kb = a.kp + (kph * PS + ((p * 64 + kr) & (PS - 1))) * HD + kpart * (16 * NL);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) kc[i] = *reinterpret_cast<const i32x4 *>(kb + 16 * i);
+      ksc = a.ks[kph];
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int key = p * 64 + 16 * (vpart * NL + i);
+        vpage[i] = checked(vid[i], key);
+        const int64_t vph = (int64_t)max(vpage[i], 0) * a.Hkv + x.h;
+        vc[i] = *reinterpret_cast<const i32x4 *>(a.vp + (vph * HD + vr) * PS + (key & (PS - 1)));
+        vsc[i] = a.vs[vph];
+      }
+    };
+    // the step in registers to LDS, converted
+    auto put = [&](int p, int buf) {
+      if (kpart == 0 && (kr & 15) == 0) there[buf][kr >> 4] = kpage >= 0;
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          *reinterpret_cast<bf16x8 *>(&kt[buf][tile_off<HD>(kr, 2 * (kpart * NL + i) + k)]) =
+              decode8(kc[i][2 * k], kc[i][2 * k + 1], ksc);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        if (p * 64 + 63 > first_lim || vpage[i] < 0) {   // zeros for what is not there, and for NaN (put back at the end)
+          const int valid = vpage[i] < 0 ? 0 : end_key - (p * 64 + 16 * (vpart * NL + i));
+          uint32_t nan = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t c = (uint32_t)vc[i][k] & first_bytes(valid - 4 * k), bad = nan_bits(c);
+            nan |= bad;
+            vc[i][k] = (int)(c & ~((bad >> 7) * 0xffu));
+          }
+          if (nan) atomicMin(&nan_step, p);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          *reinterpret_cast<bf16x8 *>(&vt[buf][tile_off<64>(vr, 2 * (vpart * NL + i) + k)]) =
+              decode8(vc[i][2 * k], vc[i][2 * k + 1], vsc[i]);
+      }
+    };
+
+    if (tid == 0) nan_step = x.steps;
+    ids(0);
+    load(0);
+    ids(1);
+    __syncthreads();
+    put(0, 0);
+    load(1);
+    ids(2);
+    __syncthreads();
+    const int pm = (l32 & 16) + ((l32 & 4) << 1) + ((l32 & 8) >> 1) + (l32 & 3);
+    for (int p = 0; p < x.steps; ++p) {
+      const int buf = p & 1;
+      if (p + 1 < x.steps) put(p + 1, buf ^ 1);
+      load(p + 2);   // past the last step: some page's, not used
+      ids(p + 3);
+      if (p * 64 <= wave_last) {
+        f32x16 s[2] = {zero16(), zero16()};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const bf16x8 kf = lds_read8(&kt[buf][tile_off<HD>(32 * t + pm, 2 * ks + hi)]);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) s[t] = mfma32<bf16_t>(kf, qf[n][ks], s[t]);
+          }
+        const i32x4 have = *reinterpret_cast<const i32x4 *>(there[buf]);
+        const bool all = have[0] && have[1] && have[2] && have[3];
+        if (p * 64 + 63 > wave_first || !all) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int key = p * 64 + 32 * t + 16 * (r >> 3) + 8 * hi + (r & 7);
+              s[t][r] = key <= lim && have[2 * t + (r >> 3)] ? s[t][r] : kNegInf;
+            }
+        }
+        float e[32], sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          e[k] = __builtin_amdgcn_exp2f(fmaf(s[k >> 4][k & 15], a.scale_log2, -m));
+          sum += e[k];
+        }
+        if (__any(!(sum <= 0x1p20f))) {
+          float mx = kNegInf;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) mx = fmaxf(mx, s[k >> 4][k & 15]);
+          mx = fmaxf(mx, xor32(mx));
+          const float now = fmaxf(m, mx * a.scale_log2);
+          const float off = now == kNegInf ? 0.f : now;
+          const float alpha = __builtin_amdgcn_exp2f(m - off);   // 0 from -inf
+          l *= alpha;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[d] *= alpha;
+          m = now;
+          sum = 0.f;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            e[k] = __builtin_amdgcn_exp2f(fmaf(s[k >> 4][k & 15], a.scale_log2, -off));
+            sum += e[k];
+          }
+        }
+        l += sum;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          bf16x8 pf[NQ];
+          split8<NQ>(e + 8 * u, pf);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const bf16x8 vf = lds_read8(&vt[buf][tile_off<64>(32 * d + l32, 2 * u + hi)]);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) o[d] = mfma32<bf16_t>(vf, pf[n], o[d]);
+          }
+        }
+      }
+      __syncthreads();
+    }
+
+    // NaNs taken out of the edge steps: for the rows that see them (see put_nan)
+    for (int p = nan_step; p < x.steps; ++p)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int key = p * 64 + 16 * u + 8 * hi;
+        const int id = checked(trow[min(key >> a.pshift, a.width - 1)], key);
+        bf16x8 sees;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sees[k] = (bf16_t)(key + k <= lim && id >= 0 ? 1.f : 0.f);
+        const uint8_t *vb = a.vp + ((int64_t)max(id, 0) * a.Hkv + x.h) * HD * PS + (key & (PS - 1));
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const i32x2 c = *reinterpret_cast<const i32x2 *>(vb + (32 * d + l32) * PS);
+          uint32_t one[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            one[k] = (nan_bits((uint32_t)c[k] & first_bytes(end_key - key - 4 * k)) >> 7) * 0x38u;
+          const f32x16 hit = mfma32<bf16_t>(decode8(one[0], one[1], 1.f), sees, zero16());
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] = hit[r] > 0.f ? __builtin_nanf("") : o[d][r];
+        }
+      }
+    const float sum = l + xor32(l), inv = sum == 0.f ? 0.f : 1.f / sum;   // no visible key: zeros
+    if (row < x.rows) {
+      T *op = row_of<T>(x, G, row, a.out, a.o_ss, a.o_hs) + 4 * hi;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+          store4(op + 32 * d + 2 * r, o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv);
+    }
+  }
+  zero_rest<HD, T>(a);
+}
+
+enum Mode { kShares, kTiles, kPrompts };
 
 struct Shape {
   Mode mode;
@@ -813,6 +1035,10 @@ Shape shape_of(int T, int B, int Hq, int Hkv, int64_t keys, int dtype) {
   const int G = Hq / Hkv;
   const int64_t rows = ((int64_t)T * G + B - 1) / B;
   const int NT = rows <= 16 && G <= 16 ? 1 : 2, parts = dtype == kDtBf16 ? 1 : dtype == kDtF16 ? 2 : 3;
+  // prompts by 128 rows where those tiles fill the chip
+  const int pm = tm_shift(kPromptRows, G, 7);
+  if (rows >= kPromptRows / 2 && (int64_t)tile_slots(T, B, pm) * Hkv >= device_cu_count())
+    return {kPrompts, 0, pm, 0};
   return {keys <= kShortKeys ? kTiles : kShares, NT, tm_shift(16 * NT, G), share_occupancy(NT, parts) * device_cu_count()};
 }
 
@@ -835,6 +1061,11 @@ void launch3(const PagedAttnArgs &a, const Shape &s, hipStream_t stream) {
 
 template <int HD, typename T>
 void launch1(const PagedAttnArgs &a, const Shape &s, hipStream_t stream) {
+  if (s.mode == kPrompts) {
+    const int slots = tile_slots(a.T, a.B, s.tmshift);
+    paged_prompt_kernel<HD, T><<<slots * a.Hkv, 256, 0, stream>>>(a, s.tmshift, a.Hq / a.Hkv, slots);
+    return;
+  }
   if (a.pshift >= 6) {
     if (s.NT == 1) launch3<HD, 1, T, true>(a, s, stream);
     else launch3<HD, 2, T, true>(a, s, stream);

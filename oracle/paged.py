@@ -68,17 +68,23 @@ def attend(q, k, v, cu, lengths, table, page_size, scale):
     T, Hq, D = q.shape
     G = Hq // k.shape[1]
     out, weight = np.zeros_like(q), np.zeros_like(q)
+    held = {}   # a sequence's positions that have a page: position, page, row
     for t, b, pos, _, _ in places(cu, lengths, table, page_size, len(k), T):
-        seen = [j for j in range(pos + 1) if j // page_size < len(table[b])
-                and 0 <= table[b][j // page_size] < len(k)]
-        if not seen:
+        if b not in held:
+            j = np.arange(len(table[b]) * page_size)
+            ids = np.repeat(np.asarray(table[b], np.int64), page_size)
+            there = (ids >= 0) & (ids < len(k))
+            held[b] = j[there], ids[there], j[there] % page_size
+        j, pg, row = held[b]
+        n = int(np.searchsorted(j, pos, side="right"))
+        if n == 0:
             continue
-        pg, row = np.array([table[b][j // page_size] for j in seen]), np.array(seen) % page_size
-        for h in range(Hq):
+        for g in range(k.shape[1]):
+            heads = slice(g * G, (g + 1) * G)
             with np.errstate(all="ignore"):
-                s = k[pg, h // G, row] @ q[t, h] * scale
-                p = np.exp(s - s.max())
-                p /= p.sum()
-                out[t, h] = p @ v[pg, h // G, row]
-                weight[t, h] = p @ np.abs(v[pg, h // G, row])
+                s = q[t, heads] @ k[pg[:n], g, row[:n]].T * scale
+                p = np.exp(s - s.max(-1, keepdims=True))
+                p /= p.sum(-1, keepdims=True)
+                out[t, heads] = p @ v[pg[:n], g, row[:n]]
+                weight[t, heads] = p @ np.abs(v[pg[:n], g, row[:n]])
     return out, weight

@@ -140,6 +140,43 @@ def test_attention_long(mga, dev, dtype, new, cached):
     check_attention(attend(mga, pool, q), q, pool, 0.125)
 
 
+PROMPTS = [([700, 30, 500, 1, 333], [0, 77, 190, 400, 3]), ([1, 129, 64, 900, 65, 200], [1000, 0, 63, 64, 500, 1])]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Hq,Hkv,D,ps", [(16, 8, 64, 64), (32, 8, 128, 64), (32, 8, 64, 16), (24, 8, 128, 128), (40, 8, 64, 32)])
+def test_attention_prompts(mga, dev, dtype, Hq, Hkv, D, ps):
+    """Batches of prompts, with sequences of few tokens among them."""
+    for i, (new, cached) in enumerate(PROMPTS):
+        print(f"case {new} {cached} {Hq} {Hkv} {D} {ps} {dtype}", flush=True)
+        pool = Pool(dev, new, cached, Hkv, D, ps, seed=i)
+        q = queries(pool, Hq, D, dtype, dev, extra=3)
+        got = attend(mga, pool, q)
+        assert not got[pool.T:].any()
+        check_attention(got, q, pool, D ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,ps", [(64, 64), (128, 16), (64, 128)])
+def test_attention_prompts_with_holes_and_nan(mga, dev, dtype, D, ps):
+    """Missing pages, NaN that some rows see, wide scores, in batches of prompts."""
+    pool = Pool(dev, [700, 30, 500, 333], [0, 77, 190, 3], 8, D, ps, seed=6, scales=(-6, 0))
+    t0 = pool.table.cpu()
+    pool.v[t0[0, 130 // ps], 0, 3, 130 % ps] = 0x7f    # position 130: the later rows of the first sequence
+    pool.v[t0[0, 699 // ps], 7, D - 1, 699 % ps] = 0xff
+    pool.k[t0[2, 400 // ps], 5, 400 % ps, 5] = 0xff    # a key of the third
+    pool.v[t0[1, 106 // ps], :, :, 107 % ps:] = 0x7f   # behind the second one's end
+    pool.table[3, 100 // ps] = -1
+    pool.table[2, 0] = pool.n
+    q = queries(pool, 16, D, dtype, dev)
+    got = attend(mga, pool, q)
+    want = check_attention(got, q, pool, D ** -0.5)
+    nan = np.isnan(want)
+    assert nan[130:700, 0:2, 3].all() and not nan[:130].any() and nan[699, 14, D - 1] and not nan[698, 14, D - 1]
+    pool.table[3, :] = -1
+    assert not attend(mga, pool, q)[1230:].any()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_many_sequences(mga, dev, dtype):
     """More sequences than threads of a workgroup, some without tokens."""
