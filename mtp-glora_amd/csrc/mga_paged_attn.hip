@@ -32,6 +32,7 @@
 // Where a value that a row may not see is NaN (a masked place), its products would be
 // NaN although p = 0: see put_nan.
 #include <algorithm>
+#include <type_traits>
 
 #include "mga_internal.hpp"
 #include "mga_paged.hpp"
@@ -799,7 +800,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttnArgs a, in
 // bytes as they lie. Bounded by the matrix unit and the softmax's vector work beside it.
 constexpr int kPromptRows = 128;
 
-template <int HD, typename T>
+template <int HD, typename T, bool UNI>
 __global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_kernel(PagedAttnArgs a, int tmshift, int G, int slots) {
   constexpr int NQ = Parts<T>::n, KS = HD / 16, DT = HD / 32;
   constexpr int NL = HD / 64;            // 16-byte loads a thread and step, for keys and for values
@@ -847,50 +848,102 @@ __global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_ke
     for (int d = 0; d < DT; ++d) o[d] = zero16();
     float m = kNegInf, l = 0.f;
 
-    // this thread's part of a step: NL * 16 bytes of key row kr, and of value row vr
-    const int kr = tid >> 2, kpart = tid & 3, vr = tid / VR, vpart = tid % VR;
-    const int32_t *trow = a.table + (int64_t)x.b * a.table_rs;
-    int kid = 0, vid[NL];   // pages of the step after the one in registers, not checked yet
-    auto ids = [&](int p) {
-      kid = trow[min((p * 64 + kr) >> a.pshift, a.width - 1)];
+    // this thread's part of a step: NL * 16 bytes of key row kr, and of value row vr; every other row
+    // (pair of rows) takes its two in the other order, so that a write's lanes meet in no bank
+    const int kr = tid >> 2, vr = tid / VR;
+    int kat[NL], vat[NL];   // 16-byte pieces of a row
 #pragma unroll
-      for (int i = 0; i < NL; ++i) vid[i] = trow[min((p * 64 + 16 * (vpart * NL + i)) >> a.pshift, a.width - 1)];
-    };
+    for (int i = 0; i < NL; ++i) {
+      kat[i] = (tid & 3) * NL + (NL == 2 ? i ^ (kr & 1) : i);
+      vat[i] = tid % VR * NL + (NL == 2 ? i ^ (vr >> 1 & 1) : i);
+    }
+    const int32_t *trow = a.table + (int64_t)x.b * a.table_rs;
     auto checked = [&](int id, int key) {
-      return (uint32_t)id < (uint32_t)a.num_pages && (key >> a.pshift) < a.width ? id : -1;
+      return (uint32_t)id < (uint32_t)a.num_pages && (key >> a.pshift) < a.width ? id * a.Hkv + x.h : -1;
     };
+    // UNI: the lanes hold the pages (page * Hkv + head, -1: none) and scales of 64 steps; else each
+    // thread its own pages of the step after the one in registers, not checked yet
+    int tph = -1, kid = 0, vid[NL];
+    float tks = 0.f, tvs = 0.f;
+    auto ids = [&](int p) {
+      if constexpr (UNI) {
+        if (p & 63) return;
+        const int key = (p + lane) * 64;
+        tph = checked(trow[min(key >> a.pshift, a.width - 1)], key);
+        tks = a.ks[max(tph, 0)];
+        tvs = a.vs[max(tph, 0)];
+        __builtin_amdgcn_s_waitcnt(wait_vm(0));   // once in 64 steps, see Stream
+      } else {
+        kid = trow[min((p * 64 + kr) >> a.pshift, a.width - 1)];
+#pragma unroll
+        for (int i = 0; i < NL; ++i) vid[i] = trow[min((p * 64 + 16 * vat[i]) >> a.pshift, a.width - 1)];
+      }
+    };
+    uint32_t klo[NL], vlo[NL];   // UNI: this thread's pieces within a page
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      klo[i] = kr * HD + 16 * kat[i];
+      vlo[i] = (vr << a.pshift) + 16 * vat[i];
+    }
     i32x4 kc[NL], vc[NL];
     float ksc, vsc[NL];
-    int kpage, vpage[NL];
+    int kph, vph[NL];
     auto load = [&](int p) {
-      kpage = checked(kid, p * 64 + kr);
-      const int64_t kph = (int64_t)max(kpage, 0) * a.Hkv + x.h;
-      const uint8_t *kb = a.kp + (kph * PS + ((p * 64 + kr) & (PS - 1))) * HD + kpart * (16 * NL);
+      if constexpr (UNI) {
+        kph = __builtin_amdgcn_readlane(tph, p & 63);
+        const int64_t ph = max(kph, 0);
+        const int in = (p * 64) & (PS - 1);
 #pragma unroll
-      for (int i = 0; i < NL; ++i) kc[i] = *reinterpret_cast<const i32x4 *>(kb + 16 * i);
-      ksc = a.ks[kph];
+        for (int i = 0; i < NL; ++i) {
+          kc[i] = load16(a.kp + ((ph << a.pshift) + in) * HD, klo[i]);
+          vc[i] = load16(a.vp + (ph * HD << a.pshift) + in, vlo[i]);
+          vph[i] = kph;
+          vsc[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, tvs), p & 63));
+        }
+        ksc = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, tks), p & 63));
+      } else {
+        kph = checked(kid, p * 64 + kr);
+        const uint8_t *kb = a.kp + (((int64_t)max(kph, 0) << a.pshift) + ((p * 64 + kr) & (PS - 1))) * HD;
 #pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int key = p * 64 + 16 * (vpart * NL + i);
-        vpage[i] = checked(vid[i], key);
-        const int64_t vph = (int64_t)max(vpage[i], 0) * a.Hkv + x.h;
-        vc[i] = *reinterpret_cast<const i32x4 *>(a.vp + (vph * HD + vr) * PS + (key & (PS - 1)));
-        vsc[i] = a.vs[vph];
+        for (int i = 0; i < NL; ++i) kc[i] = *reinterpret_cast<const i32x4 *>(kb + 16 * kat[i]);
+        ksc = a.ks[max(kph, 0)];
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const int key = p * 64 + 16 * vat[i];
+          vph[i] = checked(vid[i], key);
+          vc[i] = *reinterpret_cast<const i32x4 *>(
+              a.vp + (((int64_t)max(vph[i], 0) * HD + vr) << a.pshift) + (key & (PS - 1)));
+          vsc[i] = a.vs[max(vph[i], 0)];
+        }
       }
+    };
+    // lane offsets in the tiles, bytes: formed once
+    uint32_t kw[NL], vw[NL], ko[KS], vo[4];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      kw[i] = opaque_u32(2u * tile_off<HD>(kr, 2 * kat[i]));
+      vw[i] = opaque_u32(2u * tile_off<64>(vr, 2 * vat[i]));
+    }
+    const int pm = (l32 & 16) + ((l32 & 4) << 1) + ((l32 & 8) >> 1) + (l32 & 3);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) ko[ks] = opaque_u32(2u * tile_off<HD>(pm, 2 * ks + hi));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) vo[u] = opaque_u32(2u * tile_off<64>(l32, 2 * u + hi));
+    auto at = [](const bf16_t *tile, uint32_t off) {
+      return reinterpret_cast<bf16x8 *>(const_cast<char *>(lds_at(tile, off)));
     };
     // the step in registers to LDS, converted
     auto put = [&](int p, int buf) {
-      if (kpart == 0 && (kr & 15) == 0) there[buf][kr >> 4] = kpage >= 0;
+      if ((tid & 63) == 0) there[buf][kr >> 4] = kph >= 0;
+      // a piece's second 8 codes: the neighbouring granule
 #pragma unroll
       for (int i = 0; i < NL; ++i)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          *reinterpret_cast<bf16x8 *>(&kt[buf][tile_off<HD>(kr, 2 * (kpart * NL + i) + k)]) =
-              decode8(kc[i][2 * k], kc[i][2 * k + 1], ksc);
+        for (int k = 0; k < 2; ++k) *at(kt[buf], kw[i] ^ 16 * k) = decode8(kc[i][2 * k], kc[i][2 * k + 1], ksc);
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        if (p * 64 + 63 > first_lim || vpage[i] < 0) {   // zeros for what is not there, and for NaN (put back at the end)
-          const int valid = vpage[i] < 0 ? 0 : end_key - (p * 64 + 16 * (vpart * NL + i));
+        if (p * 64 + 63 > first_lim || vph[i] < 0) {   // zeros for what is not there, and for NaN (put back at the end)
+          const int valid = vph[i] < 0 ? 0 : end_key - (p * 64 + 16 * vat[i]);
           uint32_t nan = 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -901,9 +954,7 @@ __global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_ke
           if (nan) atomicMin(&nan_step, p);
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          *reinterpret_cast<bf16x8 *>(&vt[buf][tile_off<64>(vr, 2 * (vpart * NL + i) + k)]) =
-              decode8(vc[i][2 * k], vc[i][2 * k + 1], vsc[i]);
+        for (int k = 0; k < 2; ++k) *at(vt[buf], vw[i] ^ 16 * k) = decode8(vc[i][2 * k], vc[i][2 * k + 1], vsc[i]);
       }
     };
 
@@ -916,22 +967,25 @@ __global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_ke
     load(1);
     ids(2);
     __syncthreads();
-    const int pm = (l32 & 16) + ((l32 & 4) << 1) + ((l32 & 8) >> 1) + (l32 & 3);
-    for (int p = 0; p < x.steps; ++p) {
-      const int buf = p & 1;
+    // one step out of buffer BUF (a constant: the tiles' addresses are lane offsets plus immediates)
+    auto turn = [&](int p, auto which) {
+      constexpr int buf = decltype(which)::value;
       if (p + 1 < x.steps) put(p + 1, buf ^ 1);
       load(p + 2);   // past the last step: some page's, not used
       ids(p + 3);
       if (p * 64 <= wave_last) {
         f32x16 s[2] = {zero16(), zero16()};
+        // the products first: a SIMD's other wave fills what they leave with its softmax (5%)
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const bf16x8 kf = lds_read8(&kt[buf][tile_off<HD>(32 * t + pm, 2 * ks + hi)]);
+            const bf16x8 kf = *at(kt[buf] + 32 * t * HD, ko[ks]);
 #pragma unroll
             for (int n = 0; n < NQ; ++n) s[t] = mfma32<bf16_t>(kf, qf[n][ks], s[t]);
           }
+        __builtin_amdgcn_s_setprio(0);
         const i32x4 have = *reinterpret_cast<const i32x4 *>(there[buf]);
         const bool all = have[0] && have[1] && have[2] && have[3];
         if (p * 64 + 63 > wave_first || !all) {
@@ -969,31 +1023,37 @@ __global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_ke
           }
         }
         l += sum;
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           bf16x8 pf[NQ];
           split8<NQ>(e + 8 * u, pf);
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
-            const bf16x8 vf = lds_read8(&vt[buf][tile_off<64>(32 * d + l32, 2 * u + hi)]);
+            const bf16x8 vf = *at(vt[buf] + 32 * d * 64, vo[u]);
 #pragma unroll
             for (int n = 0; n < NQ; ++n) o[d] = mfma32<bf16_t>(vf, pf[n], o[d]);
           }
         }
+        __builtin_amdgcn_s_setprio(0);
       }
       __syncthreads();
+    };
+    for (int p = 0; p < x.steps; p += 2) {
+      turn(p, std::integral_constant<int, 0>{});
+      if (p + 1 < x.steps) turn(p + 1, std::integral_constant<int, 1>{});
     }
 
     // NaNs taken out of the edge steps: for the rows that see them (see put_nan)
     for (int p = nan_step; p < x.steps; ++p)
-#pragma unroll
+#pragma unroll 1
       for (int u = 0; u < 4; ++u) {
         const int key = p * 64 + 16 * u + 8 * hi;
-        const int id = checked(trow[min(key >> a.pshift, a.width - 1)], key);
+        const int ph = checked(trow[min(key >> a.pshift, a.width - 1)], key);
         bf16x8 sees;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sees[k] = (bf16_t)(key + k <= lim && id >= 0 ? 1.f : 0.f);
-        const uint8_t *vb = a.vp + ((int64_t)max(id, 0) * a.Hkv + x.h) * HD * PS + (key & (PS - 1));
+        for (int k = 0; k < 8; ++k) sees[k] = (bf16_t)(key + k <= lim && ph >= 0 ? 1.f : 0.f);
+        const uint8_t *vb = a.vp + ((int64_t)max(ph, 0) * HD << a.pshift) + (key & (PS - 1));
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           const i32x2 c = *reinterpret_cast<const i32x2 *>(vb + (32 * d + l32) * PS);
@@ -1063,7 +1123,10 @@ template <int HD, typename T>
 void launch1(const PagedAttnArgs &a, const Shape &s, hipStream_t stream) {
   if (s.mode == kPrompts) {
     const int slots = tile_slots(a.T, a.B, s.tmshift);
-    paged_prompt_kernel<HD, T><<<slots * a.Hkv, 256, 0, stream>>>(a, s.tmshift, a.Hq / a.Hkv, slots);
+    if (a.pshift >= 6)
+      paged_prompt_kernel<HD, T, true><<<slots * a.Hkv, 256, 0, stream>>>(a, s.tmshift, a.Hq / a.Hkv, slots);
+    else
+      paged_prompt_kernel<HD, T, false><<<slots * a.Hkv, 256, 0, stream>>>(a, s.tmshift, a.Hq / a.Hkv, slots);
     return;
   }
   if (a.pshift >= 6) {
