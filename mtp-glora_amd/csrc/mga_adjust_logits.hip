@@ -5,14 +5,14 @@
 //   y -= f * count + (count > 0 ? p : 0), count over the output;
 //   y += biases;  not allowed: y = -inf
 //
-// Bounded by HBM: each logit is read and written once. A workgroup takes a tile of
-// one row's columns. It first counts the row's tokens that fall into the tile in
-// LDS (a word a column: bits 0..30 count the output, bit 31 says that the prompt holds it;
-// integer adds, so their order does not matter), which costs a read of the row's tokens
-// for every tile, from L2, and so asks for wide tiles where the rows alone fill the chip.
-// Biases are added by one thread a column, in the order of the list: the tile's
-// entries are set in their order, 256 of the list at a time, and the first of each column
-// adds up those that follow it.
+// Bounded by HBM: each logit is read and written once. A workgroup takes a tile of one row's columns.
+// While the tile's logits are on their way it counts the row's tokens that fall into it in LDS: a count of the
+// output's in the low bits, a bit for the prompt's, a bit for columns with a bias (integer adds, so
+// their order does not matter). Every tile reads the row's tokens, from L2, which asks for wide
+// tiles where the rows alone fill the chip. Columns that nothing hit are copied as they are; the others find
+// their biases in the tile's list, kept in the caller's order, so that equal ids add up in it.
+// Counts of up to 2^14 - 1 tokens take 16 bits a column and biases of up to 1024 entries a list; longer ones
+// (the wide form) 32 bits and a sum a column, added by the first entry of each column for those after it.
 #include <type_traits>
 
 #include "mga_internal.hpp"
@@ -21,33 +21,39 @@
 namespace mga {
 namespace {
 
-constexpr uint32_t kInPrompt = 0x80000000u;
+constexpr int kListMax = 1024;
+constexpr int kNarrowTokens = (1 << 14) - 1;
 
-template <typename T>
-__device__ __forceinline__ float as_float(T v) { return (float)v; }
+template <bool WIDE> struct Count;
+template <> struct Count<false> { typedef uint16_t type; static constexpr int bits = 16; };
+template <> struct Count<true> { typedef uint32_t type; static constexpr int bits = 32; };
 
 struct RowSettings {
   float r, f, p;
 };
 
-__device__ __forceinline__ float adjusted(float x, uint32_t c, float b, const RowSettings &s) {
-  if (c) {
-    x = x > 0.f ? x / s.r : x * s.r;
-    const uint32_t n = c & ~kInPrompt;
-    if (n) x = fmaf(-s.f, (float)n, x) - s.p;
-  }
-  return x + b;
+// c: a column's count and, above it, whether it has a bias and whether the prompt holds it.
+template <int BITS>
+__device__ __forceinline__ float penalised(float x, uint32_t c, const RowSettings &s) {
+  const uint32_t n = c & ((1u << (BITS - 2)) - 1);
+  if (n || c >> (BITS - 1)) x = x > 0.f ? x / s.r : x * s.r;
+  return n ? fmaf(-s.f, (float)n, x) - s.p : x;
 }
 
 // A tile of TC columns from `base` on, which may begin before column 0 by less than a vector
 // (VEC: vectors of 16 bytes are aligned in x and out alike at base).
-template <typename T, int TC, bool VEC, bool BIAS>
+template <typename T, int TC, bool VEC, bool WIDE>
 __global__ __launch_bounds__(256) void adjust_logits_kernel(AdjustArgs a, int tiles) {
-  constexpr int VN = 16 / sizeof(T);
-  __shared__ uint32_t count[TC];
-  __shared__ float bias[BIAS ? TC : 1];
-  __shared__ int32_t list_col[BIAS ? 256 : 1];
-  __shared__ float list_val[BIAS ? 256 : 1];
+  typedef typename Count<WIDE>::type CT;
+  constexpr int VN = 16 / sizeof(T), BITS = Count<WIDE>::bits, NV = (TC + 256 * VN - 1) / (256 * VN);
+  constexpr uint32_t kPrompt = 1u << (BITS - 1), kBias = 1u << (BITS - 2);
+  // counts; where there are biases, a column's sum (wide) or the entry that holds it, and the list
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  CT *count = reinterpret_cast<CT *>(lds);
+  float *bias = reinterpret_cast<float *>(count + TC);
+  uint16_t *owner = reinterpret_cast<uint16_t *>(count + TC);
+  int32_t *list_col = reinterpret_cast<int32_t *>(WIDE ? (char *)(bias + TC) : (char *)(owner + TC));
+  float *list_val = reinterpret_cast<float *>(list_col + (WIDE ? 256 : a.K));
   __shared__ int32_t wave_n[4];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int row = blockIdx.x / tiles, tile = blockIdx.x % tiles;
@@ -58,102 +64,156 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(AdjustArgs a, int ti
   const int c0 = max(base, 0), c1 = min(base + TC, a.V);
   if (c0 >= c1) return;
 
-  for (int i = tid * 4; i < TC; i += 1024) {
-    *reinterpret_cast<i32x4 *>(&count[i]) = i32x4{0, 0, 0, 0};
-    if constexpr (BIAS) *reinterpret_cast<f32x4 *>(&bias[i]) = f32x4{0.f, 0.f, 0.f, 0.f};
+  i32x4 raw[VEC ? NV : 1];
+  if constexpr (VEC) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = (k * 256 + tid) * VN, col = base + i;
+      raw[k] = i32x4{0, 0, 0, 0};
+      if (i < TC && col >= 0 && col + VN <= a.V) raw[k] = *reinterpret_cast<const i32x4 *>(x + col);
+    }
   }
+  // the row's first tokens and biases and what says which count, all in flight before the first wait
+  constexpr int TU = 8;
+  int64_t tok[TU];
+  auto load_tokens = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < TU; ++u) {
+      const int64_t at = (int64_t)row * a.tokens_rs + min(i0 + 256 * u, a.L - 1);
+      tok[u] = a.tokens64 ? ((const int64_t *)a.tokens)[at] : ((const int32_t *)a.tokens)[at];
+    }
+  };
+  int64_t id = -1;
+  float val = 0.f;
+  auto load_bias = [&](int i) {
+    id = -1;
+    if (i >= a.K) return;
+    const int64_t at = (int64_t)row * a.bias_ids_rs + i;
+    id = a.bias64 ? ((const int64_t *)a.bias_ids)[at] : ((const int32_t *)a.bias_ids)[at];
+    val = a.bias[(int64_t)row * a.bias_rs + i];
+  };
+  if (a.L > 0) load_tokens(tid);
+  load_bias(tid);
+  const int n = a.lengths ? min(max(a.lengths[row], 0), a.L) : a.L;
+  const int m = a.prompts ? min(max(a.prompts[row], 0), n) : 0;
+  for (int i = tid; i < (int)(TC * sizeof(CT) / 16); i += 256) reinterpret_cast<i32x4 *>(count)[i] = i32x4{0, 0, 0, 0};
+  if (WIDE && a.K > 0)
+    for (int i = tid; i < TC; i += 256) bias[i] = 0.f;
   RowSettings s{a.repetition ? a.repetition[row] : a.repetition_all, a.frequency ? a.frequency[row] : a.frequency_all,
                 a.presence ? a.presence[row] : a.presence_all};
   if (!(s.r > 0.f)) s.r = 1.f;
   __syncthreads();
 
-  if (a.L > 0) {
-    const int n = a.lengths ? min(max(a.lengths[row], 0), a.L) : a.L;
-    const int m = a.prompts ? min(max(a.prompts[row], 0), n) : 0;
-    auto scan = [&](const auto *tok) {
-      for (int i0 = tid; i0 < n; i0 += 1024) {
-        int64_t t[4];   // four loads in flight, clamped instead of skipped past the end
+  // two narrow counts share a word: neither can pass its bits, nor reach the other's
+  auto shift = [&](int c) { return WIDE ? 0 : 16 * (c & 1); };
+  auto word = [&](int c) { return reinterpret_cast<uint32_t *>(count) + (WIDE ? c : c >> 1); };
+  for (int i0 = tid; i0 < n; i0 += 256 * TU) {
+    if (i0 != tid) load_tokens(i0);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) t[u] = tok[min(i0 + 256 * u, n - 1)];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int i = i0 + 256 * u;
-          if (i < n && t[u] >= c0 && t[u] < c1) {
-            uint32_t *c = &count[(int)t[u] - base];
-            if (i < m) atomicOr(c, kInPrompt);
-            else atomicAdd(c, 1u);
-          }
-        }
+    for (int u = 0; u < TU; ++u) {
+      const int i = i0 + 256 * u;
+      if (i < n && (uint64_t)(tok[u] - c0) < (uint64_t)(c1 - c0)) {
+        const int c = (int)tok[u] - base;
+        if (i < m) atomicOr(word(c), kPrompt << shift(c));
+        else atomicAdd(word(c), 1u << shift(c));
       }
-    };
-    if (a.tokens64) scan((const int64_t *)a.tokens + (int64_t)row * a.tokens_rs);
-    else scan((const int32_t *)a.tokens + (int64_t)row * a.tokens_rs);
+    }
   }
-  if constexpr (BIAS) {
-    const float *val = a.bias + (int64_t)row * a.bias_rs;
-    for (int i0 = 0; i0 < a.K; i0 += 256) {
-      const int i = i0 + tid;
-      int64_t id = -1;
-      if (i < a.K)
-        id = a.bias64 ? ((const int64_t *)a.bias_ids)[(int64_t)row * a.bias_ids_rs + i]
-                      : ((const int32_t *)a.bias_ids)[(int64_t)row * a.bias_ids_rs + i];
-      const bool mine = id >= c0 && id < c1;
-      const uint64_t who = __ballot(mine);
-      if (lane == 0) wave_n[w] = __popcll(who);
-      __syncthreads();
-      int at = __popcll(who & lanes_below()), n = 0;
-      for (int k = 0; k < 4; ++k) {
-        at += k < w ? wave_n[k] : 0;
-        n += wave_n[k];
-      }
-      if (mine) {
-        list_col[at] = (int)id - base;
-        list_val[at] = val[i];
-      }
-      __syncthreads();
-      if (tid < n) {
+  int listed = 0;
+  for (int i0 = 0; i0 < a.K; i0 += 256) {
+    if (i0) load_bias(i0 + tid);
+    const bool mine = id >= c0 && id < c1;
+    const uint64_t who = __ballot(mine);
+    if (lane == 0) wave_n[w] = __popcll(who);
+    __syncthreads();
+    int at = (WIDE ? 0 : listed) + __popcll(who & lanes_below()), found = 0;
+    for (int k = 0; k < 4; ++k) {
+      at += k < w ? wave_n[k] : 0;
+      found += wave_n[k];
+    }
+    listed += found;
+    if (mine) {
+      const int c = (int)id - base;
+      list_col[at] = c;
+      list_val[at] = val;
+      atomicOr(word(c), kBias << shift(c));
+    }
+    __syncthreads();
+    if constexpr (WIDE) {
+      if (tid < found) {
         const int c = list_col[tid];
         bool first = true;
         for (int k = 0; k < tid; ++k) first = first && list_col[k] != c;
         if (first) {
           float b = bias[c];
-          for (int k = tid; k < n; ++k) b += list_col[k] == c ? list_val[k] : 0.f;
+          for (int k = tid; k < found; ++k) b += list_col[k] == c ? list_val[k] : 0.f;
           bias[c] = b;
         }
       }
       __syncthreads();
     }
   }
+  if (!WIDE && listed) {
+    // one entry of each column, whichever, adds up all of them in their order
+    for (int t = tid; t < listed; t += 256) owner[list_col[t]] = (uint16_t)t;
+    __syncthreads();
+    for (int t = tid; t < listed; t += 256) {
+      const int c = list_col[t];
+      if (owner[c] != t) continue;
+      float b = 0.f;
+#pragma unroll 8
+      for (int k = 0; k < listed; ++k) b += list_col[k] == c ? list_val[k] : 0.f;
+      list_val[t] = b;   // read by no other column's sum
+    }
+  }
   __syncthreads();
 
   const uint32_t *ok = a.allowed ? (const uint32_t *)a.allowed + (int64_t)row * a.allowed_rs : nullptr;
+  auto value = [&](float v, uint32_t c, int i) {   // of tile column i, c != 0
+    v = penalised<BITS>(v, c, s);
+    if (c & kBias) v += WIDE ? bias[i] : list_val[owner[i]];
+    return v;
+  };
   auto one = [&](int col) {
-    const float y = adjusted(as_float(x[col]), count[col - base], BIAS ? bias[col - base] : 0.f, s);
-    out[col] = (T)(ok && !(ok[col >> 5] >> (col & 31) & 1) ? -__builtin_huge_valf() : y);
+    const uint32_t c = count[col - base];
+    T y = x[col];
+    if (c) y = (T)value((float)y, c, col - base);
+    out[col] = ok && !(ok[col >> 5] >> (col & 31) & 1) ? (T)-__builtin_huge_valf() : y;
   };
   if constexpr (VEC) {
-    for (int i = tid * VN; i < TC; i += 256 * VN) {
-      const int col = base + i;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = (k * 256 + tid) * VN, col = base + i;
+      if (i >= TC) break;
       if (col >= 0 && col + VN <= a.V) {
-        const i32x4 raw = *reinterpret_cast<const i32x4 *>(x + col);
-        const T *e = reinterpret_cast<const T *>(&raw);
-        i32x4 put;
-        T *o = reinterpret_cast<T *>(&put);
         uint32_t bits = ~0u;
         if (ok) {
           const int word = col >> 5;
           const uint32_t lo = ok[word], hi = (col + VN - 1) >> 5 != word ? ok[word + 1] : 0;
           bits = (uint32_t)((((uint64_t)hi << 32) | lo) >> (col & 31));
         }
+        uint32_t c[VN], any = 0;
 #pragma unroll
-        for (int k = 0; k < VN; ++k) {
-          const float y = adjusted(as_float(e[k]), count[i + k], BIAS ? bias[i + k] : 0.f, s);
-          o[k] = (T)(bits >> k & 1 ? y : -__builtin_huge_valf());
+        for (int e = 0; e < VN; ++e) {
+          c[e] = count[i + e];
+          any |= c[e];
+        }
+        i32x4 put = raw[k];
+        const T *src = reinterpret_cast<const T *>(&raw[k]);
+        T *o = reinterpret_cast<T *>(&put);
+        if (any) {
+#pragma unroll
+          for (int e = 0; e < VN; ++e)
+            if (c[e]) o[e] = (T)value((float)src[e], c[e], i + e);
+        }
+        if (ok) {
+#pragma unroll
+          for (int e = 0; e < VN; ++e) o[e] = bits >> e & 1 ? o[e] : (T)-__builtin_huge_valf();
         }
         *reinterpret_cast<i32x4 *>(out + col) = put;
       } else {
-        for (int k = 0; k < VN; ++k)
-          if (col + k >= 0 && col + k < a.V) one(col + k);
+        for (int e = 0; e < VN; ++e)
+          if (col + e >= 0 && col + e < a.V) one(col + e);
       }
     }
   } else {
@@ -161,10 +221,18 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(AdjustArgs a, int ti
   }
 }
 
-constexpr int kSmallTile = 1024, kLargeTile = 4096;
+// Bytes of a tile's logits: small tiles give few rows more workgroups; past the large ones' 8 KB a row's
+// tokens would be read less often, but reads and writes overlap less (80 rows of 151 936 bf16, 2048 tokens,
+// at 4 / 8 / 16 / 32 KB: 19.4 / 18.7 / 23.0 / 31.3 us).
+constexpr int kSmallTile = 2048, kLargeTile = 8192, kWideTile = 8192;
 
-int tile_of(int32_t N, int32_t V) {
-  return (int64_t)(V / kLargeTile) * N >= 4 * device_cu_count() ? kLargeTile : kSmallTile;
+bool wide_form(int32_t L, int32_t K) { return L > kNarrowTokens || K > kListMax; }
+
+// Large tiles where the rows fill the chip with them: two workgroups a CU and more.
+int tile_bytes(int32_t N, int32_t V, int32_t L, int32_t K, int eb) {
+  if (wide_form(L, K)) return kWideTile;
+  const int64_t bytes = (int64_t)V * eb;
+  return (bytes + kLargeTile - 1) / kLargeTile * N >= 2 * device_cu_count() ? kLargeTile : kSmallTile;
 }
 
 template <typename T>
@@ -173,26 +241,28 @@ void launch(const AdjustArgs &a, hipStream_t stream) {
   const auto at = [](const void *p) { return reinterpret_cast<uintptr_t>(p) / sizeof(T) % VN; };
   // rows that begin alike within a vector in x and out
   const bool vec = at(a.x) == at(a.out) && (a.N == 1 || a.xs % VN == a.os % VN);
-  auto go = [&](auto tc, auto v, auto b) {
-    constexpr int TC = decltype(tc)::value;
+  auto go = [&](auto bytes, auto v, auto wide) {
+    constexpr int TC = decltype(bytes)::value / sizeof(T);
+    constexpr bool W = decltype(wide)::value;
     const int tiles = (a.V + (decltype(v)::value ? VN - 1 : 0) + TC - 1) / TC;
-    adjust_logits_kernel<T, TC, decltype(v)::value, decltype(b)::value><<<(uint32_t)tiles * a.N, 256, 0, stream>>>(a, tiles);
+    const int lds = TC * (W ? 4 : 2) + (a.K > 0 ? TC * (W ? 4 : 2) + 8 * (W ? 256 : a.K) : 0);
+    adjust_logits_kernel<T, TC, decltype(v)::value, W><<<(uint32_t)tiles * a.N, 256, lds, stream>>>(a, tiles);
   };
-  auto go2 = [&](auto tc, auto v) {
-    if (a.K > 0) go(tc, v, std::true_type{});
-    else go(tc, v, std::false_type{});
+  auto go2 = [&](auto bytes, auto wide) {
+    if (vec) go(bytes, std::true_type{}, wide);
+    else go(bytes, std::false_type{}, wide);
   };
-  auto go3 = [&](auto tc) {
-    if (vec) go2(tc, std::true_type{});
-    else go2(tc, std::false_type{});
-  };
-  if (tile_of(a.N, a.V) == kLargeTile) go3(std::integral_constant<int, kLargeTile>{});
-  else go3(std::integral_constant<int, kSmallTile>{});
+  const int tile = tile_bytes(a.N, a.V, a.L, a.K, sizeof(T));
+  if (wide_form(a.L, a.K)) go2(std::integral_constant<int, kWideTile>{}, std::true_type{});
+  else if (tile == kLargeTile) go2(std::integral_constant<int, kLargeTile>{}, std::false_type{});
+  else go2(std::integral_constant<int, kSmallTile>{}, std::false_type{});
 }
 
 }  // namespace
 
-int64_t adjust_blocks(int32_t N, int32_t V) { return ((int64_t)V / tile_of(N, V) + 2) * N; }
+int64_t adjust_blocks(int32_t N, int32_t V, int32_t L, int32_t K, int eb) {
+  return ((int64_t)V * eb / tile_bytes(N, V, L, K, eb) + 2) * N;
+}
 
 void launch_adjust_logits(const AdjustArgs &a, int dtype, hipStream_t stream) {
   if (dtype == kDtBf16) launch<bf16_t>(a, stream);

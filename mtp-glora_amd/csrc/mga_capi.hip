@@ -1252,7 +1252,7 @@ int mga_adjust_logits(const void *logits, int64_t row_stride, int32_t n_rows, in
   if (!same && overlap(logits, row_stride, out, out_row_stride, n_rows, n_rows, n_cols, eb, eb))
     return fail(MGA_ERR_INVALID, "%s: out overlaps logits", fn);
   // a launch of fewer than 2^32 threads
-  if (mga::adjust_blocks(n_rows, n_cols) >= (int64_t(1) << 24))
+  if (mga::adjust_blocks(n_rows, n_cols, n_tokens, n_bias, eb) >= (int64_t(1) << 24))
     return fail(MGA_ERR_INVALID, "%s: %d rows of %d columns are too many", fn, n_rows, n_cols);
   const mga::AdjustArgs a{logits, row_stride, out, out_row_stride, tokens, tokens_row_stride, lengths, prompt_lengths,
                           repetition, frequency, presence, bias_ids, bias_ids_row_stride, bias, bias_row_stride, allowed,

@@ -272,7 +272,7 @@ struct AdjustArgs {
   int32_t N, V, L, K;
   bool tokens64, bias64;
 };
-int64_t adjust_blocks(int32_t N, int32_t V);   // at most
+int64_t adjust_blocks(int32_t N, int32_t V, int32_t L, int32_t K, int elem_bytes);   // at most
 void launch_adjust_logits(const AdjustArgs &a, int dtype, hipStream_t stream);
 
 // Paged 8-bit cache (mga_paged.hpp): appending with norm and rotation

@@ -82,6 +82,18 @@ def test_many_rows_of_wide_tiles(mga, dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("L,K", [(16383, 1024), (16384, 3), (20, 1025), (40000, 2000)])
+def test_long_lists(mga, dev, dtype, L, K):
+    """Histories and bias lists at and past the narrow form's ends; one token in all of a history."""
+    for V in (50, 3001):
+        a = case(3, V, L, K, dtype, dev, L, True)
+        check(run(mga, a), a)
+        a |= dict(tokens=torch.full((3, L), 17, device=dev), lengths=torch.tensor([L, L, L - 1], device=dev).int(),
+                  prompt_lengths=torch.tensor([0, L, 1], device=dev).int())
+        check(run(mga, a), a)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_settings(mga, dev, dtype):
     base = case(12, 500, 200, 0, dtype, dev, 3)
     check(run(mga, base | dict(repetition=1.3, frequency=0.4, presence=-0.3)), base | dict(repetition=1.3, frequency=0.4,
