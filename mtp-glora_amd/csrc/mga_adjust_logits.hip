@@ -42,10 +42,12 @@ __device__ __forceinline__ float penalised(float x, uint32_t c, const RowSetting
 
 // A tile of TC columns from `base` on, which may begin before column 0 by less than a vector
 // (VEC: vectors of 16 bytes are aligned in x and out alike at base).
-template <typename T, int TC, bool VEC, bool WIDE>
-__global__ __launch_bounds__(256) void adjust_logits_kernel(AdjustArgs a, int tiles) {
+constexpr int NT = 256;   // threads
+
+template <typename T, typename ID, int TC, bool VEC, bool WIDE>
+__global__ __launch_bounds__(NT) void adjust_logits_kernel(AdjustArgs a, int tiles) {
   typedef typename Count<WIDE>::type CT;
-  constexpr int VN = 16 / sizeof(T), BITS = Count<WIDE>::bits, NV = (TC + 256 * VN - 1) / (256 * VN);
+  constexpr int VN = 16 / sizeof(T), BITS = Count<WIDE>::bits, NV = (TC + NT * VN - 1) / (NT * VN);
   constexpr uint32_t kPrompt = 1u << (BITS - 1), kBias = 1u << (BITS - 2);
   // counts; where there are biases, a column's sum (wide) or the entry that holds it, and the list
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -53,8 +55,8 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(AdjustArgs a, int ti
   float *bias = reinterpret_cast<float *>(count + TC);
   uint16_t *owner = reinterpret_cast<uint16_t *>(count + TC);
   int32_t *list_col = reinterpret_cast<int32_t *>(WIDE ? (char *)(bias + TC) : (char *)(owner + TC));
-  float *list_val = reinterpret_cast<float *>(list_col + (WIDE ? 256 : a.K));
-  __shared__ int32_t wave_n[4];
+  float *list_val = reinterpret_cast<float *>(list_col + (WIDE ? NT : a.K));
+  __shared__ int32_t wave_n[NT / 64], twice;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int row = blockIdx.x / tiles, tile = blockIdx.x % tiles;
   const T *x = (const T *)a.x + (int64_t)row * a.xs;
@@ -68,19 +70,22 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(AdjustArgs a, int ti
   if constexpr (VEC) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int i = (k * 256 + tid) * VN, col = base + i;
+      const int i = (k * NT + tid) * VN, col = base + i;
       raw[k] = i32x4{0, 0, 0, 0};
       if (i < TC && col >= 0 && col + VN <= a.V) raw[k] = *reinterpret_cast<const i32x4 *>(x + col);
     }
   }
   // the row's first tokens and biases and what says which count, all in flight before the first wait
   constexpr int TU = 8;
-  int64_t tok[TU];
-  auto load_tokens = [&](int i0) {
+  const ID *tokens = (const ID *)a.tokens + (int64_t)row * a.tokens_rs;
+  ID tok[TU], tnext[TU];
+  auto load_tokens = [&](int i0, ID *tok) {   // of the TU * NT from i0 on every NT-th
+    if (i0 + TU * NT <= a.L) {
 #pragma unroll
-    for (int u = 0; u < TU; ++u) {
-      const int64_t at = (int64_t)row * a.tokens_rs + min(i0 + 256 * u, a.L - 1);
-      tok[u] = a.tokens64 ? ((const int64_t *)a.tokens)[at] : ((const int32_t *)a.tokens)[at];
+      for (int u = 0; u < TU; ++u) tok[u] = tokens[i0 + tid + NT * u];
+    } else {
+#pragma unroll
+      for (int u = 0; u < TU; ++u) tok[u] = tokens[min(i0 + tid + NT * u, a.L - 1)];
     }
   };
   int64_t id = -1;
@@ -92,42 +97,51 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(AdjustArgs a, int ti
     id = a.bias64 ? ((const int64_t *)a.bias_ids)[at] : ((const int32_t *)a.bias_ids)[at];
     val = a.bias[(int64_t)row * a.bias_rs + i];
   };
-  if (a.L > 0) load_tokens(tid);
+  if (a.L > 0) load_tokens(0, tok);
   load_bias(tid);
   const int n = a.lengths ? min(max(a.lengths[row], 0), a.L) : a.L;
   const int m = a.prompts ? min(max(a.prompts[row], 0), n) : 0;
-  for (int i = tid; i < (int)(TC * sizeof(CT) / 16); i += 256) reinterpret_cast<i32x4 *>(count)[i] = i32x4{0, 0, 0, 0};
+  for (int i = tid; i < (int)(TC * sizeof(CT) / 16); i += NT) reinterpret_cast<i32x4 *>(count)[i] = i32x4{0, 0, 0, 0};
   if (WIDE && a.K > 0)
-    for (int i = tid; i < TC; i += 256) bias[i] = 0.f;
+    for (int i = tid; i < TC; i += NT) bias[i] = 0.f;
   RowSettings s{a.repetition ? a.repetition[row] : a.repetition_all, a.frequency ? a.frequency[row] : a.frequency_all,
                 a.presence ? a.presence[row] : a.presence_all};
   if (!(s.r > 0.f)) s.r = 1.f;
+  if (tid == 0) twice = 0;
   __syncthreads();
 
   // two narrow counts share a word: neither can pass its bits, nor reach the other's
   auto shift = [&](int c) { return WIDE ? 0 : 16 * (c & 1); };
   auto word = [&](int c) { return reinterpret_cast<uint32_t *>(count) + (WIDE ? c : c >> 1); };
-  for (int i0 = tid; i0 < n; i0 += 256 * TU) {
-    if (i0 != tid) load_tokens(i0);
+  // a token within the tile: of 64 bits, the high word has to be 0
+  auto within = [&](ID t) {
+    const bool low = (uint32_t)((uint32_t)t - (uint32_t)c0) < (uint32_t)(c1 - c0);
+    if constexpr (sizeof(ID) == 8) return low && (uint32_t)((uint64_t)t >> 32) == 0;
+    else return low;
+  };
+  for (int i0 = 0; i0 < n; i0 += NT * TU) {
+    if (i0 + NT * TU < n) load_tokens(i0 + NT * TU, tnext);
 #pragma unroll
     for (int u = 0; u < TU; ++u) {
-      const int i = i0 + 256 * u;
-      if (i < n && (uint64_t)(tok[u] - c0) < (uint64_t)(c1 - c0)) {
+      const int i = i0 + tid + NT * u;
+      if (within(tok[u]) && i < n) {
         const int c = (int)tok[u] - base;
         if (i < m) atomicOr(word(c), kPrompt << shift(c));
         else atomicAdd(word(c), 1u << shift(c));
       }
     }
+#pragma unroll
+    for (int u = 0; u < TU; ++u) tok[u] = tnext[u];
   }
   int listed = 0;
-  for (int i0 = 0; i0 < a.K; i0 += 256) {
+  for (int i0 = 0; i0 < a.K; i0 += NT) {
     if (i0) load_bias(i0 + tid);
     const bool mine = id >= c0 && id < c1;
     const uint64_t who = __ballot(mine);
     if (lane == 0) wave_n[w] = __popcll(who);
     __syncthreads();
     int at = (WIDE ? 0 : listed) + __popcll(who & lanes_below()), found = 0;
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < NT / 64; ++k) {
       at += k < w ? wave_n[k] : 0;
       found += wave_n[k];
     }
@@ -154,17 +168,21 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(AdjustArgs a, int ti
     }
   }
   if (!WIDE && listed) {
-    // one entry of each column, whichever, adds up all of them in their order
-    for (int t = tid; t < listed; t += 256) owner[list_col[t]] = (uint16_t)t;
+    // one entry of each column, whichever, holds its sum
+    for (int t = tid; t < listed; t += NT) owner[list_col[t]] = (uint16_t)t;
     __syncthreads();
-    for (int t = tid; t < listed; t += 256) {
-      const int c = list_col[t];
-      if (owner[c] != t) continue;
-      float b = 0.f;
+    for (int t = tid; t < listed; t += NT)
+      if (owner[list_col[t]] != t) twice = 1;
+    __syncthreads();
+    if (twice)   // of equal ids, added in their order
+      for (int t = tid; t < listed; t += NT) {
+        const int c = list_col[t];
+        if (owner[c] != t) continue;
+        float b = 0.f;
 #pragma unroll 8
-      for (int k = 0; k < listed; ++k) b += list_col[k] == c ? list_val[k] : 0.f;
-      list_val[t] = b;   // read by no other column's sum
-    }
+        for (int k = 0; k < listed; ++k) b += list_col[k] == c ? list_val[k] : 0.f;
+        list_val[t] = b;   // read by no other column's sum
+      }
   }
   __syncthreads();
 
@@ -183,7 +201,7 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(AdjustArgs a, int ti
   if constexpr (VEC) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int i = (k * 256 + tid) * VN, col = base + i;
+      const int i = (k * NT + tid) * VN, col = base + i;
       if (i >= TC) break;
       if (col >= 0 && col + VN <= a.V) {
         uint32_t bits = ~0u;
@@ -217,13 +235,14 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(AdjustArgs a, int ti
       }
     }
   } else {
-    for (int i = tid; i < c1 - base; i += 256) one(base + i);
+    for (int i = tid; i < c1 - base; i += NT) one(base + i);
   }
 }
 
-// Bytes of a tile's logits: small tiles give few rows more workgroups; past the large ones' 8 KB a row's
-// tokens would be read less often, but reads and writes overlap less (80 rows of 151 936 bf16, 2048 tokens,
-// at 4 / 8 / 16 / 32 KB: 19.4 / 18.7 / 23.0 / 31.3 us).
+// Bytes of a tile's logits. Small tiles give few rows more workgroups; past the large ones' 8 KB a row's
+// tokens would be read less often, but reads and writes overlap less: 80 rows of 151 936 bf16 with 2048 tokens
+// at 8 KB by 256 threads, 16 KB by 512, 32 KB by 1024: 16.9 / 16.6 / 22.5 us; 256 rows of 32 003 fp32 with 4096
+// tokens and 300 biases 29.7 / 32.7 / 41.7 us.
 constexpr int kSmallTile = 2048, kLargeTile = 8192, kWideTile = 8192;
 
 bool wide_form(int32_t L, int32_t K) { return L > kNarrowTokens || K > kListMax; }
@@ -241,16 +260,20 @@ void launch(const AdjustArgs &a, hipStream_t stream) {
   const auto at = [](const void *p) { return reinterpret_cast<uintptr_t>(p) / sizeof(T) % VN; };
   // rows that begin alike within a vector in x and out
   const bool vec = at(a.x) == at(a.out) && (a.N == 1 || a.xs % VN == a.os % VN);
-  auto go = [&](auto bytes, auto v, auto wide) {
+  auto go = [&](auto id, auto bytes, auto v, auto wide) {
     constexpr int TC = decltype(bytes)::value / sizeof(T);
     constexpr bool W = decltype(wide)::value;
     const int tiles = (a.V + (decltype(v)::value ? VN - 1 : 0) + TC - 1) / TC;
-    const int lds = TC * (W ? 4 : 2) + (a.K > 0 ? TC * (W ? 4 : 2) + 8 * (W ? 256 : a.K) : 0);
-    adjust_logits_kernel<T, TC, decltype(v)::value, W><<<(uint32_t)tiles * a.N, 256, lds, stream>>>(a, tiles);
+    const int lds = TC * (W ? 4 : 2) + (a.K > 0 ? TC * (W ? 4 : 2) + 8 * (W ? NT : a.K) : 0);
+    adjust_logits_kernel<T, decltype(id), TC, decltype(v)::value, W><<<(uint32_t)tiles * a.N, NT, lds, stream>>>(a, tiles);
+  };
+  auto go1 = [&](auto bytes, auto v, auto wide) {
+    if (a.tokens64) go(int64_t{}, bytes, v, wide);
+    else go(int32_t{}, bytes, v, wide);
   };
   auto go2 = [&](auto bytes, auto wide) {
-    if (vec) go(bytes, std::true_type{}, wide);
-    else go(bytes, std::false_type{}, wide);
+    if (vec) go1(bytes, std::true_type{}, wide);
+    else go1(bytes, std::false_type{}, wide);
   };
   const int tile = tile_bytes(a.N, a.V, a.L, a.K, sizeof(T));
   if (wide_form(a.L, a.K)) go2(std::integral_constant<int, kWideTile>{}, std::true_type{});
