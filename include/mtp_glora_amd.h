@@ -583,8 +583,8 @@ int mga_paged_append(const void *key, int64_t k_stride_s, int64_t k_stride_h, co
  * Attention of the new tokens over that cache, themselves included (append first):
  *   o_i = sum_j softmax_j(scale q_i . k_j) v_j over the positions j <= lengths[b] + i
  * of the token's sequence that have a page; zeros where there is none. What a row may
- * not see does not reach it, NaN included. Scores, sums and outputs in fp32; P
- * is rounded to bf16 (bf16 queries), or kept to 16 (fp16) or 24 bits (fp32).
+ * not see does not reach it, NaN included. Scores, sums and outputs in fp32; P is
+ * held to 16 bits (fp32 queries: 24; prompts in bf16: 8).
  * q, out: [n_tokens, Hq, head_dim], rows 16-byte aligned; Hq / Hkv <= 32. Rows of
  * out behind cu_tokens[n_seqs]: zeros with zero_rest, else left as they are. workspace:
  * mga_paged_attn_workspace_bytes bytes (0: may be null), 16-byte aligned, one for each call in flight. Sums

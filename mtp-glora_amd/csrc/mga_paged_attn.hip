@@ -25,9 +25,11 @@
 // every lane's partial row sum stays <= 2^20, else the offset moves to the exact
 // maximum and the step is redone from its scores.
 //
-// Precision: scores, statistics and outputs in fp32. bf16 queries: P is rounded to
-// bf16 for its product, the row sum is not. fp16 and fp32 queries are split into 2 or 3
-// bf16 parts and P into as many (K and V are exact in bf16): 16 and 24 bits.
+// Precision: scores, statistics and outputs in fp32; K and V are exact in bf16. fp16 and fp32
+// queries are split into 2 or 3 bf16 parts. P is held in 2 parts (16 bits; fp32: 3, 24 bits) where the
+// cache's bytes bound the kernel and the matrix unit waits for them; a single part's rounding is as
+// large as that of the bf16 output. Prompts with bf16 queries are bound by the matrix unit and take one. The row
+// sum is of the unrounded P.
 //
 // Where a value that a row may not see is NaN (a masked place), its products would be
 // NaN although p = 0: see put_nan.
@@ -40,10 +42,11 @@
 namespace mga {
 namespace {
 
+// bf16 parts of the queries (n), and of the probabilities over a streamed cache (p).
 template <typename T> struct Parts;
-template <> struct Parts<bf16_t> { static constexpr int n = 1; };
-template <> struct Parts<f16_t> { static constexpr int n = 2; };
-template <> struct Parts<float> { static constexpr int n = 3; };
+template <> struct Parts<bf16_t> { static constexpr int n = 1, p = 2; };
+template <> struct Parts<f16_t> { static constexpr int n = 2, p = 2; };
+template <> struct Parts<float> { static constexpr int n = 3, p = 3; };
 
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -298,7 +301,7 @@ struct Stream {
 // One tile's queries and results.
 template <int HD, int NT, typename T, bool UNI>
 struct Rows {
-  static constexpr int NQ = Parts<T>::n, KS = HD / 32, ND = HD / 16;
+  static constexpr int NQ = Parts<T>::n, NP = Parts<T>::p, KS = HD / 32, ND = HD / 16;
   const PagedAttnArgs &a;
   const Tile &x;
   const int col, g;
@@ -376,7 +379,7 @@ struct Rows {
     // this lane's keys: key0 + 4 t + r
     const int key0 = p * 64 + 16 * g;
     const bool edge = p * 64 + 63 > x.q.len + x.tok0 || (UNI ? st.vph < 0 : (bool)__any(st.vph < 0));
-    bf16x8 pf[NT][NQ][2];
+    bf16x8 pf[NT][NP][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       if (edge) {
@@ -415,10 +418,10 @@ struct Rows {
       l[nt] += sum;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        bf16x8 part[NQ];
-        split8<NQ>(e + 8 * c, part);
+        bf16x8 part[NP];
+        split8<NP>(e + 8 * c, part);
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) pf[nt][q][c] = part[q];
+        for (int q = 0; q < NP; ++q) pf[nt][q][c] = part[q];
       }
     }
 
@@ -431,7 +434,7 @@ struct Rows {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) o[nt][d] = mfma16(vf, pf[nt][q][c], o[nt][d]);
+          for (int q = 0; q < NP; ++q) o[nt][d] = mfma16(vf, pf[nt][q][c], o[nt][d]);
         if (d % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
     st.next_v(i + 1);
