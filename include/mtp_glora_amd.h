@@ -568,7 +568,8 @@ int mga_embedding_bwd(const void *grad_out, int64_t grad_out_row_stride, const v
  * query (null: none) likewise in fp32 with q_weight into query_out, rounded once to the dtype;
  * its rows behind cu_tokens[n_seqs] are zeros. cos, sin [n_tokens, head_dim] in the dtype, or fp32
  * with cos_sin_f32. Rows behind a sequence's end in its last page, and all other pages,
- * stay as they are. n_seqs <= 4096; head_dim 64 or 128. Beside mga_kv_append and
+ * stay as they are. n_seqs <= 4096; head_dim 64 or 128; table_width * page_size + n_tokens and
+ * num_pages * Hkv <= 2^30. Beside mga_kv_append and
  * mga_qk_norm_rope_stage_fwd (mtp_glora/models/modeling_qwen3.py:274-284).
  */
 int mga_paged_append(const void *key, int64_t k_stride_s, int64_t k_stride_h, const void *value, int64_t v_stride_s,
@@ -585,7 +586,8 @@ int mga_paged_append(const void *key, int64_t k_stride_s, int64_t k_stride_h, co
  * of the token's sequence that have a page; zeros where there is none. What a row may
  * not see does not reach it, NaN included. Scores, sums and outputs in fp32; P is
  * held to 16 bits (fp32 queries: 24; prompts in bf16: 8).
- * q, out: [n_tokens, Hq, head_dim], rows 16-byte aligned; Hq / Hkv <= 32. Rows of
+ * q, out: [n_tokens, Hq, head_dim], rows 16-byte aligned; out may be q itself (the same strides), else may
+ * not overlap it; Hq / Hkv <= 32. Rows of
  * out behind cu_tokens[n_seqs]: zeros with zero_rest, else left as they are. workspace:
  * mga_paged_attn_workspace_bytes bytes (0: may be null), 16-byte aligned, one for each call in flight. Sums
  * run in a fixed order. Beside mga_attn_fwd ([tf]integrations/flex_attention.py:262-368).
@@ -613,7 +615,8 @@ int mga_paged_attn(const void *q, int64_t q_stride_s, int64_t q_stride_h, const 
  * [0, n_cols) do not count. lengths null: n_tokens; prompt_lengths null: 0.
  * repetition, frequency, presence: one value a row in device memory, or null for the
  * *_all value; a repetition that is not positive counts as 1. out may be logits itself (the same
- * rows), else may not overlap it. n_cols <= 2^30, n_rows < 2^22. No counterpart in the reference.
+ * rows), else may not overlap it. n_cols <= 2^30, n_rows < 2^22, n_tokens and n_bias < 2^30.
+ * No counterpart in the reference.
  */
 int mga_adjust_logits(const void *logits, int64_t row_stride, int32_t n_rows, int32_t n_cols, int32_t dtype,
                       const void *tokens, int32_t tokens_are_int64, int64_t tokens_row_stride, int32_t n_tokens,

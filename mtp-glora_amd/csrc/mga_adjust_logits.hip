@@ -5,7 +5,9 @@
 //   y -= f * count + (count > 0 ? p : 0), count over the output;
 //   y += biases;  not allowed: y = -inf
 //
-// Bounded by HBM: each logit is read and written once. A workgroup takes a tile of one row's columns.
+// Bounded by HBM: each logit is read and written once (80 rows of 151 936 bf16: 8.3 us without lists, a copy 7.9;
+// with 2048 tokens a row, 8 biases and a mask 16.8: the tiles' turns over the tokens). A workgroup takes a tile of
+// one row's columns.
 // While the tile's logits are on their way it counts the row's tokens that fall into it in LDS: a count of the
 // output's in the low bits, a bit for the prompt's, a bit for columns with a bias (integer adds, so
 // their order does not matter). Every tile reads the row's tokens, from L2, which asks for wide

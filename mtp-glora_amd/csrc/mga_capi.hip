@@ -1114,6 +1114,8 @@ int check_paged(const char *fn, const PagedCall &c) {
   // positions are 32-bit numbers
   if ((int64_t)c.width * c.page_size + c.T > (int64_t(1) << 30))
     return fail(MGA_ERR_INVALID, "%s: sequences of %lld tokens are too long", fn, (long long)c.width * c.page_size + c.T);
+  if ((int64_t)c.num_pages * c.Hkv > (int64_t(1) << 30))
+    return fail(MGA_ERR_INVALID, "%s: %d pages of %d heads are too many", fn, c.num_pages, c.Hkv);
   if (!c.k_pages || !c.v_pages || !aligned16(c.k_pages) || !aligned16(c.v_pages))
     return fail(MGA_ERR_INVALID, "%s: pages null or not 16-byte aligned", fn);
   if (!c.k_scale || !c.v_scale || !c.table || !c.cu || !c.lengths)
@@ -1130,6 +1132,19 @@ int check_token_rows(const char *fn, const char *name, const void *p, int64_t ss
   if (reinterpret_cast<uintptr_t>(p) % eb) return fail(MGA_ERR_INVALID, "%s: %s is not aligned to its elements", fn, name);
   *vec = *vec && aligned16(p) && ss * eb % 16 == 0 && hs * eb % 16 == 0;
   return MGA_OK;
+}
+
+// May [tokens, heads, head_dim] operands p and q share an element? Not where their tokens lie side by
+// side in rows of one buffer.
+bool token_rows_overlap(const void *p, int64_t pss, int64_t phs, const void *q, int64_t qss, int64_t qhs, int32_t T,
+                        int32_t heads, int32_t D, int eb) {
+  const int64_t pw = (heads - 1) * phs + D, qw = (heads - 1) * qhs + D;   // of a token
+  const uint64_t p0 = reinterpret_cast<uintptr_t>(p) / eb, q0 = reinterpret_cast<uintptr_t>(q) / eb;
+  if (p0 >= q0 + (T - 1) * qss + qw || q0 >= p0 + (T - 1) * pss + pw) return false;
+  if (pss != qss || pss == 0) return true;
+  const int64_t d = (int64_t)((p0 > q0 ? p0 - q0 : q0 - p0) % (uint64_t)pss);
+  const int64_t low = p0 > q0 ? qw : pw, high = p0 > q0 ? pw : qw;
+  return d < low || pss - d < high;
 }
 
 }  // namespace
@@ -1201,6 +1216,9 @@ int mga_paged_attn(const void *q, int64_t q_stride_s, int64_t q_stride_h, const 
       (rc = check_token_rows(fn, "out", out, o_stride_s, o_stride_h, eb, &vec)) != MGA_OK)
     return rc;
   if (!vec) return fail(MGA_ERR_INVALID, "%s: rows of q and out must be 16-byte aligned", fn);
+  const bool same = q == out && q_stride_s == o_stride_s && q_stride_h == o_stride_h;
+  if (!same && token_rows_overlap(q, q_stride_s, q_stride_h, out, o_stride_s, o_stride_h, n_tokens, Hq, head_dim, eb))
+    return fail(MGA_ERR_INVALID, "%s: out overlaps q", fn);
   float *ws = nullptr;
   const int64_t need = mga::paged_attn_ws_bytes(n_tokens, n_seqs, Hq, Hkv, head_dim, (int64_t)page_size * table_width, dtype);
   if (need && !workspace) return fail(MGA_ERR_INVALID, "%s: null workspace", fn);
@@ -1209,8 +1227,9 @@ int mga_paged_attn(const void *q, int64_t q_stride_s, int64_t q_stride_h, const 
                              v_scale, block_table, table_row_stride, cu_tokens, lengths, out, o_stride_s, o_stride_h, ws,
                              scale * mga::kLog2e, n_tokens, n_seqs, Hq, Hkv, num_pages, paged_shift(page_size),
                              table_width, zero_rest != 0};
-  // the list of steps is counted in 32 bits
-  if (mga::paged_attn_steps(a, dtype) >= (int64_t(1) << 31))
+  // a launch of fewer than 2^32 threads, a list of at most 2^30 steps
+  const int64_t tiles = mga::paged_attn_tiles(a, dtype), steps = ((int64_t)table_width * page_size + n_tokens + 63) / 64 + 1;
+  if (tiles >= (int64_t(1) << 23) || tiles * steps > (int64_t(1) << 30))
     return fail(MGA_ERR_INVALID, "%s: %d tokens over sequences of %lld are too many", fn, n_tokens,
                 (long long)table_width * page_size);
   mga::launch_paged_attn(a, head_dim, dtype, (hipStream_t)stream);
@@ -1230,8 +1249,8 @@ int mga_adjust_logits(const void *logits, int64_t row_stride, int32_t n_rows, in
   if (rc == MGA_OK) rc = check_matrix(fn, "out", out, out_row_stride, n_rows, n_cols, dtype);
   if (rc != MGA_OK) return rc;
   if (n_cols > (1 << 30)) return fail(MGA_ERR_INVALID, "%s: %d columns (at most 2^30)", fn, n_cols);
-  if (n_tokens < 0 || n_bias < 0)
-    return fail(MGA_ERR_INVALID, "%s: bad sizes (tokens=%d biases=%d)", fn, n_tokens, n_bias);
+  if (n_tokens < 0 || n_tokens >= (1 << 30) || n_bias < 0 || n_bias >= (1 << 30))
+    return fail(MGA_ERR_INVALID, "%s: bad sizes (tokens=%d biases=%d, below 2^30)", fn, n_tokens, n_bias);
   // rows of a list, one for all rows with a stride of 0
   const auto list = [&](const char *name, const void *p, int64_t rs, int32_t n, int eb) {
     if (n == 0) return (int)MGA_OK;

@@ -308,8 +308,8 @@ struct PagedAttnArgs {
 };
 // keys: the most that a sequence's row of the table holds
 int64_t paged_attn_ws_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int head_dim, int64_t keys, int dtype);
-// an upper bound of the 64-key steps of a call
-int64_t paged_attn_steps(const PagedAttnArgs &a, int dtype);
+// an upper bound of a call's tiles: workgroups of up to 512 threads, and of steps
+int64_t paged_attn_tiles(const PagedAttnArgs &a, int dtype);
 void launch_paged_attn(const PagedAttnArgs &a, int head_dim, int dtype, hipStream_t stream);
 
 // Compute units of the current device (queried once per device).

@@ -5,15 +5,26 @@
 // Work. A tile is up to 16 NT query rows of one sequence and KV head: TM tokens (a
 // power of two) times the G query heads of the group. It visits the cache in steps
 // of 64 keys. The steps of all tiles, sequences and heads form one list, cut into
-// equal shares, one a workgroup: ragged batches and few long sequences fill the chip
+// equal shares, one a wave: ragged batches and few long sequences fill the chip
 // alike. A tile that a cut goes through leaves fp32 partial results (at most two
-// a workgroup), joined in a fixed order by a second launch. Each workgroup finds its
-// share from the lengths on the device (a scan over the sequences; a tile's place
+// a wave), joined in a fixed order by a second launch. Each workgroup finds its
+// shares from the lengths on the device (a scan over the sequences; a tile's place
 // within its sequence has a closed form, as TM divides 64), so the launch depends on
-// no length and can be captured.
+// no length and can be captured. The K and V loads run one step ahead and on across
+// the tiles of a share.
 //
-// Step. Each of the 4 waves takes every fourth step of the share and keeps its own
-// running maximum, sum and output; they meet in LDS at the tile's end. K and V go from
+// Bounds and times (32 / 8 heads of 128, bf16, pages of 64). Few rows: HBM. A plain read of as many
+// bytes in this pattern reaches 5.85 TB/s here. 64 sequences of 177 385 tokens in all, a token each
+// (364 MB): 76 us + 5 us joining, 4.5 TB/s; 2 of 212 590 (435 MB): 82 + 6 us, 4.9 TB/s; what is left is
+// the start (cu, lengths, pages, first keys: 4 us), the join's launch, and waves that end up to 15% apart
+// with equal shares. Prompts: the matrix unit and the softmax's vector work beside it: 10 075 new
+// tokens behind up to 15 399, 1175 GFLOP visible, 1.25 ms, 940 TFLOP/s.
+//
+// Three forms share this: few rows a sequence over long ones by equal shares (paged_share_kernel), short
+// sequences by a workgroup a tile (paged_tile_kernel), prompts by 128 rows (paged_prompt_kernel, further
+// below).
+//
+// Step. A wave keeps its own running maximum, sum and output. K and V go from
 // memory to registers to the matrix unit, 16 bytes a lane, with nothing in between
 // but the conversion of two codes an instruction, under the page's scale, to bf16
 // (exact). S^T = K Q^T by v_mfma_f32_16x16x32_bf16: key m of tile t of the step is key
@@ -525,6 +536,10 @@ __device__ __forceinline__ int share_begin(int me, int workers, int total) {
   return me >= w ? total : (int)((int64_t)me * total / w);
 }
 
+// Most steps of a call. The sums stop there, so that they do not wrap for a cu_tokens that goes
+// down, whose sequences overlap.
+constexpr int kMaxSteps = 1 << 30;
+
 // Inclusive sums of the sequences' steps (all heads) and the sequences themselves in LDS;
 // returns the total.
 __device__ __forceinline__ int scan_steps(const PagedAttnArgs &a, int tmshift, int32_t *pre, SeqSpan *seqs,
@@ -536,21 +551,21 @@ __device__ __forceinline__ int scan_steps(const PagedAttnArgs &a, int tmshift, i
     int s = 0;
     if (b < a.B) {
       const SeqSpan q = seq_span(a.cu, a.lengths, b, a.T, a.width << a.pshift);
-      s = (int)(SeqTiles{q.n, q.len, tmshift}.all() * a.Hkv);
+      s = (int)min(SeqTiles{q.n, q.len, tmshift}.all() * a.Hkv, (int64_t)kMaxSteps);
       seqs[b] = q;
     }
     for (int m = 1; m < 64; m <<= 1) {
       const int o = __shfl_up(s, m, 64);
-      s += lane >= m ? o : 0;
+      s = min(s + (lane >= m ? o : 0), kMaxSteps);
     }
     if (lane == 63) wave_sum[w] = s;
     __syncthreads();
     int add = carry;
     for (int i = 0; i < 4; ++i) {
-      add += i < w ? wave_sum[i] : 0;
-      carry += wave_sum[i];
+      add = min(add + (i < w ? wave_sum[i] : 0), kMaxSteps);
+      carry = min(carry + wave_sum[i], kMaxSteps);
     }
-    if (b < a.B) pre[b] = s + add;
+    if (b < a.B) pre[b] = min(s + add, kMaxSteps);
     __syncthreads();
   }
   return carry;
@@ -588,7 +603,8 @@ __device__ __forceinline__ Place locate(const PagedAttnArgs &a, int tmshift, con
 }
 
 template <int HD, int NT, typename T, bool UNI>
-__global__ __launch_bounds__(256, share_occupancy(NT, Parts<T>::n)) void paged_share_kernel(PagedAttnArgs a, int tmshift, int G) {
+__global__ __launch_bounds__(256, share_occupancy(NT, Parts<T>::n)) void paged_share_kernel(PagedAttnArgs a, int tmshift,
+                                                                                            int G) {
   constexpr int ND = HD / 16, ROWS = 16 * NT;
   __shared__ int32_t pre[kMaxSeqs];
   __shared__ SeqSpan seqs[kMaxSeqs];
@@ -740,7 +756,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int tm
 template <int HD, int NT, typename T, bool UNI, int NW>
 __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttnArgs a, int tmshift, int G) {
   constexpr int ND = HD / 16;
-  __shared__ float om[NW][16][HD + 4];
+  __shared__ __attribute__((aligned(16))) float om[NW][16][HD + 4];
   __shared__ float ml[NW][2][16];
   const int tid = threadIdx.x, lane = tid & 63, w = wave_id(), col = lane & 15, g = lane >> 4;
   const int slot = blockIdx.x / a.Hkv;
@@ -804,13 +820,14 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttnArgs a, in
 constexpr int kPromptRows = 128;
 
 template <int HD, typename T, bool UNI>
-__global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_kernel(PagedAttnArgs a, int tmshift, int G, int slots) {
+__global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_kernel(PagedAttnArgs a, int tmshift, int G,
+                                                                                     int slots) {
   constexpr int NQ = Parts<T>::n, KS = HD / 16, DT = HD / 32;
   constexpr int NL = HD / 64;            // 16-byte loads a thread and step, for keys and for values
   constexpr int VR = 256 / HD;           // threads a value row
   __shared__ __attribute__((aligned(16))) bf16_t kt[2][64 * HD];
   __shared__ __attribute__((aligned(16))) bf16_t vt[2][HD * 64];
-  __shared__ int there[2][4];            // whether a 16-key group has a page
+  __shared__ __attribute__((aligned(16))) int there[2][4];   // whether a 16-key group has a page
   __shared__ int nan_step;               // the first edge step with a NaN among its values
   const int tid = threadIdx.x, lane = tid & 63, w = wave_id(), l32 = lane & 31, hi = lane >> 5;
   const int PS = 1 << a.pshift;
@@ -1089,7 +1106,8 @@ struct Shape {
   int NT, tmshift, nwg;
 };
 
-// Keys up to which a sequence is one workgroup's.
+// Keys up to which a sequence is one workgroup's: 1 x 1 token, 32 / 8 heads of 128, over 1000 keys 10.4 us in
+// one launch, 12.4 by shares; a CU's rate bounds it from there (20 ns a key).
 constexpr int kShortKeys = 1024;
 
 // The narrowest tile that holds an average sequence's query rows: a wide one's empty
@@ -1098,7 +1116,9 @@ Shape shape_of(int T, int B, int Hq, int Hkv, int64_t keys, int dtype) {
   const int G = Hq / Hkv;
   const int64_t rows = ((int64_t)T * G + B - 1) / B;
   const int NT = rows <= 16 && G <= 16 ? 1 : 2, parts = dtype == kDtBf16 ? 1 : dtype == kDtF16 ? 2 : 3;
-  // prompts by 128 rows where those tiles fill the chip
+  // prompts by 128 rows where those tiles fill the chip: 32 / 8 heads of 128, shares / prompts, behind 2000
+  // and 30 000 cached tokens: 1 x 512 new tokens (136 tiles) 63 / 62 and 535 / 645 us, 4 x 128 (160) 62 / 55
+  // and 562 / 644, 4 x 256 (288) 106 / 69 and 1097 / 802, 4 x 512 (544) 194 / 92 and 2131 / 988
   const int pm = tm_shift(kPromptRows, G, 7);
   if (rows >= kPromptRows / 2 && (int64_t)tile_slots(T, B, pm) * Hkv >= device_cu_count())
     return {kPrompts, 0, pm, 0};
@@ -1150,10 +1170,9 @@ int64_t paged_attn_ws_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int h
          (int64_t)tile_slots(T, B, s.tmshift) * Hkv * sizeof(JoinNote);
 }
 
-int64_t paged_attn_steps(const PagedAttnArgs &a, int dtype) {
-  const int64_t keys = (int64_t)a.width << a.pshift;
-  const Shape s = shape_of(a.T, a.B, a.Hq, a.Hkv, keys, dtype);
-  return (int64_t)tile_slots(a.T, a.B, s.tmshift) * a.Hkv * ((keys + a.T + 63) / 64 + 1);
+int64_t paged_attn_tiles(const PagedAttnArgs &a, int dtype) {
+  const Shape s = shape_of(a.T, a.B, a.Hq, a.Hkv, (int64_t)a.width << a.pshift, dtype);
+  return (int64_t)tile_slots(a.T, a.B, s.tmshift) * a.Hkv;
 }
 
 void launch_paged_attn(const PagedAttnArgs &a, int head_dim, int dtype, hipStream_t stream) {

@@ -177,7 +177,8 @@ def paged_attention(query: torch.Tensor, pages, block_table: torch.Tensor, cu_to
     ``pages`` (KVPages): token i of a sequence sees positions 0 .. lengths + i, its own
     included, so append first, with the same table, cu_tokens and lengths. Query head h
     reads KV head h // (Hq / Hkv). Positions without a page are masked; a row that sees
-    nothing is zeros. Scores and softmax in fp32. ``out`` receives the result; its rows
+    nothing is zeros. Scores and softmax in fp32. ``out`` (``query`` itself, or
+    rows that do not overlap it) receives the result; its rows
     behind the last sequence's tokens stay as they are, in a tensor made here they are
     zeros. Hq / Hkv <= 32, at most 4096 sequences."""
     _no_grad("paged_attention", query)
@@ -249,7 +250,9 @@ class PagedKVCache:
         return self._layers[layer_idx]
 
     def begin(self, block_table: torch.Tensor, cu_tokens: torch.Tensor, lengths: torch.Tensor) -> None:
-        """The batch of the appends and attentions that follow."""
+        """The batch of the appends and attentions that follow. The tensors are held, not
+        copied, if they are contiguous (a table's rows may lie apart): what is written to
+        them later, counts; a graph that begins outside its capture needs them so."""
         self._batch = _batch(block_table, cu_tokens, lengths, self._layers[0].k.device)
 
     def _step(self):

@@ -11,7 +11,7 @@ P = ctypes.c_void_p(64)
 @pytest.mark.parametrize("kw", [dict(x=None), dict(rs=99), dict(n=0), dict(v=0), dict(dtype=3), dict(n=1 << 22),
                                 dict(v=(1 << 30) + 1, rs=1 << 31, ors=1 << 31), dict(x=ctypes.c_void_p(65)), dict(out=None),
                                 dict(ors=99), dict(tokens=None), dict(tokens=ctypes.c_void_p(68)), dict(trs=3), dict(L=-1),
-                                dict(K=-1), dict(bias_ids=None), dict(bias=None), dict(bias=ctypes.c_void_p(66)), dict(brs=2),
+                                dict(L=1 << 30, trs=1 << 31), dict(K=-1), dict(bias_ids=None), dict(bias=None), dict(bias=ctypes.c_void_p(66)), dict(brs=2),
                                 dict(vrs=2), dict(allowed=ctypes.c_void_p(66)), dict(ars=3), dict(r=0.0), dict(r=-1.0),
                                 dict(r=float("nan")), dict(r=float("inf")), dict(out=ctypes.c_void_p(66)),
                                 dict(out=ctypes.c_void_p(64 + 2 * 199)), dict(out=P, ors=101),

@@ -178,6 +178,37 @@ def test_attention_prompts_with_holes_and_nan(mga, dev, dtype, D, ps):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ps", [16, 32, 64, 128])
+def test_attention_many_long_sequences(mga, dev, dtype, ps):
+    """Sequences that share their pages, of so many keys that every wave visits more steps than
+    it holds pages for at once: 48 times the same three."""
+    pool = Pool(dev, [1, 1, 1], [10000, 6999, 9990], 8, 64, ps, seed=2, scales=(-6, -2))
+    q = queries(pool, 16, 64, dtype, dev)
+    n = 48
+    one = torch.arange(3 * n + 1, dtype=torch.int32, device=dev)
+    got = mga.paged_attention(q.repeat(n, 1, 1), pool.pages, pool.table.repeat(n, 1), one, pool.len.repeat(n), 0.125)
+    got = got.view(n, 3, 16, 64)
+    for x in (got.amin(0), got.amax(0)):
+        check_attention(x, q, pool, 0.125)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ps", [16, 32, 64, 128])
+def test_attention_prompts_behind_long_sequences(mga, dev, dtype, ps):
+    """Prompts that visit more steps than the lanes hold pages for at once."""
+    pool = Pool(dev, [1000, 900, 200], [4200, 100, 8300], 8, 64, ps, seed=2)
+    q = queries(pool, 16, 64, dtype, dev)
+    got = attend(mga, pool, q)
+    for i in (0, 1, 2):   # the oracle for some rows of each: as sequences of their own
+        first, n, c = int(pool.cu[i]), [1000, 900, 200][i], [4200, 100, 8300][i]
+        at = torch.tensor([0, 1, 63, 64, n // 2, n - 2, n - 1], device=dev)
+        some = pool.clone()
+        some.table = pool.table[i:i + 1].repeat(7, 1)
+        some.cu, some.len, some.T = torch.arange(8, dtype=torch.int32, device=dev), (c + at).int(), 7
+        check_attention(got[first + at], q[first + at], some, 0.125)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_many_sequences(mga, dev, dtype):
     """More sequences than threads of a workgroup, some without tokens."""
     new = [i % 3 for i in range(700)]
@@ -401,6 +432,21 @@ def test_append_batches(mga, dev, dtype, Hq, Hkv, D, ps):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_append_few_tokens_on_average(mga, dev, dtype, D):
+    """Batches of few tokens a sequence, with sequences of many or none, and many sequences."""
+    many = [i % 3 for i in range(200)]
+    for i, (new, cached) in enumerate([([30, 1, 1, 1, 1, 1, 1], [7, 64, 15, 0, 31, 100, 3]), (many, [(i * 29) % 70 for i in range(200)]),
+                                       ([0, 0, 9, 0], [3, 16, 40, 0]), ([0, 1] * 40, [47] * 80)]):
+        for ps in (16, 64):
+            pool = Pool(dev, new, cached, 2, D, ps, seed=i, scales=(-14, -9))   # scales that have to grow
+            T = pool.T
+            q, k, v = (rows(T, h, D, dtype, dev, h + i) for h in (4, 2, 2))
+            cos, sin = tables(T, D, dtype, dev)
+            run_append(mga, pool, q, k, v, kw=(1 + 0.3 * torch.randn(D, device=dev)).to(dtype), cos=cos, sin=sin)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_append_token_by_token(mga, dev, dtype):
     """A scale that grows, stays, and begins anew with a page."""
     pool = Pool(dev, [1], [39], 1, 64, 16, seed=2, scales=(-14, -12))
@@ -490,6 +536,35 @@ def test_native_and_python_forms(mga, dev, dtype, monkeypatch):
         runs.append((e, attend(mga, pool, e), pool.k, pool.v, pool.ks, pool.vs))
     for a, b in zip(*runs):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("new,cached", [([3, 2], [90, 10]), ([3, 1], [3000, 700]), ([700, 900], [90, 0])])
+def test_attention_in_place(mga, dev, new, cached):
+    """out may be the query, or lie beside it in the rows of one buffer."""
+    pool = Pool(dev, new, cached, 8, 64, 64, scales=(-6, -2))
+    wide = torch.zeros(pool.T, 40, 64, dtype=torch.bfloat16, device=dev)
+    wide[:, :16] = q = queries(pool, 16, 64, torch.bfloat16, dev)
+    want = attend(mga, pool, q)
+    assert torch.equal(attend(mga, pool, wide[:, :16], out=wide[:, 16:32]), want)
+    assert torch.equal(wide[:, :16], q) and not wide[:, 32:].any()
+    attend(mga, pool, q, out=q)
+    assert torch.equal(q, want)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        attend(mga, pool, wide[:, 8:24], out=wide[:, 16:32])
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_inference_mode(mga, dev, native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(mga._lib, "native", lambda *a: None)
+    with torch.inference_mode():
+        pool = Pool(dev, [2, 3], [10, 20], 2, 64, 16)
+        x, q = rows(5, 2, 64, torch.bfloat16, dev, 1), rows(5, 4, 64, torch.bfloat16, dev, 2)
+        e = mga.paged_append(x, x, pool.pages, *pool.batch, query=q)
+        assert attend(mga, pool, e).shape == q.shape
+        logits = torch.randn(3, 50, device=dev)
+        assert torch.equal(mga.adjust_logits(logits, torch.zeros(3, 1, dtype=torch.long, device=dev), presence=1.0, out=logits),
+                           logits)
 
 
 def test_refusals(mga, dev):

@@ -16,7 +16,8 @@ def refused(mga, rc, text=b""):
 
 PAGED = [dict(T=-1), dict(B=0), dict(B=4097), dict(D=96), dict(Hq=3), dict(Hkv=0), dict(dtype=3), dict(ps=48),
          dict(ps=256), dict(n=0), dict(width=0), dict(trs=3), dict(width=1 << 25, trs=1 << 25), dict(kp=None), dict(vp=None),
-         dict(kp=ctypes.c_void_p(72)), dict(ks=None), dict(vs=None), dict(table=None), dict(cu=None), dict(lens=None)]
+         dict(kp=ctypes.c_void_p(72)), dict(ks=None), dict(vs=None), dict(table=None), dict(cu=None), dict(lens=None),
+         dict(n=1 << 30)]
 
 
 LONG = dict(width=1000, trs=1000)   # sequences that need a workspace
@@ -25,7 +26,7 @@ LONG = dict(width=1000, trs=1000)   # sequences that need a workspace
 def _args(**kw):
     a = dict(k=P, ss=256, hs=128, v=P, q=P, qw=None, kw=None, cos=None, sin=None, cs=128, c32=0, eps=1e-6, T=2, B=1, Hq=4,
              Hkv=2, D=128, dtype=0, kp=P, vp=P, ks=P, vs=P, n=4, ps=64, table=P, trs=4, width=4, cu=P, lens=P, qo=P,
-             scale=0.1, out=P, ws=P, nb=1 << 40)
+             scale=0.1, out=ctypes.c_void_p(1 << 20), ws=P, nb=1 << 40)
     a.update(kw)
     return a
 
@@ -59,6 +60,13 @@ def test_append(mga, kw):
                                         LONG | dict(ws=ctypes.c_void_p(72)), dict(T=1 << 28, width=1 << 22, trs=1 << 22)])
 def test_attend(mga, kw):
     refused(mga, _attend(mga.load_library(), **kw))
+
+
+# q: 2 tokens of 4 heads of 128 bf16 at 64, strides 256 and 128
+@pytest.mark.parametrize("kw", [dict(out=P), dict(out=ctypes.c_void_p(64 + 16)), dict(out=ctypes.c_void_p(64 + 1024)),
+                                dict(q=ctypes.c_void_p(64 + 1536), out=P, ss=512), dict(ss=512, out=ctypes.c_void_p(64 + 16))])
+def test_attend_out_overlaps_q(mga, kw):
+    refused(mga, _attend(mga.load_library(), **kw), b"overlaps")
 
 
 def test_no_tokens(mga):
