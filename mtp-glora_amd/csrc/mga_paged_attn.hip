@@ -518,8 +518,9 @@ __device__ __forceinline__ void zero_rest(const PagedAttnArgs &a) {
 
 // ---- equal shares of all steps, a wave each ----------------------------------------
 
-// Workgroups a CU: what the registers of a wave allow.
-constexpr int share_occupancy(int NT, int parts) { return NT == 1 && parts < 3 ? 2 : 1; }
+// Workgroups a CU: what the registers of a wave allow (2 x 5 tokens over 220 000, 32 / 8 heads of 64, bf16: one 65
+// us, two 55; heads of 128 by two would spill: 33 and 44 us for 16 x 5 tokens over 47 000).
+constexpr int share_occupancy(int HD, int NT, int parts) { return (NT == 1 || HD == 64) && parts < 3 ? 2 : 1; }
 
 // Partial results of a worker's first (0) and last (1) tile: rows of HD values, then (max, sum) pairs.
 __host__ __device__ __forceinline__ int64_t slot_floats(int rows, int HD) { return (int64_t)rows * (HD + 2); }
@@ -603,7 +604,7 @@ __device__ __forceinline__ Place locate(const PagedAttnArgs &a, int tmshift, con
 }
 
 template <int HD, int NT, typename T, bool UNI>
-__global__ __launch_bounds__(256, share_occupancy(NT, Parts<T>::n)) void paged_share_kernel(PagedAttnArgs a, int tmshift,
+__global__ __launch_bounds__(256, share_occupancy(HD, NT, Parts<T>::n)) void paged_share_kernel(PagedAttnArgs a, int tmshift,
                                                                                             int G) {
   constexpr int ND = HD / 16, ROWS = 16 * NT;
   __shared__ int32_t pre[kMaxSeqs];
@@ -645,6 +646,10 @@ __global__ __launch_bounds__(256, share_occupancy(NT, Parts<T>::n)) void paged_s
         if (p1 == x.steps) note.last = me;
       }
       Rows<HD, NT, T, UNI> rows(a, x, G);
+      // here for the queries and all before them: left to their first use, the wait would be in every step and
+      // drain the values in flight (64 tokens over 177 385: 80.6 us, 82.2 without). With one wave a SIMD, which
+      // its own instructions bound, it takes 114 us without and 119 with it (64 x 5 tokens over 197 000)
+      if constexpr (share_occupancy(HD, NT, Parts<T>::n) == 2) __builtin_amdgcn_s_waitcnt(wait_vm(0));
       for (int p = p0; p < p1; ++p, ++i) rows.step(st, i, p, find);
       // the next tile, whose first step's page is held by now
       nb = st.step_of(tb, i);
@@ -1112,7 +1117,7 @@ constexpr int kShortKeys = 1024;
 
 // The narrowest tile that holds an average sequence's query rows: a wide one's empty
 // columns cost matrix work only, a narrow one reads the cache once more a tile.
-Shape shape_of(int T, int B, int Hq, int Hkv, int64_t keys, int dtype) {
+Shape shape_of(int T, int B, int Hq, int Hkv, int HD, int64_t keys, int dtype) {
   const int G = Hq / Hkv;
   const int64_t rows = ((int64_t)T * G + B - 1) / B;
   const int NT = rows <= 16 && G <= 16 ? 1 : 2, parts = dtype == kDtBf16 ? 1 : dtype == kDtF16 ? 2 : 3;
@@ -1122,7 +1127,8 @@ Shape shape_of(int T, int B, int Hq, int Hkv, int64_t keys, int dtype) {
   const int pm = tm_shift(kPromptRows, G, 7);
   if (rows >= kPromptRows / 2 && (int64_t)tile_slots(T, B, pm) * Hkv >= device_cu_count())
     return {kPrompts, 0, pm, 0};
-  return {keys <= kShortKeys ? kTiles : kShares, NT, tm_shift(16 * NT, G), share_occupancy(NT, parts) * device_cu_count()};
+  return {keys <= kShortKeys ? kTiles : kShares, NT, tm_shift(16 * NT, G),
+          share_occupancy(HD, NT, parts) * device_cu_count()};
 }
 
 template <int HD, int NT, typename T, bool UNI>
@@ -1164,19 +1170,19 @@ void launch1(const PagedAttnArgs &a, const Shape &s, hipStream_t stream) {
 }  // namespace
 
 int64_t paged_attn_ws_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int head_dim, int64_t keys, int dtype) {
-  const Shape s = shape_of(T, B, Hq, Hkv, keys, dtype);
+  const Shape s = shape_of(T, B, Hq, Hkv, head_dim, keys, dtype);
   if (s.mode != kShares) return 0;
   return (int64_t)s.nwg * 4 * 2 * slot_floats(16 * s.NT, head_dim) * 4 +
          (int64_t)tile_slots(T, B, s.tmshift) * Hkv * sizeof(JoinNote);
 }
 
 int64_t paged_attn_tiles(const PagedAttnArgs &a, int dtype) {
-  const Shape s = shape_of(a.T, a.B, a.Hq, a.Hkv, (int64_t)a.width << a.pshift, dtype);
+  const Shape s = shape_of(a.T, a.B, a.Hq, a.Hkv, 128, (int64_t)a.width << a.pshift, dtype);   // of any head_dim
   return (int64_t)tile_slots(a.T, a.B, s.tmshift) * a.Hkv;
 }
 
 void launch_paged_attn(const PagedAttnArgs &a, int head_dim, int dtype, hipStream_t stream) {
-  const Shape s = shape_of(a.T, a.B, a.Hq, a.Hkv, (int64_t)a.width << a.pshift, dtype);
+  const Shape s = shape_of(a.T, a.B, a.Hq, a.Hkv, head_dim, (int64_t)a.width << a.pshift, dtype);
   if (head_dim == 128) {
     if (dtype == kDtBf16) launch1<128, bf16_t>(a, s, stream);
     else if (dtype == kDtF16) launch1<128, f16_t>(a, s, stream);
