@@ -15,7 +15,7 @@
 //
 // Bounds and times (32 / 8 heads of 128, bf16, pages of 64). Few rows: HBM. A plain read of as many
 // bytes in this pattern reaches 5.85 TB/s here. 64 sequences of 177 385 tokens in all, a token each
-// (364 MB): 76 us + 5 us joining, 4.5 TB/s; 2 of 212 590 (435 MB): 82 + 6 us, 4.9 TB/s; what is left is
+// (364 MB): 75 us + 5 us joining, 4.5 TB/s; 2 of 212 590 (435 MB): 81 + 7 us, 4.9 TB/s; what is left is
 // the start (cu, lengths, pages, first keys: 4 us), the join's launch, and waves that end up to 15% apart
 // with equal shares. Prompts: the matrix unit and the softmax's vector work beside it: 10 075 new
 // tokens behind up to 15 399, 1175 GFLOP visible, 1.25 ms, 940 TFLOP/s.
@@ -36,8 +36,10 @@
 // every lane's partial row sum stays <= 2^20, else the offset moves to the exact
 // maximum and the step is redone from its scores.
 //
-// Precision: scores, statistics and outputs in fp32; K and V are exact in bf16. fp16 and fp32
-// queries are split into 2 or 3 bf16 parts. P is held in 2 parts (16 bits; fp32: 3, 24 bits) where the
+// Precision: scores, statistics and outputs in fp32; K and V are exact in bf16. fp16 queries meet the
+// codes in fp16, exact too without the scale, which the scores take (16 x 5 tokens over 47 000: 32.8 us,
+// by two bf16 parts of the queries 38.3); for prompts they are split into 2 bf16
+// parts, fp32 queries into 3. P is held in 2 parts (16 bits; fp32: 3, 24 bits) where the
 // cache's bytes bound the kernel and the matrix unit waits for them; a single part's rounding is as
 // large as that of the bf16 output. Prompts with bf16 queries are bound by the matrix unit and take one. The row
 // sum is of the unrounded P.
@@ -53,7 +55,7 @@
 namespace mga {
 namespace {
 
-// bf16 parts of the queries (n), and of the probabilities over a streamed cache (p).
+// bf16 parts of the queries (n; fp16's: of prompts), and of the probabilities over a streamed cache (p).
 template <typename T> struct Parts;
 template <> struct Parts<bf16_t> { static constexpr int n = 1, p = 2; };
 template <> struct Parts<f16_t> { static constexpr int n = 2, p = 2; };
@@ -72,6 +74,17 @@ __device__ __forceinline__ bf16x8 decode8(uint32_t a, uint32_t b, float s) {
                r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, false),
                t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, true);
   return bf16x8{p[0], p[1], q[0], q[1], r[0], r[1], t[0], t[1]};
+}
+
+// The same without a scale, in fp16 (exact).
+__device__ __forceinline__ f16x8 decode8_f16(uint32_t a, uint32_t b) {
+  const auto two = [](uint32_t c, auto high) {
+    return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.f, decltype(high)::value));
+  };
+  const std::false_type lo;
+  const std::true_type hi;
+  const i32x4 r = {two(a, lo), two(a, hi), two(b, lo), two(b, hi)};
+  return __builtin_bit_cast(f16x8, r);
 }
 
 // x = the sum of N bf16 parts, up to the last one's rounding.
@@ -199,7 +212,8 @@ __device__ __forceinline__ i32x4 load16(const uint8_t *base, uint32_t off) {
 // 64 steps of one page each, or 64 / 2^pps of 2^pps pages each.
 // UNI: pages of 64 tokens or more, so that a step lies in one page: its id and scales are
 // wave-uniform, and the loads take a scalar base with a lane offset that never changes.
-template <int HD, bool UNI>
+// F16: scores take the scales, not keys.
+template <int HD, bool UNI, bool F16>
 struct Stream {
   static constexpr int ND = HD / 16, KL = HD / 64;
   const PagedAttnArgs &a;
@@ -288,7 +302,7 @@ struct Stream {
     load_k(0);
     load_v(0);
     __builtin_amdgcn_s_waitcnt(wait_vm(4 * KL + ND));   // the scales
-    ksc = held(tks, 0, kg);
+    ksc = held(tks, 0, F16 ? g : kg);   // of the keys that a lane converts, or has scores of
     vsc = held(tvs, 0, g);
   }
   template <typename F>
@@ -301,7 +315,7 @@ struct Stream {
       __builtin_amdgcn_s_waitcnt(wait_vm(0));
     }
     load_k(i);
-    ksc = held(tks, i, kg);
+    ksc = held(tks, i, F16 ? g : kg);
   }
   __device__ __forceinline__ void next_v(int i) {
     load_v(i);
@@ -312,7 +326,9 @@ struct Stream {
 // One tile's queries and results.
 template <int HD, int NT, typename T, bool UNI>
 struct Rows {
-  static constexpr int NQ = Parts<T>::n, NP = Parts<T>::p, KS = HD / 32, ND = HD / 16;
+  // fp16 queries meet the codes in fp16 and the scale in the scores
+  static constexpr bool F16 = std::is_same<T, f16_t>::value;
+  static constexpr int NQ = F16 ? 1 : Parts<T>::n, NP = Parts<T>::p, KS = HD / 32, ND = HD / 16;
   const PagedAttnArgs &a;
   const Tile &x;
   const int col, g;
@@ -339,15 +355,9 @@ struct Rows {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = 0.f;
           if (r < x.rows) {
-            if constexpr (NQ == 2) {
-              const f16x8 e = __builtin_bit_cast(f16x8, load8(qp + c));
+            const f32x4 e = *reinterpret_cast<const f32x4 *>(qp + c), f = *reinterpret_cast<const f32x4 *>(qp + c + 4);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = (float)e[i];
-            } else {
-              const f32x4 e = *reinterpret_cast<const f32x4 *>(qp + c), f = *reinterpret_cast<const f32x4 *>(qp + c + 4);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) v[i] = e[i], v[i + 4] = f[i];
-            }
+            for (int i = 0; i < 4; ++i) v[i] = e[i], v[i + 4] = f[i];
           }
           bf16x8 part[NQ];
           split8<NQ>(v, part);
@@ -364,7 +374,7 @@ struct Rows {
 
   // Step p of the tile, the stream's step i; the stream's loads go on to its next one.
   template <typename F>
-  __device__ __forceinline__ void step(Stream<HD, UNI> &st, int i, int p, F find) {
+  __device__ __forceinline__ void step(Stream<HD, UNI, F16> &st, int i, int p, F find) {
     f32x4 s[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -377,13 +387,27 @@ struct Rows {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const i32x4 c = st.kc[t][ks >> 1];
-        const bf16x8 kf = decode8(c[2 * (ks & 1)], c[2 * (ks & 1) + 1], st.ksc);
+        const uint32_t c0 = c[2 * (ks & 1)], c1 = c[2 * (ks & 1) + 1];
+        if constexpr (F16) {
+          const f16x8 kf = decode8_f16(c0, c1);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
+            s[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, __builtin_bit_cast(f16x8, qf[nt][0][ks]), s[nt][t], 0, 0, 0);
+        } else {
+          const bf16x8 kf = decode8(c0, c1, st.ksc);
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) s[nt][t] = mfma16(kf, qf[nt][q][ks], s[nt][t]);
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) s[nt][t] = mfma16(kf, qf[nt][q][ks], s[nt][t]);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (F16) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) s[nt][t] *= st.ksc;
     }
     st.next_k(i + 1, find);
 
@@ -469,7 +493,7 @@ struct Rows {
   // The NaNs taken out of the edge steps below p1 count for the rows that see them, and only for
   // those: an output becomes NaN where a product of the NaNs' places with the mask is not 0. Rare; the
   // values are read again.
-  __device__ __forceinline__ void put_nan(const Stream<HD, UNI> &st, int p1, int stride) {
+  __device__ __forceinline__ void put_nan(const Stream<HD, UNI, F16> &st, int p1, int stride) {
     for (int p = nan_from; p < p1; p += stride) {
       const int key0 = p * 64 + 16 * g, at = key0 >> a.pshift;
       const int id = at < a.width ? a.table[(int64_t)x.b * a.table_rs + at] : -1;
@@ -618,7 +642,7 @@ __global__ __launch_bounds__(256, share_occupancy(HD, NT, Parts<T>::n)) void pag
   JoinNote *notes = reinterpret_cast<JoinNote *>(a.ws + (int64_t)workers * 2 * slot_floats(ROWS, HD));
 
   if (u0 < u1) {
-    Stream<HD, UNI> st(a, u1 - u0);
+    Stream<HD, UNI, std::is_same<T, f16_t>::value> st(a, u1 - u0);
     int tb = 0, th = 0, tt = 0;   // a lane holds the tile of its step, too
     auto find = [&](int i, int &p) {
       const Place pl = locate(a, tmshift, pre, seqs, u0 + i);
@@ -769,7 +793,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttnArgs a, in
   x.h = blockIdx.x - slot * a.Hkv;
   if (tile_of_slot(a, slot, tmshift, G, x)) {
     Rows<HD, NT, T, UNI> rows(a, x, G);
-    Stream<HD, UNI> st(a, (x.steps - w + NW - 1) / NW);   // 0 or less: none
+    Stream<HD, UNI, std::is_same<T, f16_t>::value> st(a, (x.steps - w + NW - 1) / NW);   // 0 or less: none
     if (st.n > 0) {
       auto find = [&](int i, int &p) {
         p = w + i * NW;
@@ -1135,7 +1159,7 @@ template <int HD, int NT, typename T, bool UNI>
 void launch3(const PagedAttnArgs &a, const Shape &s, hipStream_t stream) {
   const int G = a.Hq / a.Hkv, tiles = tile_slots(a.T, a.B, s.tmshift) * a.Hkv;
   if (s.mode == kTiles) {
-    constexpr int NW = NT == 1 || Parts<T>::n == 1 ? 8 : 4;   // by the registers of a wave
+    constexpr int NW = NT == 1 || sizeof(T) == 2 ? 8 : 4;   // by the registers of a wave
     paged_tile_kernel<HD, NT, T, UNI, NW><<<tiles, 64 * NW, 0, stream>>>(a, s.tmshift, G);
   } else {
     paged_share_kernel<HD, NT, T, UNI><<<s.nwg, 256, 0, stream>>>(a, s.tmshift, G);

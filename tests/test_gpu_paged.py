@@ -269,6 +269,17 @@ def test_attention_wide_scores(mga, dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,cached", [([4, 1], [90, 10]), ([4, 1], [1500, 10]), ([400, 900], [500, 0])])
+def test_attention_small_queries(mga, dev, dtype, new, cached):
+    """Queries below fp16's normal range, whose products with the keys are of ordinary size."""
+    pool = Pool(dev, new, cached, 4, 64, 32, seed=8, scales=(-3, 3))
+    q = (queries(pool, 16, 64, dtype, dev).float() * 2.0 ** -17).to(dtype)
+    got = attend(mga, pool, q, scale=2.0 ** 11)
+    check_attention(got, q, pool, 2.0 ** 11)
+    assert (got[0].float() - got[0].float().mean(0)).abs().max() > 0.1   # the heads differ: the queries count
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_behind_the_last_sequence(mga, dev, dtype):
     pool = Pool(dev, [2, 3], [10, 70], 2, 64, 64)
     q = queries(pool, 4, 64, dtype, dev, extra=4)
