@@ -18,7 +18,7 @@
 // (364 MB): 75 us + 5 us joining, 4.5 TB/s; 2 of 212 590 (435 MB): 81 + 7 us, 4.9 TB/s; what is left is
 // the start (cu, lengths, pages, first keys: 4 us), the join's launch, and waves that end up to 15% apart
 // with equal shares. Prompts: the matrix unit and the softmax's vector work beside it: 10 075 new
-// tokens behind up to 15 399, 1175 GFLOP visible, 1.25 ms, 940 TFLOP/s.
+// tokens behind up to 15 399, 1175 GFLOP visible, 1.29 ms, 913 TFLOP/s.
 //
 // Three forms share this: few rows a sequence over long ones by equal shares (paged_share_kernel), short
 // sequences by a workgroup a tile (paged_tile_kernel), prompts by 128 rows (paged_prompt_kernel, further
