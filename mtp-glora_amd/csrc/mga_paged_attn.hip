@@ -231,11 +231,13 @@ struct Stream {
         pps(UNI ? 0 : 6 - a_.pshift), hold(64 >> pps), koff((16 * kg + (col & 3)) * HD + 16 * g),
         voff(col * PS + 16 * g) {}
 
-  // step p of sequence b and head h: the page of this lane's part of it
-  __device__ __forceinline__ int page_of(int b, int h, int p) const {
+  // step p of sequence b and head h: the page of this lane's part of it; none past the sequence's end,
+  // where the table may name one that was never written
+  __device__ __forceinline__ int page_of(int b, int h, int p, int end) const {
     const int at = UNI ? p >> (a.pshift - 6) : (p << pps) + (lane & ((1 << pps) - 1));
     const int id = a.table[(int64_t)b * a.table_rs + min(at, a.width - 1)];
-    return at < a.width && (uint32_t)id < (uint32_t)a.num_pages ? id * a.Hkv + h : -1;
+    const bool there = at < a.width && (UNI || at << a.pshift < end);
+    return there && (uint32_t)id < (uint32_t)a.num_pages ? id * a.Hkv + h : -1;
   }
   __device__ __forceinline__ void scales() {
     tks = a.ks[max(tph, 0)];
@@ -248,6 +250,11 @@ struct Stream {
       return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i & 63));
     else
       return __shfl(v, ((i & (hold - 1)) << pps) + (grp >> (2 - pps)), 64);
+  }
+  // of step i's values, whose page vph is; where there is none, 1: zeros under any scale could be NaN
+  __device__ __forceinline__ float v_scale(int i) const {
+    const float s = held(tvs, i, g);
+    return vph < 0 ? 1.f : s;
   }
   // a held value that a step's lanes share
   __device__ __forceinline__ int step_of(int v, int i) const {
@@ -303,7 +310,7 @@ struct Stream {
     load_v(0);
     __builtin_amdgcn_s_waitcnt(wait_vm(4 * KL + ND));   // the scales
     ksc = held(tks, 0, F16 ? g : kg);   // of the keys that a lane converts, or has scores of
-    vsc = held(tvs, 0, g);
+    vsc = v_scale(0);
   }
   template <typename F>
   __device__ __forceinline__ void next_k(int i, F find) {
@@ -319,7 +326,7 @@ struct Stream {
   }
   __device__ __forceinline__ void next_v(int i) {
     load_v(i);
-    vsc = held(tvs, i, g);
+    vsc = v_scale(i);
   }
 };
 
@@ -650,7 +657,7 @@ __global__ __launch_bounds__(256, share_occupancy(HD, NT, Parts<T>::n)) void pag
       th = pl.h;
       tt = pl.t;
       p = pl.p;
-      return st.page_of(pl.b, pl.h, pl.p);
+      return st.page_of(pl.b, pl.h, pl.p, seqs[pl.b].len + seqs[pl.b].n);
     };
     st.start(find);
     int nb = st.step_of(tb, 0), nh = st.step_of(th, 0), nt_ = st.step_of(tt, 0), np = st.step_of(st.tp, 0);
@@ -797,7 +804,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttnArgs a, in
     if (st.n > 0) {
       auto find = [&](int i, int &p) {
         p = w + i * NW;
-        return st.page_of(x.b, x.h, p);
+        return st.page_of(x.b, x.h, p, x.q.len + x.q.n);
       };
       st.start(find);
       for (int i = 0; i < st.n; ++i) rows.step(st, i, w + i * NW, find);
@@ -908,7 +915,7 @@ __global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_ke
     }
     const int32_t *trow = a.table + (int64_t)x.b * a.table_rs;
     auto checked = [&](int id, int key) {
-      return (uint32_t)id < (uint32_t)a.num_pages && (key >> a.pshift) < a.width ? id * a.Hkv + x.h : -1;
+      return (uint32_t)id < (uint32_t)a.num_pages && (key >> a.pshift) < a.width && key < end_key ? id * a.Hkv + x.h : -1;
     };
     // UNI: the lanes hold the pages (page * Hkv + head, -1: none) and scales of 64 steps; else each
     // thread its own pages of the step after the one in registers, not checked yet
@@ -922,6 +929,7 @@ __global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_ke
         tks = a.ks[max(tph, 0)];
         tvs = a.vs[max(tph, 0)];
         __builtin_amdgcn_s_waitcnt(wait_vm(0));   // once in 64 steps, see Stream
+        tvs = tph < 0 ? 1.f : tvs;                // likewise
       } else {
         kid = trow[min((p * 64 + kr) >> a.pshift, a.width - 1)];
 #pragma unroll
@@ -962,7 +970,7 @@ __global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_ke
           vph[i] = checked(vid[i], key);
           vc[i] = *reinterpret_cast<const i32x4 *>(
               a.vp + (((int64_t)max(vph[i], 0) * HD + vr) << a.pshift) + (key & (PS - 1)));
-          vsc[i] = a.vs[max(vph[i], 0)];
+          vsc[i] = a.vs[max(vph[i], 0)];   // of no page: see put
         }
       }
     };
@@ -1003,7 +1011,8 @@ __global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_ke
           if (nan) atomicMin(&nan_step, p);
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) *at(vt[buf], vw[i] ^ 16 * k) = decode8(vc[i][2 * k], vc[i][2 * k + 1], vsc[i]);
+        for (int k = 0; k < 2; ++k)
+          *at(vt[buf], vw[i] ^ 16 * k) = decode8(vc[i][2 * k], vc[i][2 * k + 1], UNI || vph[i] >= 0 ? vsc[i] : 1.f);
       }
     };
 

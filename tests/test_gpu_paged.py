@@ -252,6 +252,39 @@ def test_attention_nan_reaches_only_who_sees_it(mga, dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ps", [16, 32, 64, 128])
+@pytest.mark.parametrize("Hq,new,cached", [(4, [1, 3], [70, 5]), (8, [5, 2], [1300, 17]), (16, [700, 900], [33, 500])])
+def test_attention_of_pages_never_written(mga, dev, dtype, ps, Hq, new, cached):
+    """Scales of pages that hold no token are anything, wherever the table names them; so are page
+    0's where a page is missing."""
+    Hkv = Hq // 2
+    pool = Pool(dev, new, cached, Hkv, 64, ps, seed=4, spare=6, width=-(-1400 // ps) + 3)
+    pool.table[1, 0] = -1
+    q = queries(pool, Hq, 64, dtype, dev)
+    want = attend(mga, pool, q)
+    check_attention(want, q, pool, 0.125)
+    used = torch.zeros(pool.n + 1, dtype=torch.bool, device=dev)
+    used[pool.table.long()] = True      # -1: the last, which is none
+    free = (~used[:-1]).nonzero().flatten()
+    assert len(free) >= 6
+    move = free[0].item()
+    if used[0]:   # page 0 is to be one of them
+        for t in (pool.k, pool.v, pool.ks, pool.vs):
+            t[move] = t[0].clone()
+        pool.table[pool.table == 0] = move
+        free[0] = 0
+    bad = torch.tensor([float("nan"), float("inf"), -1.0, 0.0, 3e38, float("nan")], device=dev)
+    bad[0] = float("nan")
+    for t in (pool.ks, pool.vs):
+        t[free] = bad[torch.arange(len(free), device=dev) % 6][:, None]
+    for b in range(2):                  # behind the tokens' pages
+        n = -(-(new[b] + cached[b]) // ps)
+        tail = pool.table.shape[1] - n
+        pool.table[b, n:] = free[torch.arange(tail, device=dev) % len(free)].int()
+    assert torch.equal(attend(mga, pool, q), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_wide_scores(mga, dev, dtype):
     """Scores hundreds of units apart, rising and falling along the sequence, and queries of
     zeros, infinity and NaN."""
