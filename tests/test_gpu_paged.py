@@ -218,6 +218,22 @@ def test_attention_many_sequences(mga, dev, dtype):
     check_attention(attend(mga, pool, q), q, pool, 0.125)
 
 
+@pytest.mark.parametrize("width", [None, 80])
+def test_most_sequences(mga, dev, width):
+    """4096 sequences, a third of them without tokens, appended to and attended over, in tiles and in
+    shares; one more is refused."""
+    new = [(0, 1, 2)[i % 3] for i in range(4096)]
+    cached = [(i * 29) % 70 for i in range(4096)]
+    pool = Pool(dev, new, cached, 1, 64, 16, seed=3, width=width)
+    x, y = rows(pool.T, 1, 64, torch.bfloat16, dev, 1), rows(pool.T, 1, 64, torch.bfloat16, dev, 2)
+    run_append(mga, pool, None, x, y)
+    q = queries(pool, 2, 64, torch.bfloat16, dev)
+    check_attention(attend(mga, pool, q), q, pool, 0.125)
+    with pytest.raises(RuntimeError, match="4096"):
+        mga.paged_attention(q, pool.pages, torch.cat([pool.table, pool.table[:1]]), torch.cat([pool.cu, pool.cu[-1:]]),
+                            torch.cat([pool.len, pool.len[:1]]), 0.125)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_missing_pages(mga, dev, dtype):
     """Pages outside the cache are masked; a row with nothing else is zeros."""
