@@ -4,8 +4,9 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w            (where norm weights are given)
 //   r = y * cos + rotate_half(y) * sin            (where cos / sin are given)
 // from the projections' values; the query rows in fp32, rounded once to their type.
-// Keys are prepared in fp64 (half the rate of fp32; 4 us of the 29): an fp32 value
-// next to the middle between two codes takes the wrong one about once in 2^20 values.
+// Keys are prepared in fp64 (half the rate of fp32; 4 us of the 29) and go on in fp32
+// rounded to odd (to_float): prepared or rounded to nearest in fp32, a value next to the middle
+// between two codes takes the wrong one about once in 2^20 values.
 // Keys and values are rounded once to e4m3 under the scale of their (page, head): the
 // least power of two of which 448 hold every value the page has taken
 // since a row 0 was written. Where new rows make it grow, the rows kept from before
@@ -93,13 +94,15 @@ struct RawRow {
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 
-// fp32 next to d on the side of d: what is rounded to e4m3 from it is what d would be.
+// d in fp32, rounded to odd: towards zero, with the last bit set where anything was lost. A middle between two
+// codes and 448 times a power of two are even numbers of fp32: what is rounded to e4m3's 4 bits from the
+// result, or compared with those, comes out as from d itself. (The nearest fp32 number may be the middle.)
 __device__ __forceinline__ float to_float(double d) {
   const float f = (float)d;
-  const double r = (double)f;
-  const int bits = __builtin_bit_cast(int, f);
-  const bool more = fabs(d) > fabs(r), less = fabs(d) < fabs(r);
-  return fabsf(f) < __builtin_huge_valf() ? __builtin_bit_cast(float, bits + (more ? 1 : less ? -1 : 0)) : f;
+  int bits = __builtin_bit_cast(int, f);
+  bits -= fabs(d) < fabs((double)f) ? 1 : 0;   // from infinity, too
+  bits |= (double)__builtin_bit_cast(float, bits) != d ? 1 : 0;
+  return __builtin_bit_cast(float, bits);
 }
 
 // x <- x * rsqrt(mean(x^2) + eps) * w, then x * cos + rotate_half(x) * sin, computed in F. C: the type of cos

@@ -108,8 +108,8 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, pages, block_table: tor
 
     Keys and queries are normalised where ``k_weight`` / ``q_weight`` [D] are given (RMS
     norm) and rotated where ``cos`` / ``sin`` [T, D] are (the rotary tables of each
-    token, in the model's dtype or fp32), in fp32 with one rounding at the end, unlike
-    ``qk_norm_rope``, which rounds after every op as the reference's ops do. Keys and
+    token, in the model's dtype or fp32), keys in fp64 and queries in fp32, with one rounding at the
+    end, unlike ``qk_norm_rope``, which rounds after every op as the reference's ops do. Keys and
     values are stored in e4m3, under a power-of-two scale for each page and head that
     grows with the values the page takes; an append at a page's row 0 begins it anew.
     NaN and infinities are stored as NaN. A position without a page is not
