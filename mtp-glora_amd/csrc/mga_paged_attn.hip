@@ -727,7 +727,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int tm
   const int lane = threadIdx.x & 63, w = wave_id(), sub = w % WPR, pg = sub * PG + lane / TPP, c = lane % TPP;
   const int slot = blockIdx.x / a.Hkv;
   const JoinNote *notes = reinterpret_cast<const JoinNote *>(a.ws + (int64_t)workers * 2 * slot_floats(ROWS, HD));
-  const JoinNote n = notes[blockIdx.x];   // of a slot without a tile: anything, and not used
+  JoinNote n = notes[blockIdx.x];   // of a slot without a tile: anything, and not used
+  // so are parts of the notes where sequences of a cu_tokens that goes down overlap until the steps end at
+  // kMaxSteps: tiles behind that have no worker. Whatever they say stays among the workers' partial results
+  n.first = min(max(n.first, 0), workers - 1);
+  n.last = min(max(n.last, n.first), workers - 1);
+  n.slot = min(max(n.slot, 0), 2 * workers - 1);
   Tile x;
   x.h = blockIdx.x - slot * a.Hkv;
   if (!tile_of_slot(a, slot, tmshift, G, x) || n.first == n.last) return;
