@@ -28,6 +28,13 @@ def _dev(name: str, t: torch.Tensor) -> None:
                            "libmtp_glora_amd has no CPU path")
 
 
+def no_tangent(fn: str, *tensors) -> None:
+    """Refuse tensors with a forward-mode tangent, which ``fn`` would drop."""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{fn} computes no forward-mode derivative")
+
+
 def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.bfloat16:
         return _lib.DTYPE_BF16

@@ -17,7 +17,7 @@ rows ends at cu_tokens[B], a sequence without new tokens takes none. Rejected dr
 dropped by not adding them to ``lengths``: the next append overwrites them. Which pages a
 sequence gets is the caller's to say; no two may write to one page, any may read it.
 
-Neither call computes a gradient.
+Neither call computes a gradient; operands that ask for one, in reverse or forward mode, are refused.
 """
 from __future__ import annotations
 
@@ -26,7 +26,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .ops import _dev, _stream, dtype_code
+from .ops import _dev, _stream, dtype_code, no_tangent
 
 PAGE_SIZES = (16, 32, 64, 128)
 CODE_DTYPE = torch.float8_e4m3fn
@@ -114,11 +114,12 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, pages, block_table: tor
     grows with the values the page takes; an append at a page's row 0 begins it anew.
     NaN and infinities are stored as NaN. A position without a page is not
     stored. Rows of the result behind the last sequence's tokens are zeros."""
-    _no_grad("paged_append", key, value, query, q_weight, k_weight, cos, sin)
+    _no_grad("paged_append", key, value, query, q_weight, k_weight, cos, sin, *pages)
     r = _lib.native("paged_append", key, value, *pages, block_table, cu_tokens, lengths, query, cos, sin, q_weight,
                     k_weight, eps)
     if r is not None:
         return r[0] if query is not None else None
+    no_tangent("paged_append", key, value, query, q_weight, k_weight, cos, sin, *pages)
     p = _pages(pages)
     table, cu, lens = _batch(block_table, cu_tokens, lengths, p.k.device)
     n, Hkv, ps, D = p.k.shape
@@ -181,10 +182,11 @@ def paged_attention(query: torch.Tensor, pages, block_table: torch.Tensor, cu_to
     rows that do not overlap it) receives the result; its rows
     behind the last sequence's tokens stay as they are, in a tensor made here they are
     zeros. Hq / Hkv <= 32, at most 4096 sequences."""
-    _no_grad("paged_attention", query)
+    _no_grad("paged_attention", query, *pages)
     r = _lib.native("paged_attention", query, *pages, block_table, cu_tokens, lengths, scaling, out)
     if r is not None:
         return r
+    no_tangent("paged_attention", query, out, *pages)
     p = _pages(pages)
     table, cu, lens = _batch(block_table, cu_tokens, lengths, p.k.device)
     n, Hkv, ps, D = p.k.shape

@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _dev, _stream, dtype_code
+from .ops import _dev, _stream, dtype_code, no_tangent
 from .distill import INT32_MAX, MAX_VOCAB, row_stride, row_view
 
 
@@ -131,6 +131,7 @@ def adjust_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, l
                     *(0.0 if isinstance(v, torch.Tensor) else float(v) for v in given), bias_ids, bias, allowed, out)
     if r is not None:
         return r
+    no_tangent("adjust_logits", logits, bias, *given, out)
     _dev("logits", logits)
     lead, V, dev = logits.shape[:-1], logits.shape[-1] if logits.dim() else 0, logits.device
     x = row_view("logits", logits)
