@@ -271,9 +271,16 @@ class PagedKVCache:
         return paged_attention(query, self._layers[layer_idx], *self._step(), scaling, out=out)
 
     def dequantized(self, layer_idx: int, block_table_row: torch.Tensor, length: int):
-        """Keys and values [Hkv, length, D] (fp32) that a layer holds of a sequence, by
-        elementary operations: for inspection, and to hand a prefix to another cache."""
-        p, ids = self._layers[layer_idx], block_table_row.long()[:-(-int(length) // self.page_size)]
-        read = lambda c, s: c.view(torch.uint8)[ids].view(CODE_DTYPE).float() * s[ids][..., None, None]   # noqa: E731
+        """Keys and values [Hkv, length, D] (fp32) that a layer holds of a sequence, zeros at
+        positions without a page, by elementary operations: for inspection, and to hand a prefix to
+        another cache."""
+        p, n = self._layers[layer_idx], int(length)
+        if block_table_row.dim() != 1 or not 0 <= n <= block_table_row.shape[0] * self.page_size:
+            raise ValueError(f"{n} tokens in a table row {tuple(block_table_row.shape)} of pages of {self.page_size}")
+        ids = block_table_row.to(p.k.device).long()[:-(-n // self.page_size)]
+        there = (ids >= 0) & (ids < self.num_pages)
+        ids, there = torch.where(there, ids, 0), there[:, None, None, None]
+        read = lambda c, s: torch.where(   # noqa: E731
+            there, c.view(torch.uint8)[ids].view(CODE_DTYPE).float() * s[ids][..., None, None], 0.0)
         k, v = read(p.k, p.k_scale), read(p.v, p.v_scale).transpose(2, 3)
-        return tuple(t.transpose(0, 1).flatten(1, 2)[:, :length] for t in (k, v))
+        return tuple(t.transpose(0, 1).flatten(1, 2)[:, :n] for t in (k, v))
