@@ -26,6 +26,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
+from .distill import row_stride
 from .ops import _dev, _stream, dtype_code, no_tangent
 
 PAGE_SIZES = (16, 32, 64, 128)
@@ -168,7 +169,7 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, pages, block_table: tor
                   ptr(cos), ptr(sin), cos.stride(0) if cos is not None else 0,
                   int(cos is not None and cos.dtype == torch.float32), float(eps), T, table.shape[0],
                   q.shape[1] if q is not None else 0, Hkv, D, code, ptr(p.k), ptr(p.v), ptr(p.k_scale), ptr(p.v_scale), n,
-                  ps, ptr(table), table.stride(0), table.shape[1], ptr(cu), ptr(lens), ptr(qo), *st(qo), _stream(p.k))
+                  ps, ptr(table), row_stride(table), table.shape[1], ptr(cu), ptr(lens), ptr(qo), *st(qo), _stream(p.k))
     return qo
 
 
@@ -216,7 +217,7 @@ def paged_attention(query: torch.Tensor, pages, block_table: torch.Tensor, cu_to
         nb = int(_lib.load().mga_paged_attn_workspace_bytes(T, table.shape[0], Hq, Hkv, D, ps, table.shape[1], code))
         ws = torch.empty(nb, device=q.device, dtype=torch.uint8)
         _lib.call("mga_paged_attn", q.data_ptr(), q.stride(0), q.stride(1), p.k.data_ptr(), p.v.data_ptr(),
-                  p.k_scale.data_ptr(), p.v_scale.data_ptr(), n, ps, table.data_ptr(), table.stride(0), table.shape[1],
+                  p.k_scale.data_ptr(), p.v_scale.data_ptr(), n, ps, table.data_ptr(), row_stride(table), table.shape[1],
                   cu.data_ptr(), lens.data_ptr(), T, table.shape[0], Hq, Hkv, D, code, float(scaling), out.data_ptr(),
                   out.stride(0), out.stride(1), int(fresh), ws.data_ptr() if nb else None, nb, _stream(q))
     return out
