@@ -566,7 +566,7 @@ int mga_embedding_bwd(const void *grad_out, int64_t grad_out_row_stride, const v
  *   code = e4m3(r / scale), to nearest even; NaN and infinities become NaN codes and
  *      count in no scale.
  * query (null: none) likewise in fp32 with q_weight into query_out, rounded once to the dtype;
- * its rows behind cu_tokens[n_seqs] are zeros. cos, sin [n_tokens, head_dim] in the dtype, or fp32
+ * its rows behind cu_tokens[n_seqs] are zeros, and none may overlap. cos, sin [n_tokens, head_dim] in the dtype, or fp32
  * with cos_sin_f32. Rows behind a sequence's end in its last page, and all other pages,
  * stay as they are. n_seqs <= 4096; head_dim 64 or 128; table_width * page_size + n_tokens and
  * num_pages * Hkv <= 2^30. Beside mga_kv_append and
@@ -587,7 +587,7 @@ int mga_paged_append(const void *key, int64_t k_stride_s, int64_t k_stride_h, co
  * not see does not reach it, NaN included. Scores, sums and outputs in fp32; P is
  * held to 16 bits (fp32 queries: 24; prompts in bf16: 8).
  * q, out: [n_tokens, Hq, head_dim], rows 16-byte aligned; out may be q itself (the same strides), else may
- * not overlap it; Hq / Hkv <= 32. Rows of
+ * not overlap it, nor its rows each other; Hq / Hkv <= 32. Rows of
  * out behind cu_tokens[n_seqs]: zeros with zero_rest, else left as they are. workspace:
  * mga_paged_attn_workspace_bytes bytes (0: may be null), 16-byte aligned, one for each call in flight. Sums
  * run in a fixed order. Beside mga_attn_fwd ([tf]integrations/flex_attention.py:262-368).

@@ -1134,6 +1134,18 @@ int check_token_rows(const char *fn, const char *name, const void *p, int64_t ss
   return MGA_OK;
 }
 
+// Do the T x H rows of D elements, strides ss and hs, share none? Tokens and heads may lie in either order, or
+// one's rows between the other's.
+bool rows_apart(int64_t ss, int64_t hs, int32_t T, int32_t H, int32_t D) {
+  if ((T > 1 && ss < D) || (H > 1 && hs < D)) return false;
+  if (T <= 1 || H <= 1 || ss >= (H - 1) * hs + D || hs >= (T - 1) * ss + D) return true;
+  for (int64_t j = 1; j < H; ++j) {   // rows of other heads beside head j's of token 0: on tokens i and i + 1
+    const int64_t i = j * hs / ss, past = j * hs - i * ss;
+    if ((i < T && past < D) || (i + 1 < T && ss - past < D)) return false;
+  }
+  return true;
+}
+
 // May [tokens, heads, head_dim] operands p and q share an element? Not where their tokens lie side by
 // side in rows of one buffer.
 bool token_rows_overlap(const void *p, int64_t pss, int64_t phs, const void *q, int64_t qss, int64_t qhs, int32_t T,
@@ -1169,6 +1181,8 @@ int mga_paged_append(const void *key, int64_t k_stride_s, int64_t k_stride_h, co
     if ((rc = check_token_rows(fn, "query", query, q_stride_s, q_stride_h, eb, &vec)) != MGA_OK ||
         (rc = check_token_rows(fn, "query_out", query_out, qo_stride_s, qo_stride_h, eb, &vec)) != MGA_OK)
       return rc;
+    if (!rows_apart(qo_stride_s, qo_stride_h, n_tokens, Hq, head_dim))
+      return fail(MGA_ERR_INVALID, "%s: rows of query_out overlap", fn);
   }
   if ((cos == nullptr) != (sin == nullptr)) return fail(MGA_ERR_INVALID, "%s: one of cos and sin is null", fn);
   const int ceb = cos_sin_f32 ? 4 : eb;
@@ -1216,6 +1230,8 @@ int mga_paged_attn(const void *q, int64_t q_stride_s, int64_t q_stride_h, const 
       (rc = check_token_rows(fn, "out", out, o_stride_s, o_stride_h, eb, &vec)) != MGA_OK)
     return rc;
   if (!vec) return fail(MGA_ERR_INVALID, "%s: rows of q and out must be 16-byte aligned", fn);
+  if (!rows_apart(o_stride_s, o_stride_h, n_tokens, Hq, head_dim))
+    return fail(MGA_ERR_INVALID, "%s: rows of out overlap", fn);
   const bool same = q == out && q_stride_s == o_stride_s && q_stride_h == o_stride_h;
   if (!same && token_rows_overlap(q, q_stride_s, q_stride_h, out, o_stride_s, o_stride_h, n_tokens, Hq, head_dim, eb))
     return fail(MGA_ERR_INVALID, "%s: out overlaps q", fn);
