@@ -566,7 +566,8 @@ int mga_embedding_bwd(const void *grad_out, int64_t grad_out_row_stride, const v
  *   code = e4m3(r / scale), to nearest even; NaN and infinities become NaN codes and
  *      count in no scale.
  * query (null: none) likewise in fp32 with q_weight into query_out, rounded once to the dtype;
- * its rows behind cu_tokens[n_seqs] are zeros, and none may overlap. cos, sin [n_tokens, head_dim] in the dtype, or fp32
+ * its rows behind cu_tokens[n_seqs] are zeros. It may be query itself (the same strides), else its rows may
+ * overlap neither each other nor query, key and value. cos, sin [n_tokens, head_dim] in the dtype, or fp32
  * with cos_sin_f32. Rows behind a sequence's end in its last page, and all other pages,
  * stay as they are. n_seqs <= 4096; head_dim 64 or 128; table_width * page_size + n_tokens and
  * num_pages * Hkv <= 2^30. Beside mga_kv_append and

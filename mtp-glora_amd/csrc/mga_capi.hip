@@ -1148,9 +1148,9 @@ bool rows_apart(int64_t ss, int64_t hs, int32_t T, int32_t H, int32_t D) {
 
 // May [tokens, heads, head_dim] operands p and q share an element? Not where their tokens lie side by
 // side in rows of one buffer.
-bool token_rows_overlap(const void *p, int64_t pss, int64_t phs, const void *q, int64_t qss, int64_t qhs, int32_t T,
-                        int32_t heads, int32_t D, int eb) {
-  const int64_t pw = (heads - 1) * phs + D, qw = (heads - 1) * qhs + D;   // of a token
+bool token_rows_overlap(const void *p, int64_t pss, int64_t phs, int32_t pheads, const void *q, int64_t qss, int64_t qhs,
+                        int32_t qheads, int32_t T, int32_t D, int eb) {
+  const int64_t pw = (pheads - 1) * phs + D, qw = (qheads - 1) * qhs + D;   // of a token
   const uint64_t p0 = reinterpret_cast<uintptr_t>(p) / eb, q0 = reinterpret_cast<uintptr_t>(q) / eb;
   if (p0 >= q0 + (T - 1) * qss + qw || q0 >= p0 + (T - 1) * pss + pw) return false;
   if (pss != qss || pss == 0) return true;
@@ -1183,6 +1183,13 @@ int mga_paged_append(const void *key, int64_t k_stride_s, int64_t k_stride_h, co
       return rc;
     if (!rows_apart(qo_stride_s, qo_stride_h, n_tokens, Hq, head_dim))
       return fail(MGA_ERR_INVALID, "%s: rows of query_out overlap", fn);
+    const auto beside = [&](const void *x, int64_t ss, int64_t hs, int32_t heads) {
+      return !token_rows_overlap(x, ss, hs, heads, query_out, qo_stride_s, qo_stride_h, Hq, n_tokens, head_dim, eb);
+    };
+    const bool same = query == query_out && q_stride_s == qo_stride_s && q_stride_h == qo_stride_h;
+    if (!beside(key, k_stride_s, k_stride_h, Hkv) || !beside(value, v_stride_s, v_stride_h, Hkv) ||
+        (!same && !beside(query, q_stride_s, q_stride_h, Hq)))
+      return fail(MGA_ERR_INVALID, "%s: query_out overlaps key, value or query", fn);
   }
   if ((cos == nullptr) != (sin == nullptr)) return fail(MGA_ERR_INVALID, "%s: one of cos and sin is null", fn);
   const int ceb = cos_sin_f32 ? 4 : eb;
@@ -1233,7 +1240,7 @@ int mga_paged_attn(const void *q, int64_t q_stride_s, int64_t q_stride_h, const 
   if (!rows_apart(o_stride_s, o_stride_h, n_tokens, Hq, head_dim))
     return fail(MGA_ERR_INVALID, "%s: rows of out overlap", fn);
   const bool same = q == out && q_stride_s == o_stride_s && q_stride_h == o_stride_h;
-  if (!same && token_rows_overlap(q, q_stride_s, q_stride_h, out, o_stride_s, o_stride_h, n_tokens, Hq, head_dim, eb))
+  if (!same && token_rows_overlap(q, q_stride_s, q_stride_h, Hq, out, o_stride_s, o_stride_h, Hq, n_tokens, head_dim, eb))
     return fail(MGA_ERR_INVALID, "%s: out overlaps q", fn);
   float *ws = nullptr;
   const int64_t need = mga::paged_attn_ws_bytes(n_tokens, n_seqs, Hq, Hkv, head_dim, (int64_t)page_size * table_width, dtype);

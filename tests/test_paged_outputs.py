@@ -37,3 +37,19 @@ def test_rows_that_overlap(mga, T, H):
             apart += 1
             refused(mga, _attend(lib, ss * D // 2, hs * D // 2, T, H, ctypes.c_void_p((1 << 20) + 16)), b"out overlaps q")
     assert apart > 10
+
+
+# rows of one buffer from 1 << 20 on: 4 query heads, 2 of keys, 2 of values, then room for 4 more
+Q, K, V, MORE = (ctypes.c_void_p((1 << 20) + 2 * D * h) for h in (0, 4, 6, 8))
+
+
+@pytest.mark.parametrize("out,ss,hs,ok", [(Q, 12, 1, True), (MORE, 12, 1, True), (K, 12, 1, False), (V, 12, 1, False),
+                                          (ctypes.c_void_p((1 << 20) + 2 * D), 12, 1, False), (Q, 24, 1, False), (Q, 12, 2, False),
+                                          (ctypes.c_void_p((1 << 20) + 2 * D * 11), 12, 1, False),
+                                          (ctypes.c_void_p((1 << 20) + 2 * D * 36), 4, 1, True)])
+def test_query_out_beside_the_operands(mga, out, ss, hs, ok):
+    p = ctypes.c_void_p(64)
+    rc = mga.load_library().mga_paged_append(K, 12 * D, D, V, 12 * D, D, Q, 12 * D, D, None, None, None, None, 0, 0,
+                                             -1.0 if ok else 1e-6, 3, 1, 4, 2, D, 0, p, p, p, p, 4, 64, p, 4, 4, p, p, out,
+                                             ss * D, hs * D, None)
+    refused(mga, rc, b"eps" if ok else b"query_out overlaps")   # a good one for its eps, behind this check
