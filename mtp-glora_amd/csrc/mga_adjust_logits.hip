@@ -14,7 +14,8 @@
 // tiles where the rows alone fill the chip. Columns that nothing hit are copied as they are; the others find
 // their biases in the tile's list, kept in the caller's order, so that equal ids add up in it.
 // Counts of up to 2^14 - 1 tokens take 16 bits a column and biases of up to 1024 entries a list; longer ones
-// (the wide form) 32 bits and a sum a column, added by the first entry of each column for those after it.
+// (the wide form) 32 bits and a sum a column, added by the first entry of each column for those after it. What
+// decides is the room for a row's tokens, not its length: the 80 rows in rows of 16 383 17.3 us, of 16 384 21.8.
 #include <type_traits>
 
 #include "mga_internal.hpp"

@@ -17,8 +17,9 @@
 // bytes in this pattern reaches 5.85 TB/s here. 64 sequences of 177 385 tokens in all, a token each
 // (364 MB): 75 us + 5 us joining, 4.5 TB/s; 2 of 212 590 (435 MB): 81 + 7 us, 4.9 TB/s; what is left is
 // the start (cu, lengths, pages, first keys: 4 us), the join's launch, and waves that end up to 15% apart
-// with equal shares. Prompts: the matrix unit and the softmax's vector work beside it: 10 075 new
-// tokens behind up to 15 399, 1175 GFLOP visible, 1.29 ms, 913 TFLOP/s.
+// with equal shares. Prompts: the matrix unit and the softmax's vector work beside it, and the last tiles, which leave
+// a part of the chip idle: 10 075 new tokens behind up to 15 399, 1175 GFLOP visible, 1.24 ms, 945 TFLOP/s,
+// in the orders of the same four sequences 1.11 to 1.26 ms.
 //
 // Three forms share this: few rows a sequence over long ones by equal shares (paged_share_kernel), short
 // sequences by a workgroup a tile (paged_tile_kernel), prompts by 128 rows (paged_prompt_kernel, further
@@ -155,7 +156,7 @@ struct Tile {
   }
 };
 
-// Tiles are also numbered without a scan: sequence b owns the slots from (cu[b] >> tmshift) + b
+// Tiles are also numbered without sums over the sequences: b owns the slots from (cu[b] >> tmshift) + b
 // on, as many as n tokens can make tiles.
 __device__ __forceinline__ int tile_slot(const SeqSpan &q, int b, int t, int tmshift) {
   return (q.first >> tmshift) + b + t;
@@ -163,7 +164,8 @@ __device__ __forceinline__ int tile_slot(const SeqSpan &q, int b, int t, int tms
 __host__ __device__ __forceinline__ int tile_slots(int T, int B, int tmshift) { return (T >> tmshift) + B; }
 
 // The tile of a slot; false: none. All lanes of the wave take part. The lanes' loads find the
-// sequence and hold what is needed of it.
+// sequence, 64 a turn, and hold what is needed of it. (A token each over 100 keys, 32 / 8 heads of 128: 12.6 us for
+// 64 sequences, 95 for 512, 220 for 1024, 1496 for 4096, 760 at the rate of 512.)
 __device__ __forceinline__ bool tile_of_slot(const PagedAttnArgs &a, int slot, int tmshift, int G, Tile &x) {
   for (int i0 = 0; i0 < a.B; i0 += 64) {
     const int i = min(i0 + (int)(threadIdx.x & 63), a.B - 1);
@@ -874,7 +876,7 @@ __global__ __launch_bounds__(256, Parts<T>::n == 1 ? 2 : 1) void paged_prompt_ke
   const int PS = 1 << a.pshift;
   Tile x;
   x.h = blockIdx.x % a.Hkv;
-  const int slot = slots - 1 - (int)blockIdx.x / a.Hkv;   // long tiles first
+  const int slot = slots - 1 - (int)blockIdx.x / a.Hkv;   // the last sequence first, of each its longest tiles
   if (tile_of_slot(a, slot, tmshift, G, x)) {
     const int row = w * 32 + l32, first_lim = x.q.len + x.tok0, end_key = x.q.len + x.q.n;
     const int lim = row < x.rows ? first_lim + row / G : -1;
@@ -1150,7 +1152,8 @@ struct Shape {
 };
 
 // Keys up to which a sequence is one workgroup's: 1 x 1 token, 32 / 8 heads of 128, over 1000 keys 10.4 us in
-// one launch, 12.4 by shares; a CU's rate bounds it from there (20 ns a key).
+// one launch, 12.4 by shares; a CU's rate bounds it from there (20 ns a key). They are those that the table has
+// room for: lengths are not known on the host.
 constexpr int kShortKeys = 1024;
 
 // The narrowest tile that holds an average sequence's query rows: a wide one's empty

@@ -14,7 +14,9 @@ mask tokens, a prompt, or a part of one) as rows packed one behind the other:
 tokens in the cache. All three stay on the device and nothing is read back, so a step can
 be captured in a graph and replayed with other lengths: a batch of fewer tokens than
 rows ends at cu_tokens[B], a sequence without new tokens takes none. Rejected drafts are
-dropped by not adding them to ``lengths``: the next append overwrites them. Which pages a
+dropped by not adding them to ``lengths``: the next append overwrites them. The scale of
+their page does not shrink again, so that a page in which a large value was dropped holds
+its other values by fewer bits until it is begun anew. Which pages a
 sequence gets is the caller's to say; no two may write to one page, any may read it.
 
 Neither call computes a gradient; operands that ask for one, in reverse or forward mode, are refused.
@@ -179,7 +181,9 @@ def paged_attention(query: torch.Tensor, pages, block_table: torch.Tensor, cu_to
     ``pages`` (KVPages): token i of a sequence sees positions 0 .. lengths + i, its own
     included, so append first, with the same table, cu_tokens and lengths. Query head h
     reads KV head h // (Hq / Hkv). Positions without a page are masked; a row that sees
-    nothing is zeros. Scores and softmax in fp32. ``out`` (``query`` itself, or
+    nothing is zeros. Scores, sums and outputs in fp32; the probabilities are held to 16 bits (fp32
+    queries: 24; bf16 queries in a batch of prompts, which takes another form by its average number of new
+    tokens: 8, as the output). ``out`` (``query`` itself, or
     rows that do not overlap it) receives the result; its rows
     behind the last sequence's tokens stay as they are, in a tensor made here they are
     zeros. Hq / Hkv <= 32, at most 4096 sequences."""

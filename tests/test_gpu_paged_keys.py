@@ -29,7 +29,8 @@ def append(mga, dev, k, cos, sin, new, ps=16):
     before = pool.clone()
     mga.paged_append(k, torch.zeros_like(k), pool.pages, *pool.batch, cos=cos, sin=sin)
     torch.cuda.synchronize()
-    exact = po.prepared(f64(k), cos=f64(cos), sin=f64(sin))
+    with np.errstate(invalid="ignore"):
+        exact = po.prepared(f64(k), cos=f64(cos), sin=f64(sin))
     check_append(before, pool, exact, np.zeros(k.shape), np.zeros(k.shape), np.zeros(k.shape))
     return pool, exact
 
